@@ -462,6 +462,79 @@ int slx_gate_skip_bwd_as(const slx_glue_shape *s, const void *y, const void *u,
                          const void *d_out, void *dy, void *du, void *d_gate, void *d_skip,
                          void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- gated delta rule ------------------------------------------------------------ */
+
+/* The second recurrence of the backend, for layers that write into their state by the delta
+ * rule (no counterpart in the reference).  Per value head, state S (P, N), a_t = exp(g_t):
+ *   S_t = a_t S_{t-1} + beta_t (v_t - a_t S_{t-1} k_t) k_t^T,   o_t = scale * S_t q_t
+ * q, k (batch, key_heads, T, N); v, o (batch, heads, T, P); g, beta (batch, heads, T); value
+ * head h reads key head h / (heads / key_heads).  q, k, v, g and beta may have any strides over
+ * batch, head and token (a dense last axis; in elements, >= 0); the strides of an axis of one
+ * element are not read.  States are (batch, heads, P, N).
+ * g is a log decay; -inf (and anything below -110) drops the state.  A non-finite value in any
+ * other place makes outputs of its head from its chunk of 64 tokens on NaN. */
+typedef struct {
+  int32_t batch, heads, key_heads, T, P, N; /* N <= 128, P <= 256, heads a multiple of key_heads */
+  int32_t dtype;                            /* slx_dtype of q, k, v, o and their gradients       */
+  int32_t g_dtype, beta_dtype;              /* of g and beta and their gradients                  */
+  float scale;
+  int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3], beta_stride[3];
+} slx_gated_delta_shape;
+
+size_t slx_gated_delta_fwd_workspace_bytes(const slx_gated_delta_shape *s);
+/* What the backward needs of the forward (states before every chunk, prediction errors). */
+size_t slx_gated_delta_residual_bytes(const slx_gated_delta_shape *s);
+size_t slx_gated_delta_bwd_workspace_bytes(const slx_gated_delta_shape *s);
+
+/* o (contiguous) may be NULL: then only the states are computed.  final_state is fp32.
+ * workspace and residual 256-byte aligned. */
+int slx_gated_delta_fwd(const slx_gated_delta_shape *s, const void *q, const void *k, const void *v,
+                        const void *g, const void *beta, const void *initial_state /*[opt]*/,
+                        int32_t initial_dtype, void *o /*[opt]*/, float *final_state /*[opt]*/,
+                        void *residual /*[opt]*/, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/* VJP of slx_gated_delta_fwd.  d_o (batch, heads, T, P) contiguous; d_final (batch, heads, P, N).
+ * dq, dk (batch, key_heads, T, N), dv, dg, dbeta are contiguous and overwritten; sums run in a
+ * fixed order (no atomics). */
+int slx_gated_delta_bwd(const slx_gated_delta_shape *s, const void *q, const void *k, const void *g,
+                        const void *beta, const void *residual, const void *d_o,
+                        const void *d_final /*[opt]*/, int32_t d_final_dtype, void *dq, void *dk,
+                        void *dv, void *dg, void *dbeta, void *d_initial /*[opt]*/,
+                        int32_t d_initial_dtype, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/* One token of the same recurrence on carried states (T must be 1; strides over batch and head):
+ * o (batch, heads, P) contiguous; state_in and state_out (batch, heads, P, N) fp32, state_in NULL
+ * = zero states; state_out may be state_in.  No workspace. */
+int slx_gated_delta_step(const slx_gated_delta_shape *s, const void *q, const void *k, const void *v,
+                         const void *g, const void *beta, const float *state_in /*[opt]*/, void *o,
+                         float *state_out, void *stream);
+
+/* ---- tokens from logits ------------------------------------------------------------ */
+
+typedef struct {
+  int32_t rows, vocab;  /* vocab <= 262144 */
+  int32_t dtype;        /* slx_dtype of the logits */
+  int32_t u_bytes;      /* 4: u is float, 8: double */
+  int32_t top_k_bytes;  /* 4 or 8: size of an entry of top_k, where that is given */
+  float temperature, top_p, min_p; /* of every row, where the pointer of the same name is NULL */
+  int64_t top_k;
+  int64_t row_stride;   /* elements between rows of the logits; their last axis is dense */
+} slx_sample_shape;
+
+/* out[row] = token drawn with the random number u[row] in [0, 1).  Tokens are ranked by logit
+ * (ties: lower index first); the first top_k stay (<= 0: all), of these the shortest run that
+ * holds at least top_p of their mass (>= 1: all), of these the ones with at least min_p of the
+ * largest mass; the draw takes, in the order of the indices, the first token at which the running
+ * mass exceeds u times the whole.  Masses are exp((logit - largest) / temperature) in 64 bits.
+ * temperature <= 0 takes the first largest logit.  NaN logits count as -inf; a row without a
+ * logit above -inf gives -1.  (No counterpart in the reference.) */
+int slx_sample(const slx_sample_shape *s, const void *logits, const void *u,
+               const float *temperature /*[opt]*/, const void *top_k /*[opt]*/,
+               const float *top_p /*[opt]*/, const float *min_p /*[opt]*/, int64_t *out,
+               void *stream);
+
 /* ---- diagnostics ----------------------------------------------------------- */
 
 /* Half inputs with chunk 128, P 64 and 2N in {64,128,192,256} run on the

@@ -54,6 +54,19 @@ class ConvShape(Structure):
                 ("x_batch_stride", c_int64)]
 
 
+class GatedDeltaShape(Structure):
+    _fields_ = [("batch", c_int32), ("heads", c_int32), ("key_heads", c_int32), ("T", c_int32), ("P", c_int32),
+                ("N", c_int32), ("dtype", c_int32), ("g_dtype", c_int32), ("beta_dtype", c_int32), ("scale", c_float),
+                ("q_stride", c_int64 * 3), ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3),
+                ("g_stride", c_int64 * 3), ("beta_stride", c_int64 * 3)]
+
+
+class SampleShape(Structure):
+    _fields_ = [("rows", c_int32), ("vocab", c_int32), ("dtype", c_int32), ("u_bytes", c_int32), ("top_k_bytes", c_int32),
+                ("temperature", c_float), ("top_p", c_float), ("min_p", c_float), ("top_k", c_int64),
+                ("row_stride", c_int64)]
+
+
 # name -> (restype, argtypes); mirrors include/slinoss_b200.h one to one
 _P = c_void_p
 SIGNATURES = {
@@ -97,6 +110,14 @@ SIGNATURES = {
     "slx_segment_fold": (c_int32, [c_int32] * 4 + [_P, c_int64, _P, c_int64, c_int32, _P, _P]),
     "slx_segment_axpy": (c_int32, [c_int32] * 3 + [_P] * 3 + [c_int32, _P, _P]),
     "slx_segment_transition": (c_int32, [c_int32] * 2 + [_P] * 3),
+    "slx_gated_delta_fwd_workspace_bytes": (c_size_t, [POINTER(GatedDeltaShape)]),
+    "slx_gated_delta_residual_bytes": (c_size_t, [POINTER(GatedDeltaShape)]),
+    "slx_gated_delta_bwd_workspace_bytes": (c_size_t, [POINTER(GatedDeltaShape)]),
+    "slx_gated_delta_fwd": (c_int32, [POINTER(GatedDeltaShape)] + [_P] * 6 + [c_int32] + [_P] * 4 + [c_size_t, _P]),
+    "slx_gated_delta_bwd": (c_int32, [POINTER(GatedDeltaShape)] + [_P] * 7 + [c_int32] + [_P] * 6
+                            + [c_int32, _P, c_size_t, _P]),
+    "slx_gated_delta_step": (c_int32, [POINTER(GatedDeltaShape)] + [_P] * 9),
+    "slx_sample": (c_int32, [POINTER(SampleShape)] + [_P] * 8),
     "slx_cconv1d_bwd_workspace_bytes": (c_size_t, [POINTER(ConvShape)]),
     "slx_cconv1d_bwd": (c_int32, [POINTER(ConvShape)] + [_P] * 11 + [c_size_t, _P]),
 }

@@ -1,0 +1,476 @@
+// Shared pieces of the gated delta rule kernels: sizes, the per-chunk record, scaled fp16 operands and the matrix
+// instructions.
+//
+// Recurrence of a head, a_t = exp(g_t), state S (P, N):
+//     y_t = v_t - a_t S_{t-1} k_t,   S_t = a_t S_{t-1} + beta_t y_t k_t^T,   o_t = scale S_t q_t
+// over chunks of 64 tokens.  With G the running sum of g inside a chunk, S0 the state before it,
+// dec_ts = e^{G_t-G_s}, closing_s = e^{G_63-G_s}:
+//     M_ts = dec_ts k_t.k_s (s < t),   Tm = (I + M diag(beta))^{-1},   Y = Tm (v - e^G S0 k)
+//     P_ts = dec_ts q_t.k_s (s <= t),  o = scale (e^G S0 q + P beta Y),  S1 = e^{G_63} S0 + sum_s closing_s beta_s y_s k_s^T
+//
+// Operands.  Products run on the fp16 matrix instructions with fp32 sums.  bf16 and fp16 values are exact in fp16 once a
+// power of two per tile has brought the tile's largest magnitude to [2^14, 2^15); a computed operand is one fp16 value
+// (11 bits) where the result is rounded to bf16 anyway, and a pair hi + lo (22 bits) where it feeds an fp32 or fp16 result.
+// A pair costs two or three products instead of one.  (bf16 pairs hold 16 bits: 3e-6 in the fp32 states, against 2e-7.)
+#pragma once
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace slx {
+namespace delta {
+
+constexpr int L = 64;             // tokens of a chunk
+constexpr int kTri = 3072;        // elements of a lower triangular 64 x 64 tile, by row blocks of 16 (tri_at)
+constexpr int kThreads = 128;
+
+// What every later kernel needs of one chunk and head, written once by delta_chunk_kernel.
+struct Record {
+  __half T[2][kTri];  // Tm, hi and lo
+  __half Q[2][kTri];  // P, hi and lo
+  float gamma[L], closing[L], beta[L];
+  double G[L];
+  int eT, eQ, eq, ek;  // binary exponents: value = stored * 2^e
+  int pad[28];
+};
+static_assert(sizeof(Record) == 25984 && sizeof(Record) % 128 == 0, "record layout");
+constexpr int kHeadBytes = 3 * L * 4 + L * 8 + 16;  // gamma .. ek
+
+struct Rows {  // a (batch, head, token, :) tensor whose last axis is dense; strides in elements
+  const void *p;
+  int64_t sb, sh, st;
+  int vec;  // 16-byte accesses are aligned
+};
+
+struct Args {
+  int batch, heads, key_heads, T, P, N, NC;
+  int P16;  // P rounded up to 16
+  float scale;
+  int g_dtype, beta_dtype;
+  Rows q, k, v, g, beta, dO;
+  Record *rec;              // (batch*heads, NC)
+  // forward
+  const void *init;         // (batch, heads, P, N) or null
+  int init_dtype;
+  void *o;                  // (batch, heads, T, P) or null
+  float *final_state;       // or null
+  __half *st;               // states before every chunk: (BH, NC, planes, P16, NT), or null
+  __half *y;                // Y of every chunk: (BH, NC, planes, 64, P16), or null
+  int *est, *ey;            // (BH, NC, P16 / 16)
+  // backward
+  const void *d_final;
+  int d_final_dtype;
+  void *d_init;
+  int d_init_dtype;
+  __half *ds, *dx;          // as st and y: gradients of the states after every chunk, dX
+  int *eds, *edx, *edo;
+  void *dv;                 // (batch, heads, T, P)
+  void *dq, *dk;            // (batch, key_heads, T, N) in dtype, or fp32 per value head where heads share keys
+  void *dg, *dbeta;         // (batch, heads, T)
+};
+
+// ---- 64 x 64 lower triangular tiles: row blocks of 16 rows, block i holds columns 0 .. 16 i + 15 and 8 of padding (an odd
+// number of 16-byte units per row: ldmatrix meets no bank twice).  5/8 of the square's bytes.
+__host__ __device__ constexpr int tri_base(int i) { return 128 * i * i + 256 * i; }
+__host__ __device__ constexpr int tri_ld(int i) { return 16 * i + 24; }
+
+// ---- exponents -----------------------------------------------------------------------------------------------------
+constexpr int kZeroExp = -100;  // of a tile of zeros
+// Of a tile that holds an infinity or NaN: its powers are NaN, so that everything computed from the tile is NaN and not a
+// finite value that scaling by the infinity has wiped out.
+constexpr int kNanExp = 2000;
+__device__ __forceinline__ float pow2(int e) {
+  return abs(e) > 1000 ? __int_as_float(0x7fc00000) : __int_as_float((min(max(e, -126), 127) + 127) << 23);
+}
+// e with max * 2^-e in [2^14, 2^15), from the bits of the largest magnitude
+__device__ __forceinline__ int exp_of(unsigned bits) {
+  return bits >= 0x7f800000u ? kNanExp : bits == 0u ? kZeroExp : max((int)(bits >> 23) - 127 - 14, kZeroExp);
+}
+// an exponent for a product's operand such that an accumulator of exponent ec, brought to the product's unit e + eb, stays
+// far inside the range (what the raising rounds away is 2^-40 of the accumulator)
+__device__ __forceinline__ int floor_exp(int e, int ec, int eb) { return max(e, ec - eb - 40); }
+__device__ __forceinline__ unsigned mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+template <int n>
+__device__ __forceinline__ unsigned max_mag(const float (&c)[n][4]) {
+  unsigned m = 0;
+#pragma unroll
+  for (int j = 0; j < n; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, mag(c[j][i]));
+  return m;
+}
+template <int n>
+__device__ __forceinline__ int warp_exp(const float (&c)[n][4]) {
+  return exp_of(__reduce_max_sync(0xffffffffu, max_mag(c)));
+}
+
+// ---- matrix instructions -------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void stsm(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};"
+               :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void stsm_t(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};"
+               :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+// A 16 x 16 block of a row-major half tile at `tile` (leading dimension ld).  The four registers are
+//   block_rows:  {rows 0-7, cols 0-7}, {rows 8-15, cols 0-7}, {rows 0-7, cols 8-15}, {rows 8-15, cols 8-15}
+//   block_cols:  the same with rows and columns exchanged in the order: {0-7, 0-7}, {0-7, 8-15}, {8-15, 0-7}, {8-15, 8-15}
+// read plainly or transposed.  As operands:
+//   A (16 x 16) from [m][k]: block_rows plain;  from [k][m]: block_cols transposed
+//   B (16 x 16, two n8 tiles b[0..1], b[2..3]) from [n][k]: block_cols plain;  from [k][n]: block_rows transposed
+__device__ __forceinline__ uint32_t block_rows(const __half *tile, int ld) {
+  const int lane = threadIdx.x & 31;
+  return smem_addr(tile + (lane & 15) * ld + (lane >> 4) * 8);
+}
+__device__ __forceinline__ uint32_t block_cols(const __half *tile, int ld) {
+  const int lane = threadIdx.x & 31;
+  return smem_addr(tile + ((lane & 7) + (lane >> 4) * 8) * ld + ((lane >> 3) & 1) * 8);
+}
+__device__ __forceinline__ void a_mk(uint32_t (&r)[4], const __half *t, int ld) { ldsm(r, block_rows(t, ld)); }
+__device__ __forceinline__ void a_km(uint32_t (&r)[4], const __half *t, int ld) { ldsm_t(r, block_cols(t, ld)); }
+__device__ __forceinline__ void b_nk(uint32_t (&r)[4], const __half *t, int ld) { ldsm(r, block_cols(t, ld)); }
+__device__ __forceinline__ void b_kn(uint32_t (&r)[4], const __half *t, int ld) { ldsm_t(r, block_rows(t, ld)); }
+
+__device__ __forceinline__ uint32_t pack(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack(uint32_t r) { return __half22float2(*reinterpret_cast<const __half2 *>(&r)); }
+// planes of two values, already scaled
+template <int S>
+__device__ __forceinline__ void split(float x, float y, uint32_t *hi, uint32_t *lo) {
+  *hi = pack(x, y);
+  if constexpr (S == 2) {
+    const float2 h = unpack(*hi);
+    *lo = pack(x - h.x, y - h.y);
+  }
+}
+
+// An A operand: S planes of a 16 x 16 block.
+template <int S>
+struct Frag {
+  uint32_t r[S][4];
+};
+// from the accumulators of two neighbouring n8 tiles, times s
+template <int S>
+__device__ __forceinline__ void frag_of(Frag<S> &f, const float (&c0)[4], const float (&c1)[4], float s) {
+  uint32_t *lo = f.r[S - 1];
+  split<S>(c0[0] * s, c0[1] * s, &f.r[0][0], lo + 0);
+  split<S>(c0[2] * s, c0[3] * s, &f.r[0][1], lo + 1);
+  split<S>(c1[0] * s, c1[1] * s, &f.r[0][2], lo + 2);
+  split<S>(c1[2] * s, c1[3] * s, &f.r[0][3], lo + 3);
+}
+// c0, c1 += A B for the two n8 tiles of B; planes of A and B whose product is below 2^-22 are left out
+template <int SA, int SB>
+__device__ __forceinline__ void mma_split(float (&c0)[4], float (&c1)[4], const Frag<SA> &a, const uint32_t (&b)[SB][4]) {
+  mma(c0, a.r[0], b[0][0], b[0][1]);
+  mma(c1, a.r[0], b[0][2], b[0][3]);
+  if constexpr (SA == 2) {
+    mma(c0, a.r[1], b[0][0], b[0][1]);
+    mma(c1, a.r[1], b[0][2], b[0][3]);
+  }
+  if constexpr (SB == 2) {
+    mma(c0, a.r[0], b[1][0], b[1][1]);
+    mma(c1, a.r[0], b[1][2], b[1][3]);
+  }
+}
+template <int n>
+__device__ __forceinline__ void zero(float (&c)[n][4]) {
+#pragma unroll
+  for (int j = 0; j < n; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+}
+template <int n>
+__device__ __forceinline__ void times(float (&c)[n][4], float s) {
+#pragma unroll
+  for (int j = 0; j < n; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[j][i] *= s;
+}
+template <int n>
+__device__ __forceinline__ void times_rows(float (&c)[n][4], float s0, float s1) {  // rows lane / 4 and lane / 4 + 8
+#pragma unroll
+  for (int j = 0; j < n; ++j) {
+    c[j][0] *= s0;
+    c[j][1] *= s0;
+    c[j][2] *= s1;
+    c[j][3] *= s1;
+  }
+}
+
+// ---- asynchronous copies -------------------------------------------------------------------------------------------
+__device__ __forceinline__ void cp16(void *dst, const void *src, bool valid) {  // zeros where not valid
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(smem_addr(dst)), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(n) : "memory"); }
+
+template <typename TI>
+__device__ __forceinline__ const TI *head_base(const Rows &r, int b, int h, int t) {
+  return static_cast<const TI *>(r.p) + b * r.sb + h * r.sh + (int64_t)t * r.st;
+}
+
+// Row-major operand tiles of 64 tokens x W columns (leading dimension W + 8), SI fp16 planes one after another.
+// issue(): starts the copy of `rows` rows of `cols` columns, zeros elsewhere; finish(): what a thread has copied, brought
+// to scaled fp16 in place (called by the same threads after the copy has arrived and before the CTA's barrier).
+template <typename TI, int SI, int W>
+struct Operand {
+  static constexpr int ld = W + 8;
+  static constexpr int plane = L * ld;
+  static constexpr int bytes = SI * plane * 2;
+  static constexpr bool async_convert = sizeof(TI) == 2;
+
+  static __device__ __forceinline__ void issue(__half *dst, const TI *src, int64_t st, int rows, int cols, bool vec, int e) {
+    const float s = pow2(-e);
+    if constexpr (async_convert) {
+      if (vec) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < L * (W / 8); i += kThreads) {
+          const int r = i / (W / 8), c = (i % (W / 8)) * 8;
+          const bool ok = r < rows && c < cols;
+          cp16(dst + r * ld + c, ok ? src + r * st + c : src, ok);
+        }
+        return;
+      }
+      for (int i = threadIdx.x; i < L * W; i += kThreads) {
+        const int r = i / W, c = i % W;
+        dst[r * ld + c] = __float2half_rn(r < rows && c < cols ? to_f(src[r * st + c]) * s : 0.f);
+      }
+    } else {
+      for (int i = threadIdx.x; i < L * (W / 4); i += kThreads) {
+        const int r = i / (W / 4), c = (i % (W / 4)) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows && c < cols) {
+          const float *at = reinterpret_cast<const float *>(src) + r * st + c;
+          if (vec) x = *reinterpret_cast<const float4 *>(at);
+          else {
+            x.x = at[0];
+            if (c + 1 < cols) x.y = at[1];
+            if (c + 2 < cols) x.z = at[2];
+            if (c + 3 < cols) x.w = at[3];
+          }
+        }
+        uint2 hi, lo;
+        split<2>(x.x * s, x.y * s, &hi.x, &lo.x);
+        split<2>(x.z * s, x.w * s, &hi.y, &lo.y);
+        *reinterpret_cast<uint2 *>(dst + r * ld + c) = hi;
+        *reinterpret_cast<uint2 *>(dst + plane + r * ld + c) = lo;
+      }
+    }
+  }
+  static __device__ __forceinline__ void finish(__half *dst, bool vec, int e) {
+    if constexpr (sizeof(TI) == 2 && !std::is_same<TI, __half>::value) {
+      if (!vec) return;
+      const float s = pow2(-e);
+#pragma unroll 2
+      for (int i = threadIdx.x; i < L * (W / 8); i += kThreads) {
+        uint4 *at = reinterpret_cast<uint4 *>(dst + (i / (W / 8)) * ld + (i % (W / 8)) * 8);
+        uint4 x = *at;
+        uint32_t *w = reinterpret_cast<uint32_t *>(&x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] = pack(__uint_as_float(w[j] << 16) * s, __uint_as_float(w[j] & 0xffff0000u) * s);
+        *at = x;
+      }
+    }
+  }
+};
+
+// Largest magnitude of a tile in global memory (this thread's share), for its exponent.
+template <typename TI>
+__device__ __forceinline__ unsigned tile_mag(const TI *src, int64_t st, int rows, int cols, bool vec, int W) {
+  unsigned m = 0;
+  constexpr int V = 16 / sizeof(TI);
+  if (vec) {
+    const int per = W / V;
+    for (int i = threadIdx.x; i < L * per; i += kThreads) {
+      const int r = i / per, c = (i % per) * V;
+      if (r < rows && c < cols) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(src + r * st + c);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (sizeof(TI) == 4) m = max(m, w[j] & 0x7fffffffu);
+          else m = max(m, max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));  // bf16
+        }
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < rows * cols; i += kThreads) m = max(m, mag(to_f(src[(i / cols) * st + i % cols])));
+  }
+  return m;
+}
+
+// A raw tile of 64 tokens x up to 64 columns, kept in TI.
+template <typename TI>
+struct Raw {
+  static constexpr int ld = 64 + 16 / (int)sizeof(TI);
+  static constexpr int bytes = L * ld * (int)sizeof(TI);
+  static __device__ __forceinline__ void issue(TI *dst, const TI *src, int64_t st, int rows, int cols, int width, bool vec) {
+    constexpr int V = 16 / sizeof(TI);
+    if (vec) {
+      const int per = width / V;
+      for (int i = threadIdx.x; i < L * per; i += kThreads) {
+        const int r = i / per, c = (i % per) * V;
+        const bool ok = r < rows && c < cols;
+        cp16(dst + r * ld + c, ok ? src + r * st + c : src, ok);
+      }
+    } else {
+      for (int i = threadIdx.x; i < L * width; i += kThreads) {
+        const int r = i / width, c = i % width;
+        dst[r * ld + c] = r < rows && c < cols ? src[r * st + c] : from_f<TI>(0.f);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void copy_bytes(void *dst, const void *src, int bytes) {  // asynchronous, multiples of 16
+  for (int i = threadIdx.x * 16; i < bytes; i += kThreads * 16)
+    cp16(static_cast<char *>(dst) + i, static_cast<const char *>(src) + i, true);
+}
+
+// A warp's (16 columns p, 64 tokens) result, held transposed in accumulators (rows p, columns t), to global rows of `out`
+// at its column p0: through `buf` (64 x 24 halves of the warp's own) for half types, directly for fp32.
+template <typename TO>
+__device__ __forceinline__ void store_rows(TO *out, int64_t st, int rows, int cols, const float (&c)[8][4], __half *buf) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = 8 * j + 2 * q + (i & 1), p = g + (i >> 1) * 8;
+        if (t < rows && p < cols) out[t * st + p] = c[j][i];
+      }
+  } else {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      uint32_t r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = c[j + (i >> 1)][(i & 1) * 2], y = c[j + (i >> 1)][(i & 1) * 2 + 1];
+        if constexpr (std::is_same<TO, __half>::value) r[i] = pack(x, y);
+        else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+          r[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+      }
+      // matrices {p 0-7, t 0-7}, {p 8-15, t 0-7}, {p 0-7, t 8-15}, {p 8-15, t 8-15} of [p][t], stored as [t][p]
+      stsm_t(smem_addr(buf + (8 * j + (lane & 7) + (lane >> 4) * 8) * 24 + ((lane >> 3) & 1) * 8), r);
+    }
+    __syncwarp();
+    const bool wide = cols >= 16 && (st & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    if (wide) {
+#pragma unroll
+      for (int i = lane; i < 128; i += 32)
+        if ((i >> 1) < rows)
+          *reinterpret_cast<uint4 *>(out + (i >> 1) * st + (i & 1) * 8) =
+              *reinterpret_cast<const uint4 *>(buf + (i >> 1) * 24 + (i & 1) * 8);
+    } else {
+      for (int i = lane; i < 1024; i += 32)
+        if ((i >> 4) < rows && (i & 15) < cols)
+          out[(i >> 4) * st + (i & 15)] = reinterpret_cast<const TO *>(buf)[(i >> 4) * 24 + (i & 15)];
+    }
+  }
+}
+
+// Accumulators (rows p, columns t) as S planes of scaled fp16 rows [t][p] in global memory (leading dimension st, 64 rows,
+// always whole); returns their exponent.
+template <int S>
+__device__ __forceinline__ int store_planes(__half *out, int64_t st, int64_t plane, const float (&c)[8][4], __half *buf) {
+  const int lane = threadIdx.x & 31;
+  const int e = warp_exp(c);
+  const float s = pow2(-e);
+#pragma unroll
+  for (int pl = 0; pl < S; ++pl) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      Frag<S> f;
+      frag_of<S>(f, c[j], c[j + 1], s);
+      stsm_t(smem_addr(buf + (8 * j + (lane & 7) + (lane >> 4) * 8) * 24 + ((lane >> 3) & 1) * 8), f.r[pl]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = lane; i < 128; i += 32)
+      *reinterpret_cast<uint4 *>(out + pl * plane + (i >> 1) * st + (i & 1) * 8) =
+          *reinterpret_cast<const uint4 *>(buf + (i >> 1) * 24 + (i & 1) * 8);
+  }
+  return e;
+}
+
+// A warp's 16 rows of a state (accumulators: rows p, columns n) as S planes of fp16 rows of NT columns, scaled by 2^-e.
+template <int S, int NT>
+__device__ __forceinline__ void store_state(__half *out, int64_t plane, const float (&c)[NT / 8][4], int e, __half *buf) {
+  const int lane = threadIdx.x & 31;
+  const float s = pow2(-e);
+  constexpr int ld = NT + 8;
+#pragma unroll
+  for (int pl = 0; pl < S; ++pl) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < NT / 8; j += 2) {
+      Frag<S> f;
+      frag_of<S>(f, c[j], c[j + 1], s);
+      stsm(smem_addr(buf + (lane & 15) * ld + 8 * j + (lane >> 4) * 8), f.r[pl]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = lane; i < 16 * (NT / 8); i += 32)
+      *reinterpret_cast<uint4 *>(out + pl * plane + i * 8) =
+          *reinterpret_cast<const uint4 *>(buf + (i / (NT / 8)) * ld + (i % (NT / 8)) * 8);
+  }
+}
+
+// rows p0 .. p0 + 15 of a (P, N) matrix in any dtype, as accumulators
+template <int NT>
+__device__ __forceinline__ void load_state(float (&c)[NT / 8][4], const void *src, int dtype, size_t base, int p0, int P, int N) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+#pragma unroll
+  for (int j = 0; j < NT / 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + g + (i >> 1) * 8, n = 8 * j + 2 * q + (i & 1);
+      c[j][i] = p < P && n < N ? load_as_f(src, dtype, base + (size_t)p * N + n) : 0.f;
+    }
+}
+template <int NT>
+__device__ __forceinline__ void write_state(void *dst, int dtype, size_t base, const float (&c)[NT / 8][4], int p0, int P, int N) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+#pragma unroll
+  for (int j = 0; j < NT / 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + g + (i >> 1) * 8, n = 8 * j + 2 * q + (i & 1);
+      if (p < P && n < N) store_as(dst, dtype, base + (size_t)p * N + n, c[j][i]);
+    }
+}
+
+}  // namespace delta
+}  // namespace slx

@@ -1,0 +1,75 @@
+// Instances of the gated delta rule's kernels for one activation dtype: included by a source file each.
+#pragma once
+
+#include "delta_chunk.cuh"
+#include "delta_grad.cuh"
+#include "delta_launch.cuh"
+#include "delta_scan.cuh"
+
+namespace slx {
+namespace delta {
+
+template <int NT, int SI, int SC, typename TI>
+static int launch_chunk(const Args &a, cudaStream_t st) {
+  constexpr int bytes = chunk_smem<NT, SI>();
+  auto kernel = delta_chunk_kernel<NT, SI, TI>;
+  if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;
+  kernel<<<dim3(a.NC, a.batch * a.key_heads), kThreads, bytes, st>>>(a);
+  return check_launch("delta_chunk_kernel");
+}
+template <int NT, int SI, int SC, typename TI>
+static int launch_fwd(const Args &a, int warps, cudaStream_t st) {
+  if (const int rc = launch_chunk<NT, SI, SC, TI>(a, st)) return rc;
+  constexpr int bytes = scan_smem<NT, SI, SC, TI>(false);
+  auto kernel = delta_fwd_kernel<NT, SI, SC, TI>;
+  if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;
+  kernel<<<dim3((a.P16 / 16 + warps - 1) / warps, a.batch * a.heads), kThreads, bytes, st>>>(a, warps);
+  return check_launch("delta_fwd_kernel");
+}
+template <int NT, int SI, int SC, typename TI>
+static int launch_bwd(const Args &a, void *dq, void *dk, int warps, cudaStream_t st) {
+  if (const int rc = launch_chunk<NT, SI, SC, TI>(a, st)) return rc;
+  {
+    constexpr int bytes = scan_smem<NT, SI, SC, TI>(true);
+    auto kernel = delta_bwd_kernel<NT, SI, SC, TI>;
+    if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;
+    kernel<<<dim3((a.P16 / 16 + warps - 1) / warps, a.batch * a.heads), kThreads, bytes, st>>>(a, warps);
+    if (const int rc = check_launch("delta_bwd_kernel")) return rc;
+  }
+  {
+    constexpr int bytes = grad_smem<NT, SI, SC>();
+    auto kernel = delta_grad_kernel<NT, SI, SC, TI>;
+    if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;
+    kernel<<<dim3(a.NC, a.batch * a.heads), kThreads, bytes, st>>>(a);
+    if (const int rc = check_launch("delta_grad_kernel")) return rc;
+  }
+  if (a.heads != a.key_heads) {
+    const int64_t per = (int64_t)a.T * a.N, total = per * a.batch * a.key_heads;
+    const int64_t want = (total + 255) / 256;
+    delta_share_kernel<TI><<<dim3((unsigned)(want < 8 * kB200Sms ? want : 8 * kB200Sms), 2), 256, 0, st>>>(
+        static_cast<const float *>(a.dq), static_cast<const float *>(a.dk), static_cast<TI *>(dq), static_cast<TI *>(dk),
+        a.heads / a.key_heads, per, total);
+    return check_launch("delta_share_kernel");
+  }
+  return SLX_OK;
+}
+
+// planes of the inputs and of computed operands
+template <typename TI>
+constexpr int input_planes = sizeof(TI) == 4 ? 2 : 1;
+template <typename TI>
+constexpr int computed_planes = std::is_same<TI, __nv_bfloat16>::value ? 1 : 2;
+
+template <typename TI>
+int launch_fwd_as(const Args &a, int NT, int warps, cudaStream_t st) {
+  constexpr int SI = input_planes<TI>, SC = computed_planes<TI>;
+  return NT == 64 ? launch_fwd<64, SI, SC, TI>(a, warps, st) : launch_fwd<128, SI, SC, TI>(a, warps, st);
+}
+template <typename TI>
+int launch_bwd_as(const Args &a, int NT, void *dq, void *dk, int warps, cudaStream_t st) {
+  constexpr int SI = input_planes<TI>, SC = computed_planes<TI>;
+  return NT == 64 ? launch_bwd<64, SI, SC, TI>(a, dq, dk, warps, st) : launch_bwd<128, SI, SC, TI>(a, dq, dk, warps, st);
+}
+
+}  // namespace delta
+}  // namespace slx

@@ -1,0 +1,403 @@
+// The two passes of the gated delta rule along the sequence: states forwards (with the outputs), gradients of the states
+// backwards (with dV).
+//
+// Rows of a state (value channels) do not meet in the recurrence, so a warp owns 16 rows p for the whole sequence and keeps
+// its (16, N) part of the state in accumulators.  Every product has the 16 rows on the M side: the state and all that is
+// computed from it are A operands as they lie in registers, and the B operands (k, q, Tm, P) are tiles in shared memory
+// which the warps of a CTA share.  Per chunk, forward:
+//     X = v^T - gamma (S k^T)      Y = X Tm^T      o = gamma (S q^T) + (beta Y) P^T      S = Gam S + (closing beta Y) k
+// backward (R = dL/dS after the chunk, going down):
+//     dD = scale dO^T P + closing (R k^T)   dX = (beta dD) Tm   R = Gam R + (scale gamma dO)^T q - (gamma dX)^T k
+// The tiles of the next chunk are on their way while this one is computed: k is double-buffered, the rest is loaded again
+// as soon as its last reader is through.
+#pragma once
+
+#include "delta.cuh"
+
+namespace slx {
+namespace delta {
+
+template <int NT>
+constexpr int warp_buf() {  // halves: 64 x 24 or 16 x (NT + 8)
+  return 16 * (NT + 8) > 64 * 24 ? 16 * (NT + 8) : 64 * 24;
+}
+template <int NT, int SI, int SC, typename TI>
+constexpr int scan_smem(bool backward) {
+  return 3 * SI * L * (NT + 8) * 2 + (2 + (backward ? 2 : SC)) * kTri * 2 + kHeadBytes + Raw<TI>::bytes +
+         (kThreads / 32) * warp_buf<NT>() * 2;
+}
+
+// Columns c0 .. c0 + 15 of a raw tile, transposed: accumulators with rows p (the tile's columns) and columns t (its rows).
+template <typename TI>
+__device__ __forceinline__ void load_cols(float (&c)[8][4], const TI *tile, int c0) {
+  constexpr int ld = Raw<TI>::ld;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  if constexpr (sizeof(TI) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[j][i] = tile[(8 * j + 2 * q + (i & 1)) * ld + c0 + g + (i >> 1) * 8];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      uint32_t r[4];
+      a_km(r, reinterpret_cast<const __half *>(tile) + 8 * j * ld + c0, ld);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 x;
+        if constexpr (std::is_same<TI, __half>::value) x = unpack(r[i]);
+        else x = make_float2(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xffff0000u));
+        c[j + (i >> 1)][(i & 1) * 2] = x.x;
+        c[j + (i >> 1)][(i & 1) * 2 + 1] = x.y;
+      }
+    }
+  }
+}
+// times the entries s[t] of a vector over the columns
+__device__ __forceinline__ void times_cols(float (&c)[8][4], const float *s, float f) {
+  const int q = threadIdx.x & 3;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float2 x = *reinterpret_cast<const float2 *>(s + 8 * j + 2 * q);
+    c[j][0] *= x.x * f;
+    c[j][1] *= x.y * f;
+    c[j][2] *= x.x * f;
+    c[j][3] *= x.y * f;
+  }
+}
+template <int S>
+__device__ __forceinline__ void frags_of(Frag<S> (&f)[4], const float (&c)[8][4], int e) {
+  const float s = pow2(-e);
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb) frag_of<S>(f[kb], c[2 * kb], c[2 * kb + 1], s);
+}
+__device__ __forceinline__ int4 exps_of(const Record *r) { return __ldg(reinterpret_cast<const int4 *>(&r->eT)); }
+
+template <int NT, int SI, int SC, typename TI>
+__global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
+  using Op = Operand<TI, SI, NT>;
+  using V = Raw<TI>;
+  extern __shared__ __align__(128) char smem[];
+  __half *ks = reinterpret_cast<__half *>(smem);  // two buffers
+  __half *qs = ks + 2 * SI * Op::plane;
+  __half *Ts = qs + SI * Op::plane;  // T hi, T lo, planes of P, the record's vectors
+  __half *Ps = Ts + 2 * kTri;
+  float *hd = reinterpret_cast<float *>(Ps + SC * kTri);
+  const float *gamma = hd, *closing = hd + L, *beta = hd + 2 * L;
+  TI *vs = reinterpret_cast<TI *>(reinterpret_cast<char *>(hd) + kHeadBytes);
+
+  const int warp = threadIdx.x >> 5;
+  __half *buf = reinterpret_cast<__half *>(reinterpret_cast<char *>(vs) + V::bytes) + warp * warp_buf<NT>();
+  const int bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads, kh = h / (a.heads / a.key_heads);
+  const int first = blockIdx.x * pw * 16, p0 = first + warp * 16;  // value channels of the CTA, of the warp
+  const bool active = warp < pw && p0 < a.P16;
+  const Record *rec = a.rec + (size_t)bh * a.NC;
+  const int PB = a.P16 / 16;
+
+  auto issue_k = [&](int c, int ek) {
+    Op::issue(ks + (c & 1) * SI * Op::plane, head_base<TI>(a.k, b, kh, c * L), a.k.st, min(L, a.T - c * L), a.N, a.k.vec, ek);
+  };
+  auto issue_rest = [&](int c, int eq) {
+    const int rows = min(L, a.T - c * L);
+    Op::issue(qs, head_base<TI>(a.q, b, kh, c * L), a.q.st, rows, a.N, a.q.vec, eq);
+    copy_bytes(Ts, rec[c].T, (2 + SC) * kTri * 2);
+    copy_bytes(hd, rec[c].gamma, kHeadBytes);
+    V::issue(vs, head_base<TI>(a.v, b, h, c * L) + first, a.v.st, rows, a.P - first, pw * 16, a.v.vec);
+  };
+
+  float S[NT / 8][4];
+  if (active && a.init) load_state<NT>(S, a.init, a.init_dtype, (size_t)bh * a.P * a.N, p0, a.P, a.N);
+  else zero(S);
+  int4 ex = exps_of(rec);
+  issue_k(0, ex.w);
+  issue_rest(0, ex.z);
+  cp_commit();
+  for (int c = 0; c < a.NC; ++c) {
+    const bool more = c + 1 < a.NC;
+    const int4 nx = more ? exps_of(rec + c + 1) : ex;
+    const int eT = ex.x, eQ = ex.y, eq = ex.z, ek = ex.w;
+    const __half *kt = ks + (c & 1) * SI * Op::plane;
+    cp_wait<0>();
+    Op::finish(ks + (c & 1) * SI * Op::plane, a.k.vec, ek);
+    Op::finish(qs, a.q.vec, eq);
+    __syncthreads();
+    if (more) issue_k(c + 1, nx.w);
+    cp_commit();
+    Frag<2> fc[4];  // closing beta Y
+    int eC = 0;
+    float top = 0.f;  // Gam
+    if (active) {
+      const int eS = warp_exp(S);
+      if (a.st) {
+        const size_t at = (size_t)bh * a.NC + c;
+        store_state<SC, NT>(a.st + (at * SC * a.P16 + p0) * NT, (int64_t)a.P16 * NT, S, eS, buf);
+        if ((threadIdx.x & 31) == 0) a.est[at * PB + p0 / 16] = eS;
+      }
+      float X[8][4], O[8][4];
+      zero(X);
+      zero(O);
+      {
+        const float s = pow2(-eS);
+#pragma unroll
+        for (int kb = 0; kb < NT / 16; ++kb) {
+          Frag<2> f;
+          frag_of<2>(f, S[2 * kb], S[2 * kb + 1], s);
+          Frag<SC> fo;
+#pragma unroll
+          for (int pl = 0; pl < SC; ++pl)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fo.r[pl][i] = f.r[pl][i];
+#pragma unroll
+          for (int tb = 0; tb < 4; ++tb) {
+            uint32_t bb[SI][4];
+#pragma unroll
+            for (int s2 = 0; s2 < SI; ++s2) b_nk(bb[s2], kt + s2 * Op::plane + 16 * tb * Op::ld + 16 * kb, Op::ld);
+            mma_split<2, SI>(X[2 * tb], X[2 * tb + 1], f, bb);
+#pragma unroll
+            for (int s2 = 0; s2 < SI; ++s2) b_nk(bb[s2], qs + s2 * Op::plane + 16 * tb * Op::ld + 16 * kb, Op::ld);
+            mma_split<SC, SI>(O[2 * tb], O[2 * tb + 1], fo, bb);
+          }
+        }
+      }
+      // X = v - gamma S k
+      {
+        float v[8][4];
+        load_cols<TI>(v, vs, warp * 16);
+        times_cols(X, gamma, pow2(eS + ek));
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) X[j][i] = v[j][i] - X[j][i];
+      }
+      {
+        const int eX = warp_exp(X);
+        Frag<2> fx[4];
+        frags_of<2>(fx, X, eX);
+        zero(X);
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+          for (int kb = 0; kb <= tb; ++kb) {
+            uint32_t bb[2][4];
+            b_nk(bb[0], Ts + tri_base(tb) + 16 * kb, tri_ld(tb));
+            b_nk(bb[1], Ts + kTri + tri_base(tb) + 16 * kb, tri_ld(tb));
+            mma_split<2, 2>(X[2 * tb], X[2 * tb + 1], fx[kb], bb);
+          }
+        times(X, pow2(eX + eT));  // Y
+      }
+      if (a.y) {
+        const size_t at = (size_t)bh * a.NC + c;
+        const int e = store_planes<SC>(a.y + at * SC * L * a.P16 + p0, a.P16, (int64_t)L * a.P16, X, buf);
+        if ((threadIdx.x & 31) == 0) a.ey[at * PB + p0 / 16] = e;
+      }
+      times_cols(X, beta, 1.f);
+      if (a.o) {
+        times_cols(O, gamma, pow2(eS + eq));
+        const int eD = floor_exp(warp_exp(X), warp_exp(O), eQ);
+        times(O, pow2(-(eD + eQ)));
+        Frag<SC> fd[4];
+        frags_of<SC>(fd, X, eD);
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+          for (int kb = 0; kb <= tb; ++kb) {
+            uint32_t bb[SC][4];
+#pragma unroll
+            for (int pl = 0; pl < SC; ++pl) b_nk(bb[pl], Ps + pl * kTri + tri_base(tb) + 16 * kb, tri_ld(tb));
+            mma_split<SC, SC>(O[2 * tb], O[2 * tb + 1], fd[kb], bb);
+          }
+        times(O, a.scale * pow2(eD + eQ));
+        store_rows<TI>(static_cast<TI *>(a.o) + ((size_t)bh * a.T + c * L) * a.P + p0, a.P, min(L, a.T - c * L), a.P - p0, O, buf);
+      }
+      times_cols(X, closing, 1.f);
+      eC = floor_exp(warp_exp(X), eS, ek);
+      frags_of<2>(fc, X, eC);
+      top = gamma[L - 1];
+    }
+    __syncthreads();
+    if (more) issue_rest(c + 1, nx.z);
+    cp_commit();
+    if (active) {
+      times(S, top * pow2(-(eC + ek)));
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int nb = 0; nb < NT / 16; ++nb) {
+          uint32_t bb[SI][4];
+#pragma unroll
+          for (int s2 = 0; s2 < SI; ++s2) b_kn(bb[s2], kt + s2 * Op::plane + 16 * kb * Op::ld + 16 * nb, Op::ld);
+          mma_split<2, SI>(S[2 * nb], S[2 * nb + 1], fc[kb], bb);
+        }
+      times(S, pow2(eC + ek));
+    }
+    ex = nx;
+  }
+  cp_wait<0>();
+  if (active && a.final_state) write_state<NT>(a.final_state, SLX_F32, (size_t)bh * a.P * a.N, S, p0, a.P, a.N);
+}
+
+template <int NT, int SI, int SC, typename TI>
+__global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
+  using Op = Operand<TI, SI, NT>;
+  using V = Raw<TI>;
+  extern __shared__ __align__(128) char smem[];
+  __half *ks = reinterpret_cast<__half *>(smem);  // two buffers
+  __half *qs = ks + 2 * SI * Op::plane;
+  __half *Ts = qs + SI * Op::plane;  // T hi, T lo, P hi, P lo, the record's vectors
+  __half *Ps = Ts + 2 * kTri;
+  float *hd = reinterpret_cast<float *>(Ps + 2 * kTri);
+  const float *gamma = hd, *closing = hd + L, *beta = hd + 2 * L;
+  TI *os = reinterpret_cast<TI *>(reinterpret_cast<char *>(hd) + kHeadBytes);
+
+  const int warp = threadIdx.x >> 5;
+  __half *buf = reinterpret_cast<__half *>(reinterpret_cast<char *>(os) + V::bytes) + warp * warp_buf<NT>();
+  const int bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads, kh = h / (a.heads / a.key_heads);
+  const int first = blockIdx.x * pw * 16, p0 = first + warp * 16;
+  const bool active = warp < pw && p0 < a.P16;
+  const Record *rec = a.rec + (size_t)bh * a.NC;
+  const int PB = a.P16 / 16;
+
+  auto issue_k = [&](int c, int ek) {
+    Op::issue(ks + (c & 1) * SI * Op::plane, head_base<TI>(a.k, b, kh, c * L), a.k.st, min(L, a.T - c * L), a.N, a.k.vec, ek);
+  };
+  auto issue_rest = [&](int c) {
+    copy_bytes(Ts, rec[c].T, 4 * kTri * 2);
+    copy_bytes(hd, rec[c].gamma, kHeadBytes);
+    V::issue(os, head_base<TI>(a.dO, b, h, c * L) + first, a.dO.st, min(L, a.T - c * L), a.P - first, pw * 16, a.dO.vec);
+  };
+
+  float R[NT / 8][4];
+  if (active && a.d_final) load_state<NT>(R, a.d_final, a.d_final_dtype, (size_t)bh * a.P * a.N, p0, a.P, a.N);
+  else zero(R);
+  int4 ex = exps_of(rec + a.NC - 1);
+  issue_k(a.NC - 1, ex.w);
+  issue_rest(a.NC - 1);
+  cp_commit();
+  for (int c = a.NC - 1; c >= 0; --c) {
+    const int4 nx = c > 0 ? exps_of(rec + c - 1) : ex;
+    const int eT = ex.x, eQ = ex.y, eq = ex.z, ek = ex.w;
+    const __half *kt = ks + (c & 1) * SI * Op::plane;
+    const int rows = min(L, a.T - c * L);
+    cp_wait<0>();
+    Op::finish(ks + (c & 1) * SI * Op::plane, a.k.vec, ek);
+    __syncthreads();
+    Op::issue(qs, head_base<TI>(a.q, b, kh, c * L), a.q.st, rows, a.N, a.q.vec, eq);
+    cp_commit();
+    if (c > 0) issue_k(c - 1, nx.w);
+    cp_commit();
+    Frag<2> f1[4], f2[4];  // scale gamma dO, -gamma dX
+    int e1 = 0, e2 = 0;
+    float top = 0.f;
+    if (active) {
+      const size_t at = (size_t)bh * a.NC + c;
+      const int eR = warp_exp(R);
+      store_state<SC, NT>(a.ds + (at * SC * a.P16 + p0) * NT, (int64_t)a.P16 * NT, R, eR, buf);
+      float W[8][4], X[8][4], dO[8][4];
+      zero(X);
+      {
+        const float s = pow2(-eR);
+#pragma unroll
+        for (int kb = 0; kb < NT / 16; ++kb) {
+          Frag<2> f;
+          frag_of<2>(f, R[2 * kb], R[2 * kb + 1], s);
+#pragma unroll
+          for (int tb = 0; tb < 4; ++tb) {
+            uint32_t bb[SI][4];
+#pragma unroll
+            for (int s2 = 0; s2 < SI; ++s2) b_nk(bb[s2], kt + s2 * Op::plane + 16 * tb * Op::ld + 16 * kb, Op::ld);
+            mma_split<2, SI>(X[2 * tb], X[2 * tb + 1], f, bb);
+          }
+        }
+      }
+      load_cols<TI>(dO, os, warp * 16);
+      const int eo = std::is_same<TI, __half>::value ? 0 : warp_exp(dO);
+      zero(W);
+      {
+        Frag<SI> fo[4];
+        frags_of<SI>(fo, dO, eo);
+#pragma unroll
+        for (int sb = 0; sb < 4; ++sb)
+#pragma unroll
+          for (int kb = sb; kb < 4; ++kb) {
+            uint32_t bb[2][4];
+            b_kn(bb[0], Ps + tri_base(kb) + 16 * sb, tri_ld(kb));
+            b_kn(bb[1], Ps + kTri + tri_base(kb) + 16 * sb, tri_ld(kb));
+            mma_split<SI, 2>(W[2 * sb], W[2 * sb + 1], fo[kb], bb);
+          }
+      }
+      // beta dD
+      times_cols(X, closing, pow2(eR + ek));
+      times(W, a.scale * pow2(eo + eQ));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) X[j][i] += W[j][i];
+      times_cols(X, beta, 1.f);
+      {
+        const int eX = warp_exp(X);
+        Frag<2> fx[4];
+        frags_of<2>(fx, X, eX);
+        zero(W);
+#pragma unroll
+        for (int sb = 0; sb < 4; ++sb)
+#pragma unroll
+          for (int kb = sb; kb < 4; ++kb) {
+            uint32_t bb[2][4];
+            b_kn(bb[0], Ts + tri_base(kb) + 16 * sb, tri_ld(kb));
+            b_kn(bb[1], Ts + kTri + tri_base(kb) + 16 * sb, tri_ld(kb));
+            mma_split<2, 2>(W[2 * sb], W[2 * sb + 1], fx[kb], bb);
+          }
+        times(W, pow2(eX + eT));  // dX
+      }
+      store_rows<TI>(static_cast<TI *>(a.dv) + ((size_t)bh * a.T + c * L) * a.P + p0, a.P, rows, a.P - p0, W, buf);
+      const int exx = store_planes<SC>(a.dx + at * SC * L * a.P16 + p0, a.P16, (int64_t)L * a.P16, W, buf);
+      if ((threadIdx.x & 31) == 0) {
+        a.eds[at * PB + p0 / 16] = eR;
+        a.edx[at * PB + p0 / 16] = exx;
+        a.edo[at * PB + p0 / 16] = eo;
+      }
+      times_cols(dO, gamma, a.scale);
+      e1 = floor_exp(warp_exp(dO), eR, eq);
+      frags_of<2>(f1, dO, e1);
+      times_cols(W, gamma, -1.f);
+      // (64 products of values below 2^15 join R between the two)
+      e2 = floor_exp(warp_exp(W), max(eR, e1 + eq + 21) + 1, ek);
+      frags_of<2>(f2, W, e2);
+      top = gamma[L - 1];
+    }
+    cp_wait<1>();
+    Op::finish(qs, a.q.vec, eq);
+    __syncthreads();
+    if (c > 0) issue_rest(c - 1);
+    cp_commit();
+    if (active) {
+      times(R, top * pow2(-(e1 + eq)));
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int nb = 0; nb < NT / 16; ++nb) {
+          uint32_t bb[SI][4];
+#pragma unroll
+          for (int s2 = 0; s2 < SI; ++s2) b_kn(bb[s2], qs + s2 * Op::plane + 16 * kb * Op::ld + 16 * nb, Op::ld);
+          mma_split<2, SI>(R[2 * nb], R[2 * nb + 1], f1[kb], bb);
+        }
+      times(R, pow2(e1 + eq - (e2 + ek)));
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int nb = 0; nb < NT / 16; ++nb) {
+          uint32_t bb[SI][4];
+#pragma unroll
+          for (int s2 = 0; s2 < SI; ++s2) b_kn(bb[s2], kt + s2 * Op::plane + 16 * kb * Op::ld + 16 * nb, Op::ld);
+          mma_split<2, SI>(R[2 * nb], R[2 * nb + 1], f2[kb], bb);
+        }
+      times(R, pow2(e2 + ek));
+    }
+    ex = nx;
+  }
+  cp_wait<0>();
+  if (active && a.d_init) write_state<NT>(a.d_init, a.d_init_dtype, (size_t)bh * a.P * a.N, R, p0, a.P, a.N);
+}
+
+}  // namespace delta
+}  // namespace slx

@@ -891,6 +891,238 @@ OptTensor gate_skip(const Tensor &y_in, const Tensor &u_in, const Tensor &gate_i
   return out;
 }
 
+// ------------------------------------------------------------------------------------------------------------
+// gated delta rule
+// ------------------------------------------------------------------------------------------------------------
+struct DeltaDims {
+  int64_t b, h, hk, T, P, N;
+  at::Device dev = at::kCUDA;
+  at::ScalarType act;
+  slx_gated_delta_shape s;
+};
+// Strides over batch, head and (with tokens) token of a tensor whose last axis is dense; nothing where they are no such.
+template <int n>
+bool outer_strides(const Tensor &t, bool dense, int64_t (&out)[n]) {
+  if (dense && t.size(-1) != 1 && t.stride(-1) != 1) return false;
+  for (int i = 0; i < n; ++i) out[i] = i < t.dim() - (dense ? 1 : 0) ? t.stride(i) : 0;
+  return true;
+}
+// tokens: q, k (b, Hk, T, N), v (b, H, T, P), g, beta (b, H, T); else the same without T
+std::optional<DeltaDims> delta_dims(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta,
+                                    double scale, bool tokens) {
+  const int64_t n = tokens ? 4 : 3;
+  if (!v.is_cuda() || v.dim() != n || q.dim() != n || g.dim() != n - 1) return std::nullopt;
+  DeltaDims d;
+  d.dev = v.device();
+  d.act = v.scalar_type();
+  d.b = v.size(0);
+  d.h = v.size(1);
+  d.hk = q.size(1);
+  d.T = tokens ? v.size(2) : 1;
+  d.P = v.size(-1);
+  d.N = q.size(-1);
+  if (code_of(d.act) < 0 || code_of(g.scalar_type()) < 0 || code_of(beta.scalar_type()) < 0) return std::nullopt;
+  if (d.b == 0 || d.h == 0 || d.hk == 0 || d.T == 0 || d.P == 0 || d.N == 0 || d.h % d.hk != 0) return std::nullopt;
+  if (d.b > INT32_MAX || d.h > INT32_MAX || d.T > INT32_MAX || d.P > 256 || d.N > 128) return std::nullopt;
+  std::vector<int64_t> ksz{d.b, d.hk}, gsz{d.b, d.h};
+  if (tokens) {
+    ksz.push_back(d.T);
+    gsz.push_back(d.T);
+  }
+  ksz.push_back(d.N);
+  std::vector<int64_t> vsz = gsz;
+  vsz.push_back(d.P);
+  if (!shaped(q, ksz) || !shaped(k, ksz) || !shaped(v, vsz) || !shaped(g, gsz) || !shaped(beta, gsz)) return std::nullopt;
+  for (const Tensor *t : {&q, &k})
+    if (t->scalar_type() != d.act) return std::nullopt;
+  for (const Tensor *t : {&q, &k, &g, &beta})
+    if (t->device() != d.dev) return std::nullopt;
+  d.s = slx_gated_delta_shape{};
+  d.s.batch = (int32_t)d.b;
+  d.s.heads = (int32_t)d.h;
+  d.s.key_heads = (int32_t)d.hk;
+  d.s.T = (int32_t)d.T;
+  d.s.P = (int32_t)d.P;
+  d.s.N = (int32_t)d.N;
+  d.s.dtype = code_of(d.act);
+  d.s.g_dtype = code_of(g.scalar_type());
+  d.s.beta_dtype = code_of(beta.scalar_type());
+  d.s.scale = (float)scale;
+  if (!outer_strides(q, true, d.s.q_stride) || !outer_strides(k, true, d.s.k_stride) ||
+      !outer_strides(v, true, d.s.v_stride) || !outer_strides(g, false, d.s.g_stride) ||
+      !outer_strides(beta, false, d.s.beta_stride))
+    return std::nullopt;
+  return d;
+}
+Tensor delta_bytes(size_t n, const at::Device &dev) { return empty({(int64_t)n}, at::kByte, dev); }
+
+struct DeltaForward {
+  Tensor o, final_state, residual;
+};
+DeltaForward delta_forward(const DeltaDims &d, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
+                           const Tensor &beta, const OptTensor &init, bool want_o, bool want_state, bool want_residual) {
+  DeltaForward r;
+  if (want_o) r.o = empty({d.b, d.h, d.T, d.P}, d.act, d.dev);
+  if (want_state) r.final_state = empty({d.b, d.h, d.P, d.N}, at::kFloat, d.dev);
+  if (want_residual) r.residual = delta_bytes(slx_gated_delta_residual_bytes(&d.s), d.dev);
+  const size_t nbytes = slx_gated_delta_fwd_workspace_bytes(&d.s);
+  Tensor ws = delta_bytes(nbytes, d.dev);
+  c10::cuda::CUDAGuard guard(d.dev);
+  check(slx_gated_delta_fwd(&d.s, ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), cptr(init),
+                            init ? code_of(init->scalar_type()) : SLX_F32, ptr(r.o), fptr(r.final_state), ptr(r.residual),
+                            ptr(ws), nbytes, stream_of(d.dev)),
+        "gated delta rule forward");
+  return r;
+}
+
+struct DeltaBackward : public Node {
+  double scale = 1;
+  bool recompute = false;
+  std::optional<at::ScalarType> init_type;
+  SavedVariable q_, k_, v_, g_, beta_, init_, residual_;
+  std::vector<int64_t> v_sizes;
+  std::string name() const override { return "GatedDeltaRuleBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable *s : {&q_, &k_, &v_, &g_, &beta_, &init_, &residual_}) s->reset_data();
+  }
+  variable_list apply(variable_list &&grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(6);
+    const Tensor do_in = grads[0], df_in = grads.size() > 1 ? grads[1] : Tensor();
+    if (!do_in.defined() && !df_in.defined()) return out;
+    // (a saved-tensor hook may return other strides, also of the last axis)
+    auto dense = [](Tensor t) { return t.size(-1) != 1 && t.stride(-1) != 1 ? t.contiguous() : t; };
+    const Tensor q = dense(saved(q_)), k = dense(saved(k_)), g = saved(g_), beta = saved(beta_);
+    Tensor v, residual, init;
+    if (recompute) v = dense(saved(v_));
+    else residual = saved(residual_);
+    // (without recomputing only the sizes of v are needed, and of its strides none)
+    const std::optional<DeltaDims> dims = delta_dims(q, k, recompute ? v : at::empty({v_sizes.back()}, q.options()).expand(v_sizes),
+                                                     g, beta, scale, true);
+    TORCH_CHECK(dims, "gated delta rule backward: saved tensors have changed");
+    const DeltaDims &d = *dims;
+    if (recompute) {
+      if (init_type) init = as_read(saved(init_), *init_type);
+      residual = delta_forward(d, q, k, v, g, beta, init.defined() ? OptTensor(init) : std::nullopt, false, false, true).residual;
+    }
+    const Tensor dO = do_in.defined() ? as_read(do_in, d.act) : at::zeros(v_sizes, q.options());
+    Tensor d_final;
+    if (df_in.defined())
+      d_final = as_read(df_in, code_of(df_in.scalar_type()) < 0 ? at::kFloat : df_in.scalar_type());
+    out[0] = empty(q.sizes(), d.act, d.dev);
+    out[1] = empty(k.sizes(), d.act, d.dev);
+    out[2] = empty(v_sizes, d.act, d.dev);
+    out[3] = empty(g.sizes(), g.scalar_type(), d.dev);
+    out[4] = empty(beta.sizes(), beta.scalar_type(), d.dev);
+    if (init_type) out[5] = empty({d.b, d.h, d.P, d.N}, *init_type, d.dev);
+    const size_t nbytes = slx_gated_delta_bwd_workspace_bytes(&d.s);
+    Tensor ws = delta_bytes(nbytes, d.dev);
+    c10::cuda::CUDAGuard guard(d.dev);
+    check(slx_gated_delta_bwd(&d.s, ptr(q), ptr(k), ptr(g), ptr(beta), ptr(residual), ptr(dO), ptr(d_final),
+                              d_final.defined() ? code_of(d_final.scalar_type()) : SLX_F32, ptr(out[0]), ptr(out[1]),
+                              ptr(out[2]), ptr(out[3]), ptr(out[4]), ptr(out[5]),
+                              init_type ? code_of(*init_type) : SLX_F32, ptr(ws), nbytes, stream_of(d.dev)),
+          "gated delta rule backward");
+    return out;
+  }
+};
+
+// -> [o] or [o, final_state (fp32)].  None: not the plain case.
+std::optional<std::vector<Tensor>> gated_delta_rule(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
+                                                    const Tensor &beta, double scale, const OptTensor &init, bool want_state,
+                                                    bool recompute) {
+  const std::optional<DeltaDims> dims = delta_dims(q, k, v, g, beta, scale, true);
+  if (!dims) return std::nullopt;
+  const DeltaDims &d = *dims;
+  const int64_t ssz[4] = {d.b, d.h, d.P, d.N};
+  if (d.b * d.h > 65535) return std::nullopt;
+  if (init && (!is(*init, d.dev) || !shaped(*init, ssz) || !init->is_contiguous() || code_of(init->scalar_type()) < 0))
+    return std::nullopt;
+  refuse_tangents(q, k, v, g, beta, or_undefined(init));
+  const bool grad = torch::autograd::compute_requires_grad(q, k, v, g, beta, or_undefined(init));
+  DeltaForward r = delta_forward(d, q, k, v, g, beta, init, true, want_state, grad && !recompute);
+  if (grad) {
+    auto node = make_node<DeltaBackward>(torch::autograd::collect_next_edges(q, k, v, g, beta, or_undefined(init)));
+    node->scale = scale;
+    node->recompute = recompute;
+    node->q_ = keep(q);
+    node->k_ = keep(k);
+    node->g_ = keep(g);
+    node->beta_ = keep(beta);
+    node->v_sizes = v.sizes().vec();
+    if (init) node->init_type = init->scalar_type();
+    // Kept for the backward: the states before every chunk and the prediction errors, or (recompute) v and the initial
+    // state, from which one more pass forms them again.
+    if (recompute) {
+      node->v_ = keep(v);
+      if (init) node->init_ = keep_value(*init);
+    } else {
+      node->residual_ = keep(r.residual);
+    }
+    torch::autograd::set_history(r.o, node);
+    if (want_state) torch::autograd::set_history(r.final_state, node);
+  }
+  if (!want_state) return std::vector<Tensor>{r.o};
+  return std::vector<Tensor>{r.o, r.final_state};
+}
+
+// one token -> (o, state (fp32))
+std::optional<std::tuple<Tensor, Tensor>> gated_delta_step(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
+                                                           const Tensor &beta, double scale, const OptTensor &init,
+                                                           const OptTensor &state_out) {
+  const std::optional<DeltaDims> dims = delta_dims(q, k, v, g, beta, scale, false);
+  if (!dims) return std::nullopt;
+  const DeltaDims &d = *dims;
+  const int64_t ssz[4] = {d.b, d.h, d.P, d.N};
+  for (const OptTensor *t : {&init, &state_out})
+    if (*t && (!is(**t, d.dev) || !shaped(**t, ssz) || !(*t)->is_contiguous() || (*t)->scalar_type() != at::kFloat))
+      return std::nullopt;
+  Tensor o = empty({d.b, d.h, d.P}, d.act, d.dev);
+  Tensor out = state_out ? *state_out : empty(ssz, at::kFloat, d.dev);
+  c10::cuda::CUDAGuard guard(d.dev);
+  check(slx_gated_delta_step(&d.s, ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), static_cast<const float *>(cptr(init)), ptr(o),
+                             fptr(out), stream_of(d.dev)),
+        "gated delta step");
+  return std::make_tuple(o, out);
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// tokens from logits
+// ------------------------------------------------------------------------------------------------------------
+// A setting is a tensor of one value per row, or the number beside it for all rows.
+std::optional<Tensor> sample(const Tensor &logits, const Tensor &u, const OptTensor &temperature, double temperature0,
+                             const OptTensor &top_k, int64_t top_k0, const OptTensor &top_p, double top_p0,
+                             const OptTensor &min_p, double min_p0) {
+  if (!logits.is_cuda() || logits.dim() != 2 || code_of(logits.scalar_type()) < 0) return std::nullopt;
+  const at::Device dev = logits.device();
+  const int64_t b = logits.size(0), V = logits.size(1);
+  if (b == 0 || V == 0 || b > INT32_MAX || V > 262144 || (V != 1 && logits.stride(1) != 1)) return std::nullopt;
+  auto vector = [&](const Tensor &t) { return t.device() == dev && t.dim() == 1 && t.size(0) == b && t.is_contiguous(); };
+  if (!vector(u) || (u.scalar_type() != at::kFloat && u.scalar_type() != at::kDouble)) return std::nullopt;
+  for (const OptTensor *t : {&temperature, &top_p, &min_p})
+    if (*t && (!vector(**t) || (*t)->scalar_type() != at::kFloat)) return std::nullopt;
+  if (top_k && (!vector(*top_k) || (top_k->scalar_type() != at::kInt && top_k->scalar_type() != at::kLong))) return std::nullopt;
+  Tensor out = empty({b}, at::kLong, dev);
+  slx_sample_shape s{};
+  s.rows = (int32_t)b;
+  s.vocab = (int32_t)V;
+  s.dtype = code_of(logits.scalar_type());
+  s.u_bytes = (int32_t)u.element_size();
+  s.top_k_bytes = top_k ? (int32_t)top_k->element_size() : 8;
+  s.temperature = (float)temperature0;
+  s.top_p = (float)top_p0;
+  s.min_p = (float)min_p0;
+  s.top_k = top_k0;
+  s.row_stride = b > 1 ? logits.stride(0) : 0;
+  c10::cuda::CUDAGuard guard(dev);
+  check(slx_sample(&s, ptr(logits), ptr(u), static_cast<const float *>(cptr(temperature)), cptr(top_k),
+                   static_cast<const float *>(cptr(top_p)), static_cast<const float *>(cptr(min_p)), out.data_ptr<int64_t>(),
+                   stream_of(dev)),
+        "sample");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -903,4 +1135,7 @@ PYBIND11_MODULE(_host, m) {
   m.def("cconv1d", torch::wrap_pybind_function_no_gil(&cconv1d));
   m.def("cconv1d_update", torch::wrap_pybind_function_no_gil(&cconv1d_update));
   m.def("gate_skip", torch::wrap_pybind_function_no_gil(&gate_skip));
+  m.def("gated_delta_rule", torch::wrap_pybind_function_no_gil(&gated_delta_rule));
+  m.def("gated_delta_step", torch::wrap_pybind_function_no_gil(&gated_delta_step));
+  m.def("sample", torch::wrap_pybind_function_no_gil(&sample));
 }
