@@ -514,7 +514,7 @@ int slx_gated_delta_step(const slx_gated_delta_shape *s, const void *q, const vo
 /* ---- tokens from logits ------------------------------------------------------------ */
 
 typedef struct {
-  int32_t rows, vocab;  /* vocab <= 262144 */
+  int32_t rows, vocab;  /* rows <= 65535, vocab <= 262144 */
   int32_t dtype;        /* slx_dtype of the logits */
   int32_t u_bytes;      /* 4: u is float, 8: double */
   int32_t top_k_bytes;  /* 4 or 8: size of an entry of top_k, where that is given */

@@ -1097,7 +1097,7 @@ std::optional<Tensor> sample(const Tensor &logits, const Tensor &u, const OptTen
   if (!logits.is_cuda() || logits.dim() != 2 || code_of(logits.scalar_type()) < 0) return std::nullopt;
   const at::Device dev = logits.device();
   const int64_t b = logits.size(0), V = logits.size(1);
-  if (b == 0 || V == 0 || b > INT32_MAX || V > 262144 || (V != 1 && logits.stride(1) != 1)) return std::nullopt;
+  if (b == 0 || V == 0 || b > 65535 || V > 262144 || (V != 1 && logits.stride(1) != 1)) return std::nullopt;
   auto vector = [&](const Tensor &t) { return t.device() == dev && t.dim() == 1 && t.size(0) == b && t.is_contiguous(); };
   if (!vector(u) || (u.scalar_type() != at::kFloat && u.scalar_type() != at::kDouble)) return std::nullopt;
   for (const OptTensor *t : {&temperature, &top_p, &min_p})

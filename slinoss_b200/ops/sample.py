@@ -33,7 +33,7 @@ def sample_b200(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k
     Each setting is a number, or a tensor ``(b,)`` with one value per row (values of tensors are not checked:
     ``temperature <= 0``, ``top_p <= 0`` and ``min_p > 1`` take the first largest logit, ``top_p >= 1`` keeps all).
     ``u`` is float32 or float64.  NaN logits count as ``-inf``; where several logits are ``+inf`` they share the mass; a
-    row without any logit above ``-inf`` gives ``-1``.  ``V <= 262144``; rows may have any stride."""
+    row without any logit above ``-inf`` gives ``-1``.  ``b <= 65535``, ``V <= 262144``; rows may have any stride."""
     out = None
     if logits.ndim == 2:
         numbers = [x for x in (temperature, top_p, min_p) if not isinstance(x, torch.Tensor)]
@@ -52,6 +52,8 @@ def sample_b200(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k
     b, V = map(int, logits.shape)
     if not 1 <= V <= 262144:
         raise ValueError(f"the vocabulary must have 1..262144 tokens. Got {V}.")
+    if b > 65535:
+        raise ValueError(f"the batch must be at most 65535 rows. Got {b}.")
     if tuple(u.shape) != (b,):
         raise ValueError(f"u must be ({b},). Got {tuple(u.shape)}.")
     if u.dtype not in (torch.float32, torch.float64):
