@@ -4,16 +4,16 @@
 // top_p of their mass; of these the ones with at least min_p of the largest mass.  The draw goes through what is left in the
 // order of the indices and takes the first token at which the running mass exceeds u times the whole.
 //
-// A row is read once: a cluster of up to eight CTAs holds it in shared memory, and everything after that runs
-// there.  What a pass costs is arithmetic, so the passes are kept cheap:
+// A row is read once: a cluster of up to eight CTAs holds it in shared memory, and everything after that runs there.
 //   * The border of a filter (k tokens, or a share of the mass) is narrowed down by a histogram over steps of 1/16 in the
-//     logarithm of the mass, counted in 32-bit integers (masses relative to their bin's edge, 15 bits: a CTA's
-//     2^17 tokens may all fall into one): one bin holds the
-//     border.  Its tokens, a few dozen to a few hundred, are gathered, sorted and walked one by one.  A bin with too many
-//     is divided again by the integer keys of its logits until it is small enough or holds a single value.
-//   * Masses that decide between tokens are exponentials in 64 bits, taken only for tokens that stay, as integers of 2^-44 of
-//     the largest: their sums do not depend on an order, and a draw is decided as exact sums would decide it but for about
-//     one in 10^7 (the whole mass that top_p refers to is summed in 32-bit exponentials).
+//     logarithm of the mass, counted in 32-bit integers (masses relative to their bin's edge, 15 bits: a CTA's 2^17 tokens may
+//     all fall into one): one bin holds the border.
+//   * Where no more than a few thousand tokens lie above the bin's lower edge, CTA 0 gathers, sorts and walks them, and the
+//     other CTAs are done.  Otherwise only the bin's own tokens are gathered for the border (a bin with too many is divided
+//     again by the integer keys of its logits), and the draw sums the tokens that stay where they are.
+//   * Masses that decide between tokens are exponentials in 64 bits, taken only for tokens that may stay, as integers of 2^-44
+//     of the largest: their sums do not depend on an order, and a draw is decided as exact sums would decide it but for about
+//     one in 10^7 (the whole mass that top_p alone refers to is summed in 32-bit exponentials).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -42,31 +42,31 @@ typedef unsigned long long u64;
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kBins = 512;      // of a histogram; one per thread
 constexpr int kTail = 400;      // the bin of all masses below 2^-25 of the largest
-constexpr int kList = 2048;     // tokens that are sorted one by one
+constexpr int kList = 4096;     // tokens that are sorted and walked one by one
+constexpr int kFew = 256;       // tokens that are ranked by comparing each with each
 constexpr int kMaxVecs = 17;     // of a thread: eight CTAs hold 262144 fp32 logits that begin inside a vector
 constexpr int kMaxGroups = kMaxVecs * kSampleWarps;
 constexpr int kMaxCluster = 8;
 static_assert(kBins == kSampleThreads, "threads scan the bins one each");
 
 struct alignas(16) SampleShared {  // (the row's vectors follow it)
-  u64 list[kList];
+  u64 list[kList];              // tokens: key and inverted index, so that descending order is the ranking
   u64 group[kMaxGroups];
   double table[64];             // 2^(i/64)
-  double scan[kSampleWarps];
+  double scan[kSampleWarps], scan2[kSampleWarps];
   u64 sums[kSampleWarps];
   unsigned hist[kBins];
   // written by every CTA of the cluster into each, two sets in turn
   float gather_f[2][kMaxCluster];
   u64 gather_u[2][kMaxCluster];
-  double pick_before;
-  int pick_bin;
+  double pick_before, pick_tokens;
+  u64 start, border;
+  int pick_bin, found;
   // of CTA 0
   int count;
   unsigned lowest, highest;
   float border_x;
   int border_i;
-  u64 border_mass;
-  // of every CTA
   unsigned maxima[kSampleWarps];
 };
 
@@ -104,6 +104,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
   SampleShared &sm0 = *cluster.map_shared_rank(&sm, 0);
   const int row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const TI *x = static_cast<const TI *>(a.logits) + row * a.stride;
+  const float temperature = a.temperature ? a.temperature[row] : a.temperature0;
+  const float p = a.top_p ? a.top_p[row] : a.top_p0, minp = a.min_p ? a.min_p[row] : a.min_p0;
+  int64_t k = a.top_k0;
+  if (a.top_k) k = a.top_k_bytes == 8 ? static_cast<const int64_t *>(a.top_k)[row] : static_cast<const int *>(a.top_k)[row];
+  if (k <= 0 || k > a.V) k = a.V;
+  double u = a.u_bytes == 4 ? (double)static_cast<const float *>(a.u)[row] : static_cast<const double *>(a.u)[row];
+  u = fmin(fmax(u, 0.0), 1.0);
   // index of a thread's value (j, e): vectors lie on 16-byte boundaries, the first of a row may begin before it
   const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(TI));
   auto first_of = [&](int j) { return ((rank * NV + j) * kSampleThreads + tid) * VEC - shift; };
@@ -138,16 +145,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
   auto spread_u = [&](u64 v) {
     if (tid < C) cluster.map_shared_rank(&sm, tid)->gather_u[turn][rank] = v;
   };
-#define EACH(body_)                                                     \
+#define EACH_VECTOR(body_)                                              \
   _Pragma("unroll 1") for (int j = 0; j < NV; ++j) {                    \
-    const int i0_ = first_of(j);                                        \
-    const Vec<TI> vec_ = row_data[j * kSampleThreads];                  \
+    const int i0 = first_of(j);                                         \
+    const Vec<TI> vec = row_data[j * kSampleThreads];                   \
+    body_                                                               \
+  }
+#define EACH(body_)                                                     \
+  EACH_VECTOR({                                                         \
     _Pragma("unroll") for (int e = 0; e < VEC; ++e) {                   \
-      const float v = vec_.at(e);                                       \
-      const int i = i0_ + e;                                            \
+      const float v = vec.at(e);                                        \
+      const int i = i0 + e;                                             \
       body_                                                             \
     }                                                                   \
-  }
+  })
 
   // ---- the largest logit
   {
@@ -155,110 +166,134 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     if (lane == 0) sm.maxima[warp] = m;
     __syncthreads();
     top = value_of(__reduce_max_sync(~0u, sm.maxima[lane & (kSampleWarps - 1)]));
-    spread_f(top);
-    cluster.sync();
-    for (int c = 0; c < C; ++c) top = fmaxf(top, sm.gather_f[turn][c]);
-    turn ^= 1;
+    if (C > 1) {
+      spread_f(top);
+      cluster.sync();
+      for (int c = 0; c < C; ++c) top = fmaxf(top, sm.gather_f[turn][c]);
+      turn ^= 1;
+    }
   }
+  // (no CTA leaves while another may still write to it)
+  auto leave = [&]() {
+    if (C > 1) cluster.sync();
+  };
   if (top == -INFINITY) {  // nothing can be drawn
     if (rank == 0 && tid == 0) a.out[row] = -1;
-    cluster.sync();  // (no CTA leaves while another may still write to it)
+    leave();
     return;
   }
-  const float temperature = a.temperature ? a.temperature[row] : a.temperature0;
-  const float p = a.top_p ? a.top_p[row] : a.top_p0, minp = a.min_p ? a.min_p[row] : a.min_p0;
-  int64_t k = a.top_k0;
-  if (a.top_k) k = a.top_k_bytes == 8 ? static_cast<const int64_t *>(a.top_k)[row] : static_cast<const int *>(a.top_k)[row];
-  if (k <= 0 || k > a.V) k = a.V;
+  // the draw takes the first token with running > u z: of integers, running > its floor; below z, so that there is one
+  auto target_in = [&](u64 z) { return min((u64)(u * (double)z), z - 1); };
 
-  // Sums over groups of 32 threads' vectors in the order of the indices, sm.group[j * warps + warp]: the first index at
-  // which the running sum of `weight` exceeds `target` (which has to be below the whole), written by the warp that finds it.
-  auto group_scan = [&](u64 &before, u64 &whole) {  // -> what lies before this warp's groups j = 0, in `before`
-    // every CTA's total
+  // sum over the CTA
+  auto cta_sum = [&](u64 v) {
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
     __syncthreads();
-    u64 mine = 0;
-    for (int g = tid; g < NV * kSampleWarps; g += kSampleThreads) mine += sm.group[g];
-    for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(~0u, mine, d);
-    if (lane == 0) sm.sums[warp] = mine;
+    if (lane == 0) sm.sums[warp] = v;
     __syncthreads();
-    u64 total = 0;
-    for (int w = 0; w < kSampleWarps; ++w) total += sm.sums[w];
-    spread_u(total);
-    cluster.sync();
-    before = 0;
+    u64 s = 0;
+#pragma unroll
+    for (int w = 0; w < kSampleWarps; ++w) s += sm.sums[w];
+    return s;
+  };
+  // sum of the CTA's threads before this one, and of all
+  auto cta_scan = [&](u64 v, u64 &whole) {
+    u64 run = v;
+    for (int d = 1; d < 32; d <<= 1) {
+      const u64 o = __shfl_up_sync(~0u, run, d);
+      if (lane >= d) run += o;
+    }
+    __syncthreads();
+    if (lane == 31) sm.sums[warp] = run;
+    __syncthreads();
+    u64 before = 0;
     whole = 0;
-    for (int c = 0; c < C; ++c) {
-      const u64 t = sm.gather_u[turn][c];
-      if (c < rank) before += t;
-      whole += t;
-    }
-    turn ^= 1;
-  };
-  // (vectors of one j lie side by side over the CTA's threads: groups follow one another in the order of the indices)
-  auto locate = [&](u64 before, u64 target, auto weight, auto found) {
-    // groups before this warp's, j by j
-    for (int j = 0; j < NV; ++j) {
-      u64 start = before, here = 0;
-      for (int w = 0; w < kSampleWarps; ++w) {
-        const u64 s = sm.group[j * kSampleWarps + w];
-        if (w < warp) start += s;
-        if (w == warp) here = s;
-        before += s;
-      }
-      if (start <= target && target < start + here) {
-        u64 lanes[VEC], sum = 0;
-        const Vec<TI> vec = row_data[j * kSampleThreads];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum += lanes[e] = weight(vec.at(e), first_of(j) + e);
-        u64 run = sum;
-        for (int d = 1; d < 32; d <<= 1) {
-          const u64 o = __shfl_up_sync(~0u, run, d);
-          if (lane >= d) run += o;
-        }
-        run += start;
-        u64 at = run - sum;
-        if (at <= target && target < run) {
-          int here_e = VEC - 1;
-#pragma unroll
-          for (int e = 0; e < VEC - 1; ++e) {
-            at += lanes[e];
-            if (target < at && here_e == VEC - 1) here_e = e;
-          }
-          found(first_of(j) + here_e);
-        }
-      }
+    for (int w = 0; w < kSampleWarps; ++w) {
+      if (w < warp) before += sm.sums[w];
+      whole += sm.sums[w];
     }
+    return before + run - v;
   };
-  auto fill_groups = [&](auto weight) {
-#pragma unroll 1
-    for (int j = 0; j < NV; ++j) {
+
+  // Sums over a warp's vectors j in the order of the indices: sm.group[j * warps + warp].
+  auto fill_groups = [&](auto weights) {  // weights(vec, i0, w): of a vector's values
+    EACH_VECTOR({
+      u64 w[VEC];
+      weights(vec, i0, w);
       u64 s = 0;
-      const Vec<TI> vec = row_data[j * kSampleThreads];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s += weight(vec.at(e), first_of(j) + e);
+      for (int e = 0; e < VEC; ++e) s += w[e];
       for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
       if (lane == 0) sm.group[j * kSampleWarps + warp] = s;
+    })
+  };
+  // The first index at which the running sum of the weights (whose groups are filled) exceeds target(whole).
+  auto locate = [&](auto target_of, auto weights, auto found) {
+    __syncthreads();
+    const u64 mine = tid < NV * kSampleWarps ? sm.group[tid] : 0;
+    u64 total;
+    u64 start = cta_scan(mine, total);
+    u64 whole = total;
+    if (C > 1) {
+      spread_u(total);
+      cluster.sync();
+      whole = 0;
+      for (int c = 0; c < C; ++c) {
+        const u64 t = sm.gather_u[turn][c];
+        if (c < rank) start += t;
+        whole += t;
+      }
+      turn ^= 1;
+    }
+    const u64 target = target_of(whole);
+    if (tid == 0) sm.found = -1;
+    __syncthreads();
+    if (start <= target && target < start + mine) {
+      sm.found = tid;
+      sm.start = start;
+    }
+    __syncthreads();
+    const int g = sm.found;
+    if (g < 0 || g % kSampleWarps != warp) return;
+    const int j = g / kSampleWarps, i0 = first_of(j);
+    u64 w[VEC], sum = 0;
+    weights(row_data[j * kSampleThreads], i0, w);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum += w[e];
+    u64 run = sum;
+    for (int d = 1; d < 32; d <<= 1) {
+      const u64 o = __shfl_up_sync(~0u, run, d);
+      if (lane >= d) run += o;
+    }
+    u64 at = sm.start + run - sum;
+    if (at <= target && target < at + sum) {
+      int here = VEC - 1;
+#pragma unroll
+      for (int e = VEC - 2; e >= 0; --e) {  // (from behind: the first that exceeds stays)
+        sum -= w[e + 1];
+        if (target < at + sum) here = e;
+      }
+      found(i0 + here);
     }
   };
 
   if (!(temperature > 0.f) || k == 1 || !(p > 0.f) || !(minp <= 1.f)) {  // the first largest logit
-    auto is_top = [&](float v, int) -> u64 { return v == top; };
+    auto is_top = [&](const Vec<TI> &vec, int, u64 *w) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] = vec.at(e) == top;
+    };
     fill_groups(is_top);
-    u64 before, whole;
-    group_scan(before, whole);
-    locate(before, 0, is_top, [&](int i) { a.out[row] = i; });
-    cluster.sync();
+    locate([](u64) { return (u64)0; }, is_top, [&](int i) { a.out[row] = i; });
+    leave();
     return;
   }
   const bool infinite = top == INFINITY;  // the largest share the mass
   const double per_unit = 1.0 / (double)temperature;
-  // exp of a difference below zero by table: 2^(i/64) and the series of e^r, |r| <= ln 2 / 128 (r^6 / 720 < 2^-54); as an
-  // integer of 2^-44, zero from exp(-31) on
+  // exp of a difference below zero by table (Tang 1989): 2^(i/64) and the series of e^r, |r| <= ln 2 / 128 (r^6 / 720 <
+  // 2^-54); as an integer of 2^-44, zero from exp(-31) on.  Without branches: the chains of neighbours overlap.
   auto mass_of = [&](float v) -> u64 {
-    if (v == top) return 1ull << 44;
-    if (infinite) return 0;
-    const double y = ((double)v - (double)top) * per_unit;
-    if (!(y > -31.0)) return 0;
+    const double y = fmax(((double)v - (double)top) * per_unit, -40.0);  // (also for NaN, from two infinities)
     constexpr double kLn2 = 0.693147180559945309417232121458;
     const double t = fma(y, 64.0 / kLn2, 6755399441055744.0);  // 1.5 * 2^52: the rounded integer in the low bits
     const int n = __double2loint(t);
@@ -267,264 +302,481 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     const double b = sm.table[n & 63];
     const double f = e * __hiloint2double(__double2hiint(b) + ((n >> 6) << 20), __double2loint(b));
     const double q = fma(f, 17592186044416.0, 4503599627370496.0);  // 2^44 and 2^52
-    return ((u64)(unsigned)(__double2hiint(q) & 0xfffff) << 32) | (unsigned)__double2loint(q);
+    const u64 m = ((u64)(unsigned)(__double2hiint(q) & 0xfffff) << 32) | (unsigned)__double2loint(q);
+    return v == top ? 1ull << 44 : y > -31.0 ? m : 0;
   };
-  const float steps = (float)(16.0 * 1.4426950408889634 / (double)temperature);
-  auto step_of = [&](float v) { return v == top ? 0.f : infinite ? INFINITY : (top - v) * steps; };  // (rounding is monotone)
-  auto bin_of = [&](float t) { return t < (float)kTail ? (int)t : kTail; };
+  const double one = 17592186044416.0;
+  const u64 least = minp > 0.f ? (u64)ceil((double)minp * one) : 0;  // of a mass that min_p keeps
 
+  // ---- no border to find: the draw over everything, or over what min_p keeps
   // What stays: logits above border_x, and those at it up to index border_i.
   float border_x = -INFINITY;
   int border_i = 0x7fffffff;
-  auto stays = [&](float v, int i) { return v > border_x || (v == border_x && i <= border_i); };
+  auto stays = [&](float v, int i) { return v > border_x || (v == border_x && i <= border_i && v > -INFINITY); };
+  auto kept = [&](const Vec<TI> &vec, int i0, u64 *w) {
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) any |= stays(vec.at(e), i0 + e);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) w[e] = 0;
+    if (__any_sync(~0u, any)) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const u64 m = mass_of(vec.at(e));
+        w[e] = stays(vec.at(e), i0 + e) && m >= least ? m : 0;
+      }
+    }
+  };
+  const bool by_rank = k < a.V, by_mass = p < 1.f;
 
-  // ---- a border: the first token, from the top, with which the weights of the tokens that stay reach the target
-  // masses: weights are masses and the target p of their whole; else numbers of tokens and the target k.
-  // Leaves the border, and with masses the sums of what stays in the groups (those with at least min_p of the largest mass).
-  bool summed = false;
-  auto weight15 = [&](float part) { return (unsigned)__float2int_rn(exp2f(part * (-1.f / 16)) * 32768.f); };
-  const u64 least = minp > 0.f ? (u64)ceil((double)minp * 17592186044416.0) : 0;
-  auto narrow = [&](bool masses) {
-    float tail = 0.f;
-    EACH({
-      if (stays(v, i)) {
-        const float t = step_of(v);
-        const int b = bin_of(t);
-        if (!masses) atomicAdd(&sm.hist[b], 1u);
-        else if (b < kTail) atomicAdd(&sm.hist[b], weight15(t - (float)b));
-        else tail += exp2f(t * (-1.f / 16));
-      }
-    })
-    // picks the bin: every CTA the same from everybody's histograms; unit: of a bin's weights
-    double target = (double)k, above = 0.0, whole = 0.0;
-    auto pick = [&](auto unit, double rest, double base) {
-      cluster.sync();
-      double w = 0.0;
-      for (int c = 0; c < C; ++c) w += (double)cluster.map_shared_rank(&sm, c)->hist[tid];
-      w *= unit(tid);
-      double run = w;
-      for (int d = 1; d < 32; d <<= 1) {
-        const double o = __shfl_up_sync(~0u, run, d);
-        if (lane >= d) run += o;
-      }
-      if (lane == 31) sm.scan[warp] = run;
+  const float steps = (float)(16.0 * 1.4426950408889634 * per_unit);
+  auto step_of = [&](float v) { return v == top ? 0.f : infinite ? INFINITY : (top - v) * steps; };  // (rounding is monotone)
+  auto bin_of = [&](float t) { return t < (float)kTail ? (int)t : kTail; };
+
+  // Of the n entries of CTA 0's list, the one with which the weights (masses, or one each), from the largest entry down,
+  // reach `need`; the smallest where they do not.  In sm.border.
+  auto border_of = [&](int n, double need, bool masses) {
+    u64 *const w = sm.list + kList - kFew;
+    if (n <= kFew) {  // each looks at the others
+      if (tid < n) w[tid] = masses ? mass_of(value_of((unsigned)(sm.list[tid] >> 32))) : 1;
+      if (tid == 0) sm.border = 0;
       __syncthreads();
-      double start = base, all = base;
-      for (int i = 0; i < kSampleWarps; ++i) {
-        if (i < warp) start += sm.scan[i];
-        all += sm.scan[i];
-      }
-      whole = all + rest;
-      if (masses && base == 0.0 && rest >= 0.0) target = (double)p * whole;
-      const bool reached = start + run >= target;
-      const unsigned votes = __ballot_sync(~0u, reached);
-      if (tid == 0) sm.pick_bin = kBins;
-      __syncthreads();
-      if (reached && lane == __ffs(votes) - 1) atomicMin(&sm.pick_bin, tid);
-      __syncthreads();
-      const int b = sm.pick_bin;
-      if (b == tid) sm.pick_before = start + run - w;
-      if (b == kBins && tid == 0) sm.pick_before = all;
-      cluster.sync();  // (everybody has read the histograms)
-      above = sm.pick_before;
-      sm.hist[tid] = 0;
-      __syncthreads();
-      return b;
-    };
-    if (masses) {
-      for (int d = 16; d > 0; d >>= 1) tail += __shfl_xor_sync(~0u, tail, d);
-      if (lane == 0) sm.scan[warp] = tail;
-      __syncthreads();
-      tail = 0.f;
-      for (int w = 0; w < kSampleWarps; ++w) tail += (float)sm.scan[w];
-      spread_f(tail);
-    }
-    int bin;
-    {
-      const int t0 = turn;
-      auto unit = [&](int b) { return masses ? exp2((double)b * (-1.0 / 16)) * (1.0 / 32768) : 1.0; };
-      double rest = 0.0;
-      if (masses) {
-        cluster.sync();
-        for (int c = 0; c < C; ++c) rest += (double)sm.gather_f[t0][c];
-        turn ^= 1;
-      }
-      bin = pick(unit, rest, 0.0);
-      if (bin > kTail) bin = kTail;
-    }
-    // gathers the bin's tokens; divides it while they are too many
-    unsigned low = 0, high = ~0u;  // keys
-    auto inside = [&](float v) {
-      const unsigned key = key_of(v);
-      return key >= low && key <= high && bin_of(step_of(v)) == bin;
-    };
-    int n;
-    for (;;) {
-      unsigned lo = ~0u, hi = 0;
-      EACH({
-        const bool in = v > -INFINITY && stays(v, i) && inside(v);
-        if (in) {
-          const int at = atomicAdd(&sm0.count, 1);
-          const unsigned key = key_of(v);
-          if (at < kList) sm0.list[at] = ((u64)key << 32) | (unsigned)~i;
-          lo = min(lo, key);
-          hi = max(hi, key);
+      if (tid < n) {
+        const u64 mine = sm.list[tid];
+        u64 larger = 0;
+        bool least_of_all = true;
+        for (int o = 0; o < n; ++o) {
+          const u64 other = sm.list[o];
+          if (other > mine) larger += w[o];
+          least_of_all &= other >= mine;
         }
-      })
-      lo = __reduce_min_sync(~0u, lo);
-      hi = __reduce_max_sync(~0u, hi);
-      if (lane == 0 && hi) {
-        atomicMin(&sm0.lowest, lo);
-        atomicMax(&sm0.highest, hi);
+        const bool here = ((double)larger < need || larger == 0) && (double)(larger + w[tid]) >= need;
+        if (here || (least_of_all && (double)(larger + w[tid]) < need)) sm.border = mine;
       }
-      cluster.sync();
-      n = sm0.count;
-      const unsigned all_lo = sm0.lowest, all_hi = sm0.highest;
-      cluster.sync();
-      if (rank == 0 && tid == 0) {
-        sm.count = 0;
-        sm.lowest = ~0u;
-        sm.highest = 0;
-      }
-      if (n > 0) {
-        low = all_lo;
-        high = all_hi;
-      }
-      if (n <= kList || low == high) break;
-      // by keys, the highest first
-      const int cut = max(0, 32 - __clz(high - low) - 9);
-      const float edge = step_of(value_of(high));
-      EACH({
-        if (v > -INFINITY && stays(v, i) && inside(v))
-          atomicAdd(&sm.hist[(high - key_of(v)) >> cut], masses ? weight15(step_of(v) - edge) : 1u);
-      })
-      const double unit = masses ? exp2((double)edge * (-1.0 / 16)) * (1.0 / 32768) : 1.0;
-      int b = pick([&](int) { return unit; }, -1.0, above);
-      if (b == kBins) b = (int)((high - low) >> cut);  // (weights that rounded away: the lowest)
-      const unsigned from = high - ((unsigned)b << cut);
-      low = max(low, cut ? from - ((1u << cut) - 1) : from);
-      high = from;
-    }
-    // what lies above the bin, exactly, and in the groups
-    u64 sure = 0;
-    if (masses) {
-      const float highest = value_of(high);
-      u64 mine = 0;
-      fill_groups([&](float v, int i) -> u64 {
-        if (!(v > -INFINITY) || !stays(v, i)) return 0;
-        const int b = bin_of(step_of(v));
-        if (n > 0 ? v <= highest : b >= bin) return 0;
-        const u64 m = mass_of(v);
-        mine += m;
-        return m >= least ? m : 0;
-      });
-      for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(~0u, mine, d);
-      if (lane == 0) sm.sums[warp] = mine;
       __syncthreads();
-      mine = 0;
-      for (int w = 0; w < kSampleWarps; ++w) mine += sm.sums[w];
-      spread_u(mine);
-      cluster.sync();
-      for (int c = 0; c < C; ++c) sure += sm.gather_u[turn][c];
-      turn ^= 1;
-    }
-    const double one = 17592186044416.0;
-    if (n == 0) {  // (a tail without tokens, or weights that rounded away)
-      if (masses) summed = true;
       return;
     }
-    if (n <= kList) {
-      if (rank == 0) {
-        int size = 32;
-        while (size < n) size *= 2;
-        for (int i = n + tid; i < size; i += kSampleThreads) sm.list[i] = 0;
-        // descending by logit, ascending by index
-        for (int len = 2; len <= size; len *= 2)
-          for (int step = len / 2; step > 0; step /= 2) {
-            __syncthreads();
-            for (int i = tid; i < size / 2; i += kSampleThreads) {
-              const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-              const u64 x0 = sm.list[lo], x1 = sm.list[hi];
-              if (((lo & len) == 0) == (x0 < x1)) {
-                sm.list[lo] = x1;
-                sm.list[hi] = x0;
-              }
-            }
-          }
+    int size = 32;
+    while (size < n) size *= 2;
+    for (int i = n + tid; i < size; i += kSampleThreads) sm.list[i] = 0;
+    for (int len = 2; len <= size; len *= 2)  // bitonic, descending
+      for (int step = len / 2; step > 0; step /= 2) {
         __syncthreads();
-        if (warp == 0) {  // walks the list: 32 at a time
-          const double need = masses ? target * one - (double)sure : target - above;
-          u64 seen = 0;
-          int last = n - 1;
-          for (int i0 = 0; i0 < n; i0 += 32) {
-            u64 w = 0;
-            if (i0 + lane < n) w = masses ? mass_of(value_of((unsigned)(sm.list[i0 + lane] >> 32))) : 1;
-            u64 run = w;
-            for (int d = 1; d < 32; d <<= 1) {
-              const u64 o = __shfl_up_sync(~0u, run, d);
-              if (lane >= d) run += o;
-            }
-            const unsigned there = __ballot_sync(~0u, i0 + lane < n && (double)(seen + run) >= need);
-            if (there) {
-              last = i0 + __ffs(there) - 1;
-              break;
-            }
-            seen += __shfl_sync(~0u, run, 31);
-          }
-          if (lane == 0) {
-            sm.border_x = value_of((unsigned)(sm.list[last] >> 32));
-            sm.border_i = (int)~(unsigned)sm.list[last];
+        for (int i = tid; i < size / 2; i += kSampleThreads) {
+          const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+          const u64 x0 = sm.list[lo], x1 = sm.list[hi];
+          if (((lo & len) == 0) == (x0 < x1)) {
+            sm.list[lo] = x1;
+            sm.list[hi] = x0;
           }
         }
       }
-      cluster.sync();
-      border_x = sm0.border_x;
-      border_i = sm0.border_i;
-      if (masses) {  // the list's tokens that stay join the groups
-        EACH({
-          if (v > -INFINITY && inside(v) && stays(v, i)) {
-            const u64 m = mass_of(v);
-            if (m >= least) atomicAdd(&sm.group[j * kSampleWarps + warp], m);
-          }
-        })
-        summed = true;
+    __syncthreads();
+    if (warp == 0) {  // walks the list: 32 at a time
+      u64 seen = 0;
+      int last = n - 1;
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        u64 run = 0;
+        if (i0 + lane < n) run = masses ? mass_of(value_of((unsigned)(sm.list[i0 + lane] >> 32))) : 1;
+        for (int d = 1; d < 32; d <<= 1) {
+          const u64 o = __shfl_up_sync(~0u, run, d);
+          if (lane >= d) run += o;
+        }
+        const unsigned there = __ballot_sync(~0u, i0 + lane < n && (double)(seen + run) >= need);
+        if (there) {
+          last = i0 + __ffs(there) - 1;
+          break;
+        }
+        seen += __shfl_sync(~0u, run, 31);
       }
-      cluster.sync();
-    } else {  // many tokens of one value: their number decides, and the index of the last
-      const float value = value_of(high);
-      u64 m = mass_of(value);
-      double want = masses ? (m ? ceil((target * one - (double)sure) / (double)m) : (double)n) : target - above;
-      const u64 ties = (u64)fmin(fmax(want, 1.0), (double)n);
-      auto is_tie = [&](float v, int i) -> u64 { return v == value && stays(v, i); };
-      fill_groups(is_tie);
-      u64 before, whole_ties;
-      group_scan(before, whole_ties);
-      locate(before, ties - 1, is_tie, [&](int i) { sm0.border_i = i; });
-      cluster.sync();
-      border_i = sm0.border_i;
-      border_x = value;
-      cluster.sync();
+      if (lane == 0) sm.border = sm.list[last];
+    }
+    __syncthreads();
+  };
+
+  // ---- CTA 0 by itself: n tokens in its list, all down to the lower edge of `bin`, which holds the border of a filter:
+  // with masses top_p's, at the mass `want`; else top_k's, `above` tokens lying in the bins before.
+  auto finish = [&](int n, int bin, bool masses, double want, double above) {
+    constexpr int per = kList / kSampleThreads;
+    u64 entry[per], m[per];
+#pragma unroll
+    for (int c = 0; c < per; ++c) {
+      const int i = tid + c * kSampleThreads;
+      entry[c] = i < n ? sm.list[i] : 0;
+      m[c] = 0;
+      if (c * kSampleThreads < n && i < n) m[c] = mass_of(value_of((unsigned)(entry[c] >> 32)));
+    }
+    u64 *const runs = reinterpret_cast<u64 *>(row_data - tid);  // (the row is not needed any more)
+    auto bin_at = [&](int c) { return bin_of(step_of(value_of((unsigned)(entry[c] >> 32)))); };
+    // the entries of the bin that are still there, by themselves; then only what reaches the border stays
+    auto cut = [&](int at_bin, double need, bool by) {
+      __syncthreads();
+      if (tid == 0) sm.count = 0;
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < per; ++c)
+        if (entry[c] && bin_at(c) == at_bin) sm.list[atomicAdd(&sm.count, 1)] = entry[c];
+      __syncthreads();
+      border_of(sm.count, need, by);
+#pragma unroll
+      for (int c = 0; c < per; ++c)
+        if (entry[c] < sm.border) entry[c] = m[c] = 0;
+    };
+    u64 z;
+    if (!masses) {
+      cut(bin, (double)k - above, false);
+      if (by_mass) {  // top_p of what top_k has left
+        runs[tid] = 0;
+        __syncthreads();
+        u64 sum = 0;
+#pragma unroll
+        for (int c = 0; c < per; ++c)
+          if (m[c]) {
+            atomicAdd(&runs[bin_at(c)], m[c]);
+            sum += m[c];
+          }
+        want = (double)p * (double)cta_sum(sum);
+        if (tid == 0) sm.found = kBins;
+        const u64 mine = runs[tid], before = cta_scan(mine, z);
+        if ((double)before < want && want <= (double)(before + mine)) {
+          sm.found = tid;
+          sm.start = before;
+        }
+        __syncthreads();
+        const int at_bin = sm.found;
+        if (at_bin < kBins) cut(at_bin, want - (double)sm.start, true);
+      }
+    } else {
+      u64 sum = 0;
+#pragma unroll
+      for (int c = 0; c < per; ++c) sum += entry[c] && bin_at(c) < bin ? m[c] : 0;
+      sum = cta_sum(sum);
+      cut(bin, want - (double)sum, true);
+    }
+    // the draw in the order of the indices: sums over 512 runs of indices, then the tokens of one run among themselves
+    int shift = 0;
+    while ((a.V >> shift) >= kSampleThreads) ++shift;
+    u64 *const masses_of_run = sm.list;
+    int *const members = reinterpret_cast<int *>(sm.list + kList / 2);
+    __syncthreads();
+    runs[tid] = 0;
+    if (tid == 0) sm.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < per; ++c) {
+      if (m[c] < least) m[c] = 0;
+      if (m[c]) atomicAdd(&runs[(int)~(unsigned)entry[c] >> shift], m[c]);
+    }
+    __syncthreads();
+    const u64 run = runs[tid], start = cta_scan(run, z), target = target_in(z);
+    if (start <= target && target < start + run) {
+      sm.found = tid;
+      sm.start = start;
+    }
+    __syncthreads();
+    const int hit = sm.found;
+#pragma unroll
+    for (int c = 0; c < per; ++c) {
+      const int i = (int)~(unsigned)entry[c];
+      if (m[c] && (i >> shift) == hit) {  // (a run holds at most 2^shift <= 1024 indices)
+        const int to = atomicAdd(&sm.count, 1);
+        members[to] = i;
+        masses_of_run[to] = m[c];
+      }
+    }
+    __syncthreads();
+    const int count = sm.count;
+    for (int t = tid; t < count; t += kSampleThreads) {
+      u64 before = sm.start;
+      const int i = members[t];
+      for (int o = 0; o < count; ++o)
+        if (members[o] < i) before += masses_of_run[o];
+      if (before <= target && target < before + masses_of_run[t]) a.out[row] = i;
     }
   };
-  if (k < a.V) narrow(false);
-  if (p < 1.f) narrow(true);
 
+  if (by_rank || by_mass) {
+    auto part = [&](float t) {  // 2^(-t/16)
+      float r;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t * (-1.f / 16)));
+      return r;
+    };
+    auto weight15 = [&](float t) { return (unsigned)__float2int_rn(part(t) * 32768.f); };
+    bool summed = false, done = false;
+    // ---- a border: the first token, from the top, with which the weights of the tokens that stay reach the target.
+    // masses: weights are masses and the target p of their whole; else numbers of tokens and the target k.
+    // Leaves the border, and with masses the sums of what stays in the groups (those with at least min_p of the largest).
+    auto narrow = [&](bool masses) {
+      float tail = 0.f;
+      EACH_VECTOR({
+        int b[VEC];
+        unsigned w[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float v = vec.at(e);
+          const float t = stays(v, i0 + e) ? step_of(v) : INFINITY;
+          b[e] = bin_of(t);
+          w[e] = masses ? weight15(t - (float)b[e]) : 1u;
+          tail += b[e] == kTail ? part(t) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (b[e] < kTail) atomicAdd(&sm.hist[b[e]], w[e]);
+      })
+      if (masses) {
+        for (int d = 16; d > 0; d >>= 1) tail += __shfl_xor_sync(~0u, tail, d);
+        if (lane == 0) sm.scan[warp] = tail;
+        __syncthreads();
+        tail = 0.f;
+#pragma unroll
+        for (int w = 0; w < kSampleWarps; ++w) tail += (float)sm.scan[w];
+        spread_f(tail);
+      }
+      // Picks the bin: every CTA the same from everybody's histograms.  unit: of a bin's weights; above: what lies before
+      // the first; tokens: about how many lie above the bin's lower edge.
+      double target = (double)k, above = 0.0, tokens = 0.0;
+      auto pick = [&](double unit, bool first) {
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        unsigned n[kMaxCluster];
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) n[c] = c < C ? cluster.map_shared_rank(&sm, c)->hist[tid] : 0;
+        double w = 0.0, all = above;
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) w += (double)n[c];
+        double few = masses ? w * (1.0 / 32768) : w;
+        w *= unit;
+        double run = w;
+        for (int d = 1; d < 32; d <<= 1) {
+          const double o = __shfl_up_sync(~0u, run, d), f = __shfl_up_sync(~0u, few, d);
+          if (lane >= d) {
+            run += o;
+            few += f;
+          }
+        }
+        __syncthreads();
+        if (lane == 31) {
+          sm.scan[warp] = run;
+          sm.scan2[warp] = few;
+        }
+        if (tid == 0) sm.pick_bin = kBins;
+        __syncthreads();
+        double start = above;
+#pragma unroll
+        for (int i = 0; i < kSampleWarps; ++i) {
+          if (i < warp) {
+            start += sm.scan[i];
+            few += sm.scan2[i];
+          }
+          all += sm.scan[i];
+        }
+        if (masses && first) {
+          double whole = all;
+          for (int c = 0; c < C; ++c) whole += (double)sm.gather_f[turn][c];
+          target = (double)p * whole;
+        }
+        const bool reached = start + run >= target;
+        const unsigned votes = __ballot_sync(~0u, reached);
+        if (reached && lane == __ffs(votes) - 1) atomicMin(&sm.pick_bin, tid);
+        __syncthreads();
+        const int b = sm.pick_bin;
+        if (b == tid || (b == kBins && tid == kBins - 1)) {
+          sm.pick_before = b == tid ? start + run - w : all;
+          sm.pick_tokens = few;
+        }
+        __syncthreads();
+        above = sm.pick_before;
+        tokens = sm.pick_tokens;
+        return b;
+      };
+      // (bins' edges are powers of 2^(1/16), from the table of 2^(i/64): 2^(-b/16) = 2^(-b>>4) 2^((-b&15)/16))
+      const int e16 = -tid;
+      const double edge0 = masses ? sm.table[(e16 & 15) * 4] * __hiloint2double((1023 + (e16 >> 4)) << 20, 0) * (1.0 / 32768) : 1.0;
+      int bin = pick(edge0, true);
+      if (masses) turn ^= 1;
+      if (bin > kTail) bin = kTail;
+      // the tokens of CTA 0's list: those that stay and are `in`
+      // (each CTA lists its own; the others' lists then join CTA 0's)
+      auto gather = [&](auto in) {
+        EACH_VECTOR({
+          unsigned hits = 0;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) hits |= (unsigned)(stays(vec.at(e), i0 + e) && in(vec.at(e))) << e;
+          if (hits) {
+            int at = atomicAdd(&sm.count, __popc(hits));
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+              if (hits >> e & 1) {
+                if (at < kList) sm.list[at] = ((u64)key_of(vec.at(e)) << 32) | (unsigned)~(i0 + e);
+                ++at;
+              }
+          }
+        })
+        if (rank != 0) {
+          __syncthreads();
+          const int n = sm.count;
+          if (n > 0) {
+            if (tid == 0) sm.found = atomicAdd(&sm0.count, n);
+            __syncthreads();
+            const int base = sm.found;
+            for (int i = tid; i < min(n, kList - base); i += kSampleThreads) sm0.list[base + i] = sm.list[i];
+            __syncthreads();
+            if (tid == 0) sm.count = 0;
+          }
+        }
+      };
+      // the lowest and the highest key of what is `in`, to CTA 0
+      auto extremes = [&](auto in) {
+        unsigned lo = ~0u, hi = 0;
+        EACH({
+          if (stays(v, i) && in(v)) {
+            lo = min(lo, key_of(v));
+            hi = max(hi, key_of(v));
+          }
+        })
+        lo = __reduce_min_sync(~0u, lo);
+        hi = __reduce_max_sync(~0u, hi);
+        if (lane == 0 && hi) {
+          atomicMin(&sm0.lowest, lo);
+          atomicMax(&sm0.highest, hi);
+        }
+      };
+      if (bin < kTail && tokens * 1.05 < (double)kList) {  // (masses tell their tokens' number to within 2^(1/16))
+        const float edge = (float)(bin + 1);
+        gather([&](float v) { return step_of(v) < edge; });
+        done = true;
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        if (rank == 0) finish(sm.count, bin, masses, target * one, above);
+        return;
+      }
+      // gathers the bin's tokens; divides it while they are too many
+      unsigned low = 0, high = ~0u;  // keys
+      auto inside = [&](float v) {
+        const unsigned key = key_of(v);
+        return key >= low && key <= high && bin_of(step_of(v)) == bin;
+      };
+      int n;
+      for (;;) {
+        gather(inside);
+        extremes(inside);
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        sm.hist[tid] = 0;  // (everybody has read the histograms)
+        n = sm0.count;
+        const unsigned all_lo = sm0.lowest, all_hi = sm0.highest;
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        if (rank == 0 && tid == 0) {
+          sm.count = 0;
+          sm.lowest = ~0u;
+          sm.highest = 0;
+        }
+        if (n > 0) {
+          low = all_lo;
+          high = all_hi;
+        }
+        if (n <= kList || low == high) break;
+        // by keys, the highest first
+        const int cut = max(0, 32 - __clz(high - low) - 9);
+        const float edge = step_of(value_of(high));
+        EACH({
+          if (v > -INFINITY && stays(v, i) && inside(v))
+            atomicAdd(&sm.hist[(high - key_of(v)) >> cut], masses ? weight15(step_of(v) - edge) : 1u);
+        })
+        int b = pick(masses ? exp2((double)edge * (-1.0 / 16)) * (1.0 / 32768) : 1.0, false);
+        if (b == kBins) b = (int)((high - low) >> cut);  // (weights that rounded away: the lowest)
+        const unsigned from = high - ((unsigned)b << cut);
+        low = max(low, cut ? from - ((1u << cut) - 1) : from);
+        high = from;
+      }
+      // what lies above the bin, exactly, and in the groups
+      u64 sure = 0;
+      if (masses) {
+        const float highest = value_of(high);
+        u64 mine = 0;
+        fill_groups([&](const Vec<TI> &vec, int i0, u64 *w) {
+          unsigned hits = 0;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float v = vec.at(e);
+            if (stays(v, i0 + e) && (n > 0 ? v > highest : bin_of(step_of(v)) < bin)) hits |= 1u << e;
+            w[e] = 0;
+          }
+          if (__any_sync(~0u, hits != 0)) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const u64 m = hits >> e & 1 ? mass_of(vec.at(e)) : 0;
+              mine += m;
+              w[e] = m >= least ? m : 0;
+            }
+          }
+        });
+        sure = cta_sum(mine);
+        if (C > 1) {
+          spread_u(sure);
+          cluster.sync();
+          sure = 0;
+          for (int c = 0; c < C; ++c) sure += sm.gather_u[turn][c];
+          turn ^= 1;
+        }
+        summed = true;
+      }
+      if (n == 0) return;  // (a tail without tokens)
+      if (n <= kList) {
+        if (rank == 0) {
+          border_of(n, masses ? target * one - (double)sure : target - above, masses);
+          if (tid == 0) {
+            sm.border_x = value_of((unsigned)(sm.border >> 32));
+            sm.border_i = (int)~(unsigned)sm.border;
+          }
+        }
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        border_x = sm0.border_x;
+        border_i = sm0.border_i;
+        if (masses) {  // the list's tokens that stay join the groups
+          EACH({
+            if (stays(v, i) && inside(v)) {
+              const u64 m = mass_of(v);
+              if (m >= least) atomicAdd(&sm.group[j * kSampleWarps + warp], m);
+            }
+          })
+        }
+      } else {  // many tokens of one value: their number decides, and the index of the last
+        const float value = value_of(high);
+        const u64 m = mass_of(value);
+        const double want = masses ? (m ? ceil((target * one - (double)sure) / (double)m) : (double)n) : target - above;
+        const u64 ties = (u64)fmin(fmax(want, 1.0), (double)n);
+        auto is_tie = [&](const Vec<TI> &vec, int i0, u64 *w) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) w[e] = vec.at(e) == value && stays(vec.at(e), i0 + e);
+        };
+        __syncthreads();
+        fill_groups(is_tie);
+        locate([&](u64) { return ties - 1; }, is_tie, [&](int i) { sm0.border_i = i; });
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        border_i = sm0.border_i;
+        border_x = value;
+        summed = false;
+      }
+      if (C > 1) cluster.sync();
+      else __syncthreads();
+    };
+    if (by_rank) narrow(false);
+    if (done) return;  // (nobody reads or writes another CTA's memory after the last barrier)
+    if (by_mass) narrow(true);
+    if (done) return;
+    if (!summed) fill_groups(kept);
+  } else {
+    fill_groups(kept);
+  }
   // ---- the draw
-  auto kept = [&](float v, int i) -> u64 {
-    if (!(v > -INFINITY) || !stays(v, i)) return 0;
-    const u64 m = mass_of(v);
-    return m >= least ? m : 0;
-  };
-  if (!summed) fill_groups(kept);
-  u64 before, z;
-  group_scan(before, z);
-  double u = a.u_bytes == 4 ? (double)static_cast<const float *>(a.u)[row] : static_cast<const double *>(a.u)[row];
-  u = fmin(fmax(u, 0.0), 1.0);
-  // running > u z: of integers, running > its floor; below z, so that there always is such a token
-  const u64 target = min((u64)(u * (double)z), z - 1);
-  locate(before, target, kept, [&](int i) { a.out[row] = i; });
-  cluster.sync();
+  locate(target_in, kept, [&](int i) { a.out[row] = i; });
+  leave();
 #undef EACH
+#undef EACH_VECTOR
 }
 
 // A row's cluster: few vectors a thread where the rows leave SMs for more CTAs (two to an SM).
