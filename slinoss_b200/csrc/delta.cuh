@@ -24,18 +24,23 @@ namespace delta {
 constexpr int L = 64;             // tokens of a chunk
 constexpr int kTri = 3072;        // elements of a lower triangular 64 x 64 tile, by row blocks of 16 (tri_at)
 constexpr int kThreads = 128;
+constexpr int kTileLd = 72, kTile = L * kTileLd;  // Y and dX: 64 tokens x up to 64 value channels
 
-// What every later kernel needs of one chunk and head, written once by delta_chunk_kernel.
+// What every later kernel needs of one chunk and value head, written once by delta_chunk_kernel.
 struct Record {
   __half T[2][kTri];  // Tm, hi and lo
   __half Q[2][kTri];  // P, hi and lo
   float gamma[L], closing[L], beta[L];
+  // dec_ts for t in block i of 16 tokens and s in an earlier one is rise[t] * fall[fall_at(i) + s]: both exponents from G at
+  // the end of block i - 1, so that neither factor leaves the range where gates close
+  float rise[L], fall[96];
   double G[L];
   int eT, eQ, eq, ek;  // binary exponents: value = stored * 2^e
   int pad[28];
 };
-static_assert(sizeof(Record) == 25984 && sizeof(Record) % 128 == 0, "record layout");
-constexpr int kHeadBytes = 3 * L * 4 + L * 8 + 16;  // gamma .. ek
+static_assert(sizeof(Record) == 26624 && sizeof(Record) % 128 == 0, "record layout");
+constexpr int kHeadBytes = 3 * L * 4;  // gamma, closing, beta
+__host__ __device__ constexpr int fall_at(int i) { return 8 * i * (i - 1); }
 
 struct Rows {  // a (batch, head, token, :) tensor whose last axis is dense; strides in elements
   const void *p;
@@ -50,13 +55,14 @@ struct Args {
   int g_dtype, beta_dtype;
   Rows q, k, v, g, beta, dO;
   Record *rec;              // (batch*heads, NC)
+  __half *kq;               // (batch*key_heads, NC): k, then q, as Operand holds them in shared memory
   // forward
   const void *init;         // (batch, heads, P, N) or null
   int init_dtype;
   void *o;                  // (batch, heads, T, P) or null
   float *final_state;       // or null
-  __half *st;               // states before every chunk: (BH, NC, planes, P16, NT), or null
-  __half *y;                // Y of every chunk: (BH, NC, planes, 64, P16), or null
+  __half *st;               // states before every chunk: (BH, NC, planes, P16, NT + 8), or null
+  __half *y;                // Y of every chunk: (BH, NC, planes, tiles of 64 channels, 64, 72), or null
   int *est, *ey;            // (BH, NC, P16 / 16)
   // backward
   const void *d_final;
@@ -74,6 +80,15 @@ struct Args {
 // number of 16-byte units per row: ldmatrix meets no bank twice).  5/8 of the square's bytes.
 __host__ __device__ constexpr int tri_base(int i) { return 128 * i * i + 256 * i; }
 __host__ __device__ constexpr int tri_ld(int i) { return 16 * i + 24; }
+
+// Row-major operand tiles of 64 tokens x W columns, SI fp16 planes one after another; rows are padded to an odd number of
+// 16-byte units.
+template <int SI, int W>
+struct Operand {
+  static constexpr int ld = W + 8;
+  static constexpr int plane = L * ld;
+  static constexpr int halves = SI * plane;
+};
 
 // ---- exponents -----------------------------------------------------------------------------------------------------
 constexpr int kZeroExp = -100;  // of a tile of zeros
@@ -93,12 +108,12 @@ __device__ __forceinline__ int floor_exp(int e, int ec, int eb) { return max(e, 
 __device__ __forceinline__ unsigned mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 template <int n>
 __device__ __forceinline__ unsigned max_mag(const float (&c)[n][4]) {
-  unsigned m = 0;
+  unsigned m[4] = {0, 0, 0, 0};  // (four short chains)
 #pragma unroll
   for (int j = 0; j < n; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = max(m, mag(c[j][i]));
-  return m;
+    for (int i = 0; i < 4; ++i) m[i] = max(m[i], mag(c[j][i]));
+  return max(max(m[0], m[1]), max(m[2], m[3]));
 }
 template <int n>
 __device__ __forceinline__ int warp_exp(const float (&c)[n][4]) {
@@ -196,12 +211,94 @@ __device__ __forceinline__ void mma_split(float (&c0)[4], float (&c1)[4], const 
     mma(c1, a.r[0], b[1][2], b[1][3]);
   }
 }
+// The same for the n8 tiles 2 first .. 2 (first + n) - 1 of an accumulator and n blocks of B, plane by plane: neighbouring
+// instructions add to different tiles, so that none waits for the one before it.
+template <int SA, int SB, int n, int tiles>
+__device__ __forceinline__ void mma_group(float (&c)[tiles][4], int first, const Frag<SA> &a, const uint32_t (&b)[n][SB][4]) {
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    mma(c[2 * (first + i)], a.r[0], b[i][0][0], b[i][0][1]);
+    mma(c[2 * (first + i) + 1], a.r[0], b[i][0][2], b[i][0][3]);
+  }
+  if constexpr (SA == 2) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      mma(c[2 * (first + i)], a.r[1], b[i][0][0], b[i][0][1]);
+      mma(c[2 * (first + i) + 1], a.r[1], b[i][0][2], b[i][0][3]);
+    }
+  }
+  if constexpr (SB == 2) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      mma(c[2 * (first + i)], a.r[0], b[i][1][0], b[i][1][1]);
+      mma(c[2 * (first + i) + 1], a.r[0], b[i][1][2], b[i][1][3]);
+    }
+  }
+}
 template <int n>
 __device__ __forceinline__ void zero(float (&c)[n][4]) {
 #pragma unroll
   for (int j = 0; j < n; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+}
+// c (16 x 64 tokens) += a (16 x 64) B^T for a lower triangular tile B: columns t take the blocks s <= t.
+template <int SA, int SB, int kb>
+__device__ __forceinline__ void tri_rows_step(float (&c)[8][4], const Frag<SA> (&a)[4], const __half *tile) {
+  uint32_t b[4 - kb][SB][4];
+#pragma unroll
+  for (int i = 0; i < 4 - kb; ++i)
+#pragma unroll
+    for (int s = 0; s < SB; ++s) b_nk(b[i][s], tile + s * kTri + tri_base(kb + i) + 16 * kb, tri_ld(kb + i));
+  mma_group<SA, SB, 4 - kb>(c, kb, a[kb], b);
+}
+template <int SA, int SB>
+__device__ __forceinline__ void tri_rows(float (&c)[8][4], const Frag<SA> (&a)[4], const __half *tile) {
+  tri_rows_step<SA, SB, 0>(c, a, tile);
+  tri_rows_step<SA, SB, 1>(c, a, tile);
+  tri_rows_step<SA, SB, 2>(c, a, tile);
+  tri_rows_step<SA, SB, 3>(c, a, tile);
+}
+// c += a B: columns s take the blocks t >= s.
+template <int SA, int SB, int kb>
+__device__ __forceinline__ void tri_cols_step(float (&c)[8][4], const Frag<SA> (&a)[4], const __half *tile) {
+  uint32_t b[kb + 1][SB][4];
+#pragma unroll
+  for (int i = 0; i <= kb; ++i)
+#pragma unroll
+    for (int s = 0; s < SB; ++s) b_kn(b[i][s], tile + s * kTri + tri_base(kb) + 16 * i, tri_ld(kb));
+  mma_group<SA, SB, kb + 1>(c, 0, a[kb], b);
+}
+template <int SA, int SB>
+__device__ __forceinline__ void tri_cols(float (&c)[8][4], const Frag<SA> (&a)[4], const __half *tile) {
+  tri_cols_step<SA, SB, 3>(c, a, tile);
+  tri_cols_step<SA, SB, 2>(c, a, tile);
+  tri_cols_step<SA, SB, 1>(c, a, tile);
+  tri_cols_step<SA, SB, 0>(c, a, tile);
+}
+// c (16 x 64 tokens) += a (16 x 16 of n) B^T for columns 16 kb .. of an operand tile [t][n]
+template <int SA, int SB, int W>
+__device__ __forceinline__ void tile_rows(float (&c)[8][4], const Frag<SA> &a, const __half *tile, int kb) {
+  uint32_t b[4][SB][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int s = 0; s < SB; ++s)
+      b_nk(b[i][s], tile + s * Operand<SB, W>::plane + 16 * i * Operand<SB, W>::ld + 16 * kb, Operand<SB, W>::ld);
+  mma_group<SA, SB, 4>(c, 0, a, b);
+}
+// c (16 x W) += a (16 x 16 tokens) B for rows 16 kb .. of a row-major tile of W columns (planes `plane` apart)
+template <int SA, int SB, int W>
+__device__ __forceinline__ void tile_cols(float (&c)[W / 8][4], const Frag<SA> &a, const __half *tile, int plane, int kb) {
+#pragma unroll
+  for (int n0 = 0; n0 < W / 16; n0 += 4) {
+    uint32_t b[4][SB][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int s = 0; s < SB; ++s) b_kn(b[i][s], tile + s * plane + 16 * kb * (W + 8) + 16 * (n0 + i), W + 8);
+    mma_group<SA, SB, 4>(c, n0, a, b);
+  }
 }
 template <int n>
 __device__ __forceinline__ void times(float (&c)[n][4], float s) {
@@ -235,123 +332,108 @@ __device__ __forceinline__ const TI *head_base(const Rows &r, int b, int h, int 
   return static_cast<const TI *>(r.p) + b * r.sb + h * r.sh + (int64_t)t * r.st;
 }
 
-// Row-major operand tiles of 64 tokens x W columns (leading dimension W + 8), SI fp16 planes one after another.
-// issue(): starts the copy of `rows` rows of `cols` columns, zeros elsewhere; finish(): what a thread has copied, brought
-// to scaled fp16 in place (called by the same threads after the copy has arrived and before the CTA's barrier).
-template <typename TI, int SI, int W>
-struct Operand {
-  static constexpr int ld = W + 8;
-  static constexpr int plane = L * ld;
-  static constexpr int bytes = SI * plane * 2;
-  static constexpr bool async_convert = sizeof(TI) == 2;
-
-  static __device__ __forceinline__ void issue(__half *dst, const TI *src, int64_t st, int rows, int cols, bool vec, int e) {
-    const float s = pow2(-e);
-    if constexpr (async_convert) {
-      if (vec) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < L * (W / 8); i += kThreads) {
-          const int r = i / (W / 8), c = (i % (W / 8)) * 8;
-          const bool ok = r < rows && c < cols;
-          cp16(dst + r * ld + c, ok ? src + r * st + c : src, ok);
+// A tile of 64 tokens x W columns from global memory in 16-byte pieces, `per` of a thread, zeros outside rows and cols.
+template <typename TI, int W>
+struct Pieces {
+  static constexpr int V = 16 / (int)sizeof(TI), per = L * W / V / kThreads;
+  uint4 x[per];
+  static __device__ __forceinline__ int row(int i) { return (i * kThreads + (int)threadIdx.x) / (W / V); }
+  static __device__ __forceinline__ int col(int i) { return (i * kThreads + (int)threadIdx.x) % (W / V) * V; }
+  __device__ __forceinline__ void load(const TI *src, int64_t st, int rows, int cols, bool vec) {
+#pragma unroll
+    for (int i = 0; i < per; ++i) {
+      const int r = row(i), c = col(i);
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (r < rows && c < cols) {
+        const TI *at = src + r * st + c;
+        if (vec) x[i] = *reinterpret_cast<const uint4 *>(at);
+        else {
+          TI e[V];
+#pragma unroll
+          for (int n = 0; n < V; ++n) e[n] = c + n < cols ? at[n] : from_f<TI>(0.f);
+          memcpy(&x[i], e, 16);
         }
-        return;
-      }
-      for (int i = threadIdx.x; i < L * W; i += kThreads) {
-        const int r = i / W, c = i % W;
-        dst[r * ld + c] = __float2half_rn(r < rows && c < cols ? to_f(src[r * st + c]) * s : 0.f);
-      }
-    } else {
-      for (int i = threadIdx.x; i < L * (W / 4); i += kThreads) {
-        const int r = i / (W / 4), c = (i % (W / 4)) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < rows && c < cols) {
-          const float *at = reinterpret_cast<const float *>(src) + r * st + c;
-          if (vec) x = *reinterpret_cast<const float4 *>(at);
-          else {
-            x.x = at[0];
-            if (c + 1 < cols) x.y = at[1];
-            if (c + 2 < cols) x.z = at[2];
-            if (c + 3 < cols) x.w = at[3];
-          }
-        }
-        uint2 hi, lo;
-        split<2>(x.x * s, x.y * s, &hi.x, &lo.x);
-        split<2>(x.z * s, x.w * s, &hi.y, &lo.y);
-        *reinterpret_cast<uint2 *>(dst + r * ld + c) = hi;
-        *reinterpret_cast<uint2 *>(dst + plane + r * ld + c) = lo;
       }
     }
   }
-  static __device__ __forceinline__ void finish(__half *dst, bool vec, int e) {
-    if constexpr (sizeof(TI) == 2 && !std::is_same<TI, __half>::value) {
-      if (!vec) return;
-      const float s = pow2(-e);
-#pragma unroll 2
-      for (int i = threadIdx.x; i < L * (W / 8); i += kThreads) {
-        uint4 *at = reinterpret_cast<uint4 *>(dst + (i / (W / 8)) * ld + (i % (W / 8)) * 8);
-        uint4 x = *at;
-        uint32_t *w = reinterpret_cast<uint32_t *>(&x);
+  __device__ __forceinline__ unsigned max_bits() const {  // of the largest magnitude, as fp32
+    unsigned m = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = pack(__uint_as_float(w[j] << 16) * s, __uint_as_float(w[j] & 0xffff0000u) * s);
-        *at = x;
+    for (int i = 0; i < per; ++i) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(TI) == 4) m = max(m, w[j] & 0x7fffffffu);
+        else m = max(m, max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));  // bf16
+      }
+    }
+    return m;
+  }
+  // as scaled fp16, to an operand tile in shared memory and (COPY) to a copy of it in global memory
+  template <int SI, bool COPY>
+  __device__ __forceinline__ void store(__half *tile, __half *copy, int e) const {
+    constexpr int ld = Operand<SI, W>::ld, plane = Operand<SI, W>::plane;
+    const float s = pow2(-e);
+#pragma unroll
+    for (int i = 0; i < per; ++i) {
+      const int at = row(i) * ld + col(i);
+      if constexpr (sizeof(TI) == 4) {
+        uint2 hi, lo;
+        split<2>(__uint_as_float(x[i].x) * s, __uint_as_float(x[i].y) * s, &hi.x, &lo.x);
+        split<2>(__uint_as_float(x[i].z) * s, __uint_as_float(x[i].w) * s, &hi.y, &lo.y);
+        *reinterpret_cast<uint2 *>(tile + at) = hi;
+        *reinterpret_cast<uint2 *>(tile + plane + at) = lo;
+        if constexpr (COPY) {
+          *reinterpret_cast<uint2 *>(copy + at) = hi;
+          *reinterpret_cast<uint2 *>(copy + plane + at) = lo;
+        }
+      } else {
+        uint4 h = x[i];
+        if constexpr (!std::is_same<TI, __half>::value) {
+          uint32_t *w = reinterpret_cast<uint32_t *>(&h);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            w[j] = pack(__uint_as_float(w[j] << 16) * s, __uint_as_float(w[j] & 0xffff0000u) * s);
+        }
+        *reinterpret_cast<uint4 *>(tile + at) = h;
+        if constexpr (COPY) *reinterpret_cast<uint4 *>(copy + at) = h;
       }
     }
   }
 };
-
-// Largest magnitude of a tile in global memory (this thread's share), for its exponent.
-template <typename TI>
-__device__ __forceinline__ unsigned tile_mag(const TI *src, int64_t st, int rows, int cols, bool vec, int W) {
-  unsigned m = 0;
-  constexpr int V = 16 / sizeof(TI);
-  if (vec) {
-    const int per = W / V;
-    for (int i = threadIdx.x; i < L * per; i += kThreads) {
-      const int r = i / per, c = (i % per) * V;
-      if (r < rows && c < cols) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(src + r * st + c);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (sizeof(TI) == 4) m = max(m, w[j] & 0x7fffffffu);
-          else m = max(m, max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));  // bf16
-        }
-      }
-    }
-  } else {
-    for (int i = threadIdx.x; i < rows * cols; i += kThreads) m = max(m, mag(to_f(src[(i / cols) * st + i % cols])));
-  }
-  return m;
-}
 
 // A raw tile of 64 tokens x up to 64 columns, kept in TI.
 template <typename TI>
 struct Raw {
   static constexpr int ld = 64 + 16 / (int)sizeof(TI);
   static constexpr int bytes = L * ld * (int)sizeof(TI);
-  static __device__ __forceinline__ void issue(TI *dst, const TI *src, int64_t st, int rows, int cols, int width, bool vec) {
-    constexpr int V = 16 / sizeof(TI);
+  static __device__ __forceinline__ void issue(TI *dst, const TI *src, int64_t st, int rows, int cols, bool vec) {
+    constexpr int V = 16 / (int)sizeof(TI), per = 64 / V;
     if (vec) {
-      const int per = width / V;
-      for (int i = threadIdx.x; i < L * per; i += kThreads) {
-        const int r = i / per, c = (i % per) * V;
+#pragma unroll
+      for (int n = 0; n < L * per / kThreads; ++n) {
+        const int i = n * kThreads + threadIdx.x, r = i / per, c = i % per * V;
         const bool ok = r < rows && c < cols;
         cp16(dst + r * ld + c, ok ? src + r * st + c : src, ok);
       }
     } else {
-      for (int i = threadIdx.x; i < L * width; i += kThreads) {
-        const int r = i / width, c = i % width;
+      for (int i = threadIdx.x; i < L * 64; i += kThreads) {
+        const int r = i / 64, c = i % 64;
         dst[r * ld + c] = r < rows && c < cols ? src[r * st + c] : from_f<TI>(0.f);
       }
     }
   }
 };
 
-__device__ __forceinline__ void copy_bytes(void *dst, const void *src, int bytes) {  // asynchronous, multiples of 16
-  for (int i = threadIdx.x * 16; i < bytes; i += kThreads * 16)
-    cp16(static_cast<char *>(dst) + i, static_cast<const char *>(src) + i, true);
+template <int bytes>
+__device__ __forceinline__ void copy_bytes(void *dst, const void *src) {  // asynchronous, a multiple of 16
+  static_assert(bytes % 16 == 0, "copies of 16 bytes");
+  char *d = static_cast<char *>(dst) + threadIdx.x * 16;
+  const char *s = static_cast<const char *>(src) + threadIdx.x * 16;
+#pragma unroll
+  for (int i = 0; i < bytes / 16 / kThreads; ++i) cp16(d + i * kThreads * 16, s + i * kThreads * 16, true);
+  constexpr int whole = bytes / 16 / kThreads * kThreads * 16;
+  if (whole < bytes && (int)threadIdx.x * 16 < bytes - whole) cp16(d + whole, s + whole, true);
 }
 
 // A warp's (16 columns p, 64 tokens) result, held transposed in accumulators (rows p, columns t), to global rows of `out`
@@ -401,11 +483,10 @@ __device__ __forceinline__ void store_rows(TO *out, int64_t st, int rows, int co
 }
 
 // Accumulators (rows p, columns t) as S planes of scaled fp16 rows [t][p] in global memory (leading dimension st, 64 rows,
-// always whole); returns their exponent.
+// always whole), scaled by 2^-e.
 template <int S>
-__device__ __forceinline__ int store_planes(__half *out, int64_t st, int64_t plane, const float (&c)[8][4], __half *buf) {
+__device__ __forceinline__ void store_planes(__half *out, int64_t st, int64_t plane, const float (&c)[8][4], int e, __half *buf) {
   const int lane = threadIdx.x & 31;
-  const int e = warp_exp(c);
   const float s = pow2(-e);
 #pragma unroll
   for (int pl = 0; pl < S; ++pl) {
@@ -422,10 +503,10 @@ __device__ __forceinline__ int store_planes(__half *out, int64_t st, int64_t pla
       *reinterpret_cast<uint4 *>(out + pl * plane + (i >> 1) * st + (i & 1) * 8) =
           *reinterpret_cast<const uint4 *>(buf + (i >> 1) * 24 + (i & 1) * 8);
   }
-  return e;
 }
 
-// A warp's 16 rows of a state (accumulators: rows p, columns n) as S planes of fp16 rows of NT columns, scaled by 2^-e.
+// A warp's 16 rows of a state (accumulators: rows p, columns n) as S planes of fp16 rows of NT columns (NT + 8 apart), scaled
+// by 2^-e.
 template <int S, int NT>
 __device__ __forceinline__ void store_state(__half *out, int64_t plane, const float (&c)[NT / 8][4], int e, __half *buf) {
   const int lane = threadIdx.x & 31;
@@ -443,7 +524,7 @@ __device__ __forceinline__ void store_state(__half *out, int64_t plane, const fl
     __syncwarp();
 #pragma unroll
     for (int i = lane; i < 16 * (NT / 8); i += 32)
-      *reinterpret_cast<uint4 *>(out + pl * plane + i * 8) =
+      *reinterpret_cast<uint4 *>(out + pl * plane + (i / (NT / 8)) * ld + (i % (NT / 8)) * 8) =
           *reinterpret_cast<const uint4 *>(buf + (i / (NT / 8)) * ld + (i % (NT / 8)) * 8);
   }
 }

@@ -21,8 +21,12 @@ constexpr int kAld = 72;  // floats per row of the fp32 tile: float2 accesses of
 constexpr double kLowestGate = -110.0;
 
 template <int NT, int SI>
+constexpr int chunk_tiles() {  // bytes: k and q, then the four triangular tiles in their place
+  return 2 * Operand<SI, NT>::halves > 4 * kTri ? 2 * Operand<SI, NT>::halves * 2 : 4 * kTri * 2;
+}
+template <int NT, int SI>
 constexpr int chunk_smem() {
-  return 2 * SI * L * (NT + 8) * 2 + L * kAld * 4 + 4 * kTri * 2 + 64;
+  return chunk_tiles<NT, SI>() + L * kAld * 4;
 }
 
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
@@ -56,38 +60,53 @@ __device__ __forceinline__ void block_product(float (&c)[2][4], const float (&a)
 
 template <int NT, int SI, typename TI>
 __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
-  using Op = Operand<TI, SI, NT>;
+  using Op = Operand<SI, NT>;
+  using In = Pieces<TI, NT>;
   extern __shared__ __align__(128) char smem[];
-  __half *qs = reinterpret_cast<__half *>(smem), *ks = qs + SI * Op::plane;
-  float *A = reinterpret_cast<float *>(smem + 2 * Op::bytes);
-  __half *tri = reinterpret_cast<__half *>(A + L * kAld);  // T hi, T lo, P hi, P lo
-  unsigned *tops = reinterpret_cast<unsigned *>(tri + 4 * kTri);
+  __half *ks = reinterpret_cast<__half *>(smem), *qs = ks + Op::halves;
+  __half *tri = reinterpret_cast<__half *>(smem);  // T hi, T lo, P hi, P lo
+  float *A = reinterpret_cast<float *>(smem + chunk_tiles<NT, SI>());
   __shared__ double G[L];
-  __shared__ float beta[L];
+  __shared__ float beta[L], rise[L], fall[96];
+  __shared__ unsigned tops[8];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int chunk = blockIdx.x, b = blockIdx.y / a.key_heads, kh = blockIdx.y % a.key_heads;
   const int share = a.heads / a.key_heads, t0 = chunk * L, rows = min(L, a.T - t0);
-  const TI *qp = head_base<TI>(a.q, b, kh, t0), *kp = head_base<TI>(a.k, b, kh, t0);
 
-  int eq = 0, ek = 0;
-  if constexpr (!std::is_same<TI, __half>::value) {
-    const unsigned mq = __reduce_max_sync(~0u, tile_mag(qp, a.q.st, rows, a.N, a.q.vec, NT));
-    const unsigned mk = __reduce_max_sync(~0u, tile_mag(kp, a.k.st, rows, a.N, a.k.vec, NT));
-    if (lane == 0) {
-      tops[warp] = mq;
-      tops[4 + warp] = mk;
+  // the gates of a head, two tokens per lane of warp 0; past the end g = 0 and beta = 0
+  float gate[2], write[2];
+  auto fetch = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = 2 * lane + i;
+      gate[i] = write[i] = 0.f;
+      if (t < rows) {
+        gate[i] = load_as_f(a.g.p, a.g_dtype, b * a.g.sb + h * a.g.sh + (int64_t)(t0 + t) * a.g.st);
+        write[i] = load_as_f(a.beta.p, a.beta_dtype, b * a.beta.sb + h * a.beta.sh + (int64_t)(t0 + t) * a.beta.st);
+      }
     }
-    __syncthreads();
-    eq = exp_of(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
-    ek = exp_of(max(max(tops[4], tops[5]), max(tops[6], tops[7])));
+  };
+  if (warp == 0) fetch(kh * share);
+  int eq = 0, ek = 0;
+  {
+    In kx, qx;
+    kx.load(head_base<TI>(a.k, b, kh, t0), a.k.st, rows, a.N, a.k.vec);
+    qx.load(head_base<TI>(a.q, b, kh, t0), a.q.st, rows, a.N, a.q.vec);
+    if constexpr (!std::is_same<TI, __half>::value) {
+      const unsigned mq = __reduce_max_sync(~0u, qx.max_bits()), mk = __reduce_max_sync(~0u, kx.max_bits());
+      if (lane == 0) {
+        tops[warp] = mq;
+        tops[4 + warp] = mk;
+      }
+      __syncthreads();
+      eq = exp_of(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+      ek = exp_of(max(max(tops[4], tops[5]), max(tops[6], tops[7])));
+    }
+    __half *copy = a.kq + ((size_t)blockIdx.y * a.NC + chunk) * 2 * Op::halves;
+    kx.template store<SI, true>(ks, copy, ek);
+    qx.template store<SI, true>(qs, copy + Op::halves, eq);
   }
-  Op::issue(qs, qp, a.q.st, rows, a.N, a.q.vec, eq);
-  Op::issue(ks, kp, a.k.st, rows, a.N, a.k.vec, ek);
-  cp_commit();
-  cp_wait<0>();
-  Op::finish(qs, a.q.vec, eq);
-  Op::finish(ks, a.k.vec, ek);
   __syncthreads();
 
   // rows 16 warp .. + 15 of k k^T and q k^T, columns up to the diagonal block
@@ -121,39 +140,34 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
   for (int hs = 0; hs < share; ++hs) {
     const int h = kh * share + hs;
     Record *rec = a.rec + (size_t)(b * a.heads + h) * a.NC + chunk;
-    if (warp == 0) {  // two tokens per lane; past the end g = 0 and beta = 0
-      double s0, s1;
-      float be[2];
+    if (warp == 0) {
       double gg[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = 2 * lane + i;
-        gg[i] = 0.0;
-        be[i] = 0.f;
-        if (t < rows) {
-          const double x = load_as_f(a.g.p, a.g_dtype, b * a.g.sb + h * a.g.sh + (int64_t)(t0 + t) * a.g.st);
-          gg[i] = x < kLowestGate ? kLowestGate : x;
-          be[i] = load_as_f(a.beta.p, a.beta_dtype, b * a.beta.sb + h * a.beta.sh + (int64_t)(t0 + t) * a.beta.st);
-        }
-        beta[t] = be[i];
-      }
-      s0 = gg[0];
-      s1 = gg[0] + gg[1];
-      double run = s1;
+      for (int i = 0; i < 2; ++i) gg[i] = gate[i] < kLowestGate ? kLowestGate : (double)gate[i];
+      const double pair = gg[0] + gg[1];
+      double run = pair;
       for (int d = 1; d < 32; d <<= 1) {
         const double o = __shfl_up_sync(~0u, run, d);
         if (lane >= d) run += o;
       }
-      const double before = run - s1, last = __shfl_sync(~0u, run, 31);
-      s0 += before;
-      s1 += before;
-      G[2 * lane] = s0;
-      G[2 * lane + 1] = s1;
-      rec->G[2 * lane] = s0;
-      rec->G[2 * lane + 1] = s1;
+      const double before = run - pair, last = __shfl_sync(~0u, run, 31), s0 = before + gg[0], s1 = before + pair;
+      *reinterpret_cast<double2 *>(G + 2 * lane) = make_double2(s0, s1);
+      *reinterpret_cast<double2 *>(rec->G + 2 * lane) = make_double2(s0, s1);
       *reinterpret_cast<float2 *>(rec->gamma + 2 * lane) = make_float2(expf((float)s0), expf((float)s1));
       *reinterpret_cast<float2 *>(rec->closing + 2 * lane) = make_float2(expf((float)(last - s0)), expf((float)(last - s1)));
-      *reinterpret_cast<float2 *>(rec->beta + 2 * lane) = make_float2(be[0], be[1]);
+      *reinterpret_cast<float2 *>(rec->beta + 2 * lane) = make_float2(write[0], write[1]);
+      *reinterpret_cast<float2 *>(beta + 2 * lane) = make_float2(write[0], write[1]);
+      if (hs + 1 < share) fetch(h + 1);
+    }
+    __syncthreads();  // (also: k and q have been read)
+    if (tid < L) {
+      const float x = expf((float)(G[tid] - (tid < 16 ? 0.0 : G[(tid & ~15) - 1])));
+      rise[tid] = rec->rise[tid] = x;
+    }
+    if (tid < 96) {
+      const int i = tid < 16 ? 1 : tid < 48 ? 2 : 3;
+      const float x = expf((float)(G[16 * i - 1] - G[tid - fall_at(i)]));
+      fall[tid] = rec->fall[tid] = x;
     }
     __syncthreads();
 
@@ -163,10 +177,11 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
     for (int j = 0; j < 8; ++j)
       if (j <= 2 * warp + 1) {
         float m[4];
+        const bool diagonal = j >= 2 * warp;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 16 * warp + g + (i >> 1) * 8, c = 8 * j + 2 * q + (i & 1);
-          const float dec = c <= r ? expf((float)(G[r] - G[c])) : 0.f;
+          const float dec = !diagonal ? rise[r] * fall[fall_at(warp) + c] : c <= r ? expf((float)(G[r] - G[c])) : 0.f;
           pp[j][i] = c <= r ? dec * qk[j][i] : 0.f;
           m[i] = c < r ? dec * kk[j][i] * beta[c] : 0.f;
         }
@@ -176,20 +191,30 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
     const unsigned mp = __reduce_max_sync(~0u, max_mag(pp));
     if (lane == 0) tops[warp] = mp;
     __syncwarp();
-    // this warp's diagonal block, inverted in place: column `lane` by forward substitution
-    if (lane < 16) {
+    // this warp's diagonal block, inverted in place: a column per lane by forward substitution (two lanes do the same one)
+    {
       float *D = A + 16 * warp * kAld + 16 * warp;
+      const int col = lane & 15;
       float x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float s = i == lane ? 1.f : 0.f;
+        float s = i == col ? 1.f : 0.f, s2 = 0.f;
 #pragma unroll
-        for (int m = 0; m < i; ++m) s = fmaf(-D[i * kAld + m], x[m], s);
-        x[i] = i < lane ? 0.f : s;
+        for (int m = 0; m < i; m += 4) {
+          const float4 d = *reinterpret_cast<const float4 *>(D + i * kAld + m);
+          s = fmaf(-d.x, x[m], s);
+          if (m + 1 < i) s2 = fmaf(-d.y, x[m + 1], s2);
+          if (m + 2 < i) s = fmaf(-d.z, x[m + 2], s);
+          if (m + 3 < i) s2 = fmaf(-d.w, x[m + 3], s2);
+        }
+        x[i] = i < col ? 0.f : s + s2;
       }
-      __syncwarp(0xffffu);
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) D[i * kAld + lane] = x[i];
+      for (int i = 0; i < 8; ++i) {
+        const int r = lane < 16 ? i : i + 8;
+        D[r * kAld + col] = lane < 16 ? x[i] : x[i + 8];
+      }
     }
     __syncthreads();
 
@@ -198,17 +223,15 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
     {
       const float s = pow2(-eQ);
       const int ld = tri_ld(warp);
-      __half *at = tri + 2 * kTri + tri_base(warp) + g * ld + 2 * q;
+      __half *at = tri + 2 * kTri + tri_base(warp) + (lane & 15) * ld + (lane >> 4) * 8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j <= 2 * warp + 1)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t hi, lo;
-            split<2>(pp[j][2 * i] * s, pp[j][2 * i + 1] * s, &hi, &lo);
-            *reinterpret_cast<uint32_t *>(at + i * 8 * ld + 8 * j) = hi;
-            *reinterpret_cast<uint32_t *>(at + kTri + i * 8 * ld + 8 * j) = lo;
-          }
+      for (int j = 0; j < 8; j += 2)
+        if (j <= 2 * warp) {
+          Frag<2> f;
+          frag_of<2>(f, pp[j], pp[j + 1], s);
+          stsm(smem_addr(at + 8 * j), f.r[0]);
+          stsm(smem_addr(at + kTri + 8 * j), f.r[1]);
+        }
     }
 
     // block column `warp` of Tm, transposed: x[m] rows are the column's 16 columns, columns its rows 16 m .. + 15
@@ -243,22 +266,19 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
       const float s = pow2(-eT);
 #pragma unroll
       for (int m = 0; m < 4; ++m)
-        if (m >= warp)
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y = x[m][nt][e] * s;
-              __half *at = tri + tri_base(m) + (8 * nt + 2 * q + (e & 1)) * tri_ld(m) + 16 * warp + g + (e >> 1) * 8;
-              const __half hi = __float2half_rn(y);
-              at[0] = hi;
-              at[kTri] = __float2half_rn(y - __half2float(hi));
-            }
+        if (m >= warp) {
+          Frag<2> f;
+          frag_of<2>(f, x[m][0], x[m][1], s);
+          __half *at = tri + tri_base(m) + ((lane & 7) + (lane >> 4) * 8) * tri_ld(m) + 16 * warp + ((lane >> 3) & 1) * 8;
+          stsm_t(smem_addr(at), f.r[0]);
+          stsm_t(smem_addr(at + kTri), f.r[1]);
+        }
     }
     __syncthreads();
     uint4 *dst = reinterpret_cast<uint4 *>(rec);
     const uint4 *src = reinterpret_cast<const uint4 *>(tri);
-    for (int i = tid; i < 4 * kTri / 8; i += kThreads) dst[i] = src[i];
+#pragma unroll
+    for (int i = 0; i < 4 * kTri / 8 / kThreads; ++i) dst[tid + i * kThreads] = src[tid + i * kThreads];
     if (tid == 0) *reinterpret_cast<int4 *>(&rec->eT) = make_int4(eT, eQ, eq, ek);
     __syncthreads();  // G, beta, A and tri are written again
   }

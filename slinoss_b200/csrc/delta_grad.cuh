@@ -17,11 +17,11 @@
 namespace slx {
 namespace delta {
 
-constexpr int kGld = 72;  // halves per row of the token-major tiles of 64 value channels
+constexpr int kVectorBytes = 3 * L * 4 + L * 4 + 96 * 4 + L * 8;  // gamma .. G of the record
 
 template <int NT, int SI, int SC>
 constexpr int grad_smem() {
-  return 2 * SI * L * (NT + 8) * 2 + (SI + 2 * SC) * L * kGld * 2 + 2 * SC * 64 * (NT + 8) * 2;
+  return 2 * Operand<SI, NT>::halves * 2 + (SI + 2 * SC) * kTile * 2 + 2 * SC * 64 * (NT + 8) * 2 + kVectorBytes;
 }
 
 // sum over n of the rows' accumulators times the operand tile's rows (16 of them from `tile`); both rows of the thread
@@ -48,258 +48,226 @@ __device__ __forceinline__ float2 row_dots(const float (&c)[NT / 8][4], const __
   return make_float2(x * f, y * f);
 }
 
-// a warp's 16 rows of dq or dk
-template <int NT, typename TI>
-__device__ __forceinline__ void store_grad(const Args &a, void *out, const float (&c)[NT / 8][4], int b, int h, int kh, int t0,
-                                           int rows) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, warp = threadIdx.x >> 5;
-  const bool shared = a.heads != a.key_heads;
-  const size_t row0 = ((size_t)(shared ? b * a.heads + h : b * a.key_heads + kh)) * a.T + t0;
+// A warp's 16 rows of dq or dk, from accumulators: half types through `buf` (16 x (NT + 8) halves of the warp's own) in
+// 16-byte pieces, fp32 (also where heads share their keys and the sums are still to be added up) directly.
+template <int NT, typename TO>
+__device__ __forceinline__ void store_grad(TO *out, const float (&c)[NT / 8][4], int rows, int N, __half *buf) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  if constexpr (sizeof(TO) == 4) {
+    const bool pairs = (N & 1) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int t = 16 * warp + g + 8 * i;
-    if (t >= rows) continue;
+    for (int i = 0; i < 2; ++i) {
+      const int t = g + 8 * i;
+      if (t >= rows) continue;
+      TO *o = out + (size_t)t * N;
 #pragma unroll
-    for (int j = 0; j < NT / 8; ++j) {
-      const int n = 8 * j + 2 * q;
-      const float x = c[j][2 * i], y = c[j][2 * i + 1];
-      const size_t at = (row0 + t) * a.N + n;
-      if (shared) {
-        float *o = static_cast<float *>(out) + at;
-        if (n < a.N) o[0] = x;
-        if (n + 1 < a.N) o[1] = y;
-      } else {
-        TI *o = static_cast<TI *>(out) + at;
-        if (sizeof(TI) == 2 && (a.N & 1) == 0) {
-          if (n < a.N) {
-            const TI pair[2] = {from_f<TI>(x), from_f<TI>(y)};
-            *reinterpret_cast<uint32_t *>(o) = *reinterpret_cast<const uint32_t *>(pair);
-          }
+      for (int j = 0; j < NT / 8; ++j) {
+        const int n = 8 * j + 2 * q;
+        if (pairs) {
+          if (n < N) *reinterpret_cast<float2 *>(o + n) = make_float2(c[j][2 * i], c[j][2 * i + 1]);
         } else {
-          if (n < a.N) o[0] = from_f<TI>(x);
-          if (n + 1 < a.N) o[1] = from_f<TI>(y);
+          if (n < N) o[n] = c[j][2 * i];
+          if (n + 1 < N) o[n + 1] = c[j][2 * i + 1];
         }
       }
     }
+  } else {
+    constexpr int ld = NT + 8;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < NT / 8; j += 2) {
+      uint32_t r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = c[j + (i >> 1)][(i & 1) * 2], y = c[j + (i >> 1)][(i & 1) * 2 + 1];
+        if constexpr (std::is_same<TO, __half>::value) r[i] = pack(x, y);
+        else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+          r[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+      }
+      stsm(smem_addr(buf + (lane & 15) * ld + 8 * j + (lane >> 4) * 8), r);
+    }
+    __syncwarp();
+    if ((N & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < NT / 16; ++i) {
+        const int t = (i * 32 + lane) / (NT / 8), n = (i * 32 + lane) % (NT / 8) * 8;
+        if (t < rows && n < N)
+          *reinterpret_cast<uint4 *>(out + (size_t)t * N + n) = *reinterpret_cast<const uint4 *>(buf + t * ld + n);
+      }
+    } else {
+      for (int i = lane; i < 16 * NT; i += 32) {
+        const int t = i / NT, n = i % NT;
+        if (t < rows && n < N) out[(size_t)t * N + n] = reinterpret_cast<const TO *>(buf)[t * ld + n];
+      }
+    }
+    __syncwarp();
   }
 }
 
-__device__ __forceinline__ void rescale8(__half *at, int diff) {  // eight halves times 2^diff, diff < 0
-  const __half2 f = __float2half2_rn(pow2(diff));
-  uint4 x = *reinterpret_cast<uint4 *>(at);
-  __half2 *w = reinterpret_cast<__half2 *>(&x);
+template <int S>
+__device__ __forceinline__ Frag<S> scaled(const Frag<S> &f, int diff) {  // times 2^diff, diff <= 0
+  const __half2 m = __float2half2_rn(pow2(diff));
+  Frag<S> r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = __hmul2(w[i], f);
-  *reinterpret_cast<uint4 *>(at) = x;
-}
-__device__ __forceinline__ int top_exp(const int *e, int n) {
-  int m = __ldg(e);
-  for (int i = 1; i < n; ++i) m = max(m, __ldg(e + i));
-  return m;
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&f.r[s][i]), m);
+      r.r[s][i] = *reinterpret_cast<const uint32_t *>(&x);
+    }
+  return r;
 }
 
 template <int NT, int SI, int SC, typename TI>
 __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
-  using Op = Operand<TI, SI, NT>;
-  using Oo = Operand<TI, SI, 64>;
-  static_assert(Oo::ld == kGld, "tiles of value channels share one layout");
-  constexpr int ld = NT + 8, xplane = L * kGld, splane = 64 * ld;
+  using Op = Operand<SI, NT>;
+  constexpr int ld = NT + 8, splane = 64 * ld;
   extern __shared__ __align__(128) char smem[];
-  __half *qs = reinterpret_cast<__half *>(smem), *ks = qs + SI * Op::plane;
-  __half *os = ks + SI * Op::plane, *xs = os + SI * xplane, *ys = xs + SC * xplane;
-  __half *ss = ys + SC * xplane, *rs = ss + SC * splane;
-  __shared__ double G[L];
-  __shared__ float gamma[L], closing[L], beta[L], dGs[L], dbs[L], wsum[L], dots[4];
+  __half *ks = reinterpret_cast<__half *>(smem), *qs = ks + Op::halves;
+  __half *os = qs + Op::halves, *xs = os + SI * kTile, *ys = xs + SC * kTile;  // tokens x channels: dO, dX, Y
+  __half *ss = ys + SC * kTile, *rs = ss + SC * splane;                          // channels x N: S0, R
+  float *gamma = reinterpret_cast<float *>(rs + SC * splane), *closing = gamma + L, *beta = closing + L;
+  float *rise = beta + L, *fall = rise + L;
+  double *G = reinterpret_cast<double *>(fall + 96);
+  __shared__ float dGs[L], dbs[L], wsum[L], dots[4];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int chunk = blockIdx.x, bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads, kh = h / (a.heads / a.key_heads);
   const int t0 = chunk * L, rows = min(L, a.T - t0), PB = a.P16 / 16, tiles = (a.P16 + 63) / 64;
   const size_t at = (size_t)bh * a.NC + chunk;
   const Record *rec = a.rec + at;
-  const int eq = rec->eq, ek = rec->ek;
-  const int es = top_exp(a.est + at * PB, PB), er = top_exp(a.eds + at * PB, PB), ey = top_exp(a.ey + at * PB, PB),
-            ex = top_exp(a.edx + at * PB, PB), eo = top_exp(a.edo + at * PB, PB);
 
-  if (tid < L) {
-    G[tid] = rec->G[tid];
-    gamma[tid] = rec->gamma[tid];
-    closing[tid] = rec->closing[tid];
-    beta[tid] = rec->beta[tid];
+  // Tiles of channels come with an exponent per 16 of them.  Where channels are summed over, the A operand of a block takes
+  // what its two exponents lie below the largest such sum.  Lane l holds those of block l.
+  const int none = -100000;
+  int es = none, er = none, ey = none, ex = none, eo = none;
+  if (lane < PB) {
+    es = __ldg(a.est + at * PB + lane);
+    er = __ldg(a.eds + at * PB + lane);
+    ey = __ldg(a.ey + at * PB + lane);
+    ex = __ldg(a.edx + at * PB + lane);
+    eo = __ldg(a.edo + at * PB + lane);
   }
-  Op::issue(qs, head_base<TI>(a.q, b, kh, t0), a.q.st, rows, a.N, a.q.vec, eq);
-  Op::issue(ks, head_base<TI>(a.k, b, kh, t0), a.k.st, rows, a.N, a.k.vec, ek);
+  const int eq = rec->eq, ek = rec->ek;
 
-  // value channels 64 pt .. + 63: dO, dX and Y (tokens x channels), S0 and R (channels x N), each brought to one exponent
-  bool first = true;
-  auto load = [&](int pt) {
-    const int w = min(64, a.P16 - 64 * pt);
-    Oo::issue(os, head_base<TI>(a.dO, b, h, t0) + 64 * pt, a.dO.st, rows, a.P - 64 * pt, a.dO.vec, eo);
-    for (int i = tid; i < SC * L * 8; i += kThreads) {
-      const int pl = i / (L * 8), r = (i / 8) % L, c = (i % 8) * 8;
-      const size_t src = ((at * SC + pl) * L + r) * a.P16 + 64 * pt + c;
-      cp16(xs + pl * xplane + r * kGld + c, a.dx + (c < w ? src : 0), c < w);
-      cp16(ys + pl * xplane + r * kGld + c, a.y + (c < w ? src : 0), c < w);
+  // value channels 64 pt .. + 63: dO, dX and Y (tokens x channels), S0 and R (channels x N)
+  const int eo_top = __reduce_max_sync(~0u, eo);
+  auto load = [&](int pt, bool with_keys) {
+    if (with_keys) {
+      copy_bytes<2 * Op::halves * 2>(ks, a.kq + ((size_t)(b * a.key_heads + kh) * a.NC + chunk) * 2 * Op::halves);
+      copy_bytes<kVectorBytes>(gamma, rec->gamma);
     }
-    for (int i = tid; i < SC * 64 * (NT / 8); i += kThreads) {
-      const int pl = i / (64 * (NT / 8)), r = (i / (NT / 8)) % 64, c = (i % (NT / 8)) * 8;
-      const size_t src = ((at * SC + pl) * a.P16 + 64 * pt + r) * NT + c;
-      cp16(ss + pl * splane + r * ld + c, a.st + (r < w ? src : 0), r < w);
-      cp16(rs + pl * splane + r * ld + c, a.ds + (r < w ? src : 0), r < w);
+    const int w = min(64, a.P16 - 64 * pt);
+#pragma unroll
+    for (int s = 0; s < SC; ++s) {
+      const size_t tile = ((at * SC + s) * tiles + pt) * kTile, state = ((at * SC + s) * a.P16 + 64 * pt) * ld;
+      copy_bytes<kTile * 2>(xs + s * kTile, a.dx + tile);
+      copy_bytes<kTile * 2>(ys + s * kTile, a.y + tile);
+      if (w == 64) {
+        copy_bytes<splane * 2>(ss + s * splane, a.st + state);
+        copy_bytes<splane * 2>(rs + s * splane, a.ds + state);
+      } else {
+        for (int i = tid * 8; i < w * ld; i += kThreads * 8) {
+          cp16(ss + s * splane + i, a.st + state + i, true);
+          cp16(rs + s * splane + i, a.ds + state + i, true);
+        }
+      }
     }
     cp_commit();
+    Pieces<TI, 64> o;
+    o.load(head_base<TI>(a.dO, b, h, t0) + 64 * pt, a.dO.st, rows, a.P - 64 * pt, a.dO.vec);
+    o.template store<SI, false>(os, nullptr, eo_top);
     cp_wait<0>();
-    if (first) {
-      Op::finish(qs, a.q.vec, eq);
-      Op::finish(ks, a.k.vec, ek);
-      first = false;
-    }
-    Oo::finish(os, a.dO.vec, eo);
-    for (int i = tid; i < SC * L * 8; i += kThreads) {
-      const int pl = i / (L * 8), r = (i / 8) % L, c = (i % 8) * 8;
-      if (c < w) {
-        const int dx = __ldg(a.edx + at * PB + 4 * pt + c / 16) - ex, dy = __ldg(a.ey + at * PB + 4 * pt + c / 16) - ey;
-        if (dx) rescale8(xs + pl * xplane + r * kGld + c, dx);
-        if (dy) rescale8(ys + pl * xplane + r * kGld + c, dy);
-      }
-    }
-    for (int i = tid; i < SC * 64 * (NT / 8); i += kThreads) {
-      const int pl = i / (64 * (NT / 8)), r = (i / (NT / 8)) % 64, c = (i % (NT / 8)) * 8;
-      if (r < w) {
-        const int d1 = __ldg(a.est + at * PB + 4 * pt + r / 16) - es, d2 = __ldg(a.eds + at * PB + 4 * pt + r / 16) - er;
-        if (d1) rescale8(ss + pl * splane + r * ld + c, d1);
-        if (d2) rescale8(rs + pl * splane + r * ld + c, d2);
-      }
-    }
     __syncthreads();
   };
   auto blocks = [&](int pt) { return min(64, a.P16 - 64 * pt) / 16; };
+  auto below = [&](int e, int top, int pt, int kb) { return __shfl_sync(~0u, e, 4 * pt + kb) - top; };
   const int r0 = 16 * warp + g, r1 = r0 + 8;
   const __half *qrow = qs + 16 * warp * ld, *krow = ks + 16 * warp * ld;
-  auto load_a = [&](uint32_t (&r)[4], const __half *tile, int kb) { a_mk(r, tile + 16 * warp * kGld + 16 * kb, kGld); };
+  auto load_a = [&](auto &f, const __half *tile, int kb) {
+    constexpr int S = sizeof(f.r) / 16;
+#pragma unroll
+    for (int s = 0; s < S; ++s) a_mk(f.r[s], tile + s * kTile + 16 * warp * kTileLd + 16 * kb, kTileLd);
+  };
+  // decay from an earlier token c to a later one r of the block of 16 tokens `rb`
+  auto decay = [&](int r, int c, int rb, int cb) {
+    return rb == cb ? expf((float)(G[r] - G[c])) : rise[r] * fall[fall_at(rb) + c];
+  };
 
-  float acc[NT / 8][4], dot = 0.f;
-  float2 qdq;
-  // ---- dq
-  {
-    float Q[8][4];
-    zero(Q);
-    zero(acc);
-    for (int pt = 0; pt < tiles; ++pt) {
-      if (pt) __syncthreads();
-      load(pt);
-      for (int kb = 0; kb < blocks(pt); ++kb) {
-        Frag<SI> fo;
-#pragma unroll
-        for (int s = 0; s < SI; ++s) load_a(fo.r[s], os + s * xplane, kb);
-        uint32_t bb[SC][4];
-#pragma unroll
-        for (int sb = 0; sb < 4; ++sb)
-          if (sb <= warp) {
-#pragma unroll
-            for (int s = 0; s < SC; ++s) b_nk(bb[s], ys + s * xplane + 16 * sb * kGld + 16 * kb, kGld);
-            mma_split<SI, SC>(Q[2 * sb], Q[2 * sb + 1], fo, bb);
-          }
-#pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-#pragma unroll
-          for (int s = 0; s < SC; ++s) b_kn(bb[s], ss + s * splane + 16 * kb * ld + 16 * nb, ld);
-          mma_split<SI, SC>(acc[2 * nb], acc[2 * nb + 1], fo, bb);
-        }
-      }
-      for (int i = tid; i < blocks(pt) * 16 * (NT / 2); i += kThreads) {
-        const int r = i / (NT / 2), c = (i % (NT / 2)) * 2;
-        float2 x = make_float2(0.f, 0.f), y = x;
-#pragma unroll
-        for (int s = 0; s < SC; ++s) {
-          const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(ss + s * splane + r * ld + c));
-          const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(rs + s * splane + r * ld + c));
-          x.x += u.x;
-          x.y += u.y;
-          y.x += v.x;
-          y.y += v.y;
-        }
-        dot = fmaf(x.x, y.x, fmaf(x.y, y.y, dot));
-      }
-    }
-    const float f = a.scale * pow2(eo + ey);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i < 2 ? r0 : r1, c = 8 * j + 2 * q + (i & 1);
-        Q[j][i] = j <= 2 * warp + 1 && c <= r ? Q[j][i] * f * expf((float)(G[r] - G[c])) * beta[c] : 0.f;
-      }
-    const float fs = a.scale * pow2(eo + es);
-    times_rows(acc, gamma[r0] * fs, gamma[r1] * fs);
-    const int e = floor_exp(warp_exp(Q), warp_exp(acc), ek);
-    times(acc, pow2(-(e + ek)));
-    const float s = pow2(-e);
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-      if (kb <= warp) {
-        Frag<SC> fq;
-        frag_of<SC>(fq, Q[2 * kb], Q[2 * kb + 1], s);
-#pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-          uint32_t bb[SI][4];
-#pragma unroll
-          for (int s2 = 0; s2 < SI; ++s2) b_kn(bb[s2], ks + s2 * Op::plane + 16 * kb * ld + 16 * nb, ld);
-          mma_split<SC, SI>(acc[2 * nb], acc[2 * nb + 1], fq, bb);
-        }
-      }
-    times(acc, pow2(e + ek));
-    store_grad<NT, TI>(a, a.dq, acc, b, h, kh, t0, rows);
-    qdq = row_dots<NT, SI>(acc, qrow, eq);
-  }
-  // ---- Z
+  float acc[NT / 8][4];
+  // ---- Z, this warp's tokens as s
   float2 w, db;
+  float dot = 0.f;
   {
     float Q[8][4], H[8][4];
     zero(Q);
     zero(H);
     zero(acc);
+    const int yo = ey, yx = ey + ex, yr = ey + er, sr = es + er;
+    const int yo_top = __reduce_max_sync(~0u, yo), yx_top = __reduce_max_sync(~0u, yx), yr_top = __reduce_max_sync(~0u, yr),
+              sr_top = __reduce_max_sync(~0u, sr);
     for (int pt = 0; pt < tiles; ++pt) {
-      if (tiles > 1) {
-        __syncthreads();
-        load(pt);
-      }
+      if (pt) __syncthreads();
+      load(pt, pt == 0);
+#pragma unroll 1
       for (int kb = 0; kb < blocks(pt); ++kb) {
         Frag<SC> fy;
-#pragma unroll
-        for (int s = 0; s < SC; ++s) load_a(fy.r[s], ys + s * xplane, kb);
+        load_a(fy, ys, kb);
+        const Frag<SC> f1 = scaled(fy, below(yo, yo_top, pt, kb)), f2 = scaled(fy, below(yx, yx_top, pt, kb));
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb)
           if (tb >= warp) {
             uint32_t bo[SI][4], bx[SC][4];
 #pragma unroll
-            for (int s = 0; s < SI; ++s) b_nk(bo[s], os + s * xplane + 16 * tb * kGld + 16 * kb, kGld);
-            mma_split<SC, SI>(Q[2 * tb], Q[2 * tb + 1], fy, bo);
+            for (int s = 0; s < SI; ++s) b_nk(bo[s], os + s * kTile + 16 * tb * kTileLd + 16 * kb, kTileLd);
 #pragma unroll
-            for (int s = 0; s < SC; ++s) b_nk(bx[s], xs + s * xplane + 16 * tb * kGld + 16 * kb, kGld);
-            mma_split<SC, SC>(H[2 * tb], H[2 * tb + 1], fy, bx);
+            for (int s = 0; s < SC; ++s) b_nk(bx[s], xs + s * kTile + 16 * tb * kTileLd + 16 * kb, kTileLd);
+            mma_split<SC, SI>(Q[2 * tb], Q[2 * tb + 1], f1, bo);
+            mma_split<SC, SC>(H[2 * tb], H[2 * tb + 1], f2, bx);
           }
+        tile_cols<SC, SC, NT>(acc, scaled(fy, below(yr, yr_top, pt, kb)), rs, splane, kb);
+      }
+      // <R, S0>
+#pragma unroll 2
+      for (int n = 0; n < blocks(pt) * 16 * (NT / 8) / kThreads; ++n) {
+        const int i = n * kThreads + tid, r = i / (NT / 8), c = i % (NT / 8) * 8;
+        float x[8] = {0.f}, y[8] = {0.f}, d = 0.f;
 #pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-          uint32_t bb[SC][4];
+        for (int s = 0; s < SC; ++s) {
+          const uint4 u = *reinterpret_cast<const uint4 *>(ss + s * splane + r * ld + c);
+          const uint4 v = *reinterpret_cast<const uint4 *>(rs + s * splane + r * ld + c);
+          const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, vv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int s = 0; s < SC; ++s) b_kn(bb[s], rs + s * splane + 16 * kb * ld + 16 * nb, ld);
-          mma_split<SC, SC>(acc[2 * nb], acc[2 * nb + 1], fy, bb);
+          for (int m = 0; m < 4; ++m) {
+            const float2 p = unpack(uu[m]), o = unpack(vv[m]);
+            x[2 * m] += p.x;
+            x[2 * m + 1] += p.y;
+            y[2 * m] += o.x;
+            y[2 * m + 1] += o.y;
+          }
         }
+#pragma unroll
+        for (int m = 0; m < 8; ++m) d = fmaf(x[m], y[m], d);
+        dot = fmaf(d, pow2(below(sr, sr_top, pt, r / 16)), dot);
       }
     }
-    const float fr = pow2(ey + er);
+    dot *= pow2(sr_top);
+    const float fr = pow2(yr_top);
     times_rows(acc, closing[r0] * fr, closing[r1] * fr);
     w = row_dots<NT, SI>(acc, krow, ek);
-    const float fq = a.scale * pow2(ey + eo), fh = -pow2(ey + ex);
+    const float fq = a.scale * pow2(yo_top + eo_top), fh = -pow2(yx_top);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
+      if (j >= 2 * warp)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int s = i < 2 ? r0 : r1, t = 8 * j + 2 * q + (i & 1);
-        const float dec = t >= s ? expf((float)(G[t] - G[s])) : 0.f;
-        Q[j][i] = t >= s ? Q[j][i] * fq * dec : 0.f;
-        H[j][i] = t > s ? H[j][i] * fh * dec : 0.f;
-      }
+        for (int i = 0; i < 4; ++i) {
+          const int s = i < 2 ? r0 : r1, t = 8 * j + 2 * q + (i & 1);
+          const float dec = t >= s ? decay(t, s, j / 2, warp) : 0.f;
+          Q[j][i] = t >= s ? Q[j][i] * fq * dec : 0.f;
+          H[j][i] = t > s ? H[j][i] * fh * dec : 0.f;
+        }
     const int ec = warp_exp(acc), e1 = floor_exp(warp_exp(Q), ec, eq);
     const int e2 = floor_exp(warp_exp(H), max(ec, e1 + eq + 21) + 1, ek);
     times(acc, pow2(-(e1 + eq)));
@@ -309,13 +277,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       if (kb >= warp) {
         Frag<SC> f;
         frag_of<SC>(f, Q[2 * kb], Q[2 * kb + 1], s1);
-#pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-          uint32_t bb[SI][4];
-#pragma unroll
-          for (int s = 0; s < SI; ++s) b_kn(bb[s], qs + s * Op::plane + 16 * kb * ld + 16 * nb, ld);
-          mma_split<SC, SI>(acc[2 * nb], acc[2 * nb + 1], f, bb);
-        }
+        tile_cols<SC, SI, NT>(acc, f, qs, Op::plane, kb);
       }
     times(acc, pow2(e1 + eq - (e2 + ek)));
 #pragma unroll
@@ -323,36 +285,40 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       if (kb >= warp) {
         Frag<SC> f;
         frag_of<SC>(f, H[2 * kb], H[2 * kb + 1], s2);
-#pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-          uint32_t bb[SI][4];
-#pragma unroll
-          for (int s = 0; s < SI; ++s) b_kn(bb[s], ks + s * Op::plane + 16 * kb * ld + 16 * nb, ld);
-          mma_split<SC, SI>(acc[2 * nb], acc[2 * nb + 1], f, bb);
-        }
+        tile_cols<SC, SI, NT>(acc, f, ks, Op::plane, kb);
       }
     times(acc, pow2(e2 + ek));
     db = row_dots<NT, SI>(acc, krow, ek);
     times_rows(acc, beta[r0], beta[r1]);
   }
-  // ---- dk = beta Z - gamma (dX S0) - (H beta) k
+  __syncthreads();  // (R is not read any more: its room takes results on their way out, tile by tile of channels it is loaded again)
+  __half *buf = rs + warp * 16 * ld;
+  const bool shared = a.heads != a.key_heads;
+  const size_t row0 = ((size_t)(shared ? bh : b * a.key_heads + kh) * a.T + t0 + 16 * warp) * a.N;
+  auto store = [&](void *out) {
+    if (shared) store_grad<NT, float>(static_cast<float *>(out) + row0, acc, rows - 16 * warp, a.N, buf);
+    else store_grad<NT, TI>(static_cast<TI *>(out) + row0, acc, rows - 16 * warp, a.N, buf);
+  };
+  // ---- dk = beta Z - gamma (dX S0) - (H beta) k, this warp's tokens as t
   {
     float H[8][4];
     zero(H);
-    // -gamma dX as an operand: gamma (which exceeds one where gates do) and a small dX both enter its exponent
+    const int yx = ey + ex, xt = ex + es;
+    const int yx_top = __reduce_max_sync(~0u, yx), xt_top = __reduce_max_sync(~0u, xt);
+    // -gamma dX as an operand: gamma, which exceeds one where gates do, enters the product's unit
     const int top = __reduce_max_sync(~0u, max(mag(gamma[r0]), mag(gamma[r1])));
-    const int e3 = floor_exp(max((top >> 23) - 127 + 1, 0) + ex, warp_exp(acc), es);
-    times(acc, pow2(-(e3 + es)));
-    const float f0 = -gamma[r0] * pow2(ex - e3), f1 = -gamma[r1] * pow2(ex - e3);
+    const int unit = max(xt_top + max((top >> 23) - 127 + 1, 0), warp_exp(acc) - 40);
+    times(acc, pow2(-unit));
     for (int pt = 0; pt < tiles; ++pt) {
       if (tiles > 1) {
         __syncthreads();
-        load(pt);
+        load(pt, false);
       }
+#pragma unroll 1
       for (int kb = 0; kb < blocks(pt); ++kb) {
         Frag<SC> fx, fg;
-#pragma unroll
-        for (int s = 0; s < SC; ++s) load_a(fx.r[s], xs + s * xplane, kb);
+        load_a(fx, xs, kb);
+        const float f = -pow2(below(xt, unit, pt, kb)), f0 = gamma[r0] * f, f1 = gamma[r1] * f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float2 x = unpack(fx.r[0][i]);
@@ -361,34 +327,30 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
             x.x += y.x;
             x.y += y.y;
           }
-          const float f = i & 1 ? f1 : f0;
-          split<SC>(x.x * f, x.y * f, &fg.r[0][i], &fg.r[SC - 1][i]);
+          split<SC>(x.x * (i & 1 ? f1 : f0), x.y * (i & 1 ? f1 : f0), &fg.r[0][i], &fg.r[SC - 1][i]);
         }
-        uint32_t bb[SC][4];
+        fx = scaled(fx, below(yx, yx_top, pt, kb));
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb)
           if (sb <= warp) {
+            uint32_t bb[SC][4];
 #pragma unroll
-            for (int s = 0; s < SC; ++s) b_nk(bb[s], ys + s * xplane + 16 * sb * kGld + 16 * kb, kGld);
+            for (int s = 0; s < SC; ++s) b_nk(bb[s], ys + s * kTile + 16 * sb * kTileLd + 16 * kb, kTileLd);
             mma_split<SC, SC>(H[2 * sb], H[2 * sb + 1], fx, bb);
           }
-#pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-#pragma unroll
-          for (int s = 0; s < SC; ++s) b_kn(bb[s], ss + s * splane + 16 * kb * ld + 16 * nb, ld);
-          mma_split<SC, SC>(acc[2 * nb], acc[2 * nb + 1], fg, bb);
-        }
+        tile_cols<SC, SC, NT>(acc, fg, ss, splane, kb);
       }
     }
-    times(acc, pow2(e3 + es));
-    const float f = -pow2(ex + ey);
+    times(acc, pow2(unit));
+    const float f = -pow2(yx_top);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
+      if (j <= 2 * warp + 1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i < 2 ? r0 : r1, c = 8 * j + 2 * q + (i & 1);
-        H[j][i] = c < r ? H[j][i] * f * expf((float)(G[r] - G[c])) * beta[c] : 0.f;
-      }
+        for (int i = 0; i < 4; ++i) {
+          const int r = i < 2 ? r0 : r1, c = 8 * j + 2 * q + (i & 1);
+          H[j][i] = c < r ? H[j][i] * f * decay(r, c, warp, j / 2) * beta[c] : 0.f;
+        }
     const int e = floor_exp(warp_exp(H), warp_exp(acc), ek);
     times(acc, pow2(-(e + ek)));
     const float s = pow2(-e);
@@ -397,20 +359,67 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       if (kb <= warp) {
         Frag<SC> fh;
         frag_of<SC>(fh, H[2 * kb], H[2 * kb + 1], s);
-#pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-          uint32_t bb[SI][4];
-#pragma unroll
-          for (int s2 = 0; s2 < SI; ++s2) b_kn(bb[s2], ks + s2 * Op::plane + 16 * kb * ld + 16 * nb, ld);
-          mma_split<SC, SI>(acc[2 * nb], acc[2 * nb + 1], fh, bb);
-        }
+        tile_cols<SC, SI, NT>(acc, fh, ks, Op::plane, kb);
       }
     times(acc, pow2(e + ek));
-    store_grad<NT, TI>(a, a.dk, acc, b, h, kh, t0, rows);
   }
   const float2 kdk = row_dots<NT, SI>(acc, krow, ek);
+  if (tiles > 1) __syncthreads();  // (the last tile's R has been loaded by all threads)
+  store(a.dk);
+  // ---- dq = scale gamma (dO S0) + (Q beta) k
+  {
+    float Q[8][4];
+    zero(Q);
+    zero(acc);
+    const int es_top = __reduce_max_sync(~0u, es), ey_top = __reduce_max_sync(~0u, ey);
+    for (int pt = 0; pt < tiles; ++pt) {
+      if (tiles > 1) {
+        __syncthreads();
+        load(pt, false);
+      }
+#pragma unroll 1
+      for (int kb = 0; kb < blocks(pt); ++kb) {
+        Frag<SI> fo;
+        load_a(fo, os, kb);
+        const Frag<SI> f1 = scaled(fo, below(ey, ey_top, pt, kb));
+#pragma unroll
+        for (int sb = 0; sb < 4; ++sb)
+          if (sb <= warp) {
+            uint32_t bb[SC][4];
+#pragma unroll
+            for (int s = 0; s < SC; ++s) b_nk(bb[s], ys + s * kTile + 16 * sb * kTileLd + 16 * kb, kTileLd);
+            mma_split<SI, SC>(Q[2 * sb], Q[2 * sb + 1], f1, bb);
+          }
+        tile_cols<SI, SC, NT>(acc, scaled(fo, below(es, es_top, pt, kb)), ss, splane, kb);
+      }
+    }
+    const float f = a.scale * pow2(eo_top + ey_top);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j <= 2 * warp + 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i < 2 ? r0 : r1, c = 8 * j + 2 * q + (i & 1);
+          Q[j][i] = c <= r ? Q[j][i] * f * decay(r, c, warp, j / 2) * beta[c] : 0.f;
+        }
+    const float fs = a.scale * pow2(eo_top + es_top);
+    times_rows(acc, gamma[r0] * fs, gamma[r1] * fs);
+    const int e = floor_exp(warp_exp(Q), warp_exp(acc), ek);
+    times(acc, pow2(-(e + ek)));
+    const float s = pow2(-e);
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+      if (kb <= warp) {
+        Frag<SC> fq;
+        frag_of<SC>(fq, Q[2 * kb], Q[2 * kb + 1], s);
+        tile_cols<SC, SI, NT>(acc, fq, ks, Op::plane, kb);
+      }
+    times(acc, pow2(e + ek));
+  }
+  const float2 qdq = row_dots<NT, SI>(acc, qrow, eq);
+  if (tiles > 1) __syncthreads();
+  store(a.dq);
   // ---- gates
-  dot = dot * pow2(es + er);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(~0u, dot, d);
   if (lane == 0) dots[warp] = dot;

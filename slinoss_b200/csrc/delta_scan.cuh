@@ -23,7 +23,7 @@ constexpr int warp_buf() {  // halves: 64 x 24 or 16 x (NT + 8)
 }
 template <int NT, int SI, int SC, typename TI>
 constexpr int scan_smem(bool backward) {
-  return 3 * SI * L * (NT + 8) * 2 + (2 + (backward ? 2 : SC)) * kTri * 2 + kHeadBytes + Raw<TI>::bytes +
+  return 3 * Operand<SI, NT>::halves * 2 + (2 + (backward ? 2 : SC)) * kTri * 2 + kHeadBytes + Raw<TI>::bytes +
          (kThreads / 32) * warp_buf<NT>() * 2;
 }
 
@@ -75,12 +75,12 @@ __device__ __forceinline__ int4 exps_of(const Record *r) { return __ldg(reinterp
 
 template <int NT, int SI, int SC, typename TI>
 __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
-  using Op = Operand<TI, SI, NT>;
+  using Op = Operand<SI, NT>;
   using V = Raw<TI>;
   extern __shared__ __align__(128) char smem[];
   __half *ks = reinterpret_cast<__half *>(smem);  // two buffers
-  __half *qs = ks + 2 * SI * Op::plane;
-  __half *Ts = qs + SI * Op::plane;  // T hi, T lo, planes of P, the record's vectors
+  __half *qs = ks + 2 * Op::halves;
+  __half *Ts = qs + Op::halves;  // T hi, T lo, planes of P, the record's vectors
   __half *Ps = Ts + 2 * kTri;
   float *hd = reinterpret_cast<float *>(Ps + SC * kTri);
   const float *gamma = hd, *closing = hd + L, *beta = hd + 2 * L;
@@ -92,36 +92,32 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
   const int first = blockIdx.x * pw * 16, p0 = first + warp * 16;  // value channels of the CTA, of the warp
   const bool active = warp < pw && p0 < a.P16;
   const Record *rec = a.rec + (size_t)bh * a.NC;
-  const int PB = a.P16 / 16;
+  const int PB = a.P16 / 16, tiles = (a.P16 + 63) / 64;
 
-  auto issue_k = [&](int c, int ek) {
-    Op::issue(ks + (c & 1) * SI * Op::plane, head_base<TI>(a.k, b, kh, c * L), a.k.st, min(L, a.T - c * L), a.N, a.k.vec, ek);
-  };
-  auto issue_rest = [&](int c, int eq) {
-    const int rows = min(L, a.T - c * L);
-    Op::issue(qs, head_base<TI>(a.q, b, kh, c * L), a.q.st, rows, a.N, a.q.vec, eq);
-    copy_bytes(Ts, rec[c].T, (2 + SC) * kTri * 2);
-    copy_bytes(hd, rec[c].gamma, kHeadBytes);
-    V::issue(vs, head_base<TI>(a.v, b, h, c * L) + first, a.v.st, rows, a.P - first, pw * 16, a.v.vec);
+  const __half *kq = a.kq + (size_t)(b * a.key_heads + kh) * a.NC * 2 * Op::halves;
+  auto issue_k = [&](int c) { copy_bytes<Op::halves * 2>(ks + (c & 1) * Op::halves, kq + (size_t)c * 2 * Op::halves); };
+  auto issue_rest = [&](int c) {
+    copy_bytes<Op::halves * 2>(qs, kq + (size_t)(2 * c + 1) * Op::halves);
+    copy_bytes<(2 + SC) * kTri * 2>(Ts, rec[c].T);
+    copy_bytes<kHeadBytes>(hd, rec[c].gamma);
+    V::issue(vs, head_base<TI>(a.v, b, h, c * L) + first, a.v.st, min(L, a.T - c * L), a.P - first, a.v.vec);
   };
 
   float S[NT / 8][4];
   if (active && a.init) load_state<NT>(S, a.init, a.init_dtype, (size_t)bh * a.P * a.N, p0, a.P, a.N);
   else zero(S);
   int4 ex = exps_of(rec);
-  issue_k(0, ex.w);
-  issue_rest(0, ex.z);
+  issue_k(0);
+  issue_rest(0);
   cp_commit();
   for (int c = 0; c < a.NC; ++c) {
     const bool more = c + 1 < a.NC;
     const int4 nx = more ? exps_of(rec + c + 1) : ex;
     const int eT = ex.x, eQ = ex.y, eq = ex.z, ek = ex.w;
-    const __half *kt = ks + (c & 1) * SI * Op::plane;
+    const __half *kt = ks + (c & 1) * Op::halves;
     cp_wait<0>();
-    Op::finish(ks + (c & 1) * SI * Op::plane, a.k.vec, ek);
-    Op::finish(qs, a.q.vec, eq);
     __syncthreads();
-    if (more) issue_k(c + 1, nx.w);
+    if (more) issue_k(c + 1);
     cp_commit();
     Frag<2> fc[4];  // closing beta Y
     int eC = 0;
@@ -130,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
       const int eS = warp_exp(S);
       if (a.st) {
         const size_t at = (size_t)bh * a.NC + c;
-        store_state<SC, NT>(a.st + (at * SC * a.P16 + p0) * NT, (int64_t)a.P16 * NT, S, eS, buf);
+        store_state<SC, NT>(a.st + (at * SC * a.P16 + p0) * (NT + 8), (int64_t)a.P16 * (NT + 8), S, eS, buf);
         if ((threadIdx.x & 31) == 0) a.est[at * PB + p0 / 16] = eS;
       }
       float X[8][4], O[8][4];
@@ -147,16 +143,8 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
           for (int pl = 0; pl < SC; ++pl)
 #pragma unroll
             for (int i = 0; i < 4; ++i) fo.r[pl][i] = f.r[pl][i];
-#pragma unroll
-          for (int tb = 0; tb < 4; ++tb) {
-            uint32_t bb[SI][4];
-#pragma unroll
-            for (int s2 = 0; s2 < SI; ++s2) b_nk(bb[s2], kt + s2 * Op::plane + 16 * tb * Op::ld + 16 * kb, Op::ld);
-            mma_split<2, SI>(X[2 * tb], X[2 * tb + 1], f, bb);
-#pragma unroll
-            for (int s2 = 0; s2 < SI; ++s2) b_nk(bb[s2], qs + s2 * Op::plane + 16 * tb * Op::ld + 16 * kb, Op::ld);
-            mma_split<SC, SI>(O[2 * tb], O[2 * tb + 1], fo, bb);
-          }
+          tile_rows<2, SI, NT>(X, f, kt, kb);
+          tile_rows<SC, SI, NT>(O, fo, qs, kb);
         }
       }
       // X = v - gamma S k
@@ -174,20 +162,13 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
         Frag<2> fx[4];
         frags_of<2>(fx, X, eX);
         zero(X);
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb)
-#pragma unroll
-          for (int kb = 0; kb <= tb; ++kb) {
-            uint32_t bb[2][4];
-            b_nk(bb[0], Ts + tri_base(tb) + 16 * kb, tri_ld(tb));
-            b_nk(bb[1], Ts + kTri + tri_base(tb) + 16 * kb, tri_ld(tb));
-            mma_split<2, 2>(X[2 * tb], X[2 * tb + 1], fx[kb], bb);
-          }
+        tri_rows<2, 2>(X, fx, Ts);
         times(X, pow2(eX + eT));  // Y
       }
       if (a.y) {
         const size_t at = (size_t)bh * a.NC + c;
-        const int e = store_planes<SC>(a.y + at * SC * L * a.P16 + p0, a.P16, (int64_t)L * a.P16, X, buf);
+        const int e = warp_exp(X);
+        store_planes<SC>(a.y + (at * SC * tiles + p0 / 64) * kTile + p0 % 64, kTileLd, tiles * kTile, X, e, buf);
         if ((threadIdx.x & 31) == 0) a.ey[at * PB + p0 / 16] = e;
       }
       times_cols(X, beta, 1.f);
@@ -197,15 +178,7 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
         times(O, pow2(-(eD + eQ)));
         Frag<SC> fd[4];
         frags_of<SC>(fd, X, eD);
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb)
-#pragma unroll
-          for (int kb = 0; kb <= tb; ++kb) {
-            uint32_t bb[SC][4];
-#pragma unroll
-            for (int pl = 0; pl < SC; ++pl) b_nk(bb[pl], Ps + pl * kTri + tri_base(tb) + 16 * kb, tri_ld(tb));
-            mma_split<SC, SC>(O[2 * tb], O[2 * tb + 1], fd[kb], bb);
-          }
+        tri_rows<SC, SC>(O, fd, Ps);
         times(O, a.scale * pow2(eD + eQ));
         store_rows<TI>(static_cast<TI *>(a.o) + ((size_t)bh * a.T + c * L) * a.P + p0, a.P, min(L, a.T - c * L), a.P - p0, O, buf);
       }
@@ -215,19 +188,12 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
       top = gamma[L - 1];
     }
     __syncthreads();
-    if (more) issue_rest(c + 1, nx.z);
+    if (more) issue_rest(c + 1);
     cp_commit();
     if (active) {
       times(S, top * pow2(-(eC + ek)));
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-          uint32_t bb[SI][4];
-#pragma unroll
-          for (int s2 = 0; s2 < SI; ++s2) b_kn(bb[s2], kt + s2 * Op::plane + 16 * kb * Op::ld + 16 * nb, Op::ld);
-          mma_split<2, SI>(S[2 * nb], S[2 * nb + 1], fc[kb], bb);
-        }
+      for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(S, fc[kb], kt, Op::plane, kb);
       times(S, pow2(eC + ek));
     }
     ex = nx;
@@ -238,12 +204,12 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
 
 template <int NT, int SI, int SC, typename TI>
 __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
-  using Op = Operand<TI, SI, NT>;
+  using Op = Operand<SI, NT>;
   using V = Raw<TI>;
   extern __shared__ __align__(128) char smem[];
   __half *ks = reinterpret_cast<__half *>(smem);  // two buffers
-  __half *qs = ks + 2 * SI * Op::plane;
-  __half *Ts = qs + SI * Op::plane;  // T hi, T lo, P hi, P lo, the record's vectors
+  __half *qs = ks + 2 * Op::halves;
+  __half *Ts = qs + Op::halves;  // T hi, T lo, P hi, P lo, the record's vectors
   __half *Ps = Ts + 2 * kTri;
   float *hd = reinterpret_cast<float *>(Ps + 2 * kTri);
   const float *gamma = hd, *closing = hd + L, *beta = hd + 2 * L;
@@ -255,35 +221,33 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
   const int first = blockIdx.x * pw * 16, p0 = first + warp * 16;
   const bool active = warp < pw && p0 < a.P16;
   const Record *rec = a.rec + (size_t)bh * a.NC;
-  const int PB = a.P16 / 16;
+  const int PB = a.P16 / 16, tiles = (a.P16 + 63) / 64;
 
-  auto issue_k = [&](int c, int ek) {
-    Op::issue(ks + (c & 1) * SI * Op::plane, head_base<TI>(a.k, b, kh, c * L), a.k.st, min(L, a.T - c * L), a.N, a.k.vec, ek);
-  };
+  const __half *kq = a.kq + (size_t)(b * a.key_heads + kh) * a.NC * 2 * Op::halves;
+  auto issue_k = [&](int c) { copy_bytes<Op::halves * 2>(ks + (c & 1) * Op::halves, kq + (size_t)c * 2 * Op::halves); };
   auto issue_rest = [&](int c) {
-    copy_bytes(Ts, rec[c].T, 4 * kTri * 2);
-    copy_bytes(hd, rec[c].gamma, kHeadBytes);
-    V::issue(os, head_base<TI>(a.dO, b, h, c * L) + first, a.dO.st, min(L, a.T - c * L), a.P - first, pw * 16, a.dO.vec);
+    copy_bytes<4 * kTri * 2>(Ts, rec[c].T);
+    copy_bytes<kHeadBytes>(hd, rec[c].gamma);
+    V::issue(os, head_base<TI>(a.dO, b, h, c * L) + first, a.dO.st, min(L, a.T - c * L), a.P - first, a.dO.vec);
   };
 
   float R[NT / 8][4];
   if (active && a.d_final) load_state<NT>(R, a.d_final, a.d_final_dtype, (size_t)bh * a.P * a.N, p0, a.P, a.N);
   else zero(R);
   int4 ex = exps_of(rec + a.NC - 1);
-  issue_k(a.NC - 1, ex.w);
+  issue_k(a.NC - 1);
   issue_rest(a.NC - 1);
   cp_commit();
   for (int c = a.NC - 1; c >= 0; --c) {
     const int4 nx = c > 0 ? exps_of(rec + c - 1) : ex;
     const int eT = ex.x, eQ = ex.y, eq = ex.z, ek = ex.w;
-    const __half *kt = ks + (c & 1) * SI * Op::plane;
+    const __half *kt = ks + (c & 1) * Op::halves;
     const int rows = min(L, a.T - c * L);
     cp_wait<0>();
-    Op::finish(ks + (c & 1) * SI * Op::plane, a.k.vec, ek);
     __syncthreads();
-    Op::issue(qs, head_base<TI>(a.q, b, kh, c * L), a.q.st, rows, a.N, a.q.vec, eq);
+    copy_bytes<Op::halves * 2>(qs, kq + (size_t)(2 * c + 1) * Op::halves);
     cp_commit();
-    if (c > 0) issue_k(c - 1, nx.w);
+    if (c > 0) issue_k(c - 1);
     cp_commit();
     Frag<2> f1[4], f2[4];  // scale gamma dO, -gamma dX
     int e1 = 0, e2 = 0;
@@ -291,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
     if (active) {
       const size_t at = (size_t)bh * a.NC + c;
       const int eR = warp_exp(R);
-      store_state<SC, NT>(a.ds + (at * SC * a.P16 + p0) * NT, (int64_t)a.P16 * NT, R, eR, buf);
+      store_state<SC, NT>(a.ds + (at * SC * a.P16 + p0) * (NT + 8), (int64_t)a.P16 * (NT + 8), R, eR, buf);
       float W[8][4], X[8][4], dO[8][4];
       zero(X);
       {
@@ -300,13 +264,7 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
         for (int kb = 0; kb < NT / 16; ++kb) {
           Frag<2> f;
           frag_of<2>(f, R[2 * kb], R[2 * kb + 1], s);
-#pragma unroll
-          for (int tb = 0; tb < 4; ++tb) {
-            uint32_t bb[SI][4];
-#pragma unroll
-            for (int s2 = 0; s2 < SI; ++s2) b_nk(bb[s2], kt + s2 * Op::plane + 16 * tb * Op::ld + 16 * kb, Op::ld);
-            mma_split<2, SI>(X[2 * tb], X[2 * tb + 1], f, bb);
-          }
+          tile_rows<2, SI, NT>(X, f, kt, kb);
         }
       }
       load_cols<TI>(dO, os, warp * 16);
@@ -315,15 +273,7 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
       {
         Frag<SI> fo[4];
         frags_of<SI>(fo, dO, eo);
-#pragma unroll
-        for (int sb = 0; sb < 4; ++sb)
-#pragma unroll
-          for (int kb = sb; kb < 4; ++kb) {
-            uint32_t bb[2][4];
-            b_kn(bb[0], Ps + tri_base(kb) + 16 * sb, tri_ld(kb));
-            b_kn(bb[1], Ps + kTri + tri_base(kb) + 16 * sb, tri_ld(kb));
-            mma_split<SI, 2>(W[2 * sb], W[2 * sb + 1], fo[kb], bb);
-          }
+        tri_cols<SI, 2>(W, fo, Ps);
       }
       // beta dD
       times_cols(X, closing, pow2(eR + ek));
@@ -338,19 +288,12 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
         Frag<2> fx[4];
         frags_of<2>(fx, X, eX);
         zero(W);
-#pragma unroll
-        for (int sb = 0; sb < 4; ++sb)
-#pragma unroll
-          for (int kb = sb; kb < 4; ++kb) {
-            uint32_t bb[2][4];
-            b_kn(bb[0], Ts + tri_base(kb) + 16 * sb, tri_ld(kb));
-            b_kn(bb[1], Ts + kTri + tri_base(kb) + 16 * sb, tri_ld(kb));
-            mma_split<2, 2>(W[2 * sb], W[2 * sb + 1], fx[kb], bb);
-          }
+        tri_cols<2, 2>(W, fx, Ts);
         times(W, pow2(eX + eT));  // dX
       }
       store_rows<TI>(static_cast<TI *>(a.dv) + ((size_t)bh * a.T + c * L) * a.P + p0, a.P, rows, a.P - p0, W, buf);
-      const int exx = store_planes<SC>(a.dx + at * SC * L * a.P16 + p0, a.P16, (int64_t)L * a.P16, W, buf);
+      const int exx = warp_exp(W);
+      store_planes<SC>(a.dx + (at * SC * tiles + p0 / 64) * kTile + p0 % 64, kTileLd, tiles * kTile, W, exx, buf);
       if ((threadIdx.x & 31) == 0) {
         a.eds[at * PB + p0 / 16] = eR;
         a.edx[at * PB + p0 / 16] = exx;
@@ -366,31 +309,16 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
       top = gamma[L - 1];
     }
     cp_wait<1>();
-    Op::finish(qs, a.q.vec, eq);
     __syncthreads();
     if (c > 0) issue_rest(c - 1);
     cp_commit();
     if (active) {
       times(R, top * pow2(-(e1 + eq)));
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-          uint32_t bb[SI][4];
-#pragma unroll
-          for (int s2 = 0; s2 < SI; ++s2) b_kn(bb[s2], qs + s2 * Op::plane + 16 * kb * Op::ld + 16 * nb, Op::ld);
-          mma_split<2, SI>(R[2 * nb], R[2 * nb + 1], f1[kb], bb);
-        }
+      for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(R, f1[kb], qs, Op::plane, kb);
       times(R, pow2(e1 + eq - (e2 + ek)));
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int nb = 0; nb < NT / 16; ++nb) {
-          uint32_t bb[SI][4];
-#pragma unroll
-          for (int s2 = 0; s2 < SI; ++s2) b_kn(bb[s2], kt + s2 * Op::plane + 16 * kb * Op::ld + 16 * nb, Op::ld);
-          mma_split<2, SI>(R[2 * nb], R[2 * nb + 1], f2[kb], bb);
-        }
+      for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(R, f2[kb], kt, Op::plane, kb);
       times(R, pow2(e2 + ek));
     }
     ex = nx;

@@ -24,8 +24,11 @@ static Dims dims_of(const slx_gated_delta_shape *s) {
 }
 static size_t up(size_t n) { return (n + 255) / 256 * 256; }
 static size_t record_bytes(const Dims &d) { return up((size_t)(d.BH * d.NC) * sizeof(Record)); }
-static size_t state_bytes(const Dims &d) { return up((size_t)(d.BH * d.NC * d.planes * d.P16 * d.NT) * 2); }
-static size_t value_bytes(const Dims &d) { return up((size_t)(d.BH * d.NC * d.planes * L * d.P16) * 2); }
+static size_t keys_bytes(const slx_gated_delta_shape *s, const Dims &d) {
+  return up((size_t)s->batch * s->key_heads * d.NC * 2 * (s->dtype == SLX_F32 ? 2 : 1) * L * (d.NT + 8) * 2);
+}
+static size_t state_bytes(const Dims &d) { return up((size_t)(d.BH * d.NC * d.planes * d.P16 * (d.NT + 8)) * 2); }
+static size_t value_bytes(const Dims &d) { return up((size_t)(d.BH * d.NC * d.planes * ((d.P16 + 63) / 64) * kTile) * 2); }
 static size_t exp_bytes(const Dims &d) { return up((size_t)(d.BH * d.NC * d.PB) * 4); }
 static size_t share_bytes(const slx_gated_delta_shape *s) {
   return s->heads == s->key_heads ? 0 : up((size_t)s->batch * s->heads * s->T * s->N * 4);
@@ -60,7 +63,7 @@ static Rows rows_of(const void *p, const int64_t *st, const slx_gated_delta_shap
   return r;
 }
 static Args args_of(const slx_gated_delta_shape *s, const Dims &d, const void *q, const void *k, const void *g,
-                    const void *beta, void *rec) {
+                    const void *beta, void *workspace) {
   Args a{};
   const int size = s->dtype == SLX_F32 ? 4 : 2;
   a.batch = s->batch;
@@ -78,7 +81,8 @@ static Args args_of(const slx_gated_delta_shape *s, const Dims &d, const void *q
   a.k = rows_of(k, s->k_stride, s, s->key_heads, s->N, size);
   a.g = rows_of(g, s->g_stride, s, s->heads, 1, 4);
   a.beta = rows_of(beta, s->beta_stride, s, s->heads, 1, 4);
-  a.rec = static_cast<Record *>(rec);
+  a.rec = static_cast<Record *>(workspace);
+  a.kq = reinterpret_cast<__half *>(static_cast<char *>(workspace) + record_bytes(d));
   return a;
 }
 
@@ -96,7 +100,9 @@ using namespace slx;
 using namespace slx::delta;
 
 extern "C" size_t slx_gated_delta_fwd_workspace_bytes(const slx_gated_delta_shape *s) {
-  return check_shape(s, "gated_delta") == SLX_OK ? record_bytes(dims_of(s)) : 0;
+  if (check_shape(s, "gated_delta") != SLX_OK) return 0;
+  const Dims d = dims_of(s);
+  return record_bytes(d) + keys_bytes(s, d);
 }
 extern "C" size_t slx_gated_delta_residual_bytes(const slx_gated_delta_shape *s) {
   if (check_shape(s, "gated_delta") != SLX_OK) return 0;
@@ -106,7 +112,7 @@ extern "C" size_t slx_gated_delta_residual_bytes(const slx_gated_delta_shape *s)
 extern "C" size_t slx_gated_delta_bwd_workspace_bytes(const slx_gated_delta_shape *s) {
   if (check_shape(s, "gated_delta") != SLX_OK) return 0;
   const Dims d = dims_of(s);
-  return record_bytes(d) + state_bytes(d) + value_bytes(d) + 3 * exp_bytes(d) + 2 * share_bytes(s);
+  return record_bytes(d) + keys_bytes(s, d) + state_bytes(d) + value_bytes(d) + 3 * exp_bytes(d) + 2 * share_bytes(s);
 }
 
 static int check_common(const slx_gated_delta_shape *s, const char *what, const void *workspace, size_t have, size_t need) {
@@ -133,7 +139,8 @@ extern "C" int slx_gated_delta_fwd(const slx_gated_delta_shape *s, const void *q
   SLX_REQUIRE(q && k && v && g && beta, SLX_E_NULL, "gated_delta_fwd: q, k, v, g and beta must not be NULL");
   SLX_REQUIRE(!initial_state || known(initial_dtype), SLX_E_DTYPE, "gated_delta_fwd: unknown initial_dtype %d", initial_dtype);
   const Dims d = dims_of(s);
-  if (const int rc = check_common(s, "gated_delta_fwd", workspace, workspace_bytes, record_bytes(d))) return rc;
+  if (const int rc = check_common(s, "gated_delta_fwd", workspace, workspace_bytes,
+                                  slx_gated_delta_fwd_workspace_bytes(s))) return rc;
   Args a = args_of(s, d, q, k, g, beta, workspace);
   a.v = rows_of(v, s->v_stride, s, s->heads, s->P, s->dtype == SLX_F32 ? 4 : 2);
   a.init = initial_state;
@@ -179,7 +186,7 @@ extern "C" int slx_gated_delta_bwd(const slx_gated_delta_shape *s, const void *q
   a.y = reinterpret_cast<__half *>(r + state_bytes(d));
   a.est = reinterpret_cast<int *>(r + state_bytes(d) + value_bytes(d));
   a.ey = reinterpret_cast<int *>(r + state_bytes(d) + value_bytes(d) + exp_bytes(d));
-  w += record_bytes(d);
+  w += record_bytes(d) + keys_bytes(s, d);
   a.ds = reinterpret_cast<__half *>(w);
   w += state_bytes(d);
   a.dx = reinterpret_cast<__half *>(w);
