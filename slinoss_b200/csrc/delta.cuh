@@ -31,15 +31,17 @@ struct Record {
   __half T[2][kTri];  // Tm, hi and lo
   __half Q[2][kTri];  // P, hi and lo
   float gamma[L], closing[L], beta[L];
-  // dec_ts for t in block i of 16 tokens and s in an earlier one is rise[t] * fall[fall_at(i) + s]: both exponents from G at
-  // the end of block i - 1, so that neither factor leaves the range where gates close
-  float rise[L], fall[96];
-  double G[L];
+  // dec_ts for t and s in the same block of 16 tokens is near[block][t][s]; for t in block i and s in an earlier one it is
+  // rise[t] * fall[fall_at(i) + s]: both exponents from G at the end of block i - 1, so that neither factor leaves the range
+  // where gates close
+  float rise[L], fall[96], near[4][16 * 20];
   int eT, eQ, eq, ek;  // binary exponents: value = stored * 2^e
   int pad[28];
 };
-static_assert(sizeof(Record) == 26624 && sizeof(Record) % 128 == 0, "record layout");
+static_assert(sizeof(Record) == 31232 && sizeof(Record) % 128 == 0, "record layout");
 constexpr int kHeadBytes = 3 * L * 4;  // gamma, closing, beta
+constexpr int kVectorBytes = kHeadBytes + L * 4 + 96 * 4 + 4 * 16 * 20 * 4;  // gamma .. near
+constexpr int kNearLd = 20;
 __host__ __device__ constexpr int fall_at(int i) { return 8 * i * (i - 1); }
 
 struct Rows {  // a (batch, head, token, :) tensor whose last axis is dense; strides in elements
@@ -339,22 +341,25 @@ struct Pieces {
   uint4 x[per];
   static __device__ __forceinline__ int row(int i) { return (i * kThreads + (int)threadIdx.x) / (W / V); }
   static __device__ __forceinline__ int col(int i) { return (i * kThreads + (int)threadIdx.x) % (W / V) * V; }
-  __device__ __forceinline__ void load(const TI *src, int64_t st, int rows, int cols, bool vec) {
+  // (room: as many bytes of shared memory as the tile has, for rows that no 16-byte access fits)
+  __device__ __forceinline__ void load(const TI *src, int64_t st, int rows, int cols, bool vec, void *room) {
+    if (!vec) {
+      TI *raw = static_cast<TI *>(room);
+#pragma unroll 1
+      for (int i = threadIdx.x; i < L * W; i += kThreads) {
+        const int r = i / W, c = i % W;
+        raw[i] = r < rows && c < cols ? src[r * st + c] : from_f<TI>(0.f);
+      }
+      __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < per; ++i) {
       const int r = row(i), c = col(i);
       x[i] = make_uint4(0, 0, 0, 0);
-      if (r < rows && c < cols) {
-        const TI *at = src + r * st + c;
-        if (vec) x[i] = *reinterpret_cast<const uint4 *>(at);
-        else {
-          TI e[V];
-#pragma unroll
-          for (int n = 0; n < V; ++n) e[n] = c + n < cols ? at[n] : from_f<TI>(0.f);
-          memcpy(&x[i], e, 16);
-        }
-      }
+      if (!vec) x[i] = static_cast<const uint4 *>(room)[i * kThreads + threadIdx.x];
+      else if (r < rows && c < cols) x[i] = *reinterpret_cast<const uint4 *>(src + r * st + c);
     }
+    if (!vec) __syncthreads();
   }
   __device__ __forceinline__ unsigned max_bits() const {  // of the largest magnitude, as fp32
     unsigned m = 0;

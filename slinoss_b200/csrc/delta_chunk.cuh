@@ -59,7 +59,7 @@ __device__ __forceinline__ void block_product(float (&c)[2][4], const float (&a)
 }
 
 template <int NT, int SI, typename TI>
-__global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
+__global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_chunk_kernel(Args a) {
   using Op = Operand<SI, NT>;
   using In = Pieces<TI, NT>;
   extern __shared__ __align__(128) char smem[];
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
   __half *tri = reinterpret_cast<__half *>(smem);  // T hi, T lo, P hi, P lo
   float *A = reinterpret_cast<float *>(smem + chunk_tiles<NT, SI>());
   __shared__ double G[L];
-  __shared__ float beta[L], rise[L], fall[96];
+  __shared__ float beta[L], rise[L], fall[96], near[4][16 * kNearLd];
   __shared__ unsigned tops[8];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
   int eq = 0, ek = 0;
   {
     In kx, qx;
-    kx.load(head_base<TI>(a.k, b, kh, t0), a.k.st, rows, a.N, a.k.vec);
-    qx.load(head_base<TI>(a.q, b, kh, t0), a.q.st, rows, a.N, a.q.vec);
+    kx.load(head_base<TI>(a.k, b, kh, t0), a.k.st, rows, a.N, a.k.vec, ks);
+    qx.load(head_base<TI>(a.q, b, kh, t0), a.q.st, rows, a.N, a.q.vec, qs);
     if constexpr (!std::is_same<TI, __half>::value) {
       const unsigned mq = __reduce_max_sync(~0u, qx.max_bits()), mk = __reduce_max_sync(~0u, kx.max_bits());
       if (lane == 0) {
@@ -152,7 +152,6 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
       }
       const double before = run - pair, last = __shfl_sync(~0u, run, 31), s0 = before + gg[0], s1 = before + pair;
       *reinterpret_cast<double2 *>(G + 2 * lane) = make_double2(s0, s1);
-      *reinterpret_cast<double2 *>(rec->G + 2 * lane) = make_double2(s0, s1);
       *reinterpret_cast<float2 *>(rec->gamma + 2 * lane) = make_float2(expf((float)s0), expf((float)s1));
       *reinterpret_cast<float2 *>(rec->closing + 2 * lane) = make_float2(expf((float)(last - s0)), expf((float)(last - s1)));
       *reinterpret_cast<float2 *>(rec->beta + 2 * lane) = make_float2(write[0], write[1]);
@@ -169,6 +168,12 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
       const float x = expf((float)(G[16 * i - 1] - G[tid - fall_at(i)]));
       fall[tid] = rec->fall[tid] = x;
     }
+#pragma unroll 2
+    for (int i = lane; i < 256; i += 32) {  // this warp's block of near pairs
+      const int r = i / 16, c = i % 16;
+      const float x = c <= r ? expf((float)(G[16 * warp + r] - G[16 * warp + c])) : 0.f;
+      near[warp][r * kNearLd + c] = rec->near[warp][r * kNearLd + c] = x;
+    }
     __syncthreads();
 
     float pp[8][4];
@@ -181,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunk_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 16 * warp + g + (i >> 1) * 8, c = 8 * j + 2 * q + (i & 1);
-          const float dec = !diagonal ? rise[r] * fall[fall_at(warp) + c] : c <= r ? expf((float)(G[r] - G[c])) : 0.f;
+          const float dec = diagonal ? near[warp][(r & 15) * kNearLd + (c & 15)] : rise[r] * fall[fall_at(warp) + c];
           pp[j][i] = c <= r ? dec * qk[j][i] : 0.f;
           m[i] = c < r ? dec * kk[j][i] * beta[c] : 0.f;
         }

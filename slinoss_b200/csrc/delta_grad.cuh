@@ -17,11 +17,9 @@
 namespace slx {
 namespace delta {
 
-constexpr int kVectorBytes = 3 * L * 4 + L * 4 + 96 * 4 + L * 8;  // gamma .. G of the record
-
 template <int NT, int SI, int SC>
 constexpr int grad_smem() {
-  return 2 * Operand<SI, NT>::halves * 2 + (SI + 2 * SC) * kTile * 2 + 2 * SC * 64 * (NT + 8) * 2 + kVectorBytes;
+  return 2 * Operand<SI, NT>::halves * 2 + 3 * SC * kTile * 2 + 2 * SC * 64 * (NT + 8) * 2 + kVectorBytes;
 }
 
 // sum over n of the rows' accumulators times the operand tile's rows (16 of them from `tile`); both rows of the thread
@@ -126,11 +124,10 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
   constexpr int ld = NT + 8, splane = 64 * ld;
   extern __shared__ __align__(128) char smem[];
   __half *ks = reinterpret_cast<__half *>(smem), *qs = ks + Op::halves;
-  __half *os = qs + Op::halves, *xs = os + SI * kTile, *ys = xs + SC * kTile;  // tokens x channels: dO, dX, Y
+  __half *os = qs + Op::halves, *xs = os + SC * kTile, *ys = xs + SC * kTile;  // tokens x channels: dO, dX, Y
   __half *ss = ys + SC * kTile, *rs = ss + SC * splane;                          // channels x N: S0, R
   float *gamma = reinterpret_cast<float *>(rs + SC * splane), *closing = gamma + L, *beta = closing + L;
-  float *rise = beta + L, *fall = rise + L;
-  double *G = reinterpret_cast<double *>(fall + 96);
+  float *rise = beta + L, *fall = rise + L, *near = fall + 96;
   __shared__ float dGs[L], dbs[L], wsum[L], dots[4];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
@@ -151,49 +148,48 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     eo = __ldg(a.edo + at * PB + lane);
   }
   const int eq = rec->eq, ek = rec->ek;
+  const int eo_top = __reduce_max_sync(~0u, eo);  // (dO is brought to one exponent as it is read)
+  copy_bytes<2 * Op::halves * 2>(ks, a.kq + ((size_t)(b * a.key_heads + kh) * a.NC + chunk) * 2 * Op::halves);
+  copy_bytes<kVectorBytes>(gamma, rec->gamma);
 
   // value channels 64 pt .. + 63: dO, dX and Y (tokens x channels), S0 and R (channels x N)
-  const int eo_top = __reduce_max_sync(~0u, eo);
-  auto load = [&](int pt, bool with_keys) {
-    if (with_keys) {
-      copy_bytes<2 * Op::halves * 2>(ks, a.kq + ((size_t)(b * a.key_heads + kh) * a.NC + chunk) * 2 * Op::halves);
-      copy_bytes<kVectorBytes>(gamma, rec->gamma);
-    }
+  auto load = [&](int pt) {
     const int w = min(64, a.P16 - 64 * pt);
 #pragma unroll
     for (int s = 0; s < SC; ++s) {
       const size_t tile = ((at * SC + s) * tiles + pt) * kTile, state = ((at * SC + s) * a.P16 + 64 * pt) * ld;
       copy_bytes<kTile * 2>(xs + s * kTile, a.dx + tile);
       copy_bytes<kTile * 2>(ys + s * kTile, a.y + tile);
-      if (w == 64) {
-        copy_bytes<splane * 2>(ss + s * splane, a.st + state);
-        copy_bytes<splane * 2>(rs + s * splane, a.ds + state);
-      } else {
-        for (int i = tid * 8; i < w * ld; i += kThreads * 8) {
-          cp16(ss + s * splane + i, a.st + state + i, true);
-          cp16(rs + s * splane + i, a.ds + state + i, true);
-        }
+#pragma unroll 1
+      for (int i = tid * 8; i < w * ld; i += kThreads * 8) {
+        cp16(ss + s * splane + i, a.st + state + i, true);
+        cp16(rs + s * splane + i, a.ds + state + i, true);
       }
     }
     cp_commit();
     Pieces<TI, 64> o;
-    o.load(head_base<TI>(a.dO, b, h, t0) + 64 * pt, a.dO.st, rows, a.P - 64 * pt, a.dO.vec);
+    o.load(head_base<TI>(a.dO, b, h, t0) + 64 * pt, a.dO.st, rows, a.P - 64 * pt, a.dO.vec, os);
     o.template store<SI, false>(os, nullptr, eo_top);
+    if constexpr (SI < SC) {  // (a second plane of zeros: one code for dO and dX)
+      for (int i = tid * 8; i < kTile; i += kThreads * 8) *reinterpret_cast<uint4 *>(os + kTile + i) = make_uint4(0, 0, 0, 0);
+    }
     cp_wait<0>();
     __syncthreads();
   };
-  auto blocks = [&](int pt) { return min(64, a.P16 - 64 * pt) / 16; };
   auto below = [&](int e, int top, int pt, int kb) { return __shfl_sync(~0u, e, 4 * pt + kb) - top; };
   const int r0 = 16 * warp + g, r1 = r0 + 8;
-  const __half *qrow = qs + 16 * warp * ld, *krow = ks + 16 * warp * ld;
-  auto load_a = [&](auto &f, const __half *tile, int kb) {
-    constexpr int S = sizeof(f.r) / 16;
+  const __half *krow = ks + 16 * warp * ld;
+  auto load_a = [&](Frag<SC> &f, const __half *tile, int kb) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) a_mk(f.r[s], tile + s * kTile + 16 * warp * kTileLd + 16 * kb, kTileLd);
+    for (int s = 0; s < SC; ++s) a_mk(f.r[s], tile + s * kTile + 16 * warp * kTileLd + 16 * kb, kTileLd);
   };
-  // decay from an earlier token c to a later one r of the block of 16 tokens `rb`
+  auto load_b = [&](uint32_t (&f)[SC][4], const __half *tile, int rb, int kb) {
+#pragma unroll
+    for (int s = 0; s < SC; ++s) b_nk(f[s], tile + s * kTile + 16 * rb * kTileLd + 16 * kb, kTileLd);
+  };
+  // decay from an earlier token c of block cb to a later one r of block rb (zero where c comes later in the same block)
   auto decay = [&](int r, int c, int rb, int cb) {
-    return rb == cb ? expf((float)(G[r] - G[c])) : rise[r] * fall[fall_at(rb) + c];
+    return rb == cb ? near[rb * 16 * kNearLd + (r & 15) * kNearLd + (c & 15)] : rise[r] * fall[fall_at(rb) + c];
   };
 
   float acc[NT / 8][4];
@@ -205,33 +201,33 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     zero(Q);
     zero(H);
     zero(acc);
-    const int yo = ey, yx = ey + ex, yr = ey + er, sr = es + er;
-    const int yo_top = __reduce_max_sync(~0u, yo), yx_top = __reduce_max_sync(~0u, yx), yr_top = __reduce_max_sync(~0u, yr),
+    const int yx = ey + ex, yr = ey + er, sr = es + er;
+    const int y_top = __reduce_max_sync(~0u, ey), yx_top = __reduce_max_sync(~0u, yx), yr_top = __reduce_max_sync(~0u, yr),
               sr_top = __reduce_max_sync(~0u, sr);
+#pragma unroll 1
     for (int pt = 0; pt < tiles; ++pt) {
       if (pt) __syncthreads();
-      load(pt, pt == 0);
+      load(pt);
+      const int blocks = min(4, PB - 4 * pt);
 #pragma unroll 1
-      for (int kb = 0; kb < blocks(pt); ++kb) {
+      for (int kb = 0; kb < blocks; ++kb) {
         Frag<SC> fy;
         load_a(fy, ys, kb);
-        const Frag<SC> f1 = scaled(fy, below(yo, yo_top, pt, kb)), f2 = scaled(fy, below(yx, yx_top, pt, kb));
+        const Frag<SC> f1 = scaled(fy, below(ey, y_top, pt, kb)), f2 = scaled(fy, below(yx, yx_top, pt, kb));
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb)
           if (tb >= warp) {
-            uint32_t bo[SI][4], bx[SC][4];
-#pragma unroll
-            for (int s = 0; s < SI; ++s) b_nk(bo[s], os + s * kTile + 16 * tb * kTileLd + 16 * kb, kTileLd);
-#pragma unroll
-            for (int s = 0; s < SC; ++s) b_nk(bx[s], xs + s * kTile + 16 * tb * kTileLd + 16 * kb, kTileLd);
-            mma_split<SC, SI>(Q[2 * tb], Q[2 * tb + 1], f1, bo);
+            uint32_t bo[SC][4], bx[SC][4];
+            load_b(bo, os, tb, kb);
+            load_b(bx, xs, tb, kb);
+            mma_split<SC, SC>(Q[2 * tb], Q[2 * tb + 1], f1, bo);
             mma_split<SC, SC>(H[2 * tb], H[2 * tb + 1], f2, bx);
           }
         tile_cols<SC, SC, NT>(acc, scaled(fy, below(yr, yr_top, pt, kb)), rs, splane, kb);
       }
       // <R, S0>
-#pragma unroll 2
-      for (int n = 0; n < blocks(pt) * 16 * (NT / 8) / kThreads; ++n) {
+#pragma unroll 1
+      for (int n = 0; n < blocks * 16 * (NT / 8) / kThreads; ++n) {
         const int i = n * kThreads + tid, r = i / (NT / 8), c = i % (NT / 8) * 8;
         float x[8] = {0.f}, y[8] = {0.f}, d = 0.f;
 #pragma unroll
@@ -257,14 +253,14 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     const float fr = pow2(yr_top);
     times_rows(acc, closing[r0] * fr, closing[r1] * fr);
     w = row_dots<NT, SI>(acc, krow, ek);
-    const float fq = a.scale * pow2(yo_top + eo_top), fh = -pow2(yx_top);
+    const float fq = a.scale * pow2(y_top + eo_top), fh = -pow2(yx_top);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (j >= 2 * warp)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int s = i < 2 ? r0 : r1, t = 8 * j + 2 * q + (i & 1);
-          const float dec = t >= s ? decay(t, s, j / 2, warp) : 0.f;
+          const float dec = decay(t, s, j / 2, warp);
           Q[j][i] = t >= s ? Q[j][i] * fq * dec : 0.f;
           H[j][i] = t > s ? H[j][i] * fh * dec : 0.f;
         }
@@ -291,65 +287,69 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     db = row_dots<NT, SI>(acc, krow, ek);
     times_rows(acc, beta[r0], beta[r1]);
   }
-  __syncthreads();  // (R is not read any more: its room takes results on their way out, tile by tile of channels it is loaded again)
+  __syncthreads();  // (R is not read any more: its room takes results on their way out)
   __half *buf = rs + warp * 16 * ld;
-  const bool shared = a.heads != a.key_heads;
-  const size_t row0 = ((size_t)(shared ? bh : b * a.key_heads + kh) * a.T + t0 + 16 * warp) * a.N;
-  auto store = [&](void *out) {
-    if (shared) store_grad<NT, float>(static_cast<float *>(out) + row0, acc, rows - 16 * warp, a.N, buf);
-    else store_grad<NT, TI>(static_cast<TI *>(out) + row0, acc, rows - 16 * warp, a.N, buf);
-  };
-  // ---- dk = beta Z - gamma (dX S0) - (H beta) k, this warp's tokens as t
-  {
+  // ---- this warp's tokens as t: dk = beta Z + f gamma (dX S0) + f (H beta) k with f = -1, then the same with dO, Q and
+  // f = scale: dq (whose sum starts at zero and has t itself)
+  float2 dots_k = make_float2(0.f, 0.f), dots_q = dots_k;
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {
+    const bool is_q = part == 1;
+    const __half *tile = is_q ? os : xs;
+    const int ea = is_q ? (lane < PB ? eo_top : none) : ex;
+    const float f = is_q ? a.scale : -1.f;
     float H[8][4];
     zero(H);
-    const int yx = ey + ex, xt = ex + es;
-    const int yx_top = __reduce_max_sync(~0u, yx), xt_top = __reduce_max_sync(~0u, xt);
-    // -gamma dX as an operand: gamma, which exceeds one where gates do, enters the product's unit
-    const int top = __reduce_max_sync(~0u, max(mag(gamma[r0]), mag(gamma[r1])));
-    const int unit = max(xt_top + max((top >> 23) - 127 + 1, 0), warp_exp(acc) - 40);
+    if (is_q) zero(acc);
+    const int ya = ey + ea, sa = es + ea;
+    const int ya_top = __reduce_max_sync(~0u, ya), sa_top = __reduce_max_sync(~0u, sa);
+    // f gamma times the tile as an operand: the factor, which exceeds one where gates do, enters the product's unit
+    const float g0 = f * gamma[r0], g1 = f * gamma[r1];
+    const int top = __reduce_max_sync(~0u, max(mag(g0), mag(g1)));
+    const int unit = max(sa_top + max((top >> 23) - 127 + 1, 0), warp_exp(acc) - 40);
     times(acc, pow2(-unit));
+#pragma unroll 1
     for (int pt = 0; pt < tiles; ++pt) {
       if (tiles > 1) {
         __syncthreads();
-        load(pt, false);
+        load(pt);
       }
+      const int blocks = min(4, PB - 4 * pt);
 #pragma unroll 1
-      for (int kb = 0; kb < blocks(pt); ++kb) {
-        Frag<SC> fx, fg;
-        load_a(fx, xs, kb);
-        const float f = -pow2(below(xt, unit, pt, kb)), f0 = gamma[r0] * f, f1 = gamma[r1] * f;
+      for (int kb = 0; kb < blocks; ++kb) {
+        Frag<SC> fa, fg;
+        load_a(fa, tile, kb);
+        const float m = pow2(below(sa, unit, pt, kb)), f0 = g0 * m, f1 = g1 * m;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float2 x = unpack(fx.r[0][i]);
+          float2 x = unpack(fa.r[0][i]);
           if constexpr (SC == 2) {
-            const float2 y = unpack(fx.r[1][i]);
+            const float2 y = unpack(fa.r[1][i]);
             x.x += y.x;
             x.y += y.y;
           }
           split<SC>(x.x * (i & 1 ? f1 : f0), x.y * (i & 1 ? f1 : f0), &fg.r[0][i], &fg.r[SC - 1][i]);
         }
-        fx = scaled(fx, below(yx, yx_top, pt, kb));
+        fa = scaled(fa, below(ya, ya_top, pt, kb));
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb)
           if (sb <= warp) {
             uint32_t bb[SC][4];
-#pragma unroll
-            for (int s = 0; s < SC; ++s) b_nk(bb[s], ys + s * kTile + 16 * sb * kTileLd + 16 * kb, kTileLd);
-            mma_split<SC, SC>(H[2 * sb], H[2 * sb + 1], fx, bb);
+            load_b(bb, ys, sb, kb);
+            mma_split<SC, SC>(H[2 * sb], H[2 * sb + 1], fa, bb);
           }
         tile_cols<SC, SC, NT>(acc, fg, ss, splane, kb);
       }
     }
     times(acc, pow2(unit));
-    const float f = -pow2(yx_top);
+    const float fh = f * pow2(ya_top);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (j <= 2 * warp + 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = i < 2 ? r0 : r1, c = 8 * j + 2 * q + (i & 1);
-          H[j][i] = c < r ? H[j][i] * f * decay(r, c, warp, j / 2) * beta[c] : 0.f;
+          H[j][i] = c < r + part ? H[j][i] * fh * decay(r, c, warp, j / 2) * beta[c] : 0.f;
         }
     const int e = floor_exp(warp_exp(H), warp_exp(acc), ek);
     times(acc, pow2(-(e + ek)));
@@ -357,75 +357,27 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
       if (kb <= warp) {
-        Frag<SC> fh;
-        frag_of<SC>(fh, H[2 * kb], H[2 * kb + 1], s);
-        tile_cols<SC, SI, NT>(acc, fh, ks, Op::plane, kb);
+        Frag<SC> fh2;
+        frag_of<SC>(fh2, H[2 * kb], H[2 * kb + 1], s);
+        tile_cols<SC, SI, NT>(acc, fh2, ks, Op::plane, kb);
       }
     times(acc, pow2(e + ek));
+    dots_k = dots_q;
+    dots_q = row_dots<NT, SI>(acc, (is_q ? qs : ks) + 16 * warp * ld, is_q ? eq : ek);
+    if (tiles > 1) __syncthreads();  // (the last tile's R has been loaded by all threads)
+    const bool shared = a.heads != a.key_heads;
+    const size_t row0 = ((size_t)(shared ? bh : b * a.key_heads + kh) * a.T + t0 + 16 * warp) * a.N;
+    void *out = is_q ? a.dq : a.dk;
+    if (shared) store_grad<NT, float>(static_cast<float *>(out) + row0, acc, rows - 16 * warp, a.N, buf);
+    else store_grad<NT, TI>(static_cast<TI *>(out) + row0, acc, rows - 16 * warp, a.N, buf);
   }
-  const float2 kdk = row_dots<NT, SI>(acc, krow, ek);
-  if (tiles > 1) __syncthreads();  // (the last tile's R has been loaded by all threads)
-  store(a.dk);
-  // ---- dq = scale gamma (dO S0) + (Q beta) k
-  {
-    float Q[8][4];
-    zero(Q);
-    zero(acc);
-    const int es_top = __reduce_max_sync(~0u, es), ey_top = __reduce_max_sync(~0u, ey);
-    for (int pt = 0; pt < tiles; ++pt) {
-      if (tiles > 1) {
-        __syncthreads();
-        load(pt, false);
-      }
-#pragma unroll 1
-      for (int kb = 0; kb < blocks(pt); ++kb) {
-        Frag<SI> fo;
-        load_a(fo, os, kb);
-        const Frag<SI> f1 = scaled(fo, below(ey, ey_top, pt, kb));
-#pragma unroll
-        for (int sb = 0; sb < 4; ++sb)
-          if (sb <= warp) {
-            uint32_t bb[SC][4];
-#pragma unroll
-            for (int s = 0; s < SC; ++s) b_nk(bb[s], ys + s * kTile + 16 * sb * kTileLd + 16 * kb, kTileLd);
-            mma_split<SI, SC>(Q[2 * sb], Q[2 * sb + 1], f1, bb);
-          }
-        tile_cols<SI, SC, NT>(acc, scaled(fo, below(es, es_top, pt, kb)), ss, splane, kb);
-      }
-    }
-    const float f = a.scale * pow2(eo_top + ey_top);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j <= 2 * warp + 1)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i < 2 ? r0 : r1, c = 8 * j + 2 * q + (i & 1);
-          Q[j][i] = c <= r ? Q[j][i] * f * decay(r, c, warp, j / 2) * beta[c] : 0.f;
-        }
-    const float fs = a.scale * pow2(eo_top + es_top);
-    times_rows(acc, gamma[r0] * fs, gamma[r1] * fs);
-    const int e = floor_exp(warp_exp(Q), warp_exp(acc), ek);
-    times(acc, pow2(-(e + ek)));
-    const float s = pow2(-e);
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-      if (kb <= warp) {
-        Frag<SC> fq;
-        frag_of<SC>(fq, Q[2 * kb], Q[2 * kb + 1], s);
-        tile_cols<SC, SI, NT>(acc, fq, ks, Op::plane, kb);
-      }
-    times(acc, pow2(e + ek));
-  }
-  const float2 qdq = row_dots<NT, SI>(acc, qrow, eq);
-  if (tiles > 1) __syncthreads();
-  store(a.dq);
   // ---- gates
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(~0u, dot, d);
   if (lane == 0) dots[warp] = dot;
   if (q == 0) {
-    dGs[r0] = qdq.x + kdk.x - 2.f * beta[r0] * db.x;
-    dGs[r1] = qdq.y + kdk.y - 2.f * beta[r1] * db.y;
+    dGs[r0] = dots_q.x + dots_k.x - 2.f * beta[r0] * db.x;
+    dGs[r1] = dots_q.y + dots_k.y - 2.f * beta[r1] * db.y;
     dbs[r0] = db.x;
     dbs[r1] = db.y;
     wsum[r0] = beta[r0] * w.x;
