@@ -199,6 +199,20 @@ __device__ __forceinline__ void frag_of(Frag<S> &f, const float (&c0)[4], const 
   split<S>(c1[0] * s, c1[1] * s, &f.r[0][2], lo + 2);
   split<S>(c1[2] * s, c1[3] * s, &f.r[0][3], lo + 3);
 }
+template <int S>
+__device__ __forceinline__ Frag<S> scaled(const Frag<S> &f, int diff) {  // times 2^diff, diff <= 0
+  const __half2 m = __float2half2_rn(pow2(diff));
+  Frag<S> r;
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&f.r[s][i]), m);
+      r.r[s][i] = *reinterpret_cast<const uint32_t *>(&x);
+    }
+  return r;
+}
+
 // c0, c1 += A B for the two n8 tiles of B; planes of A and B whose product is below 2^-22 are left out
 template <int SA, int SB>
 __device__ __forceinline__ void mma_split(float (&c0)[4], float (&c1)[4], const Frag<SA> &a, const uint32_t (&b)[SB][4]) {

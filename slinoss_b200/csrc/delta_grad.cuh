@@ -104,20 +104,6 @@ __device__ __forceinline__ void store_grad(TO *out, const float (&c)[NT / 8][4],
   }
 }
 
-template <int S>
-__device__ __forceinline__ Frag<S> scaled(const Frag<S> &f, int diff) {  // times 2^diff, diff <= 0
-  const __half2 m = __float2half2_rn(pow2(diff));
-  Frag<S> r;
-#pragma unroll
-  for (int s = 0; s < S; ++s)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&f.r[s][i]), m);
-      r.r[s][i] = *reinterpret_cast<const uint32_t *>(&x);
-    }
-  return r;
-}
-
 template <int NT, int SI, int SC, typename TI>
 __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
   using Op = Operand<SI, NT>;

@@ -5,6 +5,7 @@
 #include "delta_grad.cuh"
 #include "delta_launch.cuh"
 #include "delta_scan.cuh"
+#include "delta_team.cuh"
 
 namespace slx {
 namespace delta {
@@ -17,9 +18,23 @@ static int launch_chunk(const Args &a, cudaStream_t st) {
   kernel<<<dim3(a.NC, a.batch * a.key_heads), kThreads, bytes, st>>>(a);
   return check_launch("delta_chunk_kernel");
 }
+// warps == 0: teams of four warps on 16 value channels (where their tiles fit an SM: not fp32 of more than 64 columns)
+template <int NT, int SI>
+constexpr bool has_team = SI == 1 || NT == 64;
+
 template <int NT, int SI, int SC, typename TI>
 static int launch_fwd(const Args &a, int warps, cudaStream_t st) {
   if (const int rc = launch_chunk<NT, SI, SC, TI>(a, st)) return rc;
+  if constexpr (has_team<NT, SI>) {
+    if (warps == 0) {
+      constexpr int bytes = sizeof(TeamShared<NT, SI, SC, TI>);
+      auto kernel = delta_fwd_team_kernel<NT, SI, SC, TI>;
+      if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;
+      kernel<<<dim3(a.P16 / 16, a.batch * a.heads), kThreads, bytes, st>>>(a);
+      return check_launch("delta_fwd_team_kernel");
+    }
+  }
+  if (warps == 0) warps = a.P16 < 64 ? a.P16 / 16 : 4;
   constexpr int bytes = scan_smem<NT, SI, SC, TI>(false);
   auto kernel = delta_fwd_kernel<NT, SI, SC, TI>;
   if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;
@@ -29,7 +44,19 @@ static int launch_fwd(const Args &a, int warps, cudaStream_t st) {
 template <int NT, int SI, int SC, typename TI>
 static int launch_bwd(const Args &a, void *dq, void *dk, int warps, cudaStream_t st) {
   if (const int rc = launch_chunk<NT, SI, SC, TI>(a, st)) return rc;
-  {
+  bool done = false;
+  if constexpr (has_team<NT, SI>) {
+    if (warps == 0) {
+      constexpr int bytes = sizeof(TeamShared<NT, SI, 2, TI>);
+      auto kernel = delta_bwd_team_kernel<NT, SI, SC, TI>;
+      if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;
+      kernel<<<dim3(a.P16 / 16, a.batch * a.heads), kThreads, bytes, st>>>(a);
+      if (const int rc = check_launch("delta_bwd_team_kernel")) return rc;
+      done = true;
+    }
+  }
+  if (warps == 0) warps = a.P16 < 64 ? a.P16 / 16 : 4;
+  if (!done) {
     constexpr int bytes = scan_smem<NT, SI, SC, TI>(true);
     auto kernel = delta_bwd_kernel<NT, SI, SC, TI>;
     if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;

@@ -86,11 +86,13 @@ static Args args_of(const slx_gated_delta_shape *s, const Dims &d, const void *q
   return a;
 }
 
-// Warps of a CTA that hold rows of states: 64 value channels share a CTA's tiles, fewer where that leaves SMs without a CTA.
+// Zero: teams of four warps on 16 value channels, where each can have an SM to itself.  Else the warps of a CTA that hold 16
+// channels each: as many as there are, up to four, which share a CTA's tiles.  Measured (T 2048, N 128, P 64, bf16, forward
+// and training, us) with 128 blocks of 16 channels: teams 141 / 384, warps 199 / 557; with 256 blocks: 269 / 708, 235 / 694;
+// fewer than four warps a CTA are never faster (512 blocks: four 316 / 1001, two 362 / 1114, one 455 / 1308).
 static int scan_warps(const Dims &d) {
-  int w = (int)(d.PB < 4 ? d.PB : 4);
-  while (w > 1 && d.BH * ((d.PB + w - 1) / w) < kB200Sms) w = (w + 1) / 2;
-  return w;
+  if (d.BH * d.PB <= kB200Sms) return 0;
+  return (int)(d.PB < 4 ? d.PB : 4);
 }
 
 }  // namespace delta
