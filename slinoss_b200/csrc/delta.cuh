@@ -444,15 +444,20 @@ struct Raw {
   }
 };
 
+// asynchronous, a multiple of 16 bytes, by kThreads threads of which this is number `tid`
 template <int bytes>
-__device__ __forceinline__ void copy_bytes(void *dst, const void *src) {  // asynchronous, a multiple of 16
+__device__ __forceinline__ void copy_bytes(void *dst, const void *src, int tid) {
   static_assert(bytes % 16 == 0, "copies of 16 bytes");
-  char *d = static_cast<char *>(dst) + threadIdx.x * 16;
-  const char *s = static_cast<const char *>(src) + threadIdx.x * 16;
+  char *d = static_cast<char *>(dst) + tid * 16;
+  const char *s = static_cast<const char *>(src) + tid * 16;
 #pragma unroll
   for (int i = 0; i < bytes / 16 / kThreads; ++i) cp16(d + i * kThreads * 16, s + i * kThreads * 16, true);
   constexpr int whole = bytes / 16 / kThreads * kThreads * 16;
-  if (whole < bytes && (int)threadIdx.x * 16 < bytes - whole) cp16(d + whole, s + whole, true);
+  if (whole < bytes && tid * 16 < bytes - whole) cp16(d + whole, s + whole, true);
+}
+template <int bytes>
+__device__ __forceinline__ void copy_bytes(void *dst, const void *src) {
+  copy_bytes<bytes>(dst, src, threadIdx.x);
 }
 
 // A warp's (16 columns p, 64 tokens) result, held transposed in accumulators (rows p, columns t), to global rows of `out`

@@ -18,7 +18,7 @@ static int launch_chunk(const Args &a, cudaStream_t st) {
   kernel<<<dim3(a.NC, a.batch * a.key_heads), kThreads, bytes, st>>>(a);
   return check_launch("delta_chunk_kernel");
 }
-// warps == 0: teams of four warps on 16 value channels (where their tiles fit an SM: not fp32 of more than 64 columns)
+// warps == 0: teams on 16 value channels (where their tiles fit an SM: not fp32 of more than 64 columns)
 template <int NT, int SI>
 constexpr bool has_team = SI == 1 || NT == 64;
 
@@ -30,7 +30,7 @@ static int launch_fwd(const Args &a, int warps, cudaStream_t st) {
       constexpr int bytes = sizeof(TeamShared<NT, SI, SC, TI>);
       auto kernel = delta_fwd_team_kernel<NT, SI, SC, TI>;
       if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;
-      kernel<<<dim3(a.P16 / 16, a.batch * a.heads), kThreads, bytes, st>>>(a);
+      kernel<<<dim3(a.P16 / 16, a.batch * a.heads), kTeamThreads, bytes, st>>>(a);
       return check_launch("delta_fwd_team_kernel");
     }
   }
@@ -50,7 +50,7 @@ static int launch_bwd(const Args &a, void *dq, void *dk, int warps, cudaStream_t
       constexpr int bytes = sizeof(TeamShared<NT, SI, 2, TI>);
       auto kernel = delta_bwd_team_kernel<NT, SI, SC, TI>;
       if (const int rc = ensure_dyn_smem(kernel, bytes)) return rc;
-      kernel<<<dim3(a.P16 / 16, a.batch * a.heads), kThreads, bytes, st>>>(a);
+      kernel<<<dim3(a.P16 / 16, a.batch * a.heads), kTeamThreads, bytes, st>>>(a);
       if (const int rc = check_launch("delta_bwd_team_kernel")) return rc;
       done = true;
     }

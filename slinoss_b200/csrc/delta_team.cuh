@@ -1,11 +1,12 @@
-// The passes along the sequence for calls with few heads: a team of four warps on 16 value channels.
+// The passes along the sequence for calls with few heads: a team of eight warps on 16 value channels.
 //
 // Where the channels of all heads together are fewer than the SMs have warps for, a chunk's time is that of one warp's chain of
-// products (delta_scan.cuh: some 8000 clocks a chunk), and three quarters of every SM stand idle.  Here four warps share it.
-// The state lies by columns: warp w holds N / 4 of them for the 16 rows.  Products with the state are partial sums over the
-// columns, added up through shared memory by 16 tokens a warp; what a warp computes for its 16 tokens the others need as
-// operands comes back the same way, as fragments.  Four barriers a chunk and a quarter of the instructions each.  All tiles
-// are double-buffered: a CTA has its SM to itself.
+// products (delta_scan.cuh: some 8000 clocks a chunk), and three quarters of every SM stand idle.  Here four warps share the
+// chain and four more do what does not lie on it.  The state lies by columns: warp w of the first four holds N / 4 of them for
+// the 16 rows.  Products with the state are partial sums over the columns, added up through shared memory by 16 tokens a warp;
+// what a warp computes for its 16 tokens the others need as operands comes back the same way, as fragments.  The other four
+// warps copy the next chunk's tiles in, form the outputs (from the state's fragments, 16 tokens each) and write everything that
+// goes to memory.  Four barriers a chunk.  All tiles are double-buffered: a CTA has its SM to itself.
 #pragma once
 
 #include "delta_scan.cuh"
@@ -18,18 +19,18 @@ template <typename TI>
 struct RawTeam {
   static constexpr int ld = 16 + 16 / (int)sizeof(TI);
   static constexpr int size = L * ld;
-  static __device__ __forceinline__ void issue(TI *dst, const TI *src, int64_t st, int rows, int cols, bool vec) {
+  static __device__ __forceinline__ void issue(TI *dst, const TI *src, int64_t st, int rows, int cols, bool vec, int tid) {
     constexpr int V = 16 / (int)sizeof(TI), per = 16 / V;
     if (vec) {
 #pragma unroll
       for (int n = 0; n < L * per / kThreads; ++n) {
-        const int i = n * kThreads + threadIdx.x, r = i / per, c = i % per * V;
+        const int i = n * kThreads + tid, r = i / per, c = i % per * V;
         const bool ok = r < rows && c < cols;
         cp16(dst + r * ld + c, ok ? src + r * st + c : src, ok);
       }
     } else {
 #pragma unroll 1
-      for (int i = threadIdx.x; i < L * 16; i += kThreads) {
+      for (int i = tid; i < L * 16; i += kThreads) {
         const int r = i / 16, c = i % 16;
         dst[r * ld + c] = r < rows && c < cols ? src[r * st + c] : from_f<TI>(0.f);
       }
@@ -67,11 +68,14 @@ struct TeamStage {  // the tiles of a chunk
 template <int NT, int SI, int SP, typename TI>
 struct alignas(16) TeamShared {
   TeamStage<NT, SI, SP, TI> stage[2];
-  float2 part[2][4][8][2][32];       // partial sums: of X and of O, by warp, tile, row half, lane
-  uint4 frag[3][4][2][32];           // fragments: kind, warp, plane, lane
-  int exps[2][5][4];                 // exponents by kind and warp (3: of the states, 4: of Y or dX); two sets in turn
+  float2 part[4][8][2][32];          // partial sums by warp, tile, row half, lane
+  uint4 state[NT / 16][2][32];       // the state's fragments: columns, plane, lane
+  uint4 frag[4][4][2][32];           // fragments: kind, warp, plane, lane
+  int exps[2][5][4];                 // their exponents, and (4) the state's; two sets in turn
   __half buf[4][16 * (NT / 4 + 8) > 16 * 24 ? 16 * (NT / 4 + 8) : 16 * 24];
 };
+constexpr int kTeamThreads = 2 * kThreads;
+__device__ __forceinline__ void team_barrier() { asm volatile("barrier.sync 1, %0;" ::"n"(kTeamThreads) : "memory"); }
 
 template <int S>
 __device__ __forceinline__ void put_frag(uint4 (&dst)[2][32], const Frag<S> &f) {
@@ -130,10 +134,8 @@ __device__ __forceinline__ void store_rows16(TO *out, int64_t st, int rows, int 
   }
 }
 template <int S>
-__device__ __forceinline__ void store_planes16(__half *out, int64_t plane, const float (&c)[2][4], int e, __half *buf) {
+__device__ __forceinline__ void store_planes16(__half *out, int64_t plane, const Frag<S> &f, __half *buf) {
   const int lane = threadIdx.x & 31;
-  Frag<S> f;
-  frag_of<S>(f, c[0], c[1], pow2(-e));
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     __syncwarp();
@@ -143,20 +145,19 @@ __device__ __forceinline__ void store_planes16(__half *out, int64_t plane, const
         *reinterpret_cast<const uint4 *>(buf + (lane >> 1) * 24 + (lane & 1) * 8);
   }
 }
-// this warp's NT / 4 columns of 16 rows of a state
+// NT / 4 columns of 16 rows of a state, from its fragments
 template <int S, int NT>
-__device__ __forceinline__ void store_state16(__half *out, int64_t plane, const float (&c)[NT / 32][4], int e, __half *buf) {
+__device__ __forceinline__ void store_state16(__half *out, int64_t plane, const uint4 (*state)[2][32], __half *buf) {
   const int lane = threadIdx.x & 31;
   constexpr int W = NT / 4, ld = W + 8;
-  const float s = pow2(-e);
 #pragma unroll
   for (int pl = 0; pl < S; ++pl) {
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < W / 8; j += 2) {
-      Frag<S> f;
-      frag_of<S>(f, c[j], c[j + 1], s);
-      stsm(smem_addr(buf + (lane & 15) * ld + 8 * j + (lane >> 4) * 8), f.r[pl]);
+    for (int j = 0; j < W / 16; ++j) {
+      const uint4 x = state[j][pl][lane];
+      const uint32_t r[4] = {x.x, x.y, x.z, x.w};
+      stsm(smem_addr(buf + (lane & 15) * ld + 16 * j + (lane >> 4) * 8), r);
     }
     __syncwarp();
 #pragma unroll
@@ -250,321 +251,396 @@ __device__ __forceinline__ void write_state16(void *dst, int dtype, size_t base,
     }
 }
 
+// hi + lo of a fragment as accumulators, times s
+template <int S>
+__device__ __forceinline__ void frag_values(float (&c)[2][4], const Frag<S> &f, float s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 x = unpack(f.r[0][i]);
+    if constexpr (S == 2) {
+      const float2 y = unpack(f.r[1][i]);
+      x.x += y.x;
+      x.y += y.y;
+    }
+    c[i >> 1][(i & 1) * 2] = x.x * s;
+    c[i >> 1][(i & 1) * 2 + 1] = x.y * s;
+  }
+}
+
 template <int NT, int SI, int SC, typename TI>
-__global__ void __launch_bounds__(kThreads) delta_fwd_team_kernel(Args a) {
+__global__ void __launch_bounds__(kTeamThreads) delta_fwd_team_kernel(Args a) {
   using Op = Operand<SI, NT>;
   using Shared = TeamShared<NT, SI, SC, TI>;
   extern __shared__ __align__(128) char smem[];
   Shared &sm = *reinterpret_cast<Shared *>(smem);
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __half *buf = sm.buf[w];
+  const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const bool chain = threadIdx.x < kThreads;
   const int bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads, kh = h / (a.heads / a.key_heads);
   const int p0 = blockIdx.x * 16, n0 = w * (NT / 4), PB = a.P16 / 16, tiles = (a.P16 + 63) / 64;
   const Record *rec = a.rec + (size_t)bh * a.NC;
-  const __half *kq = a.kq + (size_t)(b * a.key_heads + kh) * a.NC * 2 * Op::halves;
-  auto issue = [&](int c) {
-    auto &st = sm.stage[c & 1];
-    copy_bytes<2 * Op::halves * 2>(st.k, kq + (size_t)c * 2 * Op::halves);  // k, q
-    copy_bytes<(2 + SC) * kTri * 2>(st.T, rec[c].T);                        // T, P
-    copy_bytes<kHeadBytes>(st.gamma, rec[c].gamma);
-    RawTeam<TI>::issue(st.v, head_base<TI>(a.v, b, h, c * L) + p0, a.v.st, min(L, a.T - c * L), a.P - p0, a.v.vec);
-    cp_commit();
-  };
-  float S[NT / 32][4];
-  if (a.init) load_state16<NT>(S, a.init, a.init_dtype, (size_t)bh * a.P * a.N, p0, n0, a.P, a.N);
-  else zero(S);
-  int4 ex = exps_of(rec);
-  issue(0);
-  {
-    const int e = warp_exp(S);
-    if (lane == 0) sm.exps[0][3][w] = e;
-  }
-  for (int c = 0; c < a.NC; ++c) {
-    const bool more = c + 1 < a.NC;
-    const int4 nx = more ? exps_of(rec + c + 1) : ex;
-    const int eT = ex.x, eQ = ex.y, eq = ex.z, ek = ex.w;
-    const auto &st = sm.stage[c & 1];
-    int(&exps)[5][4] = sm.exps[c & 1];
-    const size_t at = (size_t)bh * a.NC + c;
-    cp_wait<0>();
-    __syncthreads();
-    if (more) issue(c + 1);
-    const int eS = max4(exps[3]);
-    if (a.st) {
-      store_state16<SC, NT>(a.st + (at * SC * a.P16 + p0) * (NT + 8) + n0, (int64_t)a.P16 * (NT + 8), S, eS, buf);
-      if (threadIdx.x == 0) a.est[at * PB + p0 / 16] = eS;
-    }
-    {  // over this warp's columns: S k^T and S q^T
-      float X[8][4], O[8][4];
-      zero(X);
-      zero(O);
-      const float s = pow2(-eS);
-#pragma unroll
-      for (int kb = 0; kb < NT / 64; ++kb) {
-        Frag<2> f;
-        frag_of<2>(f, S[2 * kb], S[2 * kb + 1], s);
-        Frag<SC> fo;
-#pragma unroll
-        for (int pl = 0; pl < SC; ++pl)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) fo.r[pl][i] = f.r[pl][i];
-        team_rows<2, SI, NT>(X, f, st.k, n0 + 16 * kb);
-        team_rows<SC, SI, NT>(O, fo, st.q, n0 + 16 * kb);
-      }
-      put_part(sm.part[0][w], X);
-      put_part(sm.part[1][w], O);
-    }
-    __syncthreads();
-    float x[2][4], o[2][4];  // this warp's 16 tokens
-    sum_parts(x, sm.part[0], w);
-    sum_parts(o, sm.part[1], w);
-    {
-      float v[2][4];
-      RawTeam<TI>::load(v, st.v, w);
-      times_cols16(x, st.gamma + 16 * w, pow2(eS + ek));
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[j][i] = v[j][i] - x[j][i];
-      const int e = warp_exp(x);
-      Frag<2> f;
-      frag_of<2>(f, x[0], x[1], pow2(-e));
-      put_frag<2>(sm.frag[0][w], f);
-      if (lane == 0) exps[0][w] = e;
-    }
-    __syncthreads();
-    {
-      const int eX = max4(exps[0]);
-      zero(x);
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-        if (kb <= w) {
-          const Frag<2> f = get_frag<2>(sm.frag[0][kb], exps[0][kb] - eX);
-          uint32_t bb[2][4];
-          b_nk(bb[0], st.T + tri_base(w) + 16 * kb, tri_ld(w));
-          b_nk(bb[1], st.T + kTri + tri_base(w) + 16 * kb, tri_ld(w));
-          mma_split<2, 2>(x[0], x[1], f, bb);
-        }
-      times(x, pow2(eX + eT));  // Y
-    }
-    float y[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[j][i] = x[j][i];
-    {
-      const int eY = warp_exp(x);
-      times_cols16(x, st.beta + 16 * w, 1.f);
-      const int eD = warp_exp(x);
-      Frag<SC> fd;
-      frag_of<SC>(fd, x[0], x[1], pow2(-eD));
-      put_frag<SC>(sm.frag[1][w], fd);
-      times_cols16(x, st.closing + 16 * w, 1.f);
-      const int eC = warp_exp(x);
-      Frag<2> fc;
-      frag_of<2>(fc, x[0], x[1], pow2(-eC));
-      put_frag<2>(sm.frag[2][w], fc);
-      if (lane == 0) {
-        exps[4][w] = eY;
-        exps[1][w] = eD;
-        exps[2][w] = eC;
-      }
-    }
-    __syncthreads();
-    if (a.y) {
-      const int e = max4(exps[4]);
-      store_planes16<SC>(a.y + (at * SC * tiles + p0 / 64) * kTile + 16 * w * kTileLd + p0 % 64, (int64_t)tiles * kTile, y, e, buf);
-      if (threadIdx.x == 0) a.ey[at * PB + p0 / 16] = e;
-    }
-    if (a.o) {
-      times_cols16(o, st.gamma + 16 * w, pow2(eS + eq));
-      const int eD = floor_exp(max4(exps[1]), warp_exp(o), eQ);
-      times(o, pow2(-(eD + eQ)));
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-        if (kb <= w) {
-          const Frag<SC> f = get_frag<SC>(sm.frag[1][kb], exps[1][kb] - eD);
-          uint32_t bb[SC][4];
-#pragma unroll
-          for (int s = 0; s < SC; ++s) b_nk(bb[s], st.P + s * kTri + tri_base(w) + 16 * kb, tri_ld(w));
-          mma_split<SC, SC>(o[0], o[1], f, bb);
-        }
-      times(o, a.scale * pow2(eD + eQ));
-      store_rows16<TI>(static_cast<TI *>(a.o) + ((size_t)bh * a.T + c * L + 16 * w) * a.P + p0, a.P, a.T - c * L - 16 * w,
-                       a.P - p0, o, buf);
-    }
-    const int eC = floor_exp(max4(exps[2]), eS, ek);
-    times(S, st.gamma[L - 1] * pow2(-(eC + ek)));
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-      team_cols<2, SI, NT>(S, get_frag<2>(sm.frag[2][kb], exps[2][kb] - eC), st.k, kb, n0);
-    times(S, pow2(eC + ek));
+  // kinds of fragments and exponents: X, beta Y, closing beta Y, Y; the state's
+  enum { kX, kD, kC, kY, kS };
+  if (chain) {
+    float S[NT / 32][4];
+    if (a.init) load_state16<NT>(S, a.init, a.init_dtype, (size_t)bh * a.P * a.N, p0, n0, a.P, a.N);
+    else zero(S);
+    int4 nx = exps_of(rec);
     {
       const int e = warp_exp(S);
-      if (lane == 0) sm.exps[(c + 1) & 1][3][w] = e;
+      if (lane == 0) sm.exps[0][kS][w] = e;
     }
-    ex = nx;
+    for (int c = 0; c < a.NC; ++c) {
+      const int4 ex = nx;
+      const int eT = ex.x, ek = ex.w;
+      const auto &st = sm.stage[c & 1];
+      int(&exps)[5][4] = sm.exps[c & 1];
+      team_barrier();
+      if (c + 1 < a.NC) nx = exps_of(rec + c + 1);
+      const int eS = max4(exps[kS]);
+      {  // over this warp's columns: S k^T
+        float X[8][4];
+        zero(X);
+        const float s = pow2(-eS);
+#pragma unroll
+        for (int kb = 0; kb < NT / 64; ++kb) {
+          Frag<2> f;
+          frag_of<2>(f, S[2 * kb], S[2 * kb + 1], s);
+          put_frag<2>(sm.state[w * (NT / 64) + kb], f);
+          team_rows<2, SI, NT>(X, f, st.k, n0 + 16 * kb);
+        }
+        put_part(sm.part[w], X);
+      }
+      team_barrier();
+      float x[2][4];  // this warp's 16 tokens
+      {
+        float v[2][4];
+        RawTeam<TI>::load(v, st.v, w);
+        sum_parts(x, sm.part, w);
+        times_cols16(x, st.gamma + 16 * w, pow2(eS + ek));
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j][i] = v[j][i] - x[j][i];
+        const int e = warp_exp(x);
+        Frag<2> f;
+        frag_of<2>(f, x[0], x[1], pow2(-e));
+        put_frag<2>(sm.frag[kX][w], f);
+        if (lane == 0) exps[kX][w] = e;
+      }
+      team_barrier();
+      {
+        const int eX = max4(exps[kX]);
+        float z[2][2][4];  // (two chains)
+        zero(z[0]);
+        zero(z[1]);
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+          if (kb <= w) {
+            const Frag<2> f = get_frag<2>(sm.frag[kX][kb], exps[kX][kb] - eX);
+            uint32_t bb[2][4];
+            b_nk(bb[0], st.T + tri_base(w) + 16 * kb, tri_ld(w));
+            b_nk(bb[1], st.T + kTri + tri_base(w) + 16 * kb, tri_ld(w));
+            mma_split<2, 2>(z[kb & 1][0], z[kb & 1][1], f, bb);
+          }
+        const float s = pow2(eX + eT);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j][i] = (z[0][j][i] + z[1][j][i]) * s;  // Y
+        if (a.y) {
+          const int e = warp_exp(x);
+          Frag<SC> f;
+          frag_of<SC>(f, x[0], x[1], pow2(-e));
+          put_frag<SC>(sm.frag[kY][w], f);
+          if (lane == 0) exps[kY][w] = e;
+        }
+        times_cols16(x, st.beta + 16 * w, 1.f);
+        const int eD = warp_exp(x);
+        Frag<SC> fd;
+        frag_of<SC>(fd, x[0], x[1], pow2(-eD));
+        put_frag<SC>(sm.frag[kD][w], fd);
+        times_cols16(x, st.closing + 16 * w, 1.f);
+        const int eC = warp_exp(x);
+        Frag<2> fc;
+        frag_of<2>(fc, x[0], x[1], pow2(-eC));
+        put_frag<2>(sm.frag[kC][w], fc);
+        if (lane == 0) {
+          exps[kD][w] = eD;
+          exps[kC][w] = eC;
+        }
+      }
+      team_barrier();
+      const int eC = floor_exp(max4(exps[kC]), eS, ek);
+      times(S, st.gamma[L - 1] * pow2(-(eC + ek)));
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+        team_cols<2, SI, NT>(S, get_frag<2>(sm.frag[kC][kb], exps[kC][kb] - eC), st.k, kb, n0);
+      times(S, pow2(eC + ek));
+      const int e = warp_exp(S);
+      if (lane == 0) sm.exps[(c + 1) & 1][kS][w] = e;
+    }
+    if (a.final_state) write_state16<NT>(a.final_state, SLX_F32, (size_t)bh * a.P * a.N, S, p0, n0, a.P, a.N);
+  } else {
+    const int tid = threadIdx.x - kThreads;
+    __half *buf = sm.buf[w];
+    const __half *kq = a.kq + (size_t)(b * a.key_heads + kh) * a.NC * 2 * Op::halves;
+    auto issue = [&](int c) {
+      auto &st = sm.stage[c & 1];
+      copy_bytes<2 * Op::halves * 2>(st.k, kq + (size_t)c * 2 * Op::halves, tid);  // k, q
+      copy_bytes<(2 + SC) * kTri * 2>(st.T, rec[c].T, tid);                        // T, P
+      copy_bytes<kHeadBytes>(st.gamma, rec[c].gamma, tid);
+      RawTeam<TI>::issue(st.v, head_base<TI>(a.v, b, h, c * L) + p0, a.v.st, min(L, a.T - c * L), a.P - p0, a.v.vec, tid);
+      cp_commit();
+    };
+    issue(0);
+    for (int c = 0; c < a.NC; ++c) {
+      const int4 ex = exps_of(rec + c);
+      const int eQ = ex.y, eq = ex.z;
+      const auto &st = sm.stage[c & 1];
+      int(&exps)[5][4] = sm.exps[c & 1];
+      const size_t at = (size_t)bh * a.NC + c;
+      cp_wait<0>();
+      team_barrier();
+      if (c + 1 < a.NC) issue(c + 1);
+      const int eS = max4(exps[kS]);
+      team_barrier();
+      float o[2][4];
+      {
+        float z[2][2][4];
+        zero(z[0]);
+        zero(z[1]);
+        if (a.o) {
+#pragma unroll
+          for (int kb = 0; kb < NT / 16; ++kb) {
+            const Frag<SC> f = get_frag<SC>(sm.state[kb], 0);
+            uint32_t bb[SI][4];
+#pragma unroll
+            for (int s = 0; s < SI; ++s) b_nk(bb[s], st.q + s * Op::plane + 16 * w * Op::ld + 16 * kb, Op::ld);
+            mma_split<SC, SI>(z[kb & 1][0], z[kb & 1][1], f, bb);
+          }
+        }
+        const float s = pow2(eS + eq);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[j][i] = (z[0][j][i] + z[1][j][i]) * s;
+      }
+      team_barrier();
+      if (a.st) {
+        store_state16<SC, NT>(a.st + (at * SC * a.P16 + p0) * (NT + 8) + n0, (int64_t)a.P16 * (NT + 8),
+                              sm.state + w * (NT / 64), buf);
+        if (tid == 0) a.est[at * PB + p0 / 16] = eS;
+      }
+      times_cols16(o, st.gamma + 16 * w, 1.f);
+      const int eo = warp_exp(o);
+      team_barrier();
+      if (a.o) {
+        const int eD = floor_exp(max4(exps[kD]), eo, eQ);
+        times(o, pow2(-(eD + eQ)));
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+          if (kb <= w) {
+            const Frag<SC> f = get_frag<SC>(sm.frag[kD][kb], exps[kD][kb] - eD);
+            uint32_t bb[SC][4];
+#pragma unroll
+            for (int s = 0; s < SC; ++s) b_nk(bb[s], st.P + s * kTri + tri_base(w) + 16 * kb, tri_ld(w));
+            mma_split<SC, SC>(o[0], o[1], f, bb);
+          }
+        times(o, a.scale * pow2(eD + eQ));
+        store_rows16<TI>(static_cast<TI *>(a.o) + ((size_t)bh * a.T + c * L + 16 * w) * a.P + p0, a.P, a.T - c * L - 16 * w,
+                         a.P - p0, o, buf);
+      }
+      if (a.y) {
+        const int e = max4(exps[kY]);
+        store_planes16<SC>(a.y + (at * SC * tiles + p0 / 64) * kTile + 16 * w * kTileLd + p0 % 64, (int64_t)tiles * kTile,
+                           get_frag<SC>(sm.frag[kY][w], exps[kY][w] - e), buf);
+        if (tid == 0) a.ey[at * PB + p0 / 16] = e;
+      }
+    }
+    cp_wait<0>();
   }
-  cp_wait<0>();
-  if (a.final_state) write_state16<NT>(a.final_state, SLX_F32, (size_t)bh * a.P * a.N, S, p0, n0, a.P, a.N);
 }
 
 template <int NT, int SI, int SC, typename TI>
-__global__ void __launch_bounds__(kThreads) delta_bwd_team_kernel(Args a) {
+__global__ void __launch_bounds__(kTeamThreads) delta_bwd_team_kernel(Args a) {
   using Op = Operand<SI, NT>;
   using Shared = TeamShared<NT, SI, 2, TI>;
   extern __shared__ __align__(128) char smem[];
   Shared &sm = *reinterpret_cast<Shared *>(smem);
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __half *buf = sm.buf[w];
+  const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const bool chain = threadIdx.x < kThreads;
   const int bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads, kh = h / (a.heads / a.key_heads);
   const int p0 = blockIdx.x * 16, n0 = w * (NT / 4), PB = a.P16 / 16, tiles = (a.P16 + 63) / 64;
   const Record *rec = a.rec + (size_t)bh * a.NC;
-  const __half *kq = a.kq + (size_t)(b * a.key_heads + kh) * a.NC * 2 * Op::halves;
-  auto issue = [&](int c) {
-    auto &st = sm.stage[c & 1];
-    copy_bytes<2 * Op::halves * 2>(st.k, kq + (size_t)c * 2 * Op::halves);  // k, q
-    copy_bytes<4 * kTri * 2>(st.T, rec[c].T);                               // T, P
-    copy_bytes<kHeadBytes>(st.gamma, rec[c].gamma);
-    RawTeam<TI>::issue(st.v, head_base<TI>(a.dO, b, h, c * L) + p0, a.dO.st, min(L, a.T - c * L), a.P - p0, a.dO.vec);
-    cp_commit();
-  };
-  float R[NT / 32][4];
-  if (a.d_final) load_state16<NT>(R, a.d_final, a.d_final_dtype, (size_t)bh * a.P * a.N, p0, n0, a.P, a.N);
-  else zero(R);
-  int4 ex = exps_of(rec + a.NC - 1);
-  issue(a.NC - 1);
-  {
-    const int e = warp_exp(R);
-    if (lane == 0) sm.exps[(a.NC - 1) & 1][3][w] = e;
-  }
-  for (int c = a.NC - 1; c >= 0; --c) {
-    const int4 nx = c > 0 ? exps_of(rec + c - 1) : ex;
-    const int eT = ex.x, eQ = ex.y, eq = ex.z, ek = ex.w;
-    const auto &st = sm.stage[c & 1];
-    int(&exps)[5][4] = sm.exps[c & 1];
-    const size_t at = (size_t)bh * a.NC + c;
-    cp_wait<0>();
-    __syncthreads();
-    if (c > 0) issue(c - 1);
-    const int eR = max4(exps[3]);
-    store_state16<SC, NT>(a.ds + (at * SC * a.P16 + p0) * (NT + 8) + n0, (int64_t)a.P16 * (NT + 8), R, eR, buf);
-    {  // over this warp's columns: R k^T
-      float X[8][4];
-      zero(X);
-      const float s = pow2(-eR);
+  // kinds of fragments and exponents: dO, then beta dD in the same place; scale gamma dO; -gamma dX; dX; the state's
+  enum { kO, kG, kN, kX, kR };
+  if (chain) {
+    float R[NT / 32][4];
+    if (a.d_final) load_state16<NT>(R, a.d_final, a.d_final_dtype, (size_t)bh * a.P * a.N, p0, n0, a.P, a.N);
+    else zero(R);
+    int4 nx = exps_of(rec + a.NC - 1);
+    {
+      const int e = warp_exp(R);
+      if (lane == 0) sm.exps[(a.NC - 1) & 1][kR][w] = e;
+    }
+    for (int c = a.NC - 1; c >= 0; --c) {
+      const int4 ex = nx;
+      const int eT = ex.x, eQ = ex.y, eq = ex.z, ek = ex.w;
+      const auto &st = sm.stage[c & 1];
+      int(&exps)[5][4] = sm.exps[c & 1];
+      team_barrier();
+      if (c > 0) nx = exps_of(rec + c - 1);
+      const int eR = max4(exps[kR]);
+      {  // over this warp's columns: R k^T
+        float X[8][4];
+        zero(X);
+        const float s = pow2(-eR);
 #pragma unroll
-      for (int kb = 0; kb < NT / 64; ++kb) {
+        for (int kb = 0; kb < NT / 64; ++kb) {
+          Frag<2> f;
+          frag_of<2>(f, R[2 * kb], R[2 * kb + 1], s);
+          put_frag<2>(sm.state[w * (NT / 64) + kb], f);
+          team_rows<2, SI, NT>(X, f, st.k, n0 + 16 * kb);
+        }
+        put_part(sm.part[w], X);
+      }
+      team_barrier();
+      float x[2][4], y[2][4];
+      {
+        const int eo = max4(exps[kO]);
+        zero(y);
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+          if (kb >= w) {
+            const Frag<SI> f = get_frag<SI>(sm.frag[kO][kb], exps[kO][kb] - eo);
+            uint32_t bb[2][4];
+            b_kn(bb[0], st.P + tri_base(kb) + 16 * w, tri_ld(kb));
+            b_kn(bb[1], st.P + kTri + tri_base(kb) + 16 * w, tri_ld(kb));
+            mma_split<SI, 2>(y[0], y[1], f, bb);
+          }
+        sum_parts(x, sm.part, w);
+        times_cols16(x, st.closing + 16 * w, pow2(eR + ek));
+        const float s = a.scale * pow2(eo + eQ);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j][i] = fmaf(y[j][i], s, x[j][i]);
+        times_cols16(x, st.beta + 16 * w, 1.f);
+        const int e = warp_exp(x);
         Frag<2> f;
-        frag_of<2>(f, R[2 * kb], R[2 * kb + 1], s);
-        team_rows<2, SI, NT>(X, f, st.k, n0 + 16 * kb);
+        frag_of<2>(f, x[0], x[1], pow2(-e));
+        put_frag<2>(sm.frag[kX][w], f);  // (beta dD, until dX takes the place)
+        if (lane == 0) exps[kX][w] = e;
       }
-      put_part(sm.part[0][w], X);
+      team_barrier();
+      {
+        const int eX = max4(exps[kX]);
+        float z[2][2][4];  // (two chains)
+        zero(z[0]);
+        zero(z[1]);
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+          if (kb >= w) {
+            const Frag<2> f = get_frag<2>(sm.frag[kX][kb], exps[kX][kb] - eX);
+            uint32_t bb[2][4];
+            b_kn(bb[0], st.T + tri_base(kb) + 16 * w, tri_ld(kb));
+            b_kn(bb[1], st.T + kTri + tri_base(kb) + 16 * w, tri_ld(kb));
+            mma_split<2, 2>(z[kb & 1][0], z[kb & 1][1], f, bb);
+          }
+        const float s = pow2(eX + eT);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j][i] = (z[0][j][i] + z[1][j][i]) * s;  // dX
+        const int eW = warp_exp(x);
+        Frag<2> f;
+        frag_of<2>(f, x[0], x[1], pow2(-eW));
+        put_frag<2>(sm.frag[kO][w], f);  // (dO's place: everybody has read it)
+        times_cols16(x, st.gamma + 16 * w, -1.f);
+        const int eN = warp_exp(x);
+        frag_of<2>(f, x[0], x[1], pow2(-eN));
+        put_frag<2>(sm.frag[kN][w], f);
+        if (lane == 0) {
+          exps[kO][w] = eW;
+          exps[kN][w] = eN;
+        }
+      }
+      team_barrier();
+      const int u1 = floor_exp(max4(exps[kG]), eR, eq);
+      const int u2 = floor_exp(max4(exps[kN]), max(eR, u1 + eq + 21) + 1, ek);
+      times(R, st.gamma[L - 1] * pow2(-(u1 + eq)));
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) team_cols<2, SI, NT>(R, get_frag<2>(sm.frag[kG][kb], exps[kG][kb] - u1), st.q, kb, n0);
+      times(R, pow2(u1 + eq - (u2 + ek)));
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) team_cols<2, SI, NT>(R, get_frag<2>(sm.frag[kN][kb], exps[kN][kb] - u2), st.k, kb, n0);
+      times(R, pow2(u2 + ek));
+      const int e = warp_exp(R);
+      if (lane == 0) sm.exps[(c + 1) & 1][kR][w] = e;
     }
-    float x[2][4], d[2][4];
-    RawTeam<TI>::load(d, st.v, w);
-    {  // dO of this warp's tokens
-      const int e = std::is_same<TI, __half>::value ? 0 : warp_exp(d);
-      Frag<SI> f;
-      frag_of<SI>(f, d[0], d[1], pow2(-e));
-      put_frag<SI>(sm.frag[0][w], f);
-      if (lane == 0) exps[0][w] = e;
-    }
-    __syncthreads();
-    int e1;
-    {
-      const int eo = max4(exps[0]);
+    if (a.d_init) write_state16<NT>(a.d_init, a.d_init_dtype, (size_t)bh * a.P * a.N, R, p0, n0, a.P, a.N);
+  } else {
+    const int tid = threadIdx.x - kThreads;
+    __half *buf = sm.buf[w];
+    const __half *kq = a.kq + (size_t)(b * a.key_heads + kh) * a.NC * 2 * Op::halves;
+    auto issue = [&](int c) {
+      auto &st = sm.stage[c & 1];
+      copy_bytes<2 * Op::halves * 2>(st.k, kq + (size_t)c * 2 * Op::halves, tid);  // k, q
+      copy_bytes<4 * kTri * 2>(st.T, rec[c].T, tid);                               // T, P
+      copy_bytes<kHeadBytes>(st.gamma, rec[c].gamma, tid);
+      RawTeam<TI>::issue(st.v, head_base<TI>(a.dO, b, h, c * L) + p0, a.dO.st, min(L, a.T - c * L), a.P - p0, a.dO.vec, tid);
+      cp_commit();
+    };
+    issue(a.NC - 1);
+    for (int c = a.NC - 1; c >= 0; --c) {
+      const auto &st = sm.stage[c & 1];
+      int(&exps)[5][4] = sm.exps[c & 1];
+      const size_t at = (size_t)bh * a.NC + c;
+      cp_wait<0>();
+      team_barrier();
+      const int eR = max4(exps[kR]);
+      float d[2][4];
+      RawTeam<TI>::load(d, st.v, w);
+      {  // dO of 16 tokens
+        const int e = std::is_same<TI, __half>::value ? 0 : warp_exp(d);
+        Frag<SI> f;
+        frag_of<SI>(f, d[0], d[1], pow2(-e));
+        put_frag<SI>(sm.frag[kO][w], f);
+        if (lane == 0) exps[kO][w] = e;
+      }
+      if (c > 0) issue(c - 1);
+      team_barrier();
+      if (tid == 0) {
+        a.edo[at * PB + p0 / 16] = max4(exps[kO]);
+        a.eds[at * PB + p0 / 16] = eR;
+      }
+      {
+        times_cols16(d, st.gamma + 16 * w, a.scale);
+        const int e = warp_exp(d);
+        Frag<2> f;
+        frag_of<2>(f, d[0], d[1], pow2(-e));
+        put_frag<2>(sm.frag[kG][w], f);
+        if (lane == 0) exps[kG][w] = e;
+      }
+      team_barrier();
+      store_state16<SC, NT>(a.ds + (at * SC * a.P16 + p0) * (NT + 8) + n0, (int64_t)a.P16 * (NT + 8), sm.state + w * (NT / 64), buf);
+      team_barrier();
+      const int e = max4(exps[kO]);  // of dX by now
+      const Frag<2> f = get_frag<2>(sm.frag[kO][w], exps[kO][w] - e);
+      Frag<SC> fs;
+#pragma unroll
+      for (int s = 0; s < SC; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fs.r[s][i] = f.r[s][i];
+      store_planes16<SC>(a.dx + (at * SC * tiles + p0 / 64) * kTile + 16 * w * kTileLd + p0 % 64, (int64_t)tiles * kTile, fs, buf);
       float y[2][4];
-      zero(y);
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-        if (kb >= w) {
-          const Frag<SI> f = get_frag<SI>(sm.frag[0][kb], exps[0][kb] - eo);
-          uint32_t bb[2][4];
-          b_kn(bb[0], st.P + tri_base(kb) + 16 * w, tri_ld(kb));
-          b_kn(bb[1], st.P + kTri + tri_base(kb) + 16 * w, tri_ld(kb));
-          mma_split<SI, 2>(y[0], y[1], f, bb);
-        }
-      sum_parts(x, sm.part[0], w);
-      times_cols16(x, st.closing + 16 * w, pow2(eR + ek));
-      times(y, a.scale * pow2(eo + eQ));
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[j][i] += y[j][i];
-      times_cols16(x, st.beta + 16 * w, 1.f);
-      const int e = warp_exp(x);
-      Frag<2> f;
-      frag_of<2>(f, x[0], x[1], pow2(-e));
-      put_frag<2>(sm.frag[1][w], f);
-      times_cols16(d, st.gamma + 16 * w, a.scale);
-      e1 = warp_exp(d);
-      if (lane == 0) {
-        exps[1][w] = e;
-        if (w == 0) a.edo[at * PB + p0 / 16] = eo;
-      }
+      frag_values<2>(y, get_frag<2>(sm.frag[kO][w], 0), pow2(exps[kO][w]));
+      store_rows16<TI>(static_cast<TI *>(a.dv) + ((size_t)bh * a.T + c * L + 16 * w) * a.P + p0, a.P, a.T - c * L - 16 * w,
+                       a.P - p0, y, buf);
+      if (tid == 0) a.edx[at * PB + p0 / 16] = e;
     }
-    __syncthreads();
-    {
-      const int eX = max4(exps[1]);
-      zero(x);
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-        if (kb >= w) {
-          const Frag<2> f = get_frag<2>(sm.frag[1][kb], exps[1][kb] - eX);
-          uint32_t bb[2][4];
-          b_kn(bb[0], st.T + tri_base(kb) + 16 * w, tri_ld(kb));
-          b_kn(bb[1], st.T + kTri + tri_base(kb) + 16 * w, tri_ld(kb));
-          mma_split<2, 2>(x[0], x[1], f, bb);
-        }
-      times(x, pow2(eX + eT));  // dX
-    }
-    float y[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[j][i] = x[j][i];
-    {
-      const int eX = warp_exp(x);
-      times_cols16(x, st.gamma + 16 * w, -1.f);
-      const int e2 = warp_exp(x);
-      Frag<2> f;
-      frag_of<2>(f, x[0], x[1], pow2(-e2));
-      put_frag<2>(sm.frag[2][w], f);
-      frag_of<2>(f, d[0], d[1], pow2(-e1));
-      put_frag<2>(sm.frag[0][w], f);  // (dO itself has been read by everybody)
-      if (lane == 0) {
-        exps[0][w] = e1;
-        exps[2][w] = e2;
-        exps[4][w] = eX;
-      }
-    }
-    __syncthreads();
-    const int e = max4(exps[4]);
-    store_planes16<SC>(a.dx + (at * SC * tiles + p0 / 64) * kTile + 16 * w * kTileLd + p0 % 64, (int64_t)tiles * kTile, y, e, buf);
-    store_rows16<TI>(static_cast<TI *>(a.dv) + ((size_t)bh * a.T + c * L + 16 * w) * a.P + p0, a.P, a.T - c * L - 16 * w, a.P - p0,
-                     y, buf);
-    if (threadIdx.x == 0) {
-      a.eds[at * PB + p0 / 16] = eR;
-      a.edx[at * PB + p0 / 16] = e;
-    }
-    const int u1 = floor_exp(max4(exps[0]), eR, eq);
-    const int u2 = floor_exp(max4(exps[2]), max(eR, u1 + eq + 21) + 1, ek);
-    times(R, st.gamma[L - 1] * pow2(-(u1 + eq)));
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) team_cols<2, SI, NT>(R, get_frag<2>(sm.frag[0][kb], exps[0][kb] - u1), st.q, kb, n0);
-    times(R, pow2(u1 + eq - (u2 + ek)));
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) team_cols<2, SI, NT>(R, get_frag<2>(sm.frag[2][kb], exps[2][kb] - u2), st.k, kb, n0);
-    times(R, pow2(u2 + ek));
-    {
-      const int e3 = warp_exp(R);
-      if (lane == 0) sm.exps[(c + 1) & 1][3][w] = e3;
-    }
-    ex = nx;
+    cp_wait<0>();
   }
-  cp_wait<0>();
-  if (a.d_init) write_state16<NT>(a.d_init, a.d_init_dtype, (size_t)bh * a.P * a.N, R, p0, n0, a.P, a.N);
 }
 
 }  // namespace delta

@@ -86,7 +86,7 @@ static Args args_of(const slx_gated_delta_shape *s, const Dims &d, const void *q
   return a;
 }
 
-// Zero: teams of four warps on 16 value channels, where each can have an SM to itself.  Else the warps of a CTA that hold 16
+// Zero: teams of eight warps on 16 value channels, where each can have an SM to itself.  Else the warps of a CTA that hold 16
 // channels each: as many as there are, up to four, which share a CTA's tiles.  Measured (T 2048, N 128, P 64, bf16, forward
 // and training, us) with 128 blocks of 16 channels: teams 141 / 384, warps 199 / 557; with 256 blocks: 269 / 708, 235 / 694;
 // fewer than four warps a CTA are never faster (512 blocks: four 316 / 1001, two 362 / 1114, one 455 / 1308).
