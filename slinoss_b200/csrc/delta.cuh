@@ -104,6 +104,11 @@ __device__ __forceinline__ float pow2(int e) {
 __device__ __forceinline__ int exp_of(unsigned bits) {
   return bits >= 0x7f800000u ? kNanExp : bits == 0u ? kZeroExp : max((int)(bits >> 23) - 127 - 14, kZeroExp);
 }
+// least e with |x| < 2^e (for the exponent of values times x)
+__device__ __forceinline__ int above(float x) {
+  const unsigned b = __float_as_uint(x) & 0x7fffffffu;
+  return b >= 0x7f800000u ? kNanExp : (int)(b >> 23) - 126;
+}
 // an exponent for a product's operand such that an accumulator of exponent ec, brought to the product's unit e + eb, stays
 // far inside the range (what the raising rounds away is 2^-40 of the accumulator)
 __device__ __forceinline__ int floor_exp(int e, int ec, int eb) { return max(e, ec - eb - 40); }

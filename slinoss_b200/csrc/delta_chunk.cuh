@@ -67,32 +67,69 @@ __global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_c
   __half *tri = reinterpret_cast<__half *>(smem);  // T hi, T lo, P hi, P lo
   float *A = reinterpret_cast<float *>(smem + chunk_tiles<NT, SI>());
   __shared__ double G[L];
-  __shared__ float beta[L], rise[L], fall[96], near[4][16 * kNearLd];
+  __shared__ float beta[L], rise[L], fall[96];
   __shared__ unsigned tops[8];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int chunk = blockIdx.x, b = blockIdx.y / a.key_heads, kh = blockIdx.y % a.key_heads;
   const int share = a.heads / a.key_heads, t0 = chunk * L, rows = min(L, a.T - t0);
 
-  // the gates of a head, two tokens per lane of warp 0; past the end g = 0 and beta = 0
-  float gate[2], write[2];
-  auto fetch = [&](int h) {
+  // near pairs of block w lie in a block of A above the diagonal
+  auto near_at = [&](int w, int r, int c) -> float & { return A[((w < 3 ? 0 : 16) + r) * kAld + (w < 3 ? 16 * w + 16 : 32) + c]; };
+  In kx, qx;  // (on their way while the gates are read)
+  kx.load(head_base<TI>(a.k, b, kh, t0), a.k.st, rows, a.N, a.k.vec, ks);
+  qx.load(head_base<TI>(a.q, b, kh, t0), a.q.st, rows, a.N, a.q.vec, qs);
+  float kk[8][4], qk[8][4];  // rows 16 warp .. + 15 of k k^T and q k^T, columns up to the diagonal block
+  int eq = 0, ek = 0;
+
+  auto gates = [&](int h, Record *rec) {  // of one head, to shared memory and its record
+    if (warp == 0) {  // two tokens per lane; past the end g = 0 and beta = 0
+      double gg[2];
+      float write[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = 2 * lane + i;
-      gate[i] = write[i] = 0.f;
-      if (t < rows) {
-        gate[i] = load_as_f(a.g.p, a.g_dtype, b * a.g.sb + h * a.g.sh + (int64_t)(t0 + t) * a.g.st);
-        write[i] = load_as_f(a.beta.p, a.beta_dtype, b * a.beta.sb + h * a.beta.sh + (int64_t)(t0 + t) * a.beta.st);
+      for (int i = 0; i < 2; ++i) {
+        const int t = 2 * lane + i;
+        gg[i] = 0.0;
+        write[i] = 0.f;
+        if (t < rows) {
+          const double x = load_as_f(a.g.p, a.g_dtype, b * a.g.sb + h * a.g.sh + (int64_t)(t0 + t) * a.g.st);
+          gg[i] = x < kLowestGate ? kLowestGate : x;
+          write[i] = load_as_f(a.beta.p, a.beta_dtype, b * a.beta.sb + h * a.beta.sh + (int64_t)(t0 + t) * a.beta.st);
+        }
       }
+      const double pair = gg[0] + gg[1];
+      double run = pair;
+      for (int d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_up_sync(~0u, run, d);
+        if (lane >= d) run += o;
+      }
+      *reinterpret_cast<double2 *>(G + 2 * lane) = make_double2(run - pair + gg[0], run);
+      *reinterpret_cast<float2 *>(rec->beta + 2 * lane) = make_float2(write[0], write[1]);
+      *reinterpret_cast<float2 *>(beta + 2 * lane) = make_float2(write[0], write[1]);
+    }
+    __syncthreads();
+    if (tid < L) {
+      const float x = expf((float)(G[tid] - (tid < 16 ? 0.0 : G[(tid & ~15) - 1])));
+      rise[tid] = rec->rise[tid] = x;
+      rec->gamma[tid] = expf((float)G[tid]);
+    } else {
+      rec->closing[tid - L] = expf((float)(G[L - 1] - G[tid - L]));
+    }
+    if (tid < 96) {
+      const int i = tid < 16 ? 1 : tid < 48 ? 2 : 3;
+      const float x = expf((float)(G[16 * i - 1] - G[tid - fall_at(i)]));
+      fall[tid] = rec->fall[tid] = x;
+    }
+#pragma unroll 4
+    for (int i = lane; i < 256; i += 32) {  // this warp's block of near pairs
+      const int r = i / 16, c = i % 16;
+      const float x = c <= r ? expf((float)(G[16 * warp + r] - G[16 * warp + c])) : 0.f;
+      near_at(warp, r, c) = rec->near[warp][r * kNearLd + c] = x;
     }
   };
-  if (warp == 0) fetch(kh * share);
-  int eq = 0, ek = 0;
+  auto record_of = [&](int h) { return a.rec + (size_t)(b * a.heads + h) * a.NC + chunk; };
+  gates(kh * share, record_of(kh * share));
   {
-    In kx, qx;
-    kx.load(head_base<TI>(a.k, b, kh, t0), a.k.st, rows, a.N, a.k.vec, ks);
-    qx.load(head_base<TI>(a.q, b, kh, t0), a.q.st, rows, a.N, a.q.vec, qs);
     if constexpr (!std::is_same<TI, __half>::value) {
       const unsigned mq = __reduce_max_sync(~0u, qx.max_bits()), mk = __reduce_max_sync(~0u, kx.max_bits());
       if (lane == 0) {
@@ -106,75 +143,38 @@ __global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_c
     __half *copy = a.kq + ((size_t)blockIdx.y * a.NC + chunk) * 2 * Op::halves;
     kx.template store<SI, true>(ks, copy, ek);
     qx.template store<SI, true>(qs, copy + Op::halves, eq);
-  }
-  __syncthreads();
-
-  // rows 16 warp .. + 15 of k k^T and q k^T, columns up to the diagonal block
-  float kk[8][4], qk[8][4];
-  zero(kk);
-  zero(qk);
-#pragma unroll 2
-  for (int kb = 0; kb < NT / 16; ++kb) {
-    Frag<SI> fk, fq;
-#pragma unroll
-    for (int s = 0; s < SI; ++s) {
-      a_mk(fk.r[s], ks + s * Op::plane + 16 * warp * Op::ld + 16 * kb, Op::ld);
-      a_mk(fq.r[s], qs + s * Op::plane + 16 * warp * Op::ld + 16 * kb, Op::ld);
-    }
-#pragma unroll
-    for (int sb = 0; sb < 4; ++sb)
-      if (sb <= warp) {
-        uint32_t bb[SI][4];
-#pragma unroll
-        for (int s = 0; s < SI; ++s) b_nk(bb[s], ks + s * Op::plane + 16 * sb * Op::ld + 16 * kb, Op::ld);
-        mma_split<SI, SI>(kk[2 * sb], kk[2 * sb + 1], fk, bb);
-        mma_split<SI, SI>(qk[2 * sb], qk[2 * sb + 1], fq, bb);
-      }
-  }
-  const float fkk = pow2(ek), fqk = pow2(eq);  // (two factors: their product may leave the range where the results do not)
-  times(kk, fkk);
-  times(kk, fkk);
-  times(qk, fqk);
-  times(qk, fkk);
-
-  for (int hs = 0; hs < share; ++hs) {
-    const int h = kh * share + hs;
-    Record *rec = a.rec + (size_t)(b * a.heads + h) * a.NC + chunk;
-    if (warp == 0) {
-      double gg[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) gg[i] = gate[i] < kLowestGate ? kLowestGate : (double)gate[i];
-      const double pair = gg[0] + gg[1];
-      double run = pair;
-      for (int d = 1; d < 32; d <<= 1) {
-        const double o = __shfl_up_sync(~0u, run, d);
-        if (lane >= d) run += o;
-      }
-      const double before = run - pair, last = __shfl_sync(~0u, run, 31), s0 = before + gg[0], s1 = before + pair;
-      *reinterpret_cast<double2 *>(G + 2 * lane) = make_double2(s0, s1);
-      *reinterpret_cast<float2 *>(rec->gamma + 2 * lane) = make_float2(expf((float)s0), expf((float)s1));
-      *reinterpret_cast<float2 *>(rec->closing + 2 * lane) = make_float2(expf((float)(last - s0)), expf((float)(last - s1)));
-      *reinterpret_cast<float2 *>(rec->beta + 2 * lane) = make_float2(write[0], write[1]);
-      *reinterpret_cast<float2 *>(beta + 2 * lane) = make_float2(write[0], write[1]);
-      if (hs + 1 < share) fetch(h + 1);
-    }
-    __syncthreads();  // (also: k and q have been read)
-    if (tid < L) {
-      const float x = expf((float)(G[tid] - (tid < 16 ? 0.0 : G[(tid & ~15) - 1])));
-      rise[tid] = rec->rise[tid] = x;
-    }
-    if (tid < 96) {
-      const int i = tid < 16 ? 1 : tid < 48 ? 2 : 3;
-      const float x = expf((float)(G[16 * i - 1] - G[tid - fall_at(i)]));
-      fall[tid] = rec->fall[tid] = x;
-    }
-#pragma unroll 2
-    for (int i = lane; i < 256; i += 32) {  // this warp's block of near pairs
-      const int r = i / 16, c = i % 16;
-      const float x = c <= r ? expf((float)(G[16 * warp + r] - G[16 * warp + c])) : 0.f;
-      near[warp][r * kNearLd + c] = rec->near[warp][r * kNearLd + c] = x;
-    }
     __syncthreads();
+    zero(kk);
+    zero(qk);
+#pragma unroll 2
+    for (int kb = 0; kb < NT / 16; ++kb) {
+      Frag<SI> fk, fq;
+#pragma unroll
+      for (int s = 0; s < SI; ++s) {
+        a_mk(fk.r[s], ks + s * Op::plane + 16 * warp * Op::ld + 16 * kb, Op::ld);
+        a_mk(fq.r[s], qs + s * Op::plane + 16 * warp * Op::ld + 16 * kb, Op::ld);
+      }
+#pragma unroll
+      for (int sb = 0; sb < 4; ++sb)
+        if (sb <= warp) {
+          uint32_t bb[SI][4];
+#pragma unroll
+          for (int s = 0; s < SI; ++s) b_nk(bb[s], ks + s * Op::plane + 16 * sb * Op::ld + 16 * kb, Op::ld);
+          mma_split<SI, SI>(kk[2 * sb], kk[2 * sb + 1], fk, bb);
+          mma_split<SI, SI>(qk[2 * sb], qk[2 * sb + 1], fq, bb);
+        }
+    }
+    const float fkk = pow2(ek), fqk = pow2(eq);  // (two factors: their product may leave the range where the results do not)
+    times(kk, fkk);
+    times(kk, fkk);
+    times(qk, fqk);
+    times(qk, fkk);
+  }
+  __syncthreads();  // (the tables are there; k and q have been read)
+
+#pragma unroll 1
+  for (int hs = 0; hs < share; ++hs) {
+    Record *rec = record_of(kh * share + hs);
 
     float pp[8][4];
     zero(pp);
@@ -182,16 +182,27 @@ __global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_c
     for (int j = 0; j < 8; ++j)
       if (j <= 2 * warp + 1) {
         float m[4];
-        const bool diagonal = j >= 2 * warp;
+        const int c = 8 * j + 2 * q;
+        const float2 be = *reinterpret_cast<const float2 *>(beta + c);
+        if (j >= 2 * warp) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 16 * warp + g + (i >> 1) * 8, c = 8 * j + 2 * q + (i & 1);
-          const float dec = diagonal ? near[warp][(r & 15) * kNearLd + (c & 15)] : rise[r] * fall[fall_at(warp) + c];
-          pp[j][i] = c <= r ? dec * qk[j][i] : 0.f;
-          m[i] = c < r ? dec * kk[j][i] * beta[c] : 0.f;
+          for (int i = 0; i < 4; ++i) {
+            const int r = g + (i >> 1) * 8, cc = (c & 15) + (i & 1);
+            const float dec = near_at(warp, r, cc);  // (zero above the diagonal)
+            pp[j][i] = cc <= r ? dec * qk[j][i] : 0.f;
+            m[i] = cc < r ? dec * kk[j][i] * (i & 1 ? be.y : be.x) : 0.f;
+          }
+        } else {
+          const float2 fa = *reinterpret_cast<const float2 *>(fall + fall_at(warp) + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float dec = rise[16 * warp + g + (i >> 1) * 8] * (i & 1 ? fa.y : fa.x);
+            pp[j][i] = dec * qk[j][i];
+            m[i] = dec * kk[j][i] * (i & 1 ? be.y : be.x);
+          }
         }
-        *reinterpret_cast<float2 *>(A + (16 * warp + g) * kAld + 8 * j + 2 * q) = make_float2(m[0], m[1]);
-        *reinterpret_cast<float2 *>(A + (16 * warp + g + 8) * kAld + 8 * j + 2 * q) = make_float2(m[2], m[3]);
+        *reinterpret_cast<float2 *>(A + (16 * warp + g) * kAld + c) = make_float2(m[0], m[1]);
+        *reinterpret_cast<float2 *>(A + (16 * warp + g + 8) * kAld + c) = make_float2(m[2], m[3]);
       }
     const unsigned mp = __reduce_max_sync(~0u, max_mag(pp));
     if (lane == 0) tops[warp] = mp;
@@ -285,7 +296,11 @@ __global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_c
 #pragma unroll
     for (int i = 0; i < 4 * kTri / 8 / kThreads; ++i) dst[tid + i * kThreads] = src[tid + i * kThreads];
     if (tid == 0) *reinterpret_cast<int4 *>(&rec->eT) = make_int4(eT, eQ, eq, ek);
-    __syncthreads();  // G, beta, A and tri are written again
+    if (hs + 1 < share) {  // G, beta, A and tri are written again
+      __syncthreads();
+      gates(kh * share + hs + 1, record_of(kh * share + hs + 1));
+      __syncthreads();
+    }
   }
 }
 

@@ -173,13 +173,9 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
 #pragma unroll
     for (int s = 0; s < SC; ++s) b_nk(f[s], tile + s * kTile + 16 * rb * kTileLd + 16 * kb, kTileLd);
   };
-  // decay from an earlier token c of block cb to a later one r of block rb (zero where c comes later in the same block)
-  auto decay = [&](int r, int c, int rb, int cb) {
-    return rb == cb ? near[rb * 16 * kNearLd + (r & 15) * kNearLd + (c & 15)] : rise[r] * fall[fall_at(rb) + c];
-  };
-
   float acc[NT / 8][4];
   // ---- Z, this warp's tokens as s
+  int unit;  // of acc
   float2 w, db;
   float dot = 0.f;
   {
@@ -237,23 +233,45 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     }
     dot *= pow2(sr_top);
     const float fr = pow2(yr_top);
-    times_rows(acc, closing[r0] * fr, closing[r1] * fr);
     w = row_dots<NT, SI>(acc, krow, ek);
-    const float fq = a.scale * pow2(y_top + eo_top), fh = -pow2(yx_top);
+    w.x *= closing[r0] * fr;
+    w.y *= closing[r1] * fr;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j >= 2 * warp)
+    for (int tb = 0; tb < 4; ++tb)
+      if (tb >= warp) {
+        const float f0 = tb > warp ? fall[fall_at(tb) + r0] : 1.f, f1 = tb > warp ? fall[fall_at(tb) + r1] : 1.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int s = i < 2 ? r0 : r1, t = 8 * j + 2 * q + (i & 1);
-          const float dec = decay(t, s, j / 2, warp);
-          Q[j][i] = t >= s ? Q[j][i] * fq * dec : 0.f;
-          H[j][i] = t > s ? H[j][i] * fh * dec : 0.f;
+        for (int j = 2 * tb; j < 2 * tb + 2; ++j) {
+          const int t = 8 * j + 2 * q;
+          if (tb == warp) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int s = g + (i >> 1) * 8, tt = (t & 15) + (i & 1);
+              const float dec = near[(warp * 16 + tt) * kNearLd + s];  // (zero where s comes later)
+              Q[j][i] = tt >= s ? Q[j][i] * dec : 0.f;
+              H[j][i] = tt > s ? H[j][i] * dec : 0.f;
+            }
+          } else {
+            const float2 up = *reinterpret_cast<const float2 *>(rise + t);
+            const float d[4] = {up.x * f0, up.y * f0, up.x * f1, up.y * f1};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              Q[j][i] *= d[i];
+              H[j][i] *= d[i];
+            }
+          }
         }
-    const int ec = warp_exp(acc), e1 = floor_exp(warp_exp(Q), ec, eq);
-    const int e2 = floor_exp(warp_exp(H), max(ec, e1 + eq + 21) + 1, ek);
-    times(acc, pow2(-(e1 + eq)));
-    const float s1 = pow2(-e1), s2 = pow2(-e2);
+      }
+    // Q and H still lack a factor each, which joins their scaling; the sum takes closing and its unit in one
+    const float fq = a.scale * pow2(y_top + eo_top), fh = -pow2(yx_top);
+    const float top = __uint_as_float(__reduce_max_sync(~0u, max(mag(closing[r0]), mag(closing[r1]))));
+    const int ec = warp_exp(acc) + yr_top + above(top), e1 = floor_exp(warp_exp(Q) + above(fq), ec, eq);
+    const int e2 = floor_exp(warp_exp(H) + yx_top, max(ec, e1 + eq + 21) + 1, ek);
+    {
+      const float u = fr * pow2(-(e1 + eq));
+      times_rows(acc, closing[r0] * u, closing[r1] * u);
+    }
+    const float s1 = fq * pow2(-e1), s2 = fh * pow2(-e2);
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
       if (kb >= warp) {
@@ -269,9 +287,10 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
         frag_of<SC>(f, H[2 * kb], H[2 * kb + 1], s2);
         tile_cols<SC, SI, NT>(acc, f, ks, Op::plane, kb);
       }
-    times(acc, pow2(e2 + ek));
+    unit = e2 + ek;  // (acc is Z without its unit)
     db = row_dots<NT, SI>(acc, krow, ek);
-    times_rows(acc, beta[r0], beta[r1]);
+    db.x *= pow2(unit);
+    db.y *= pow2(unit);
   }
   __syncthreads();  // (R is not read any more: its room takes results on their way out)
   __half *buf = rs + warp * 16 * ld;
@@ -286,14 +305,25 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     const float f = is_q ? a.scale : -1.f;
     float H[8][4];
     zero(H);
-    if (is_q) zero(acc);
     const int ya = ey + ea, sa = es + ea;
     const int ya_top = __reduce_max_sync(~0u, ya), sa_top = __reduce_max_sync(~0u, sa);
     // f gamma times the tile as an operand: the factor, which exceeds one where gates do, enters the product's unit
     const float g0 = f * gamma[r0], g1 = f * gamma[r1];
     const int top = __reduce_max_sync(~0u, max(mag(g0), mag(g1)));
-    const int unit = max(sa_top + max((top >> 23) - 127 + 1, 0), warp_exp(acc) - 40);
-    times(acc, pow2(-unit));
+    float b0 = 0.f, b1 = 0.f;  // dk takes beta Z over
+    int held = kZeroExp;
+    if (!is_q) {
+      b0 = beta[r0];
+      b1 = beta[r1];
+      held = warp_exp(acc) + unit + above(__uint_as_float(__reduce_max_sync(~0u, max(mag(b0), mag(b1)))));
+    }
+    const int before = unit;
+    unit = max(sa_top + max((top >> 23) - 127 + 1, 0), held - 40);
+    {
+      const float u = pow2(max(before - unit, -126));
+      if (is_q) zero(acc);
+      else times_rows(acc, b0 * u, b1 * u);
+    }
 #pragma unroll 1
     for (int pt = 0; pt < tiles; ++pt) {
       if (tiles > 1) {
@@ -327,19 +357,33 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
         tile_cols<SC, SC, NT>(acc, fg, ss, splane, kb);
       }
     }
-    times(acc, pow2(unit));
-    const float fh = f * pow2(ya_top);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j <= 2 * warp + 1)
+    for (int sb = 0; sb < 4; ++sb)
+      if (sb <= warp) {
+        const float f0 = sb < warp ? rise[r0] : 1.f, f1 = sb < warp ? rise[r1] : 1.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i < 2 ? r0 : r1, c = 8 * j + 2 * q + (i & 1);
-          H[j][i] = c < r + part ? H[j][i] * fh * decay(r, c, warp, j / 2) * beta[c] : 0.f;
+        for (int j = 2 * sb; j < 2 * sb + 2; ++j) {
+          const int c = 8 * j + 2 * q;
+          const float2 be = *reinterpret_cast<const float2 *>(beta + c);
+          if (sb == warp) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = g + (i >> 1) * 8, cc = (c & 15) + (i & 1);
+              const float dec = near[(warp * 16 + r) * kNearLd + cc] * (i & 1 ? be.y : be.x);
+              H[j][i] = cc < r + part ? H[j][i] * dec : 0.f;
+            }
+          } else {
+            const float2 fa = *reinterpret_cast<const float2 *>(fall + fall_at(warp) + c);
+            const float x = fa.x * be.x, y = fa.y * be.y;
+            const float d[4] = {f0 * x, f0 * y, f1 * x, f1 * y};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) H[j][i] *= d[i];
+          }
         }
-    const int e = floor_exp(warp_exp(H), warp_exp(acc), ek);
-    times(acc, pow2(-(e + ek)));
-    const float s = pow2(-e);
+      }
+    const int e = floor_exp(warp_exp(H) + ya_top + above(f), warp_exp(acc) + unit, ek);
+    times(acc, pow2(unit - (e + ek)));
+    const float s = f * pow2(ya_top - e);
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
       if (kb <= warp) {
