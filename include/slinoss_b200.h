@@ -482,12 +482,14 @@ typedef struct {
 } slx_gated_delta_shape;
 
 size_t slx_gated_delta_fwd_workspace_bytes(const slx_gated_delta_shape *s);
-/* What the backward needs of the forward (states before every chunk, prediction errors). */
+/* What the forward keeps for the backward, in the place of its inputs: per 64 tokens the triangular
+ * matrices, scaled fp16 tiles of k and q, the states before them and the prediction errors. */
 size_t slx_gated_delta_residual_bytes(const slx_gated_delta_shape *s);
 size_t slx_gated_delta_bwd_workspace_bytes(const slx_gated_delta_shape *s);
 
 /* o (contiguous) may be NULL: then only the states are computed.  final_state is fp32.
- * workspace and residual 256-byte aligned. */
+ * workspace and residual 256-byte aligned; the workspace is needed (and read) only without a
+ * residual. */
 int slx_gated_delta_fwd(const slx_gated_delta_shape *s, const void *q, const void *k, const void *v,
                         const void *g, const void *beta, const void *initial_state /*[opt]*/,
                         int32_t initial_dtype, void *o /*[opt]*/, float *final_state /*[opt]*/,
@@ -496,9 +498,8 @@ int slx_gated_delta_fwd(const slx_gated_delta_shape *s, const void *q, const voi
 
 /* VJP of slx_gated_delta_fwd.  d_o (batch, heads, T, P) contiguous; d_final (batch, heads, P, N).
  * dq, dk (batch, key_heads, T, N), dv, dg, dbeta are contiguous and overwritten; sums run in a
- * fixed order (no atomics). */
-int slx_gated_delta_bwd(const slx_gated_delta_shape *s, const void *q, const void *k, const void *g,
-                        const void *beta, const void *residual, const void *d_o,
+ * fixed order (no atomics).  The strides of the shape are not read. */
+int slx_gated_delta_bwd(const slx_gated_delta_shape *s, const void *residual, const void *d_o,
                         const void *d_final /*[opt]*/, int32_t d_final_dtype, void *dq, void *dk,
                         void *dv, void *dg, void *dbeta, void *d_initial /*[opt]*/,
                         int32_t d_initial_dtype, void *workspace, size_t workspace_bytes,

@@ -114,7 +114,7 @@ SIGNATURES = {
     "slx_gated_delta_residual_bytes": (c_size_t, [POINTER(GatedDeltaShape)]),
     "slx_gated_delta_bwd_workspace_bytes": (c_size_t, [POINTER(GatedDeltaShape)]),
     "slx_gated_delta_fwd": (c_int32, [POINTER(GatedDeltaShape)] + [_P] * 6 + [c_int32] + [_P] * 4 + [c_size_t, _P]),
-    "slx_gated_delta_bwd": (c_int32, [POINTER(GatedDeltaShape)] + [_P] * 7 + [c_int32] + [_P] * 6
+    "slx_gated_delta_bwd": (c_int32, [POINTER(GatedDeltaShape)] + [_P] * 3 + [c_int32] + [_P] * 6
                             + [c_int32, _P, c_size_t, _P]),
     "slx_gated_delta_step": (c_int32, [POINTER(GatedDeltaShape)] + [_P] * 9),
     "slx_sample": (c_int32, [POINTER(SampleShape)] + [_P] * 8),

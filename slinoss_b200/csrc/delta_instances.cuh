@@ -43,7 +43,6 @@ static int launch_fwd(const Args &a, int warps, cudaStream_t st) {
 }
 template <int NT, int SI, int SC, typename TI>
 static int launch_bwd(const Args &a, void *dq, void *dk, int warps, cudaStream_t st) {
-  if (const int rc = launch_chunk<NT, SI, SC, TI>(a, st)) return rc;
   bool done = false;
   if constexpr (has_team<NT, SI>) {
     if (warps == 0) {

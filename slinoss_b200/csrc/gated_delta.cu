@@ -1,8 +1,9 @@
 // Gated delta rule: C-ABI entry points of the chunked operator (forward, backward).
 //
-// Forward: the chunks' triangular matrices (delta_chunk.cuh), then one pass along the sequence (delta_scan.cuh).  Backward:
-// the triangular matrices again (they are 26 KB per chunk and head, more than the inputs they come from), the pass back along
-// the sequence, then the gradients of every chunk by itself (delta_grad.cuh).
+// Forward: the chunks' triangular matrices (delta_chunk.cuh), then one pass along the sequence (delta_scan.cuh, delta_team.cuh).
+// Backward: the pass back along the sequence, then the gradients of every chunk by itself (delta_grad.cuh).  What the forward
+// has made of a chunk is kept for it: the matrices, the scaled tiles of k and q (in the place of k and q themselves), the states
+// and the prediction errors.
 #include "delta_launch.cuh"
 
 namespace slx {
@@ -62,10 +63,8 @@ static Rows rows_of(const void *p, const int64_t *st, const slx_gated_delta_shap
   r.vec = (reinterpret_cast<uintptr_t>(p) & 15) == 0 && r.sb % v == 0 && r.sh % v == 0 && r.st % v == 0 && width % v == 0;
   return r;
 }
-static Args args_of(const slx_gated_delta_shape *s, const Dims &d, const void *q, const void *k, const void *g,
-                    const void *beta, void *workspace) {
+static Args args_of(const slx_gated_delta_shape *s, const Dims &d) {
   Args a{};
-  const int size = s->dtype == SLX_F32 ? 4 : 2;
   a.batch = s->batch;
   a.heads = s->heads;
   a.key_heads = s->key_heads;
@@ -77,12 +76,6 @@ static Args args_of(const slx_gated_delta_shape *s, const Dims &d, const void *q
   a.scale = s->scale;
   a.g_dtype = s->g_dtype;
   a.beta_dtype = s->beta_dtype;
-  a.q = rows_of(q, s->q_stride, s, s->key_heads, s->N, size);
-  a.k = rows_of(k, s->k_stride, s, s->key_heads, s->N, size);
-  a.g = rows_of(g, s->g_stride, s, s->heads, 1, 4);
-  a.beta = rows_of(beta, s->beta_stride, s, s->heads, 1, 4);
-  a.rec = static_cast<Record *>(workspace);
-  a.kq = reinterpret_cast<__half *>(static_cast<char *>(workspace) + record_bytes(d));
   return a;
 }
 
@@ -101,23 +94,44 @@ static int scan_warps(const Dims &d) {
 using namespace slx;
 using namespace slx::delta;
 
+// what the forward keeps, in this order: records, tiles of k and q, states, errors, exponents of both
+struct Kept {
+  size_t keys, states, values, exps, bytes;
+};
+static Kept kept_of(const slx_gated_delta_shape *s, const Dims &d) {
+  Kept k;
+  k.keys = record_bytes(d);
+  k.states = k.keys + keys_bytes(s, d);
+  k.values = k.states + state_bytes(d);
+  k.exps = k.values + value_bytes(d);
+  k.bytes = k.exps + 2 * exp_bytes(d);
+  return k;
+}
+static void place_kept(Args &a, const Kept &k, const Dims &d, const void *residual) {
+  char *r = static_cast<char *>(const_cast<void *>(residual));
+  a.rec = reinterpret_cast<Record *>(r);
+  a.kq = reinterpret_cast<__half *>(r + k.keys);
+  a.st = reinterpret_cast<__half *>(r + k.states);
+  a.y = reinterpret_cast<__half *>(r + k.values);
+  a.est = reinterpret_cast<int *>(r + k.exps);
+  a.ey = reinterpret_cast<int *>(r + k.exps + exp_bytes(d));
+}
+
 extern "C" size_t slx_gated_delta_fwd_workspace_bytes(const slx_gated_delta_shape *s) {
   if (check_shape(s, "gated_delta") != SLX_OK) return 0;
   const Dims d = dims_of(s);
   return record_bytes(d) + keys_bytes(s, d);
 }
 extern "C" size_t slx_gated_delta_residual_bytes(const slx_gated_delta_shape *s) {
-  if (check_shape(s, "gated_delta") != SLX_OK) return 0;
-  const Dims d = dims_of(s);
-  return state_bytes(d) + value_bytes(d) + 2 * exp_bytes(d);
+  return check_shape(s, "gated_delta") == SLX_OK ? kept_of(s, dims_of(s)).bytes : 0;
 }
 extern "C" size_t slx_gated_delta_bwd_workspace_bytes(const slx_gated_delta_shape *s) {
   if (check_shape(s, "gated_delta") != SLX_OK) return 0;
   const Dims d = dims_of(s);
-  return record_bytes(d) + keys_bytes(s, d) + state_bytes(d) + value_bytes(d) + 3 * exp_bytes(d) + 2 * share_bytes(s);
+  return state_bytes(d) + value_bytes(d) + 3 * exp_bytes(d) + 2 * share_bytes(s);
 }
 
-static int check_common(const slx_gated_delta_shape *s, const char *what, const void *workspace, size_t have, size_t need) {
+static int check_workspace(const char *what, const void *workspace, size_t have, size_t need) {
   SLX_REQUIRE(workspace, SLX_E_NULL, "%s: workspace is NULL", what);
   SLX_REQUIRE(have >= need, SLX_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, have, need);
   SLX_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, SLX_E_WORKSPACE, "%s: workspace must be 256-byte aligned",
@@ -141,10 +155,13 @@ extern "C" int slx_gated_delta_fwd(const slx_gated_delta_shape *s, const void *q
   SLX_REQUIRE(q && k && v && g && beta, SLX_E_NULL, "gated_delta_fwd: q, k, v, g and beta must not be NULL");
   SLX_REQUIRE(!initial_state || known(initial_dtype), SLX_E_DTYPE, "gated_delta_fwd: unknown initial_dtype %d", initial_dtype);
   const Dims d = dims_of(s);
-  if (const int rc = check_common(s, "gated_delta_fwd", workspace, workspace_bytes,
-                                  slx_gated_delta_fwd_workspace_bytes(s))) return rc;
-  Args a = args_of(s, d, q, k, g, beta, workspace);
-  a.v = rows_of(v, s->v_stride, s, s->heads, s->P, s->dtype == SLX_F32 ? 4 : 2);
+  Args a = args_of(s, d);
+  const int size = s->dtype == SLX_F32 ? 4 : 2;
+  a.q = rows_of(q, s->q_stride, s, s->key_heads, s->N, size);
+  a.k = rows_of(k, s->k_stride, s, s->key_heads, s->N, size);
+  a.v = rows_of(v, s->v_stride, s, s->heads, s->P, size);
+  a.g = rows_of(g, s->g_stride, s, s->heads, 1, 4);
+  a.beta = rows_of(beta, s->beta_stride, s, s->heads, 1, 4);
   a.init = initial_state;
   a.init_dtype = initial_dtype;
   a.o = o;
@@ -152,11 +169,12 @@ extern "C" int slx_gated_delta_fwd(const slx_gated_delta_shape *s, const void *q
   if (residual) {
     SLX_REQUIRE((reinterpret_cast<uintptr_t>(residual) & 255) == 0, SLX_E_WORKSPACE,
                 "gated_delta_fwd: residual must be 256-byte aligned");
-    char *r = static_cast<char *>(residual);
-    a.st = reinterpret_cast<__half *>(r);
-    a.y = reinterpret_cast<__half *>(r + state_bytes(d));
-    a.est = reinterpret_cast<int *>(r + state_bytes(d) + value_bytes(d));
-    a.ey = reinterpret_cast<int *>(r + state_bytes(d) + value_bytes(d) + exp_bytes(d));
+    place_kept(a, kept_of(s, d), d, residual);
+  } else {
+    if (const int rc = check_workspace("gated_delta_fwd", workspace, workspace_bytes, slx_gated_delta_fwd_workspace_bytes(s)))
+      return rc;
+    a.rec = static_cast<Record *>(workspace);
+    a.kq = reinterpret_cast<__half *>(static_cast<char *>(workspace) + record_bytes(d));
   }
   const int warps = scan_warps(d);
   cudaStream_t st = as_stream(stream);
@@ -165,30 +183,23 @@ extern "C" int slx_gated_delta_fwd(const slx_gated_delta_shape *s, const void *q
 #undef ARGS_
 }
 
-extern "C" int slx_gated_delta_bwd(const slx_gated_delta_shape *s, const void *q, const void *k, const void *g,
-                                   const void *beta, const void *residual, const void *d_o, const void *d_final,
+extern "C" int slx_gated_delta_bwd(const slx_gated_delta_shape *s, const void *residual, const void *d_o, const void *d_final,
                                    int32_t d_final_dtype, void *dq, void *dk, void *dv, void *dg, void *dbeta, void *d_initial,
                                    int32_t d_initial_dtype, void *workspace, size_t workspace_bytes, void *stream) {
   if (const int rc = check_shape(s, "gated_delta_bwd")) return rc;
-  SLX_REQUIRE(q && k && g && beta && residual && d_o && dq && dk && dv && dg && dbeta, SLX_E_NULL,
-              "gated_delta_bwd: a required pointer is NULL");
+  SLX_REQUIRE(residual && d_o && dq && dk && dv && dg && dbeta, SLX_E_NULL, "gated_delta_bwd: a required pointer is NULL");
   SLX_REQUIRE(!d_final || known(d_final_dtype), SLX_E_DTYPE, "gated_delta_bwd: unknown d_final_dtype %d", d_final_dtype);
   SLX_REQUIRE(!d_initial || known(d_initial_dtype), SLX_E_DTYPE, "gated_delta_bwd: unknown d_initial_dtype %d", d_initial_dtype);
   const Dims d = dims_of(s);
-  if (const int rc = check_common(s, "gated_delta_bwd", workspace, workspace_bytes, slx_gated_delta_bwd_workspace_bytes(s)))
+  if (const int rc = check_workspace("gated_delta_bwd", workspace, workspace_bytes, slx_gated_delta_bwd_workspace_bytes(s)))
     return rc;
   SLX_REQUIRE((reinterpret_cast<uintptr_t>(residual) & 255) == 0, SLX_E_WORKSPACE,
               "gated_delta_bwd: residual must be 256-byte aligned");
   char *w = static_cast<char *>(workspace);
-  Args a = args_of(s, d, q, k, g, beta, w);
+  Args a = args_of(s, d);
+  place_kept(a, kept_of(s, d), d, residual);
   const int64_t o_stride[3] = {(int64_t)s->heads * s->T * s->P, (int64_t)s->T * s->P, s->P};
   a.dO = rows_of(d_o, o_stride, s, s->heads, s->P, s->dtype == SLX_F32 ? 4 : 2);
-  char *r = static_cast<char *>(const_cast<void *>(residual));
-  a.st = reinterpret_cast<__half *>(r);
-  a.y = reinterpret_cast<__half *>(r + state_bytes(d));
-  a.est = reinterpret_cast<int *>(r + state_bytes(d) + value_bytes(d));
-  a.ey = reinterpret_cast<int *>(r + state_bytes(d) + value_bytes(d) + exp_bytes(d));
-  w += record_bytes(d) + keys_bytes(s, d);
   a.ds = reinterpret_cast<__half *>(w);
   w += state_bytes(d);
   a.dx = reinterpret_cast<__half *>(w);

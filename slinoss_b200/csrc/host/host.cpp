@@ -965,8 +965,9 @@ DeltaForward delta_forward(const DeltaDims &d, const Tensor &q, const Tensor &k,
   if (want_o) r.o = empty({d.b, d.h, d.T, d.P}, d.act, d.dev);
   if (want_state) r.final_state = empty({d.b, d.h, d.P, d.N}, at::kFloat, d.dev);
   if (want_residual) r.residual = delta_bytes(slx_gated_delta_residual_bytes(&d.s), d.dev);
-  const size_t nbytes = slx_gated_delta_fwd_workspace_bytes(&d.s);
-  Tensor ws = delta_bytes(nbytes, d.dev);
+  const size_t nbytes = want_residual ? 0 : slx_gated_delta_fwd_workspace_bytes(&d.s);
+  Tensor ws;
+  if (nbytes) ws = delta_bytes(nbytes, d.dev);
   c10::cuda::CUDAGuard guard(d.dev);
   check(slx_gated_delta_fwd(&d.s, ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), cptr(init),
                             init ? code_of(init->scalar_type()) : SLX_F32, ptr(r.o), fptr(r.final_state), ptr(r.residual),
@@ -976,11 +977,12 @@ DeltaForward delta_forward(const DeltaDims &d, const Tensor &q, const Tensor &k,
 }
 
 struct DeltaBackward : public Node {
-  double scale = 1;
+  DeltaDims d{};
   bool recompute = false;
   std::optional<at::ScalarType> init_type;
+  std::vector<int64_t> k_sizes, v_sizes, g_sizes;
+  at::ScalarType g_type, beta_type;
   SavedVariable q_, k_, v_, g_, beta_, init_, residual_;
-  std::vector<int64_t> v_sizes;
   std::string name() const override { return "GatedDeltaRuleBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -991,35 +993,34 @@ struct DeltaBackward : public Node {
     variable_list out(6);
     const Tensor do_in = grads[0], df_in = grads.size() > 1 ? grads[1] : Tensor();
     if (!do_in.defined() && !df_in.defined()) return out;
-    // (a saved-tensor hook may return other strides, also of the last axis)
-    auto dense = [](Tensor t) { return t.size(-1) != 1 && t.stride(-1) != 1 ? t.contiguous() : t; };
-    const Tensor q = dense(saved(q_)), k = dense(saved(k_)), g = saved(g_), beta = saved(beta_);
-    Tensor v, residual, init;
-    if (recompute) v = dense(saved(v_));
-    else residual = saved(residual_);
-    // (without recomputing only the sizes of v are needed, and of its strides none)
-    const std::optional<DeltaDims> dims = delta_dims(q, k, recompute ? v : at::empty({v_sizes.back()}, q.options()).expand(v_sizes),
-                                                     g, beta, scale, true);
-    TORCH_CHECK(dims, "gated delta rule backward: saved tensors have changed");
-    const DeltaDims &d = *dims;
+    Tensor residual;
     if (recompute) {
+      // (a saved-tensor hook may return other strides, also of the last axis)
+      auto dense = [](Tensor t) { return t.size(-1) != 1 && t.stride(-1) != 1 ? t.contiguous() : t; };
+      const Tensor q = dense(saved(q_)), k = dense(saved(k_)), v = dense(saved(v_)), g = saved(g_), beta = saved(beta_);
+      OptTensor init;
       if (init_type) init = as_read(saved(init_), *init_type);
-      residual = delta_forward(d, q, k, v, g, beta, init.defined() ? OptTensor(init) : std::nullopt, false, false, true).residual;
+      const std::optional<DeltaDims> now = delta_dims(q, k, v, g, beta, d.s.scale, true);
+      TORCH_CHECK(now, "gated delta rule backward: a saved tensor has another form than in the forward");
+      residual = delta_forward(*now, q, k, v, g, beta, init, false, false, true).residual;
+    } else {
+      residual = as_read(saved(residual_), at::kByte);
     }
-    const Tensor dO = do_in.defined() ? as_read(do_in, d.act) : at::zeros(v_sizes, q.options());
+    const auto options = at::TensorOptions().dtype(d.act).device(d.dev);
+    const Tensor dO = do_in.defined() ? as_read(do_in, d.act) : at::zeros(v_sizes, options);
     Tensor d_final;
     if (df_in.defined())
       d_final = as_read(df_in, code_of(df_in.scalar_type()) < 0 ? at::kFloat : df_in.scalar_type());
-    out[0] = empty(q.sizes(), d.act, d.dev);
-    out[1] = empty(k.sizes(), d.act, d.dev);
+    out[0] = empty(k_sizes, d.act, d.dev);
+    out[1] = empty(k_sizes, d.act, d.dev);
     out[2] = empty(v_sizes, d.act, d.dev);
-    out[3] = empty(g.sizes(), g.scalar_type(), d.dev);
-    out[4] = empty(beta.sizes(), beta.scalar_type(), d.dev);
+    out[3] = empty(g_sizes, g_type, d.dev);
+    out[4] = empty(g_sizes, beta_type, d.dev);
     if (init_type) out[5] = empty({d.b, d.h, d.P, d.N}, *init_type, d.dev);
     const size_t nbytes = slx_gated_delta_bwd_workspace_bytes(&d.s);
     Tensor ws = delta_bytes(nbytes, d.dev);
     c10::cuda::CUDAGuard guard(d.dev);
-    check(slx_gated_delta_bwd(&d.s, ptr(q), ptr(k), ptr(g), ptr(beta), ptr(residual), ptr(dO), ptr(d_final),
+    check(slx_gated_delta_bwd(&d.s, ptr(residual), ptr(dO), ptr(d_final),
                               d_final.defined() ? code_of(d_final.scalar_type()) : SLX_F32, ptr(out[0]), ptr(out[1]),
                               ptr(out[2]), ptr(out[3]), ptr(out[4]), ptr(out[5]),
                               init_type ? code_of(*init_type) : SLX_F32, ptr(ws), nbytes, stream_of(d.dev)),
@@ -1044,18 +1045,22 @@ std::optional<std::vector<Tensor>> gated_delta_rule(const Tensor &q, const Tenso
   DeltaForward r = delta_forward(d, q, k, v, g, beta, init, true, want_state, grad && !recompute);
   if (grad) {
     auto node = make_node<DeltaBackward>(torch::autograd::collect_next_edges(q, k, v, g, beta, or_undefined(init)));
-    node->scale = scale;
+    node->d = d;
     node->recompute = recompute;
-    node->q_ = keep(q);
-    node->k_ = keep(k);
-    node->g_ = keep(g);
-    node->beta_ = keep(beta);
+    node->k_sizes = k.sizes().vec();
     node->v_sizes = v.sizes().vec();
+    node->g_sizes = g.sizes().vec();
+    node->g_type = g.scalar_type();
+    node->beta_type = beta.scalar_type();
     if (init) node->init_type = init->scalar_type();
-    // Kept for the backward: the states before every chunk and the prediction errors, or (recompute) v and the initial
-    // state, from which one more pass forms them again.
+    // Kept for the backward: what the forward's kernels have made of the inputs, and none of these, or (recompute) the
+    // inputs, from which one more pass forms it again.
     if (recompute) {
+      node->q_ = keep(q);
+      node->k_ = keep(k);
       node->v_ = keep(v);
+      node->g_ = keep(g);
+      node->beta_ = keep(beta);
       if (init) node->init_ = keep_value(*init);
     } else {
       node->residual_ = keep(r.residual);

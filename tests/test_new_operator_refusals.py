@@ -36,7 +36,7 @@ def test_shapes_that_no_kernel_takes(lib, kw, code):
     s = ctypes.byref(_shape(**kw))
     one = ctypes.c_void_p(256)
     assert lib.slx_gated_delta_fwd(s, *([one] * 5), None, 0, one, None, None, one, 1 << 40, None) == code
-    assert lib.slx_gated_delta_bwd(s, *([one] * 6), None, 0, *([one] * 5), None, 0, one, 1 << 40, None) == code
+    assert lib.slx_gated_delta_bwd(s, one, one, None, 0, *([one] * 5), None, 0, one, 1 << 40, None) == code
     assert lib.slx_gated_delta_fwd_workspace_bytes(s) == 0
     assert lib.slx_gated_delta_residual_bytes(s) == 0 and lib.slx_gated_delta_bwd_workspace_bytes(s) == 0
 
@@ -55,10 +55,12 @@ def test_pointers_and_workspaces(lib):
     assert fwd(*([one] * 5), one, 9, one, None, None, one, n) == -5
     m = lib.slx_gated_delta_bwd_workspace_bytes(r)
     bwd = lambda *a: lib.slx_gated_delta_bwd(r, *a, None)
-    assert bwd(*([one] * 4), None, one, None, 0, *([one] * 5), None, 0, one, m) == -1
-    assert bwd(*([one] * 6), None, 0, *([one] * 5), None, 0, one, m - 1) == -4
-    assert bwd(*([one] * 6), one, 5, *([one] * 5), None, 0, one, m) == -5
-    assert bwd(*([one] * 6), None, 0, *([one] * 5), one, 5, one, m) == -5
+    assert bwd(None, one, None, 0, *([one] * 5), None, 0, one, m) == -1
+    assert bwd(one, one, None, 0, *([one] * 4), None, None, 0, one, m) == -1
+    assert bwd(one, one, None, 0, *([one] * 5), None, 0, one, m - 1) == -4
+    assert bwd(ctypes.c_void_p(264), one, None, 0, *([one] * 5), None, 0, one, m) == -4
+    assert bwd(one, one, one, 5, *([one] * 5), None, 0, one, m) == -5
+    assert bwd(one, one, None, 0, *([one] * 5), one, 5, one, m) == -5
     one_token = _shape(T=1)
     step = lambda sh, *a: lib.slx_gated_delta_step(ctypes.byref(sh), *a, None)
     assert step(s, *([one] * 5), None, one, one) == -2  # T is not 1
