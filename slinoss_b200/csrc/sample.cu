@@ -11,9 +11,10 @@
 //   * Where no more than a few thousand tokens lie above the bin's lower edge, CTA 0 gathers, sorts and walks them, and the
 //     other CTAs are done.  Otherwise only the bin's own tokens are gathered for the border (a bin with too many is divided
 //     again by the integer keys of its logits), and the draw sums the tokens that stay where they are.
-//   * Masses that decide between tokens are exponentials in 64 bits, taken only for tokens that may stay, as integers of 2^-44
-//     of the largest: their sums do not depend on an order, and a draw is decided as exact sums would decide it but for about
-//     one in 10^7 (the whole mass that top_p alone refers to is summed in 32-bit exponentials).
+//   * Masses that decide anything are exponentials in 64 bits, held as integers of 2^-44 of the largest: their sums do not
+//     depend on an order.  The whole mass that top_p refers to is such a sum over every token: an error of 10^-6 in it moves
+//     the border past a token in ten, every draw by that token's mass, and one draw in a hundred into the neighbour, where ten
+//     thousand tokens stay.  Only the histogram is coarser; it names a bin, and its neighbours are looked at too.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -394,8 +395,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     __syncthreads();
   };
 
-  // ---- CTA 0 by itself: n tokens in its list, all down to the lower edge of `bin`, which holds the border of a filter:
-  // with masses top_p's, at the mass `want`; else top_k's, `above` tokens lying in the bins before.
+  // ---- CTA 0 by itself: n tokens in its list.  With masses all down to the bin after `bin`, near which top_p's border lies,
+  // at the mass `want`; else all down to `bin`, which holds top_k's, `above` tokens lying in the bins before.
   auto finish = [&](int n, int bin, bool masses, double want, double above) {
     constexpr int per = kList / kSampleThreads;
     u64 entry[per], m[per];
@@ -422,36 +423,47 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       for (int c = 0; c < per; ++c)
         if (entry[c] < sm.border) entry[c] = m[c] = 0;
     };
+    auto mass_in = [&](int from, int to) {  // of the bins from .. to - 1
+      u64 sum = 0;
+#pragma unroll
+      for (int c = 0; c < per; ++c) {
+        const int at = entry[c] ? bin_at(c) : -1;
+        sum += at >= from && at < to ? m[c] : 0;
+      }
+      return cta_sum(sum);
+    };
     u64 z;
     if (!masses) {
       cut(bin, (double)k - above, false);
-      if (by_mass) {  // top_p of what top_k has left
-        runs[tid] = 0;
+      if (by_mass) {  // top_p of what top_k has left: a histogram of rounded masses says where about
+        unsigned *const rough = sm.hist;
         __syncthreads();
-        u64 sum = 0;
+        rough[tid] = 0;
+        __syncthreads();
 #pragma unroll
         for (int c = 0; c < per; ++c)
-          if (m[c]) {
-            atomicAdd(&runs[bin_at(c)], m[c]);
-            sum += m[c];
-          }
-        want = (double)p * (double)cta_sum(sum);
-        if (tid == 0) sm.found = kBins;
-        const u64 mine = runs[tid], before = cta_scan(mine, z);
-        if ((double)before < want && want <= (double)(before + mine)) {
-          sm.found = tid;
-          sm.start = before;
-        }
+          if (entry[c]) atomicAdd(&rough[bin_at(c)], (unsigned)(m[c] >> 25));  // (4096 tokens of 2^19)
+        want = (double)p * (double)mass_in(0, kBins);
+        if (tid == 0) sm.found = kTail;
+        const u64 mine = rough[tid], before = cta_scan(mine, z);
+        if ((double)before < want * 0x1p-25 && want * 0x1p-25 <= (double)(before + mine)) sm.found = tid;
         __syncthreads();
-        const int at_bin = sm.found;
-        if (at_bin < kBins) cut(at_bin, want - (double)sm.start, true);
+        bin = sm.found;
       }
-    } else {
-      u64 sum = 0;
-#pragma unroll
-      for (int c = 0; c < per; ++c) sum += entry[c] && bin_at(c) < bin ? m[c] : 0;
-      sum = cta_sum(sum);
-      cut(bin, want - (double)sum, true);
+    }
+    if (by_mass) {
+      // the exact sums have the last word: bins below while they do not reach, above while they would do without this one
+      u64 before = mass_in(0, bin), here = mass_in(bin, bin + 1);
+      while (bin < kTail && (double)(before + here) < want) {
+        before += here;
+        ++bin;
+        here = mass_in(bin, bin + 1);
+      }
+      while (bin > 0 && (double)before >= want) {
+        --bin;
+        before -= mass_in(bin, bin + 1);
+      }
+      cut(bin, want - (double)before, true);
     }
     // the draw in the order of the indices: sums over 512 runs of indices, then the tokens of one run among themselves
     int shift = 0;
@@ -507,33 +519,29 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     // masses: weights are masses and the target p of their whole; else numbers of tokens and the target k.
     // Leaves the border, and with masses the sums of what stays in the groups (those with at least min_p of the largest).
     auto narrow = [&](bool masses) {
-      float tail = 0.f;
+      u64 mass = 0;
+      unsigned tail = 0;
       EACH_VECTOR({
         int b[VEC];
         unsigned w[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const float v = vec.at(e);
-          const float t = stays(v, i0 + e) ? step_of(v) : INFINITY;
+          const bool in = stays(v, i0 + e);
+          const float t = in ? step_of(v) : INFINITY;
           b[e] = bin_of(t);
           w[e] = masses ? weight15(t - (float)b[e]) : 1u;
-          tail += b[e] == kTail ? part(t) : 0.f;
+          if (masses) mass += in ? mass_of(v) : 0;
+          tail += in && b[e] == kTail;
         }
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
           if (b[e] < kTail) atomicAdd(&sm.hist[b[e]], w[e]);
       })
-      if (masses) {
-        for (int d = 16; d > 0; d >>= 1) tail += __shfl_xor_sync(~0u, tail, d);
-        if (lane == 0) sm.scan[warp] = tail;
-        __syncthreads();
-        tail = 0.f;
-#pragma unroll
-        for (int w = 0; w < kSampleWarps; ++w) tail += (float)sm.scan[w];
-        spread_f(tail);
-      }
-      // Picks the bin: every CTA the same from everybody's histograms.  unit: of a bin's weights; above: what lies before
-      // the first; tokens: about how many lie above the bin's lower edge.
+      if (masses) spread_u(cta_sum(mass));
+      else if ((tail = __reduce_add_sync(~0u, tail)) && lane == 0) atomicAdd(&sm.hist[kTail], tail);
+      // Picks the bin: every CTA the same from everybody's histograms.  unit: of a bin's weights; above: what lies before the
+      // first, then before the bin (with masses: before its neighbour); tokens: about how many lie above the lower edge of the bin after it.
       double target = (double)k, above = 0.0, tokens = 0.0;
       auto pick = [&](double unit, bool first) {
         if (C > 1) cluster.sync();
@@ -571,19 +579,18 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
           all += sm.scan[i];
         }
         if (masses && first) {
-          double whole = all;
-          for (int c = 0; c < C; ++c) whole += (double)sm.gather_f[turn][c];
-          target = (double)p * whole;
+          u64 whole = 0;
+          for (int c = 0; c < C; ++c) whole += sm.gather_u[turn][c];
+          target = (double)p * (double)whole * (1.0 / one);
         }
         const bool reached = start + run >= target;
         const unsigned votes = __ballot_sync(~0u, reached);
         if (reached && lane == __ffs(votes) - 1) atomicMin(&sm.pick_bin, tid);
         __syncthreads();
         const int b = sm.pick_bin;
-        if (b == tid || (b == kBins && tid == kBins - 1)) {
-          sm.pick_before = b == tid ? start + run - w : all;
-          sm.pick_tokens = few;
-        }
+        const int from = masses && first ? max(min(b, kTail) - 1, 0) : min(b, kBins - 1);
+        if (tid == from) sm.pick_before = b == kBins && !(masses && first) ? all : start + run - w;
+        if (tid == min(b + 1, kBins - 1)) sm.pick_tokens = few;
         __syncthreads();
         above = sm.pick_before;
         tokens = sm.pick_tokens;
@@ -641,8 +648,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
           atomicMax(&sm0.highest, hi);
         }
       };
-      if (bin < kTail && tokens * 1.05 < (double)kList) {  // (masses tell their tokens' number to within 2^(1/16))
-        const float edge = (float)(bin + 1);
+      if (bin + 1 < kTail && tokens * 1.05 < (double)kList) {  // (masses tell their tokens' number to within 2^(1/16))
+        const float edge = (float)(bin + (masses ? 2 : 1));
         gather([&](float v) { return step_of(v) < edge; });
         done = true;
         if (C > 1) cluster.sync();
@@ -652,9 +659,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       }
       // gathers the bin's tokens; divides it while they are too many
       unsigned low = 0, high = ~0u;  // keys
+      const int first_bin = masses ? bin - 1 : bin, last_bin = masses ? bin + 1 : bin;
       auto inside = [&](float v) {
         const unsigned key = key_of(v);
-        return key >= low && key <= high && bin_of(step_of(v)) == bin;
+        const int b = bin_of(step_of(v));
+        return key >= low && key <= high && b >= first_bin && b <= last_bin;
       };
       int n;
       for (;;) {
@@ -700,7 +709,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             const float v = vec.at(e);
-            if (stays(v, i0 + e) && (n > 0 ? v > highest : bin_of(step_of(v)) < bin)) hits |= 1u << e;
+            if (stays(v, i0 + e) && (n > 0 ? v > highest : bin_of(step_of(v)) < first_bin)) hits |= 1u << e;
             w[e] = 0;
           }
           if (__any_sync(~0u, hits != 0)) {

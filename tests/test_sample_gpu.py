@@ -72,6 +72,17 @@ def test_ties_go_by_index(dtype):
             assert (got[:4] < k).all()
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("b,V,spread", [(256, 20000, 1.0), (256, 9000, 2.0), (40, 131072, 3.0), (300, 3000, 0.2)])
+def test_wide_nuclei_draw_exactly(dtype, b, V, spread):
+    """Thousands of tokens stay: an error of 1e-6 in the whole mass would give one row in a hundred its neighbour."""
+    logits, u = rows(b, V, dtype, seed=V, spread=spread)
+    gen = torch.Generator().manual_seed(9)
+    top_p = (0.9 + 0.099 * torch.rand(b, generator=gen)).cuda()
+    check(logits, u, 1.1, 0, top_p, 0.0)
+    check(logits, u, 0.9, V // 2, top_p, 0.001)
+
+
 def test_signed_zeros_are_one_value():
     logits = torch.tensor([[-0.0, 0.0, -0.0, -1.0]], device="cuda").repeat(3, 1)
     got = check(logits, torch.tensor([0.0, 0.4, 0.9]).cuda(), 1.0, 2, 1.0, 0.0)
