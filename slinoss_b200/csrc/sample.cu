@@ -55,11 +55,11 @@ struct alignas(16) SampleShared {  // (the row's vectors follow it)
   u64 group[kMaxGroups];
   double table[64];             // 2^(i/64)
   double scan[kSampleWarps], scan2[kSampleWarps];
-  u64 sums[kSampleWarps];
+  u64 sums[kSampleWarps], sums2[kSampleWarps];
   unsigned hist[kBins];
   // written by every CTA of the cluster into each, two sets in turn
   float gather_f[2][kMaxCluster];
-  u64 gather_u[2][kMaxCluster];
+  u64 gather_u[2][kMaxCluster], gather_v[2][kMaxCluster];
   double pick_before, pick_tokens;
   u64 start, border;
   int pick_bin, found;
@@ -93,6 +93,338 @@ struct Vec {
     return fmaxf(x, -INFINITY);  // (a NaN counts as -inf)
   }
 };
+
+// sum over the CTA
+__device__ __forceinline__ u64 sum_over_cta(SampleShared &sm, u64 v) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  __syncthreads();
+  if (lane == 0) sm.sums[warp] = v;
+  __syncthreads();
+  u64 s = 0;
+#pragma unroll
+  for (int w = 0; w < kSampleWarps; ++w) s += sm.sums[w];
+  return s;
+}
+struct Pair {
+  u64 x, y;
+};
+__device__ __forceinline__ Pair sum_over_cta(SampleShared &sm, Pair v) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int d = 16; d > 0; d >>= 1) {
+    v.x += __shfl_xor_sync(~0u, v.x, d);
+    v.y += __shfl_xor_sync(~0u, v.y, d);
+  }
+  __syncthreads();
+  if (lane == 0) {
+    sm.sums[warp] = v.x;
+    sm.sums2[warp] = v.y;
+  }
+  __syncthreads();
+  Pair s{0, 0};
+#pragma unroll
+  for (int w = 0; w < kSampleWarps; ++w) {
+    s.x += sm.sums[w];
+    s.y += sm.sums2[w];
+  }
+  return s;
+}
+// sum of the CTA's threads before this one, and of all
+__device__ __forceinline__ u64 scan_over_cta(SampleShared &sm, u64 v, u64 &whole) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  u64 run = v;
+  for (int d = 1; d < 32; d <<= 1) {
+    const u64 o = __shfl_up_sync(~0u, run, d);
+    if (lane >= d) run += o;
+  }
+  __syncthreads();
+  if (lane == 31) sm.sums[warp] = run;
+  __syncthreads();
+  u64 before = 0;
+  whole = 0;
+#pragma unroll
+  for (int w = 0; w < kSampleWarps; ++w) {
+    if (w < warp) before += sm.sums[w];
+    whole += sm.sums[w];
+  }
+  return before + run - v;
+}
+
+// A token's mass: exp of a difference below zero by table (Tang 1989): 2^(i/64) and the series of e^r, |r| <= ln 2 / 128
+// (r^6 / 720 < 2^-54); as an integer of 2^-44, zero from exp(-31) on.  Without branches: the chains of neighbours overlap.
+struct Mass {
+  const double *table;
+  double per_unit;  // 1 / temperature
+  float top;        // (where it is infinite, the largest share the mass)
+  __device__ __forceinline__ u64 operator()(float v) const {
+    const double y = fmax(((double)v - (double)top) * per_unit, -40.0);  // (also for NaN, from two infinities)
+    constexpr double kLn2 = 0.693147180559945309417232121458;
+    const double t = fma(y, 64.0 / kLn2, 6755399441055744.0);  // 1.5 * 2^52: the rounded integer in the low bits
+    const int n = __double2loint(t);
+    const double s = fma(t - 6755399441055744.0, -kLn2 / 64.0, y);
+    const double e = fma(s, fma(s, fma(s, fma(s, fma(s, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0);
+    const double b = table[n & 63];
+    const double f = e * __hiloint2double(__double2hiint(b) + ((n >> 6) << 20), __double2loint(b));
+    const double q = fma(f, 17592186044416.0, 4503599627370496.0);  // 2^44 and 2^52
+    const u64 m = ((u64)(unsigned)(__double2hiint(q) & 0xfffff) << 32) | (unsigned)__double2loint(q);
+    return v == top ? 1ull << 44 : y > -31.0 ? m : 0;
+  }
+};
+
+// Of the n entries of CTA 0's list, the one with which the weights (masses, or one each), from the largest entry down,
+// reach `need`; the smallest where they do not.  In sm.border.  While they are many they are divided into 512 ranges of equal
+// width, of which one stays; then each looks at the others.
+// (per: entries of a thread that n needs at most)
+template <int per>
+__device__ __noinline__ void border_of(SampleShared &sm, Mass mass_of, int n, double need, bool masses) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  u64 *const few = sm.list + kList - kFew;  // their weights
+  auto weight_of = [&](u64 entry) -> u64 { return masses ? mass_of(value_of((unsigned)(entry >> 32))) : 1; };
+  if (n > kFew) {
+    u64 entry[per], w[per];
+#pragma unroll
+    for (int c = 0; c < per; ++c) {
+      const int i = tid + c * kSampleThreads;
+      entry[c] = i < n ? sm.list[i] : 0;
+      w[c] = i < n ? weight_of(entry[c]) : 0;
+    }
+    u64 above = 0;
+    for (;;) {
+      u64 lo = ~0ull, hi = 0;
+#pragma unroll
+      for (int c = 0; c < per; ++c)
+        if (entry[c]) {
+          lo = min(lo, entry[c]);
+          hi = max(hi, entry[c]);
+        }
+      for (int d = 16; d > 0; d >>= 1) {
+        lo = min(lo, __shfl_xor_sync(~0u, lo, d));
+        hi = max(hi, __shfl_xor_sync(~0u, hi, d));
+      }
+      __syncthreads();
+      if (lane == 0) {
+        sm.sums[warp] = lo;
+        sm.sums2[warp] = hi;
+      }
+      sm.hist[tid] = 0;
+      if (tid == 0) sm.found = kBins - 1;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kSampleWarps; ++i) {
+        lo = min(lo, sm.sums[i]);
+        hi = max(hi, sm.sums2[i]);
+      }
+      const int cut = max(0, 64 - __clzll((long long)(hi - lo)) - 9);
+      const int coarse = max(0, 64 - __clzll((long long)weight_of(hi)) - 19);  // (4096 weights of 2^19 fit 32 bits)
+      int range[per];
+#pragma unroll
+      for (int c = 0; c < per; ++c) {
+        range[c] = entry[c] ? (int)((hi - entry[c]) >> cut) : -1;
+        if (entry[c]) atomicAdd(&sm.hist[range[c]], (unsigned)(w[c] >> coarse));
+      }
+      __syncthreads();
+      u64 all;
+      const unsigned mine = sm.hist[tid];
+      const u64 before = scan_over_cta(sm, mine, all);
+      const double rough = (need - (double)above) / (double)(1ull << coarse);
+      if ((double)before < rough && rough <= (double)(before + mine)) sm.found = tid;
+      __syncthreads();
+      int at = sm.found;
+      // the exact sums have the last word: {weight of the ranges before `at`, of this one}
+      auto weights = [&]() {
+        Pair s{0, 0};
+#pragma unroll
+        for (int c = 0; c < per; ++c) {
+          s.x += range[c] >= 0 && range[c] < at ? w[c] : 0;
+          s.y += range[c] == at ? w[c] : 0;
+        }
+        s = sum_over_cta(sm, s);
+        s.x += above;
+        return s;
+      };
+      Pair s = weights();
+      while (at < kBins - 1 && (double)(s.x + s.y) < need) {
+        ++at;
+        s = weights();
+      }
+      while (at > 0 && (double)s.x >= need) {
+        --at;
+        s = weights();
+      }
+      above = s.x;
+      unsigned left = 0;
+#pragma unroll
+      for (int c = 0; c < per; ++c) {
+        if (range[c] != at) entry[c] = 0;
+        left += entry[c] != 0;
+      }
+      n = (int)sum_over_cta(sm, left);
+      if (n <= kFew) break;
+    }
+    if (tid == 0) sm.count = 0;
+    sm.hist[tid] = 0;  // (as it was found: the histogram of the next filter begins with it)
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < per; ++c)
+      if (entry[c]) sm.list[atomicAdd(&sm.count, 1)] = entry[c];
+    __syncthreads();
+    if (tid == 0) sm.count = 0;
+    need -= (double)above;
+  }
+  if (tid < n) few[tid] = weight_of(sm.list[tid]);
+  if (tid == 0) sm.border = 0;
+  __syncthreads();
+  if (tid < n) {
+    const u64 mine = sm.list[tid];
+    u64 larger = 0;
+    bool least_of_all = true;
+#pragma unroll 8
+    for (int o = 0; o < n; ++o) {
+      const u64 other = sm.list[o];
+      if (other > mine) larger += few[o];
+      least_of_all &= other >= mine;
+    }
+    const bool reaches = (double)(larger + few[tid]) >= need;
+    if ((((double)larger < need || larger == 0) && reaches) || (least_of_all && !reaches)) sm.border = mine;
+  }
+  __syncthreads();
+}
+
+
+// Steps of 1/16 in the logarithm of the mass below the largest logit (rounding is monotone), and bins of them.
+struct Steps {
+  float top, per_logit;
+  __device__ __forceinline__ float of(float v) const {
+    return v == top ? 0.f : top == INFINITY ? INFINITY : (top - v) * per_logit;
+  }
+  static __device__ __forceinline__ int bin_of(float t) { return t < (float)kTail ? (int)t : kTail; }
+  __device__ __forceinline__ int bin(float v) const { return bin_of(of(v)); }
+};
+
+// ---- CTA 0 by itself: n tokens in its list.  With masses all down to the bin after `bin`, near which top_p's border lies,
+// at the mass `want`; else all down to `bin`, which holds top_k's, `above` tokens lying in the bins before.
+// The draw takes the first token with running > u z: of integers, running > its floor; below z, so that there is one.
+__device__ __forceinline__ u64 target_in(double u, u64 z) { return min((u64)(u * (double)z), z - 1); }
+struct Row {  // of one row, what its last steps need
+  Steps step;
+  int V;
+  bool by_mass;
+  int64_t k;
+  float p;
+  u64 least;
+  double u;
+  int64_t *out;
+};
+template <int per>
+__device__ __noinline__ void finish(SampleShared &sm, u64 *runs, Mass mass_of, Row row, int n, int bin, bool masses, double want,
+                                    double above) {
+  const int tid = threadIdx.x;
+  u64 entry[per], m[per];
+#pragma unroll
+  for (int c = 0; c < per; ++c) {
+    const int i = tid + c * kSampleThreads;
+    entry[c] = i < n ? sm.list[i] : 0;
+    m[c] = 0;
+    if (c * kSampleThreads < n && i < n) m[c] = mass_of(value_of((unsigned)(entry[c] >> 32)));
+  }
+  // (runs: the row's room, which is not needed any more)
+  int bins[per];
+#pragma unroll
+  for (int c = 0; c < per; ++c) bins[c] = entry[c] ? row.step.bin(value_of((unsigned)(entry[c] >> 32))) : -1;
+  // the entries of the bin that are still there, by themselves; then only what reaches the border stays
+  auto cut = [&](int at_bin, double need, bool by) {
+    __syncthreads();
+    if (tid == 0) sm.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < per; ++c)
+      if (bins[c] == at_bin) sm.list[atomicAdd(&sm.count, 1)] = entry[c];
+    __syncthreads();
+    border_of<per>(sm, mass_of, sm.count, need, by);
+#pragma unroll
+    for (int c = 0; c < per; ++c)
+      if (entry[c] < sm.border) {
+        entry[c] = m[c] = 0;
+        bins[c] = -1;
+      }
+  };
+  auto around = [&](int at) {  // {mass of the bins before `at`, of this one}
+    Pair s{0, 0};
+#pragma unroll
+    for (int c = 0; c < per; ++c) {
+      s.x += bins[c] < at ? m[c] : 0;
+      s.y += bins[c] == at ? m[c] : 0;
+    }
+    return sum_over_cta(sm, s);
+  };
+  u64 z;
+  if (!masses) {
+    cut(bin, (double)row.k - above, false);
+    if (row.by_mass) {  // top_p of what top_k has left: a histogram of rounded masses says where about
+      unsigned *const rough = sm.hist;
+      __syncthreads();
+      rough[tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < per; ++c)
+        if (entry[c]) atomicAdd(&rough[bins[c]], (unsigned)(m[c] >> 25));  // (4096 tokens of 2^19)
+      want = (double)row.p * (double)around(kBins).x;
+      if (tid == 0) sm.found = kTail;
+      const u64 mine = rough[tid], before = scan_over_cta(sm, mine, z);
+      if ((double)before < want * 0x1p-25 && want * 0x1p-25 <= (double)(before + mine)) sm.found = tid;
+      __syncthreads();
+      bin = sm.found;
+    }
+  }
+  if (row.by_mass) {
+    // the exact sums have the last word: bins below while they do not reach, above while they would do without this one
+    Pair s = around(bin);
+    while (bin < kTail && (double)(s.x + s.y) < want) s = around(++bin);
+    while (bin > 0 && (double)s.x >= want) s = around(--bin);
+    cut(bin, want - (double)s.x, true);
+  }
+  // the draw in the order of the indices: sums over 512 runs of indices, then the tokens of one run among themselves
+  int shift = 0;
+  while ((row.V >> shift) >= kSampleThreads) ++shift;
+  u64 *const masses_of_run = sm.list;
+  int *const members = reinterpret_cast<int *>(sm.list + kList / 2);
+  __syncthreads();
+  runs[tid] = 0;
+  if (tid == 0) sm.count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < per; ++c) {
+    if (m[c] < row.least) m[c] = 0;
+    if (m[c]) atomicAdd(&runs[(int)~(unsigned)entry[c] >> shift], m[c]);
+  }
+  __syncthreads();
+  const u64 run = runs[tid], start = scan_over_cta(sm, run, z), target = target_in(row.u, z);
+  if (start <= target && target < start + run) {
+    sm.found = tid;
+    sm.start = start;
+  }
+  __syncthreads();
+  const int hit = sm.found;
+#pragma unroll
+  for (int c = 0; c < per; ++c) {
+    const int i = (int)~(unsigned)entry[c];
+    if (m[c] && (i >> shift) == hit) {  // (a run holds at most 2^shift <= 1024 indices)
+      const int to = atomicAdd(&sm.count, 1);
+      members[to] = i;
+      masses_of_run[to] = m[c];
+    }
+  }
+  __syncthreads();
+  const int count = sm.count;
+  for (int t = tid; t < count; t += kSampleThreads) {
+    u64 before = sm.start;
+    const int i = members[t];
+    for (int o = 0; o < count; ++o)
+      if (members[o] < i) before += masses_of_run[o];
+    if (before <= target && target < before + masses_of_run[t]) *row.out = i;
+  }
+}
+
 
 template <typename TI>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a, int NV) {  // NV vectors a thread
@@ -183,39 +515,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     leave();
     return;
   }
-  // the draw takes the first token with running > u z: of integers, running > its floor; below z, so that there is one
-  auto target_in = [&](u64 z) { return min((u64)(u * (double)z), z - 1); };
 
-  // sum over the CTA
-  auto cta_sum = [&](u64 v) {
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
-    __syncthreads();
-    if (lane == 0) sm.sums[warp] = v;
-    __syncthreads();
-    u64 s = 0;
-#pragma unroll
-    for (int w = 0; w < kSampleWarps; ++w) s += sm.sums[w];
-    return s;
-  };
-  // sum of the CTA's threads before this one, and of all
-  auto cta_scan = [&](u64 v, u64 &whole) {
-    u64 run = v;
-    for (int d = 1; d < 32; d <<= 1) {
-      const u64 o = __shfl_up_sync(~0u, run, d);
-      if (lane >= d) run += o;
-    }
-    __syncthreads();
-    if (lane == 31) sm.sums[warp] = run;
-    __syncthreads();
-    u64 before = 0;
-    whole = 0;
-#pragma unroll
-    for (int w = 0; w < kSampleWarps; ++w) {
-      if (w < warp) before += sm.sums[w];
-      whole += sm.sums[w];
-    }
-    return before + run - v;
-  };
+  auto cta_sum = [&](u64 v) { return sum_over_cta(sm, v); };
+  auto cta_scan = [&](u64 v, u64 &whole) { return scan_over_cta(sm, v, whole); };
 
   // Sums over a warp's vectors j in the order of the indices: sm.group[j * warps + warp].
   auto fill_groups = [&](auto weights) {  // weights(vec, i0, w): of a vector's values
@@ -289,23 +591,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     leave();
     return;
   }
-  const bool infinite = top == INFINITY;  // the largest share the mass
   const double per_unit = 1.0 / (double)temperature;
-  // exp of a difference below zero by table (Tang 1989): 2^(i/64) and the series of e^r, |r| <= ln 2 / 128 (r^6 / 720 <
-  // 2^-54); as an integer of 2^-44, zero from exp(-31) on.  Without branches: the chains of neighbours overlap.
-  auto mass_of = [&](float v) -> u64 {
-    const double y = fmax(((double)v - (double)top) * per_unit, -40.0);  // (also for NaN, from two infinities)
-    constexpr double kLn2 = 0.693147180559945309417232121458;
-    const double t = fma(y, 64.0 / kLn2, 6755399441055744.0);  // 1.5 * 2^52: the rounded integer in the low bits
-    const int n = __double2loint(t);
-    const double s = fma(t - 6755399441055744.0, -kLn2 / 64.0, y);
-    const double e = fma(s, fma(s, fma(s, fma(s, fma(s, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0);
-    const double b = sm.table[n & 63];
-    const double f = e * __hiloint2double(__double2hiint(b) + ((n >> 6) << 20), __double2loint(b));
-    const double q = fma(f, 17592186044416.0, 4503599627370496.0);  // 2^44 and 2^52
-    const u64 m = ((u64)(unsigned)(__double2hiint(q) & 0xfffff) << 32) | (unsigned)__double2loint(q);
-    return v == top ? 1ull << 44 : y > -31.0 ? m : 0;
-  };
+  const Mass mass_of{sm.table, per_unit, top};
   const double one = 17592186044416.0;
   const u64 least = minp > 0.f ? (u64)ceil((double)minp * one) : 0;  // of a mass that min_p keeps
 
@@ -330,182 +617,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
   };
   const bool by_rank = k < a.V, by_mass = p < 1.f;
 
-  const float steps = (float)(16.0 * 1.4426950408889634 * per_unit);
-  auto step_of = [&](float v) { return v == top ? 0.f : infinite ? INFINITY : (top - v) * steps; };  // (rounding is monotone)
-  auto bin_of = [&](float t) { return t < (float)kTail ? (int)t : kTail; };
-
-  // Of the n entries of CTA 0's list, the one with which the weights (masses, or one each), from the largest entry down,
-  // reach `need`; the smallest where they do not.  In sm.border.
-  auto border_of = [&](int n, double need, bool masses) {
-    u64 *const w = sm.list + kList - kFew;
-    if (n <= kFew) {  // each looks at the others
-      if (tid < n) w[tid] = masses ? mass_of(value_of((unsigned)(sm.list[tid] >> 32))) : 1;
-      if (tid == 0) sm.border = 0;
-      __syncthreads();
-      if (tid < n) {
-        const u64 mine = sm.list[tid];
-        u64 larger = 0;
-        bool least_of_all = true;
-        for (int o = 0; o < n; ++o) {
-          const u64 other = sm.list[o];
-          if (other > mine) larger += w[o];
-          least_of_all &= other >= mine;
-        }
-        const bool here = ((double)larger < need || larger == 0) && (double)(larger + w[tid]) >= need;
-        if (here || (least_of_all && (double)(larger + w[tid]) < need)) sm.border = mine;
-      }
-      __syncthreads();
-      return;
-    }
-    int size = 32;
-    while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += kSampleThreads) sm.list[i] = 0;
-    for (int len = 2; len <= size; len *= 2)  // bitonic, descending
-      for (int step = len / 2; step > 0; step /= 2) {
-        __syncthreads();
-        for (int i = tid; i < size / 2; i += kSampleThreads) {
-          const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-          const u64 x0 = sm.list[lo], x1 = sm.list[hi];
-          if (((lo & len) == 0) == (x0 < x1)) {
-            sm.list[lo] = x1;
-            sm.list[hi] = x0;
-          }
-        }
-      }
-    __syncthreads();
-    if (warp == 0) {  // walks the list: 32 at a time
-      u64 seen = 0;
-      int last = n - 1;
-      for (int i0 = 0; i0 < n; i0 += 32) {
-        u64 run = 0;
-        if (i0 + lane < n) run = masses ? mass_of(value_of((unsigned)(sm.list[i0 + lane] >> 32))) : 1;
-        for (int d = 1; d < 32; d <<= 1) {
-          const u64 o = __shfl_up_sync(~0u, run, d);
-          if (lane >= d) run += o;
-        }
-        const unsigned there = __ballot_sync(~0u, i0 + lane < n && (double)(seen + run) >= need);
-        if (there) {
-          last = i0 + __ffs(there) - 1;
-          break;
-        }
-        seen += __shfl_sync(~0u, run, 31);
-      }
-      if (lane == 0) sm.border = sm.list[last];
-    }
-    __syncthreads();
-  };
-
-  // ---- CTA 0 by itself: n tokens in its list.  With masses all down to the bin after `bin`, near which top_p's border lies,
-  // at the mass `want`; else all down to `bin`, which holds top_k's, `above` tokens lying in the bins before.
-  auto finish = [&](int n, int bin, bool masses, double want, double above) {
-    constexpr int per = kList / kSampleThreads;
-    u64 entry[per], m[per];
-#pragma unroll
-    for (int c = 0; c < per; ++c) {
-      const int i = tid + c * kSampleThreads;
-      entry[c] = i < n ? sm.list[i] : 0;
-      m[c] = 0;
-      if (c * kSampleThreads < n && i < n) m[c] = mass_of(value_of((unsigned)(entry[c] >> 32)));
-    }
-    u64 *const runs = reinterpret_cast<u64 *>(row_data - tid);  // (the row is not needed any more)
-    auto bin_at = [&](int c) { return bin_of(step_of(value_of((unsigned)(entry[c] >> 32)))); };
-    // the entries of the bin that are still there, by themselves; then only what reaches the border stays
-    auto cut = [&](int at_bin, double need, bool by) {
-      __syncthreads();
-      if (tid == 0) sm.count = 0;
-      __syncthreads();
-#pragma unroll
-      for (int c = 0; c < per; ++c)
-        if (entry[c] && bin_at(c) == at_bin) sm.list[atomicAdd(&sm.count, 1)] = entry[c];
-      __syncthreads();
-      border_of(sm.count, need, by);
-#pragma unroll
-      for (int c = 0; c < per; ++c)
-        if (entry[c] < sm.border) entry[c] = m[c] = 0;
-    };
-    auto mass_in = [&](int from, int to) {  // of the bins from .. to - 1
-      u64 sum = 0;
-#pragma unroll
-      for (int c = 0; c < per; ++c) {
-        const int at = entry[c] ? bin_at(c) : -1;
-        sum += at >= from && at < to ? m[c] : 0;
-      }
-      return cta_sum(sum);
-    };
-    u64 z;
-    if (!masses) {
-      cut(bin, (double)k - above, false);
-      if (by_mass) {  // top_p of what top_k has left: a histogram of rounded masses says where about
-        unsigned *const rough = sm.hist;
-        __syncthreads();
-        rough[tid] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < per; ++c)
-          if (entry[c]) atomicAdd(&rough[bin_at(c)], (unsigned)(m[c] >> 25));  // (4096 tokens of 2^19)
-        want = (double)p * (double)mass_in(0, kBins);
-        if (tid == 0) sm.found = kTail;
-        const u64 mine = rough[tid], before = cta_scan(mine, z);
-        if ((double)before < want * 0x1p-25 && want * 0x1p-25 <= (double)(before + mine)) sm.found = tid;
-        __syncthreads();
-        bin = sm.found;
-      }
-    }
-    if (by_mass) {
-      // the exact sums have the last word: bins below while they do not reach, above while they would do without this one
-      u64 before = mass_in(0, bin), here = mass_in(bin, bin + 1);
-      while (bin < kTail && (double)(before + here) < want) {
-        before += here;
-        ++bin;
-        here = mass_in(bin, bin + 1);
-      }
-      while (bin > 0 && (double)before >= want) {
-        --bin;
-        before -= mass_in(bin, bin + 1);
-      }
-      cut(bin, want - (double)before, true);
-    }
-    // the draw in the order of the indices: sums over 512 runs of indices, then the tokens of one run among themselves
-    int shift = 0;
-    while ((a.V >> shift) >= kSampleThreads) ++shift;
-    u64 *const masses_of_run = sm.list;
-    int *const members = reinterpret_cast<int *>(sm.list + kList / 2);
-    __syncthreads();
-    runs[tid] = 0;
-    if (tid == 0) sm.count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < per; ++c) {
-      if (m[c] < least) m[c] = 0;
-      if (m[c]) atomicAdd(&runs[(int)~(unsigned)entry[c] >> shift], m[c]);
-    }
-    __syncthreads();
-    const u64 run = runs[tid], start = cta_scan(run, z), target = target_in(z);
-    if (start <= target && target < start + run) {
-      sm.found = tid;
-      sm.start = start;
-    }
-    __syncthreads();
-    const int hit = sm.found;
-#pragma unroll
-    for (int c = 0; c < per; ++c) {
-      const int i = (int)~(unsigned)entry[c];
-      if (m[c] && (i >> shift) == hit) {  // (a run holds at most 2^shift <= 1024 indices)
-        const int to = atomicAdd(&sm.count, 1);
-        members[to] = i;
-        masses_of_run[to] = m[c];
-      }
-    }
-    __syncthreads();
-    const int count = sm.count;
-    for (int t = tid; t < count; t += kSampleThreads) {
-      u64 before = sm.start;
-      const int i = members[t];
-      for (int o = 0; o < count; ++o)
-        if (members[o] < i) before += masses_of_run[o];
-      if (before <= target && target < before + masses_of_run[t]) a.out[row] = i;
-    }
-  };
+  const Steps step{top, (float)(16.0 * 1.4426950408889634 * per_unit)};
+  auto step_of = [&](float v) { return step.of(v); };
+  auto bin_of = [&](float t) { return Steps::bin_of(t); };
 
   if (by_rank || by_mass) {
     auto part = [&](float t) {  // 2^(-t/16)
@@ -541,7 +655,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       if (masses) spread_u(cta_sum(mass));
       else if ((tail = __reduce_add_sync(~0u, tail)) && lane == 0) atomicAdd(&sm.hist[kTail], tail);
       // Picks the bin: every CTA the same from everybody's histograms.  unit: of a bin's weights; above: what lies before the
-      // first, then before the bin (with masses: before its neighbour); tokens: about how many lie above the lower edge of the bin after it.
+      // first, then before the bin; tokens: about how many lie above the lower edge of the bin after it.
       double target = (double)k, above = 0.0, tokens = 0.0;
       auto pick = [&](double unit, bool first) {
         if (C > 1) cluster.sync();
@@ -588,8 +702,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         if (reached && lane == __ffs(votes) - 1) atomicMin(&sm.pick_bin, tid);
         __syncthreads();
         const int b = sm.pick_bin;
-        const int from = masses && first ? max(min(b, kTail) - 1, 0) : min(b, kBins - 1);
-        if (tid == from) sm.pick_before = b == kBins && !(masses && first) ? all : start + run - w;
+        if (b == tid || (b == kBins && tid == kBins - 1)) sm.pick_before = b == tid ? start + run - w : all;
         if (tid == min(b + 1, kBins - 1)) sm.pick_tokens = few;
         __syncthreads();
         above = sm.pick_before;
@@ -654,18 +767,71 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         done = true;
         if (C > 1) cluster.sync();
         else __syncthreads();
-        if (rank == 0) finish(sm.count, bin, masses, target * one, above);
+        if (rank == 0) {
+          const Row rest{step, a.V, by_mass, k, p, least, u, a.out + row};
+          u64 *const room = reinterpret_cast<u64 *>(row_data - tid);
+          const int n = sm.count;
+          if (n <= kSampleThreads) finish<1>(sm, room, mass_of, rest, n, bin, masses, target * one, above);
+          else finish<kList / kSampleThreads>(sm, room, mass_of, rest, n, bin, masses, target * one, above);
+        }
         return;
+      }
+      // with masses: what lies above the bin, exactly, and in the groups.  The exact sums have the last word on the bin.
+      u64 sure = 0;
+      while (masses) {
+        Pair mine{0, 0};
+        __syncthreads();
+        fill_groups([&](const Vec<TI> &vec, int i0, u64 *w) {
+          unsigned hits = 0, here = 0;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float v = vec.at(e);
+            const int b = bin_of(step_of(v));
+            if (stays(v, i0 + e)) {
+              hits |= (unsigned)(b < bin) << e;
+              here |= (unsigned)(b == bin) << e;
+            }
+            w[e] = 0;
+          }
+          if (__any_sync(~0u, (hits | here) != 0)) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const u64 m = mass_of(vec.at(e));
+              mine.x += hits >> e & 1 ? m : 0;
+              mine.y += here >> e & 1 ? m : 0;
+              w[e] = (hits >> e & 1) && m >= least ? m : 0;
+            }
+          }
+        });
+        Pair s = sum_over_cta(sm, mine);
+        if (C > 1) {
+          spread_u(s.x);
+          if (tid < C) cluster.map_shared_rank(&sm, tid)->gather_v[turn][rank] = s.y;
+          cluster.sync();
+          s = Pair{0, 0};
+          for (int c = 0; c < C; ++c) {
+            s.x += sm.gather_u[turn][c];
+            s.y += sm.gather_v[turn][c];
+          }
+          turn ^= 1;
+        }
+        sure = s.x;
+        if (bin > 0 && (double)s.x >= target * one) --bin;
+        else if (bin < kTail && (double)(s.x + s.y) < target * one) ++bin;
+        else break;
+      }
+      if (masses) {
+        summed = true;
+        above = (double)sure * (1.0 / one);
       }
       // gathers the bin's tokens; divides it while they are too many
       unsigned low = 0, high = ~0u;  // keys
-      const int first_bin = masses ? bin - 1 : bin, last_bin = masses ? bin + 1 : bin;
       auto inside = [&](float v) {
         const unsigned key = key_of(v);
-        const int b = bin_of(step_of(v));
-        return key >= low && key <= high && b >= first_bin && b <= last_bin;
+        return key >= low && key <= high && bin_of(step_of(v)) == bin;
       };
       int n;
+      bool divided = false;
       for (;;) {
         gather(inside);
         extremes(inside);
@@ -686,11 +852,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
           high = all_hi;
         }
         if (n <= kList || low == high) break;
+        divided = true;
         // by keys, the highest first
         const int cut = max(0, 32 - __clz(high - low) - 9);
         const float edge = step_of(value_of(high));
         EACH({
-          if (v > -INFINITY && stays(v, i) && inside(v))
+          if (stays(v, i) && inside(v))
             atomicAdd(&sm.hist[(high - key_of(v)) >> cut], masses ? weight15(step_of(v) - edge) : 1u);
         })
         int b = pick(masses ? exp2((double)edge * (-1.0 / 16)) * (1.0 / 32768) : 1.0, false);
@@ -699,42 +866,30 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         low = max(low, cut ? from - ((1u << cut) - 1) : from);
         high = from;
       }
-      // what lies above the bin, exactly, and in the groups
-      u64 sure = 0;
-      if (masses) {
+      if (masses && divided && n > 0) {  // the bin's tokens above what is left of it join what lies above
         const float highest = value_of(high);
-        u64 mine = 0;
-        fill_groups([&](const Vec<TI> &vec, int i0, u64 *w) {
-          unsigned hits = 0;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float v = vec.at(e);
-            if (stays(v, i0 + e) && (n > 0 ? v > highest : bin_of(step_of(v)) < first_bin)) hits |= 1u << e;
-            w[e] = 0;
+        u64 more = 0;
+        EACH({
+          if (stays(v, i) && bin_of(step_of(v)) == bin && v > highest) {
+            const u64 m = mass_of(v);
+            more += m;
+            if (m >= least) atomicAdd(&sm.group[j * kSampleWarps + warp], m);
           }
-          if (__any_sync(~0u, hits != 0)) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const u64 m = hits >> e & 1 ? mass_of(vec.at(e)) : 0;
-              mine += m;
-              w[e] = m >= least ? m : 0;
-            }
-          }
-        });
-        sure = cta_sum(mine);
+        })
+        more = cta_sum(more);
         if (C > 1) {
-          spread_u(sure);
+          spread_u(more);
           cluster.sync();
-          sure = 0;
-          for (int c = 0; c < C; ++c) sure += sm.gather_u[turn][c];
+          more = 0;
+          for (int c = 0; c < C; ++c) more += sm.gather_u[turn][c];
           turn ^= 1;
         }
-        summed = true;
+        sure += more;
       }
       if (n == 0) return;  // (a tail without tokens)
       if (n <= kList) {
         if (rank == 0) {
-          border_of(n, masses ? target * one - (double)sure : target - above, masses);
+          border_of<kList / kSampleThreads>(sm, mass_of, n, masses ? target * one - (double)sure : target - above, masses);
           if (tid == 0) {
             sm.border_x = value_of((unsigned)(sm.border >> 32));
             sm.border_i = (int)~(unsigned)sm.border;
@@ -782,7 +937,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     fill_groups(kept);
   }
   // ---- the draw
-  locate(target_in, kept, [&](int i) { a.out[row] = i; });
+  locate([&](u64 z) { return target_in(u, z); }, kept, [&](int i) { a.out[row] = i; });
   leave();
 #undef EACH
 #undef EACH_VECTOR
