@@ -31,15 +31,17 @@ struct Record {
   __half T[2][kTri];  // Tm, hi and lo
   __half Q[2][kTri];  // P, hi and lo
   float gamma[L], closing[L], beta[L];
+  int tops[3][4];  // of gamma, beta and closing beta in each 16 tokens: least e with all magnitudes below 2^e
+  int pad0[20];    // (what is copied whole keeps its neighbours on 128-byte lines)
   // dec_ts for t and s in the same block of 16 tokens is near[block][t][s]; for t in block i and s in an earlier one it is
   // rise[t] * fall[fall_at(i) + s]: both exponents from G at the end of block i - 1, so that neither factor leaves the range
   // where gates close
   float rise[L], fall[96], near[4][16 * 20];
   int eT, eQ, eq, ek;  // binary exponents: value = stored * 2^e
-  int pad[28];
+  int pad1[28];
 };
-static_assert(sizeof(Record) == 31232 && sizeof(Record) % 128 == 0, "record layout");
-constexpr int kHeadBytes = 3 * L * 4;  // gamma, closing, beta
+static_assert(sizeof(Record) == 31360 && sizeof(Record) % 128 == 0, "record layout");
+constexpr int kHeadBytes = 3 * L * 4 + 128;  // gamma, closing, beta, tops
 constexpr int kVectorBytes = kHeadBytes + L * 4 + 96 * 4 + 4 * 16 * 20 * 4;  // gamma .. near
 constexpr int kNearLd = 20;
 __host__ __device__ constexpr int fall_at(int i) { return 8 * i * (i - 1); }

@@ -104,6 +104,20 @@ __global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_c
         if (lane >= d) run += o;
       }
       *reinterpret_cast<double2 *>(G + 2 * lane) = make_double2(run - pair + gg[0], run);
+      const double last = __shfl_sync(~0u, run, 31);
+      unsigned bits[3] = {0, 0, 0};  // (of magnitudes: a NaN is the largest)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const double s = i ? run : run - gg[1];
+        const float x[3] = {expf((float)s), write[i], write[i] * expf((float)(last - s))};
+#pragma unroll
+        for (int n = 0; n < 3; ++n) bits[n] = max(bits[n], mag(x[n]));
+      }
+#pragma unroll
+      for (int n = 0; n < 3; ++n) {
+        for (int d = 1; d < 8; d <<= 1) bits[n] = max(bits[n], __shfl_xor_sync(~0u, bits[n], d));
+        if (lane % 8 == 0) rec->tops[n][lane / 8] = above(__uint_as_float(bits[n]));
+      }
       *reinterpret_cast<float2 *>(rec->beta + 2 * lane) = make_float2(write[0], write[1]);
       *reinterpret_cast<float2 *>(beta + 2 * lane) = make_float2(write[0], write[1]);
     }

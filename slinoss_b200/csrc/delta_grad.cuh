@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
   __half *os = qs + Op::halves, *xs = os + SC * kTile, *ys = xs + SC * kTile;  // tokens x channels: dO, dX, Y
   __half *ss = ys + SC * kTile, *rs = ss + SC * splane;                          // channels x N: S0, R
   float *gamma = reinterpret_cast<float *>(rs + SC * splane), *closing = gamma + L, *beta = closing + L;
-  float *rise = beta + L, *fall = rise + L, *near = fall + 96;
+  float *rise = beta + L + 32, *fall = rise + L, *near = fall + 96;
   __shared__ float dGs[L], dbs[L], wsum[L], dots[4];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;

@@ -65,6 +65,29 @@ __device__ __forceinline__ void times_cols(float (&c)[8][4], const float *s, flo
     c[j][3] *= x.y * f;
   }
 }
+__device__ __forceinline__ int max4(const int (&e)[4]) { return max(max(e[0], e[1]), max(e[2], e[3])); }
+// a warp's 16 rows of a state from its buffer
+template <int NT>
+__device__ __forceinline__ void copy_state(__half *out, const __half *buf) {
+  constexpr int ld = NT + 8;
+#pragma unroll
+  for (int i = threadIdx.x & 31; i < 16 * (NT / 8); i += 32)
+    *reinterpret_cast<uint4 *>(out + (i / (NT / 8)) * ld + (i % (NT / 8)) * 8) =
+        *reinterpret_cast<const uint4 *>(buf + (i / (NT / 8)) * ld + (i % (NT / 8)) * 8);
+}
+// v less c, times the entries s[t] of a vector over the columns
+__device__ __forceinline__ void minus_cols(float (&c)[8][4], const float (&v)[8][4], const float *s, float f) {
+  const int q = threadIdx.x & 3;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float2 x = *reinterpret_cast<const float2 *>(s + 8 * j + 2 * q);
+    const float a = -x.x * f, b = -x.y * f;
+    c[j][0] = fmaf(a, c[j][0], v[j][0]);
+    c[j][1] = fmaf(b, c[j][1], v[j][1]);
+    c[j][2] = fmaf(a, c[j][2], v[j][2]);
+    c[j][3] = fmaf(b, c[j][3], v[j][3]);
+  }
+}
 template <int S>
 __device__ __forceinline__ void frags_of(Frag<S> (&f)[4], const float (&c)[8][4], int e) {
   const float s = pow2(-e);
@@ -84,6 +107,7 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
   __half *Ps = Ts + 2 * kTri;
   float *hd = reinterpret_cast<float *>(Ps + SC * kTri);
   const float *gamma = hd, *closing = hd + L, *beta = hd + 2 * L;
+  const int(*tops)[4] = reinterpret_cast<const int(*)[4]>(hd + 3 * L);
   TI *vs = reinterpret_cast<TI *>(reinterpret_cast<char *>(hd) + kHeadBytes);
 
   const int warp = threadIdx.x >> 5;
@@ -103,7 +127,8 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
     V::issue(vs, head_base<TI>(a.v, b, h, c * L) + first, a.v.st, min(L, a.T - c * L), a.P - first, a.v.vec);
   };
 
-  float S[NT / 8][4];
+  float S[NT / 8][4];  // times 2^unit
+  int unit = 0;
   if (active && a.init) load_state<NT>(S, a.init, a.init_dtype, (size_t)bh * a.P * a.N, p0, a.P, a.N);
   else zero(S);
   int4 ex = exps_of(rec);
@@ -123,21 +148,23 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
     int eC = 0;
     float top = 0.f;  // Gam
     if (active) {
-      const int eS = warp_exp(S);
-      if (a.st) {
-        const size_t at = (size_t)bh * a.NC + c;
-        store_state<SC, NT>(a.st + (at * SC * a.P16 + p0) * (NT + 8), (int64_t)a.P16 * (NT + 8), S, eS, buf);
-        if ((threadIdx.x & 31) == 0) a.est[at * PB + p0 / 16] = eS;
-      }
+      const size_t at = (size_t)bh * a.NC + c;
+      const int e0 = warp_exp(S), eS = e0 + unit;
+      __half *const st = a.st ? a.st + (at * SC * a.P16 + p0) * (NT + 8) : nullptr;
+      if (st && (threadIdx.x & 31) == 0) a.est[at * PB + p0 / 16] = eS;
+      if (SC > 1 && st) store_state<SC, NT>(st, (int64_t)a.P16 * (NT + 8), S, e0, buf);
       float X[8][4], O[8][4];
       zero(X);
       zero(O);
       {
-        const float s = pow2(-eS);
+        const float s = pow2(-e0);
+        const int lane = threadIdx.x & 31;
+        if (SC == 1 && st) __syncwarp();
 #pragma unroll
         for (int kb = 0; kb < NT / 16; ++kb) {
           Frag<2> f;
           frag_of<2>(f, S[2 * kb], S[2 * kb + 1], s);
+          if (SC == 1 && st) stsm(smem_addr(buf + (lane & 15) * (NT + 8) + 16 * kb + (lane >> 4) * 8), f.r[0]);
           Frag<SC> fo;
 #pragma unroll
           for (int pl = 0; pl < SC; ++pl)
@@ -146,60 +173,64 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
           tile_rows<2, SI, NT>(X, f, kt, kb);
           tile_rows<SC, SI, NT>(O, fo, qs, kb);
         }
+        if (SC == 1 && st) {
+          __syncwarp();
+          copy_state<NT>(st, buf);
+          __syncwarp();
+        }
       }
       // X = v - gamma S k
       {
         float v[8][4];
         load_cols<TI>(v, vs, warp * 16);
-        times_cols(X, gamma, pow2(eS + ek));
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) X[j][i] = v[j][i] - X[j][i];
+        minus_cols(X, v, gamma, pow2(eS + ek));
       }
+      int y;  // the unit of Y
       {
         const int eX = warp_exp(X);
         Frag<2> fx[4];
         frags_of<2>(fx, X, eX);
         zero(X);
         tri_rows<2, 2>(X, fx, Ts);
-        times(X, pow2(eX + eT));  // Y
+        y = eX + eT;
       }
+      const int eY = warp_exp(X);
       if (a.y) {
-        const size_t at = (size_t)bh * a.NC + c;
-        const int e = warp_exp(X);
-        store_planes<SC>(a.y + (at * SC * tiles + p0 / 64) * kTile + p0 % 64, kTileLd, tiles * kTile, X, e, buf);
-        if ((threadIdx.x & 31) == 0) a.ey[at * PB + p0 / 16] = e;
+        store_planes<SC>(a.y + (at * SC * tiles + p0 / 64) * kTile + p0 % 64, kTileLd, tiles * kTile, X, eY, buf);
+        if ((threadIdx.x & 31) == 0) a.ey[at * PB + p0 / 16] = eY + y;
       }
       times_cols(X, beta, 1.f);
       if (a.o) {
-        times_cols(O, gamma, pow2(eS + eq));
-        const int eD = floor_exp(warp_exp(X), warp_exp(O), eQ);
-        times(O, pow2(-(eD + eQ)));
+        // (exponents from bounds: of beta Y by the largest beta, of S q by its operands')
+        const int eD = floor_exp(eY + y + max4(tops[1]), eS + eq + 22 + max4(tops[0]), eQ);
+        times_cols(O, gamma, pow2(eS + eq - (eD + eQ)));
         Frag<SC> fd[4];
-        frags_of<SC>(fd, X, eD);
+        frags_of<SC>(fd, X, eD - y);
         tri_rows<SC, SC>(O, fd, Ps);
         times(O, a.scale * pow2(eD + eQ));
         store_rows<TI>(static_cast<TI *>(a.o) + ((size_t)bh * a.T + c * L) * a.P + p0, a.P, min(L, a.T - c * L), a.P - p0, O, buf);
       }
       times_cols(X, closing, 1.f);
-      eC = floor_exp(warp_exp(X), eS, ek);
-      frags_of<2>(fc, X, eC);
+      eC = floor_exp(eY + y + max4(tops[2]), eS, ek);
+      frags_of<2>(fc, X, eC - y);
       top = gamma[L - 1];
     }
     __syncthreads();
     if (more) issue_rest(c + 1);
     cp_commit();
     if (active) {
-      times(S, top * pow2(-(eC + ek)));
+      times(S, top * pow2(unit - (eC + ek)));
+      unit = eC + ek;
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(S, fc[kb], kt, Op::plane, kb);
-      times(S, pow2(eC + ek));
     }
     ex = nx;
   }
   cp_wait<0>();
-  if (active && a.final_state) write_state<NT>(a.final_state, SLX_F32, (size_t)bh * a.P * a.N, S, p0, a.P, a.N);
+  if (active && a.final_state) {
+    times(S, pow2(unit));
+    write_state<NT>(a.final_state, SLX_F32, (size_t)bh * a.P * a.N, S, p0, a.P, a.N);
+  }
 }
 
 template <int NT, int SI, int SC, typename TI>
@@ -213,6 +244,7 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
   __half *Ps = Ts + 2 * kTri;
   float *hd = reinterpret_cast<float *>(Ps + 2 * kTri);
   const float *gamma = hd, *closing = hd + L, *beta = hd + 2 * L;
+  const int(*tops)[4] = reinterpret_cast<const int(*)[4]>(hd + 3 * L);
   TI *os = reinterpret_cast<TI *>(reinterpret_cast<char *>(hd) + kHeadBytes);
 
   const int warp = threadIdx.x >> 5;
@@ -231,7 +263,8 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
     V::issue(os, head_base<TI>(a.dO, b, h, c * L) + first, a.dO.st, min(L, a.T - c * L), a.P - first, a.dO.vec);
   };
 
-  float R[NT / 8][4];
+  float R[NT / 8][4];  // times 2^unit
+  int unit = 0;
   if (active && a.d_final) load_state<NT>(R, a.d_final, a.d_final_dtype, (size_t)bh * a.P * a.N, p0, a.P, a.N);
   else zero(R);
   int4 ex = exps_of(rec + a.NC - 1);
@@ -254,35 +287,50 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
     float top = 0.f;
     if (active) {
       const size_t at = (size_t)bh * a.NC + c;
-      const int eR = warp_exp(R);
-      store_state<SC, NT>(a.ds + (at * SC * a.P16 + p0) * (NT + 8), (int64_t)a.P16 * (NT + 8), R, eR, buf);
+      const int e0 = warp_exp(R), eR = e0 + unit;
+      __half *const st = a.ds + (at * SC * a.P16 + p0) * (NT + 8);
+      if (SC > 1) store_state<SC, NT>(st, (int64_t)a.P16 * (NT + 8), R, e0, buf);
       float W[8][4], X[8][4], dO[8][4];
       zero(X);
       {
-        const float s = pow2(-eR);
+        const float s = pow2(-e0);
+        const int lane = threadIdx.x & 31;
+        if (SC == 1) __syncwarp();
 #pragma unroll
         for (int kb = 0; kb < NT / 16; ++kb) {
           Frag<2> f;
           frag_of<2>(f, R[2 * kb], R[2 * kb + 1], s);
+          if (SC == 1) stsm(smem_addr(buf + (lane & 15) * (NT + 8) + 16 * kb + (lane >> 4) * 8), f.r[0]);
           tile_rows<2, SI, NT>(X, f, kt, kb);
+        }
+        if (SC == 1) {
+          __syncwarp();
+          copy_state<NT>(st, buf);
+          __syncwarp();
         }
       }
       load_cols<TI>(dO, os, warp * 16);
-      const int eo = std::is_same<TI, __half>::value ? 0 : warp_exp(dO);
+      const int eG = warp_exp(dO), eo = std::is_same<TI, __half>::value ? 0 : eG;
       zero(W);
       {
         Frag<SI> fo[4];
         frags_of<SI>(fo, dO, eo);
         tri_cols<SI, 2>(W, fo, Ps);
       }
-      // beta dD
-      times_cols(X, closing, pow2(eR + ek));
-      times(W, a.scale * pow2(eo + eQ));
+      {  // beta dD
+        const float fx = pow2(eR + ek), fw = a.scale * pow2(eo + eQ);
+        const int q = threadIdx.x & 3;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 8; ++j) {
+          const float2 be = *reinterpret_cast<const float2 *>(beta + 8 * j + 2 * q);
+          const float2 cl = *reinterpret_cast<const float2 *>(closing + 8 * j + 2 * q);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) X[j][i] += W[j][i];
-      times_cols(X, beta, 1.f);
+          for (int i = 0; i < 4; ++i) {
+            const float b = i & 1 ? be.y : be.x, l = i & 1 ? cl.y : cl.x;
+            X[j][i] = b * fmaf(l * fx, X[j][i], W[j][i] * fw);
+          }
+        }
+      }
       {
         const int eX = warp_exp(X);
         Frag<2> fx[4];
@@ -292,19 +340,20 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
         times(W, pow2(eX + eT));  // dX
       }
       store_rows<TI>(static_cast<TI *>(a.dv) + ((size_t)bh * a.T + c * L) * a.P + p0, a.P, rows, a.P - p0, W, buf);
-      const int exx = warp_exp(W);
-      store_planes<SC>(a.dx + (at * SC * tiles + p0 / 64) * kTile + p0 % 64, kTileLd, tiles * kTile, W, exx, buf);
+      const int eW = warp_exp(W);
+      store_planes<SC>(a.dx + (at * SC * tiles + p0 / 64) * kTile + p0 % 64, kTileLd, tiles * kTile, W, eW, buf);
       if ((threadIdx.x & 31) == 0) {
         a.eds[at * PB + p0 / 16] = eR;
-        a.edx[at * PB + p0 / 16] = exx;
+        a.edx[at * PB + p0 / 16] = eW;
         a.edo[at * PB + p0 / 16] = eo;
       }
+      // (exponents from bounds: by the largest gamma)
       times_cols(dO, gamma, a.scale);
-      e1 = floor_exp(warp_exp(dO), eR, eq);
+      e1 = floor_exp(eG + max4(tops[0]) + above(a.scale), eR, eq);
       frags_of<2>(f1, dO, e1);
       times_cols(W, gamma, -1.f);
       // (64 products of values below 2^15 join R between the two)
-      e2 = floor_exp(warp_exp(W), max(eR, e1 + eq + 21) + 1, ek);
+      e2 = floor_exp(eW + max4(tops[0]), max(eR, e1 + eq + 21) + 1, ek);
       frags_of<2>(f2, W, e2);
       top = gamma[L - 1];
     }
@@ -313,18 +362,21 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
     if (c > 0) issue_rest(c - 1);
     cp_commit();
     if (active) {
-      times(R, top * pow2(-(e1 + eq)));
+      times(R, top * pow2(unit - (e1 + eq)));
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(R, f1[kb], qs, Op::plane, kb);
       times(R, pow2(e1 + eq - (e2 + ek)));
+      unit = e2 + ek;
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(R, f2[kb], kt, Op::plane, kb);
-      times(R, pow2(e2 + ek));
     }
     ex = nx;
   }
   cp_wait<0>();
-  if (active && a.d_init) write_state<NT>(a.d_init, a.d_init_dtype, (size_t)bh * a.P * a.N, R, p0, a.P, a.N);
+  if (active && a.d_init) {
+    times(R, pow2(unit));
+    write_state<NT>(a.d_init, a.d_init_dtype, (size_t)bh * a.P * a.N, R, p0, a.P, a.N);
+  }
 }
 
 }  // namespace delta

@@ -60,13 +60,14 @@ struct RawTeam {
 };
 
 template <int NT, int SI, int SP, typename TI>  // SP: planes of P
-struct TeamStage {  // the tiles of a chunk
+struct alignas(128) TeamStage {  // the tiles of a chunk
   __half k[Operand<SI, NT>::halves], q[Operand<SI, NT>::halves], T[2 * kTri], P[SP * kTri];
   float gamma[L], closing[L], beta[L];
+  int tops[3][4], pad[20];
   TI v[RawTeam<TI>::size];
 };
 template <int NT, int SI, int SP, typename TI>
-struct alignas(16) TeamShared {
+struct alignas(128) TeamShared {
   TeamStage<NT, SI, SP, TI> stage[2];
   float2 part[4][8][2][32];          // partial sums by warp, tile, row half, lane
   uint4 state[NT / 16][2][32];       // the state's fragments: columns, plane, lane
@@ -224,7 +225,6 @@ __device__ __forceinline__ void times_cols16(float (&c)[2][4], const float *s, f
     c[j][3] *= x.y * f;
   }
 }
-__device__ __forceinline__ int max4(const int (&e)[4]) { return max(max(e[0], e[1]), max(e[2], e[3])); }
 
 template <int NT>
 __device__ __forceinline__ void load_state16(float (&c)[NT / 32][4], const void *src, int dtype, size_t base, int p0, int n0, int P,
@@ -347,20 +347,19 @@ __global__ void __launch_bounds__(kTeamThreads) delta_fwd_team_kernel(Args a) {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[j][i] = (z[0][j][i] + z[1][j][i]) * s;  // Y
+        // (the exponents of beta Y and closing beta Y: Y's and the factors' largest)
+        const int eY = warp_exp(x), eD = eY + st.tops[1][w], eC = eY + st.tops[2][w];
         if (a.y) {
-          const int e = warp_exp(x);
           Frag<SC> f;
-          frag_of<SC>(f, x[0], x[1], pow2(-e));
+          frag_of<SC>(f, x[0], x[1], pow2(-eY));
           put_frag<SC>(sm.frag[kY][w], f);
-          if (lane == 0) exps[kY][w] = e;
+          if (lane == 0) exps[kY][w] = eY;
         }
         times_cols16(x, st.beta + 16 * w, 1.f);
-        const int eD = warp_exp(x);
         Frag<SC> fd;
         frag_of<SC>(fd, x[0], x[1], pow2(-eD));
         put_frag<SC>(sm.frag[kD][w], fd);
         times_cols16(x, st.closing + 16 * w, 1.f);
-        const int eC = warp_exp(x);
         Frag<2> fc;
         frag_of<2>(fc, x[0], x[1], pow2(-eC));
         put_frag<2>(sm.frag[kC][w], fc);
@@ -373,8 +372,9 @@ __global__ void __launch_bounds__(kTeamThreads) delta_fwd_team_kernel(Args a) {
       const int eC = floor_exp(max4(exps[kC]), eS, ek);
       times(S, st.gamma[L - 1] * pow2(-(eC + ek)));
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
+      for (int kb = 0; kb < 4; ++kb) {
         team_cols<2, SI, NT>(S, get_frag<2>(sm.frag[kC][kb], exps[kC][kb] - eC), st.k, kb, n0);
+      }
       times(S, pow2(eC + ek));
       const int e = warp_exp(S);
       if (lane == 0) sm.exps[(c + 1) & 1][kS][w] = e;
@@ -552,12 +552,11 @@ __global__ void __launch_bounds__(kTeamThreads) delta_bwd_team_kernel(Args a) {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[j][i] = (z[0][j][i] + z[1][j][i]) * s;  // dX
-        const int eW = warp_exp(x);
+        const int eW = warp_exp(x), eN = eW + st.tops[0][w];
         Frag<2> f;
         frag_of<2>(f, x[0], x[1], pow2(-eW));
         put_frag<2>(sm.frag[kO][w], f);  // (dO's place: everybody has read it)
         times_cols16(x, st.gamma + 16 * w, -1.f);
-        const int eN = warp_exp(x);
         frag_of<2>(f, x[0], x[1], pow2(-eN));
         put_frag<2>(sm.frag[kN][w], f);
         if (lane == 0) {
@@ -570,10 +569,14 @@ __global__ void __launch_bounds__(kTeamThreads) delta_bwd_team_kernel(Args a) {
       const int u2 = floor_exp(max4(exps[kN]), max(eR, u1 + eq + 21) + 1, ek);
       times(R, st.gamma[L - 1] * pow2(-(u1 + eq)));
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb) team_cols<2, SI, NT>(R, get_frag<2>(sm.frag[kG][kb], exps[kG][kb] - u1), st.q, kb, n0);
+      for (int kb = 0; kb < 4; ++kb) {
+        team_cols<2, SI, NT>(R, get_frag<2>(sm.frag[kG][kb], exps[kG][kb] - u1), st.q, kb, n0);
+      }
       times(R, pow2(u1 + eq - (u2 + ek)));
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb) team_cols<2, SI, NT>(R, get_frag<2>(sm.frag[kN][kb], exps[kN][kb] - u2), st.k, kb, n0);
+      for (int kb = 0; kb < 4; ++kb) {
+        team_cols<2, SI, NT>(R, get_frag<2>(sm.frag[kN][kb], exps[kN][kb] - u2), st.k, kb, n0);
+      }
       times(R, pow2(u2 + ek));
       const int e = warp_exp(R);
       if (lane == 0) sm.exps[(c + 1) & 1][kR][w] = e;
