@@ -1,4 +1,4 @@
-"""Gated delta rule in float64, token by token, with its adjoint (numpy; the checker of the CUDA kernels).
+"""Gated delta rule in float64, token by token, with its adjoint (numpy; what the CUDA kernels are compared with).
 
     S' = a_t S_{t-1},  y_t = v_t - S' k_t,  S_t = S' + beta_t y_t k_t^T,  o_t = scale S_t q_t,  a_t = exp(g_t)
 

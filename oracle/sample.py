@@ -1,4 +1,4 @@
-"""Token sampling in float64, one row at a time (numpy; the checker of the CUDA kernel)."""
+"""Token sampling in float64, one row at a time (numpy; what the CUDA kernel is compared with)."""
 
 from __future__ import annotations
 

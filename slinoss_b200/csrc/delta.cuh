@@ -22,7 +22,7 @@ namespace slx {
 namespace delta {
 
 constexpr int L = 64;             // tokens of a chunk
-constexpr int kTri = 3072;        // elements of a lower triangular 64 x 64 tile, by row blocks of 16 (tri_at)
+constexpr int kTri = 128 * 4 * 4 + 256 * 4;  // elements of a lower triangular 64 x 64 tile, by row blocks of 16 (tri_at)
 constexpr int kThreads = 128;
 constexpr int kTileLd = 72, kTile = L * kTileLd;  // Y and dX: 64 tokens x up to 64 value channels
 

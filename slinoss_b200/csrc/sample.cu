@@ -42,9 +42,11 @@ struct SampleArgs {
 typedef unsigned long long u64;
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kBins = 512;      // of a histogram; one per thread
-constexpr int kTail = 400;      // the bin of all masses below 2^-25 of the largest
+constexpr int kTail = 400;      // counting tokens: the bin of all masses below 2^-25 of the largest
+constexpr int kMassTail = 320;  // adding masses: of all below 2^-20
 constexpr int kList = 4096;     // tokens that are sorted and walked one by one
-constexpr int kFew = 256;       // tokens that are ranked by comparing each with each
+constexpr int kRuns = 1024;     // of indices, in the order of which tokens are drawn
+constexpr int kQueue = 32 + 32 * 8;  // values of a warp that wait for their masses
 constexpr int kMaxVecs = 17;     // of a thread: eight CTAs hold 262144 fp32 logits that begin inside a vector
 constexpr int kMaxGroups = kMaxVecs * kSampleWarps;
 constexpr int kMaxCluster = 8;
@@ -57,8 +59,9 @@ struct alignas(16) SampleShared {  // (the row's vectors follow it)
   double scan[kSampleWarps], scan2[kSampleWarps];
   u64 sums[kSampleWarps], sums2[kSampleWarps];
   unsigned hist[kBins];
+  unsigned short waiting[kSampleWarps][64];
   // written by every CTA of the cluster into each, two sets in turn
-  float gather_f[2][kMaxCluster];
+  float gather_top[kMaxCluster], gather_bound[kMaxCluster];
   u64 gather_u[2][kMaxCluster], gather_v[2][kMaxCluster];
   double pick_before, pick_tokens;
   u64 start, border;
@@ -68,8 +71,9 @@ struct alignas(16) SampleShared {  // (the row's vectors follow it)
   unsigned lowest, highest;
   float border_x;
   int border_i;
-  unsigned maxima[kSampleWarps];
+  unsigned maxima[kSampleWarps], bounds[kSampleWarps];
 };
+static_assert(kSampleWarps * kQueue * 4 <= kList * 8, "the queues lie in the list's place");
 
 // Unsigned integers in the order of the values (zeros of both signs are one value).
 __device__ __forceinline__ unsigned key_of(float x) {
@@ -92,6 +96,17 @@ struct Vec {
     else x = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
     return fmaxf(x, -INFINITY);  // (a NaN counts as -inf)
   }
+  __device__ __forceinline__ float most() const {  // (NaN where all are)
+    if constexpr (sizeof(TI) == 4) {
+      return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)), fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+    } else {
+      using T2 = std::conditional_t<std::is_same<TI, __half>::value, __half2, __nv_bfloat162>;
+      const T2 *w = reinterpret_cast<const T2 *>(&raw);
+      const T2 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+      if constexpr (std::is_same<TI, __half>::value) return fmaxf(__low2float(m), __high2float(m));
+      else return fmaxf(__bfloat162float(__low2bfloat16(m)), __bfloat162float(__high2bfloat16(m)));
+    }
+  }
 };
 
 // sum over the CTA
@@ -101,10 +116,9 @@ __device__ __forceinline__ u64 sum_over_cta(SampleShared &sm, u64 v) {
   __syncthreads();
   if (lane == 0) sm.sums[warp] = v;
   __syncthreads();
-  u64 s = 0;
-#pragma unroll
-  for (int w = 0; w < kSampleWarps; ++w) s += sm.sums[w];
-  return s;
+  v = sm.sums[lane % kSampleWarps];
+  for (int d = kSampleWarps / 2; d > 0; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  return v;
 }
 struct Pair {
   u64 x, y;
@@ -121,14 +135,11 @@ __device__ __forceinline__ Pair sum_over_cta(SampleShared &sm, Pair v) {
     sm.sums2[warp] = v.y;
   }
   __syncthreads();
-  Pair s{0, 0};
-#pragma unroll
-  for (int w = 0; w < kSampleWarps; ++w) {
-    s.x += sm.sums[w];
-    s.y += sm.sums2[w];
-  }
-  return s;
+  u64 s = (lane < kSampleWarps ? sm.sums : sm.sums2)[lane % kSampleWarps];  // one sum in each half of the warp
+  for (int d = kSampleWarps / 2; d > 0; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+  return Pair{__shfl_sync(~0u, s, 0), __shfl_sync(~0u, s, 31)};
 }
+static_assert(kSampleWarps == 16, "the sums of the warps are taken by half a warp");
 // sum of the CTA's threads before this one, and of all
 __device__ __forceinline__ u64 scan_over_cta(SampleShared &sm, u64 v, u64 &whole) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -140,14 +151,13 @@ __device__ __forceinline__ u64 scan_over_cta(SampleShared &sm, u64 v, u64 &whole
   __syncthreads();
   if (lane == 31) sm.sums[warp] = run;
   __syncthreads();
-  u64 before = 0;
-  whole = 0;
-#pragma unroll
-  for (int w = 0; w < kSampleWarps; ++w) {
-    if (w < warp) before += sm.sums[w];
-    whole += sm.sums[w];
+  u64 upto = sm.sums[lane % kSampleWarps];
+  for (int d = 1; d < kSampleWarps; d <<= 1) {
+    const u64 o = __shfl_up_sync(~0u, upto, d, kSampleWarps);
+    if (lane % kSampleWarps >= d) upto += o;
   }
-  return before + run - v;
+  whole = __shfl_sync(~0u, upto, kSampleWarps - 1);
+  return (warp ? __shfl_sync(~0u, upto, warp - 1) : 0) + run - v;
 }
 
 // A token's mass: exp of a difference below zero by table (Tang 1989): 2^(i/64) and the series of e^r, |r| <= ln 2 / 128
@@ -171,138 +181,91 @@ struct Mass {
   }
 };
 
+// The list's n entries in descending order: thread t gets the ranks per t .. per t + per - 1 (zeros behind the n).  Bitonic:
+// steps within a thread, within a warp by shuffles, and across warps through the list's memory; as many as n needs.
+template <int per>
+__device__ __forceinline__ void sorted_list(SampleShared &sm, int n, u64 (&e)[per]) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int c = 0; c < per; ++c) e[c] = tid * per + c < n ? sm.list[tid * per + c] : 0;
+  auto within = [&](int k, auto stride) {
+    constexpr int J = decltype(stride)::value;
+#pragma unroll
+    for (int c = 0; c < per; ++c)
+      if (!(c & J) && c + J < per) {
+        const u64 x = e[c], y = e[c + J];
+        const bool change = (x < y) == (((tid * per + c) & k) == 0);
+        e[c] = change ? y : x;
+        e[c + J] = change ? x : y;
+      }
+  };
+#pragma unroll 1
+  for (int k = 2; k < 2 * n; k <<= 1) {
+    const bool down = (tid * per & k) == 0;
+#pragma unroll 1
+    for (int j = k >> 1; j >= 32 * per; j >>= 1) {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < per; ++c) sm.list[c * kSampleThreads + tid] = e[c];
+      __syncthreads();
+      const int other = tid ^ (j / per);
+#pragma unroll
+      for (int c = 0; c < per; ++c) {
+        const u64 o = sm.list[c * kSampleThreads + other];
+        e[c] = (e[c] > o) == (down == (tid < other)) ? e[c] : o;
+      }
+    }
+#pragma unroll 1
+    for (int j = min(k >> 1, 16 * per); j >= per; j >>= 1) {
+      const int mask = j / per;
+      const bool larger = down == ((tid & mask) == 0);
+#pragma unroll
+      for (int c = 0; c < per; ++c) {
+        const u64 o = __shfl_xor_sync(~0u, e[c], mask);
+        e[c] = (e[c] > o) == larger ? e[c] : o;
+      }
+    }
+    if (per > 4 && k > 4) within(k, std::integral_constant<int, 4>());
+    if (per > 2 && k > 2) within(k, std::integral_constant<int, 2>());
+    if (per > 1) within(k, std::integral_constant<int, 1>());
+  }
+  __syncthreads();  // (the list may be written again)
+}
+
 // Of the n entries of CTA 0's list, the one with which the weights (masses, or one each), from the largest entry down,
-// reach `need`; the smallest where they do not.  In sm.border.  While they are many they are divided into 512 ranges of equal
-// width, of which one stays; then each looks at the others.
+// reach `need`; the smallest where they do not.  In sm.border, which is read after a barrier.
 // (per: entries of a thread that n needs at most)
 template <int per>
 __device__ __noinline__ void border_of(SampleShared &sm, Mass mass_of, int n, double need, bool masses) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  u64 *const few = sm.list + kList - kFew;  // their weights
-  auto weight_of = [&](u64 entry) -> u64 { return masses ? mass_of(value_of((unsigned)(entry >> 32))) : 1; };
-  if (n > kFew) {
-    u64 entry[per], w[per];
+  u64 e[per], w[per], sum = 0, whole;
+  sorted_list<per>(sm, n, e);
 #pragma unroll
-    for (int c = 0; c < per; ++c) {
-      const int i = tid + c * kSampleThreads;
-      entry[c] = i < n ? sm.list[i] : 0;
-      w[c] = i < n ? weight_of(entry[c]) : 0;
-    }
-    u64 above = 0;
-    for (;;) {
-      u64 lo = ~0ull, hi = 0;
-#pragma unroll
-      for (int c = 0; c < per; ++c)
-        if (entry[c]) {
-          lo = min(lo, entry[c]);
-          hi = max(hi, entry[c]);
-        }
-      for (int d = 16; d > 0; d >>= 1) {
-        lo = min(lo, __shfl_xor_sync(~0u, lo, d));
-        hi = max(hi, __shfl_xor_sync(~0u, hi, d));
-      }
-      __syncthreads();
-      if (lane == 0) {
-        sm.sums[warp] = lo;
-        sm.sums2[warp] = hi;
-      }
-      sm.hist[tid] = 0;
-      if (tid == 0) sm.found = kBins - 1;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kSampleWarps; ++i) {
-        lo = min(lo, sm.sums[i]);
-        hi = max(hi, sm.sums2[i]);
-      }
-      const int cut = max(0, 64 - __clzll((long long)(hi - lo)) - 9);
-      const int coarse = max(0, 64 - __clzll((long long)weight_of(hi)) - 19);  // (4096 weights of 2^19 fit 32 bits)
-      int range[per];
-#pragma unroll
-      for (int c = 0; c < per; ++c) {
-        range[c] = entry[c] ? (int)((hi - entry[c]) >> cut) : -1;
-        if (entry[c]) atomicAdd(&sm.hist[range[c]], (unsigned)(w[c] >> coarse));
-      }
-      __syncthreads();
-      u64 all;
-      const unsigned mine = sm.hist[tid];
-      const u64 before = scan_over_cta(sm, mine, all);
-      const double rough = (need - (double)above) / (double)(1ull << coarse);
-      if ((double)before < rough && rough <= (double)(before + mine)) sm.found = tid;
-      __syncthreads();
-      int at = sm.found;
-      // the exact sums have the last word: {weight of the ranges before `at`, of this one}
-      auto weights = [&]() {
-        Pair s{0, 0};
-#pragma unroll
-        for (int c = 0; c < per; ++c) {
-          s.x += range[c] >= 0 && range[c] < at ? w[c] : 0;
-          s.y += range[c] == at ? w[c] : 0;
-        }
-        s = sum_over_cta(sm, s);
-        s.x += above;
-        return s;
-      };
-      Pair s = weights();
-      while (at < kBins - 1 && (double)(s.x + s.y) < need) {
-        ++at;
-        s = weights();
-      }
-      while (at > 0 && (double)s.x >= need) {
-        --at;
-        s = weights();
-      }
-      above = s.x;
-      unsigned left = 0;
-#pragma unroll
-      for (int c = 0; c < per; ++c) {
-        if (range[c] != at) entry[c] = 0;
-        left += entry[c] != 0;
-      }
-      n = (int)sum_over_cta(sm, left);
-      if (n <= kFew) break;
-    }
-    if (tid == 0) sm.count = 0;
-    sm.hist[tid] = 0;  // (as it was found: the histogram of the next filter begins with it)
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < per; ++c)
-      if (entry[c]) sm.list[atomicAdd(&sm.count, 1)] = entry[c];
-    __syncthreads();
-    if (tid == 0) sm.count = 0;
-    need -= (double)above;
+  for (int c = 0; c < per; ++c) {
+    w[c] = !e[c] ? 0 : masses ? mass_of(value_of((unsigned)(e[c] >> 32))) : 1;
+    sum += w[c];
   }
-  if (tid < n) few[tid] = weight_of(sm.list[tid]);
-  if (tid == 0) sm.border = 0;
-  __syncthreads();
-  if (tid < n) {
-    const u64 mine = sm.list[tid];
-    u64 larger = 0;
-    bool least_of_all = true;
-#pragma unroll 8
-    for (int o = 0; o < n; ++o) {
-      const u64 other = sm.list[o];
-      if (other > mine) larger += few[o];
-      least_of_all &= other >= mine;
-    }
-    const bool reaches = (double)(larger + few[tid]) >= need;
-    if ((((double)larger < need || larger == 0) && reaches) || (least_of_all && !reaches)) sm.border = mine;
+  u64 run = scan_over_cta(sm, sum, whole);
+#pragma unroll
+  for (int c = 0; c < per; ++c) {
+    const int rank = threadIdx.x * per + c;
+    if (rank < n && (rank == 0 || (double)run < need) && (rank == n - 1 || (double)(run + w[c]) >= need)) sm.border = e[c];
+    run += w[c];
   }
-  __syncthreads();
 }
 
-
-// Steps of 1/16 in the logarithm of the mass below the largest logit (rounding is monotone), and bins of them.
+// Steps of 1/16 in the logarithm of the mass below the largest logit (rounding is monotone).
 struct Steps {
   float top, per_logit;
   __device__ __forceinline__ float of(float v) const {
     return v == top ? 0.f : top == INFINITY ? INFINITY : (top - v) * per_logit;
   }
-  static __device__ __forceinline__ int bin_of(float t) { return t < (float)kTail ? (int)t : kTail; }
-  __device__ __forceinline__ int bin(float v) const { return bin_of(of(v)); }
+  // all values of fewer steps than `edge` are at least this (two roundings are 2^-23)
+  __device__ __forceinline__ float floor(float edge) const {
+    return fmaxf(__fsub_rd(top, edge * 1.0001f / per_logit), -INFINITY);
+  }
 };
 
-// ---- CTA 0 by itself: n tokens in its list.  With masses all down to the bin after `bin`, near which top_p's border lies,
-// at the mass `want`; else all down to `bin`, which holds top_k's, `above` tokens lying in the bins before.
+// ---- CTA 0 by itself: n tokens in its list, all that may stay and some below them.
 // The draw takes the first token with running > u z: of integers, running > its floor; below z, so that there is one.
 __device__ __forceinline__ u64 target_in(double u, u64 z) { return min((u64)(u * (double)z), z - 1); }
 struct Row {  // of one row, what its last steps need
@@ -315,24 +278,30 @@ struct Row {  // of one row, what its last steps need
   double u;
   int64_t *out;
 };
+// n tokens are in CTA 0's list.  With masses all down to the bin after `bin`, near which top_p's border lies, at the mass
+// `want`; else all down to `bin`, which holds top_k's, `above` tokens lying in the bins before.
 template <int per>
-__device__ __noinline__ void finish(SampleShared &sm, u64 *runs, Mass mass_of, Row row, int n, int bin, bool masses, double want,
-                                    double above) {
+__device__ __noinline__ void finish(SampleShared &sm, unsigned *runs, Mass mass_of, Row row, int n, int bin, bool masses,
+                                    double want, double above) {
   const int tid = threadIdx.x;
-  u64 entry[per], m[per];
+  u64 entry[per], m[per], z;
+  int bins[per];
 #pragma unroll
   for (int c = 0; c < per; ++c) {
     const int i = tid + c * kSampleThreads;
-    entry[c] = i < n ? sm.list[i] : 0;
-    m[c] = 0;
-    if (c * kSampleThreads < n && i < n) m[c] = mass_of(value_of((unsigned)(entry[c] >> 32)));
+    entry[c] = m[c] = 0;
+    bins[c] = -1;
+    if (i < n) {
+      entry[c] = sm.list[i];
+      const float v = value_of((unsigned)(entry[c] >> 32));
+      m[c] = mass_of(v);
+      bins[c] = (int)row.step.of(v);
+    }
   }
-  // (runs: the row's room, which is not needed any more)
-  int bins[per];
-#pragma unroll
-  for (int c = 0; c < per; ++c) bins[c] = entry[c] ? row.step.bin(value_of((unsigned)(entry[c] >> 32))) : -1;
-  // the entries of the bin that are still there, by themselves; then only what reaches the border stays
+  const int last = masses ? bin + 1 : bin;  // (no entry lies in a later bin)
+  // Of the entries of one bin, by themselves, what lies below the one that reaches `need` is dropped.
   auto cut = [&](int at_bin, double need, bool by) {
+    u64 *const weight = sm.list + kList - kSampleThreads;
     __syncthreads();
     if (tid == 0) sm.count = 0;
     __syncthreads();
@@ -340,11 +309,34 @@ __device__ __noinline__ void finish(SampleShared &sm, u64 *runs, Mass mass_of, R
     for (int c = 0; c < per; ++c)
       if (bins[c] == at_bin) sm.list[atomicAdd(&sm.count, 1)] = entry[c];
     __syncthreads();
-    border_of<per>(sm, mass_of, sm.count, need, by);
+    const int some = sm.count;
+    if (some > kSampleThreads) border_of<kList / kSampleThreads>(sm, mass_of, some, need, by);
+    else {  // each looks at the others
+      u64 mine = 0;
+      if (tid < some) {
+        mine = sm.list[tid];
+        weight[tid] = by ? mass_of(value_of((unsigned)(mine >> 32))) : 1;
+      }
+      __syncthreads();
+      if (tid < some) {
+        u64 larger = 0;
+        int below = 0;
+#pragma unroll 4
+        for (int o = 0; o < some; ++o) {
+          const u64 other = sm.list[o];
+          if (other > mine) larger += weight[o];
+          below += other < mine;
+        }
+        const bool reaches = (double)(larger + weight[tid]) >= need;
+        if (((double)larger < need || larger == 0) && (reaches || below == 0)) sm.border = mine;
+      }
+    }
+    __syncthreads();
+    const u64 border = sm.border;
 #pragma unroll
     for (int c = 0; c < per; ++c)
-      if (entry[c] < sm.border) {
-        entry[c] = m[c] = 0;
+      if (bins[c] == at_bin ? entry[c] < border : bins[c] > at_bin) {
+        m[c] = 0;
         bins[c] = -1;
       }
   };
@@ -357,58 +349,66 @@ __device__ __noinline__ void finish(SampleShared &sm, u64 *runs, Mass mass_of, R
     }
     return sum_over_cta(sm, s);
   };
-  u64 z;
   if (!masses) {
     cut(bin, (double)row.k - above, false);
     if (row.by_mass) {  // top_p of what top_k has left: a histogram of rounded masses says where about
       unsigned *const rough = sm.hist;
-      __syncthreads();
       rough[tid] = 0;
-      __syncthreads();
+      want = (double)row.p * (double)around(last + 1).x;
+      if (tid == 0) sm.found = last;
 #pragma unroll
       for (int c = 0; c < per; ++c)
-        if (entry[c]) atomicAdd(&rough[bins[c]], (unsigned)(m[c] >> 25));  // (4096 tokens of 2^19)
-      want = (double)row.p * (double)around(kBins).x;
-      if (tid == 0) sm.found = kTail;
+        if (m[c]) atomicAdd(&rough[bins[c]], (unsigned)(m[c] >> 25));  // (4096 tokens of 2^19)
+      __syncthreads();
       const u64 mine = rough[tid], before = scan_over_cta(sm, mine, z);
       if ((double)before < want * 0x1p-25 && want * 0x1p-25 <= (double)(before + mine)) sm.found = tid;
       __syncthreads();
-      bin = sm.found;
+      bin = min(sm.found, last);
     }
   }
   if (row.by_mass) {
     // the exact sums have the last word: bins below while they do not reach, above while they would do without this one
     Pair s = around(bin);
-    while (bin < kTail && (double)(s.x + s.y) < want) s = around(++bin);
+    while (bin < last && (double)(s.x + s.y) < want) s = around(++bin);
     while (bin > 0 && (double)s.x >= want) s = around(--bin);
     cut(bin, want - (double)s.x, true);
   }
-  // the draw in the order of the indices: sums over 512 runs of indices, then the tokens of one run among themselves
-  int shift = 0;
-  while ((row.V >> shift) >= kSampleThreads) ++shift;
-  u64 *const masses_of_run = sm.list;
-  int *const members = reinterpret_cast<int *>(sm.list + kList / 2);
-  __syncthreads();
-  runs[tid] = 0;
+  // (runs: the row's room, which is not needed any more)
+#pragma unroll
+  for (int i = 0; i < 2 * kRuns; i += kSampleThreads) runs[tid + i] = 0;
   if (tid == 0) sm.count = 0;
   __syncthreads();
+  // The draw in the order of the indices: sums over 1024 runs of indices (at most 512 of one run, so that two halves of 22
+  // bits fit 32 each), then the tokens of one run among themselves.
+  int shift = 0;
+  while ((row.V >> shift) >= kRuns) ++shift;
+  unsigned *const upper = runs + kRuns;
+  u64 *const masses_of_run = sm.list;
+  int *const members = reinterpret_cast<int *>(sm.list + kList / 2);
 #pragma unroll
   for (int c = 0; c < per; ++c) {
     if (m[c] < row.least) m[c] = 0;
-    if (m[c]) atomicAdd(&runs[(int)~(unsigned)entry[c] >> shift], m[c]);
+    if (m[c]) {
+      const int to = (int)~(unsigned)entry[c] >> shift;
+      atomicAdd(&runs[to], (unsigned)m[c] & 0x3fffffu);
+      atomicAdd(&upper[to], (unsigned)(m[c] >> 22));
+    }
   }
   __syncthreads();
-  const u64 run = runs[tid], start = scan_over_cta(sm, run, z), target = target_in(row.u, z);
-  if (start <= target && target < start + run) {
-    sm.found = tid;
-    sm.start = start;
+  const uint2 lo = reinterpret_cast<const uint2 *>(runs)[tid], hi = reinterpret_cast<const uint2 *>(upper)[tid];
+  const u64 first = ((u64)hi.x << 22) + lo.x, second = ((u64)hi.y << 22) + lo.y;
+  const u64 start = scan_over_cta(sm, first + second, z), target = target_in(row.u, z);
+  if (start <= target && target < start + first + second) {
+    const bool later = target >= start + first;
+    sm.found = 2 * tid + later;
+    sm.start = later ? start + first : start;
   }
   __syncthreads();
   const int hit = sm.found;
 #pragma unroll
   for (int c = 0; c < per; ++c) {
     const int i = (int)~(unsigned)entry[c];
-    if (m[c] && (i >> shift) == hit) {  // (a run holds at most 2^shift <= 1024 indices)
+    if (m[c] && (i >> shift) == hit) {
       const int to = atomicAdd(&sm.count, 1);
       members[to] = i;
       masses_of_run[to] = m[c];
@@ -416,15 +416,14 @@ __device__ __noinline__ void finish(SampleShared &sm, u64 *runs, Mass mass_of, R
   }
   __syncthreads();
   const int count = sm.count;
-  for (int t = tid; t < count; t += kSampleThreads) {
-    u64 before = sm.start;
-    const int i = members[t];
+  if (tid < count) {
+    u64 at = sm.start;
+    const int i = members[tid];
     for (int o = 0; o < count; ++o)
-      if (members[o] < i) before += masses_of_run[o];
-    if (before <= target && target < before + masses_of_run[t]) *row.out = i;
+      if (members[o] < i) at += masses_of_run[o];
+    if (at <= target && target < at + masses_of_run[tid]) *row.out = i;
   }
 }
-
 
 template <typename TI>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a, int NV) {  // NV vectors a thread
@@ -472,9 +471,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
   }
   int turn = 0;
   // the same value from every CTA to every CTA: read after the next cluster barrier
-  auto spread_f = [&](float v) {
-    if (tid < C) cluster.map_shared_rank(&sm, tid)->gather_f[turn][rank] = v;
-  };
   auto spread_u = [&](u64 v) {
     if (tid < C) cluster.map_shared_rank(&sm, tid)->gather_u[turn][rank] = v;
   };
@@ -493,17 +489,41 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     }                                                                   \
   })
 
-  // ---- the largest logit
+  // ---- the largest logit, and (where k is small) a value that k tokens reach: of each warp's threads the largest logits are
+  // the first k / warps at least this
+  float bound = -INFINITY;
   {
-    const unsigned m = __reduce_max_sync(~0u, key_of(top));
-    if (lane == 0) sm.maxima[warp] = m;
+    const unsigned key = key_of(top), m = __reduce_max_sync(~0u, key);
+    const int64_t of_warp = (k + C * kSampleWarps - 1) / (C * kSampleWarps);
+    unsigned least_of = 0;
+    if (k < a.V && of_warp <= 32) {
+      int rank_of = 0;
+#pragma unroll 8
+      for (int l = 0; l < 32; ++l) {
+        const unsigned o = __shfl_sync(~0u, key, l);
+        rank_of += o > key || (o == key && l < lane);
+      }
+      least_of = __shfl_sync(~0u, key, __ffs(__ballot_sync(~0u, rank_of == (int)of_warp - 1)) - 1);
+    }
+    if (lane == 0) {
+      sm.maxima[warp] = m;
+      sm.bounds[warp] = least_of;
+    }
     __syncthreads();
     top = value_of(__reduce_max_sync(~0u, sm.maxima[lane & (kSampleWarps - 1)]));
+    least_of = __reduce_min_sync(~0u, sm.bounds[lane & (kSampleWarps - 1)]);
+    if (least_of) bound = value_of(least_of);
     if (C > 1) {
-      spread_f(top);
+      if (tid < C) {
+        SampleShared &to = *cluster.map_shared_rank(&sm, tid);
+        to.gather_top[rank] = top;
+        to.gather_bound[rank] = bound;
+      }
       cluster.sync();
-      for (int c = 0; c < C; ++c) top = fmaxf(top, sm.gather_f[turn][c]);
-      turn ^= 1;
+      for (int c = 0; c < C; ++c) {
+        top = fmaxf(top, sm.gather_top[c]);
+        bound = fminf(bound, sm.gather_bound[c]);
+      }
     }
   }
   // (no CTA leaves while another may still write to it)
@@ -515,6 +535,61 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     leave();
     return;
   }
+
+  // body(vec, i0, valid), by whole warps, for the vectors with a value of at least `floor` (few of them, mostly: a warp
+  // collects their places and takes 32 at a time)
+  auto each_above = [&](float floor, auto body) {
+    unsigned short *const queue = sm.waiting[warp];
+    int waiting = 0;
+    auto take = [&](int n) {
+      waiting -= n;
+      const bool valid = lane < n;
+      const int at = valid ? queue[waiting + lane] : lane, other = at % 32 - lane;
+      body(row_data[at / 32 * kSampleThreads + other], first_of(at / 32) + other * VEC, valid);
+    };
+#pragma unroll 1
+    for (int j = 0; j < NV; ++j) {
+      const bool in = row_data[j * kSampleThreads].most() >= floor;
+      const unsigned mask = __ballot_sync(~0u, in);
+      if (in) queue[waiting + __popc(mask & ((1u << lane) - 1))] = (unsigned short)(32 * j + lane);
+      waiting += __popc(mask);
+      if (waiting >= 32) {
+        __syncwarp();
+        take(32);
+        __syncwarp();
+      }
+    }
+    __syncwarp();
+    if (waiting) take(waiting);
+  };
+
+  // body(v, i, j, valid), by whole warps, for the values of at least `floor`, of which j is the thread's vector
+  auto each_value = [&](float floor, auto body) {
+    unsigned short *const queue = sm.waiting[warp];
+    int waiting = 0;
+    auto take = [&](int n) {
+      waiting -= n;
+      const bool valid = lane < n;
+      const int at = valid ? queue[waiting + lane] : lane, other = at % 32 - lane, e = at / 32 % VEC, j = at / 32 / VEC;
+      body(to_f(reinterpret_cast<const TI *>(&row_data[j * kSampleThreads + other])[e]), first_of(j) + other * VEC + e, j, valid);
+    };
+    EACH_VECTOR({
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const bool in = vec.at(e) >= floor;
+        const unsigned mask = __ballot_sync(~0u, in);
+        if (in) queue[waiting + __popc(mask & ((1u << lane) - 1))] = (unsigned short)((j * VEC + e) * 32 + lane);
+        waiting += __popc(mask);
+        if (waiting >= 32) {
+          __syncwarp();
+          take(32);
+          __syncwarp();
+        }
+      }
+    })
+    __syncwarp();
+    if (waiting) take(waiting);
+  };
 
   auto cta_sum = [&](u64 v) { return sum_over_cta(sm, v); };
   auto cta_scan = [&](u64 v, u64 &whole) { return scan_over_cta(sm, v, whole); };
@@ -619,7 +694,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
 
   const Steps step{top, (float)(16.0 * 1.4426950408889634 * per_unit)};
   auto step_of = [&](float v) { return step.of(v); };
-  auto bin_of = [&](float t) { return Steps::bin_of(t); };
 
   if (by_rank || by_mass) {
     auto part = [&](float t) {  // 2^(-t/16)
@@ -628,30 +702,73 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       return r;
     };
     auto weight15 = [&](float t) { return (unsigned)__float2int_rn(part(t) * 32768.f); };
-    bool summed = false, done = false;
+    bool done = false;
     // ---- a border: the first token, from the top, with which the weights of the tokens that stay reach the target.
     // masses: weights are masses and the target p of their whole; else numbers of tokens and the target k.
     // Leaves the border, and with masses the sums of what stays in the groups (those with at least min_p of the largest).
-    auto narrow = [&](bool masses) {
+    auto narrow = [&](auto kind) {
+      constexpr bool masses = decltype(kind)::value;
+      const int last = masses ? kMassTail : kTail;  // the bin of all that lies below the others
+      auto bin_of = [&](float t) { return t < (float)last ? (int)t : last; };
       u64 mass = 0;
       unsigned tail = 0;
-      EACH_VECTOR({
-        int b[VEC];
-        unsigned w[VEC];
+      if (masses) {
+        // The many tokens below 2^-20 need no more than an exponential in 32 bits: off by 2^-21 of themselves, in no common
+        // direction (the factor is held in two parts), which is 2^-41 of the largest mass each.  As integers of 2^-43 they
+        // fit the mantissa of 2^23.  The others queue up, so that whole warps take the 64-bit exponentials.
+        const double c = 1.4426950408889634 * per_unit;
+        const float c0 = (float)c, c1 = (float)(c - (double)c0), least_heavy = fmaxf(step.floor((float)last), -3.402823466e38f);
+        float *const queue = reinterpret_cast<float *>(sm.list) + warp * kQueue;
+        unsigned light = 0;
+        auto weigh = [&](float v) {
+          const float t = step_of(v);
+          const int b = bin_of(t);
+          if (b < last) atomicAdd(&sm.hist[b], weight15(t - (float)b));
+          mass += mass_of(v);
+        };
+        auto add_up = [&](auto all) {  // (all: no border lies before this one)
+          int waiting = 0;
+          EACH_VECTOR({
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float v = vec.at(e);
-          const bool in = stays(v, i0 + e);
-          const float t = in ? step_of(v) : INFINITY;
-          b[e] = bin_of(t);
-          w[e] = masses ? weight15(t - (float)b[e]) : 1u;
-          if (masses) mass += in ? mass_of(v) : 0;
-          tail += in && b[e] == kTail;
-        }
+            for (int e = 0; e < VEC; ++e) {
+              const float v = vec.at(e);
+              const bool in = decltype(all)::value || stays(v, i0 + e);
+              const bool heavy = in && v >= least_heavy;
+              const unsigned mask = __ballot_sync(~0u, heavy);
+              if (heavy) queue[waiting + __popc(mask & ((1u << lane) - 1))] = v;
+              waiting += __popc(mask);
+              float r;
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaxf(fmaf(v - top, c1, fmaf(v - top, c0, 43.f)), -200.f)));
+              if (in && !heavy) light += __float_as_uint(r + 8388608.f) - __float_as_uint(8388608.f);
+            }
+            if (waiting >= 32) {
+              __syncwarp();
+              do {
+                waiting -= 32;
+                weigh(queue[waiting + lane]);
+              } while (waiting >= 32);
+              __syncwarp();
+            }
+          })
+          __syncwarp();
+          if (lane < waiting) weigh(queue[lane]);
+        };
+        if (border_x == -INFINITY) add_up(std::true_type());
+        else add_up(std::false_type());
+        mass += 2 * (u64)light;
+      } else {
+        each_above(bound, [&](const Vec<TI> &vec, int, bool valid) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (b[e] < kTail) atomicAdd(&sm.hist[b[e]], w[e]);
-      })
+          for (int e = 0; e < VEC; ++e) {
+            const float v = vec.at(e);
+            if (valid && v >= bound && v > -INFINITY) {
+              const int b = bin_of(step_of(v));
+              if (b < kTail) atomicAdd(&sm.hist[b], 1u);
+              else ++tail;
+            }
+          }
+        });
+      }
       if (masses) spread_u(cta_sum(mass));
       else if ((tail = __reduce_add_sync(~0u, tail)) && lane == 0) atomicAdd(&sm.hist[kTail], tail);
       // Picks the bin: every CTA the same from everybody's histograms.  unit: of a bin's weights; above: what lies before the
@@ -714,24 +831,29 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       const double edge0 = masses ? sm.table[(e16 & 15) * 4] * __hiloint2double((1023 + (e16 >> 4)) << 20, 0) * (1.0 / 32768) : 1.0;
       int bin = pick(edge0, true);
       if (masses) turn ^= 1;
-      if (bin > kTail) bin = kTail;
+      if (bin > last) bin = last;
       // the tokens of CTA 0's list: those that stay and are `in`
       // (each CTA lists its own; the others' lists then join CTA 0's)
-      auto gather = [&](auto in) {
-        EACH_VECTOR({
+      auto gather = [&](float floor, auto in) {  // (floor: no value below it is in)
+        each_above(floor, [&](const Vec<TI> &vec, int i0, bool valid) {
           unsigned hits = 0;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) hits |= (unsigned)(stays(vec.at(e), i0 + e) && in(vec.at(e))) << e;
-          if (hits) {
-            int at = atomicAdd(&sm.count, __popc(hits));
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-              if (hits >> e & 1) {
-                if (at < kList) sm.list[at] = ((u64)key_of(vec.at(e)) << 32) | (unsigned)~(i0 + e);
-                ++at;
-              }
+          for (int e = 0; e < VEC; ++e) hits |= (unsigned)(valid && stays(vec.at(e), i0 + e) && in(vec.at(e))) << e;
+          int run = __popc(hits);
+          for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(~0u, run, d);
+            if (lane >= d) run += o;
           }
-        })
+          int at = 0;
+          if (lane == 31 && run) at = atomicAdd(&sm.count, run);
+          at = __shfl_sync(~0u, at, 31) + run - __popc(hits);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (hits >> e & 1) {
+              if (at < kList) sm.list[at] = ((u64)key_of(vec.at(e)) << 32) | (unsigned)~(i0 + e);
+              ++at;
+            }
+        });
         if (rank != 0) {
           __syncthreads();
           const int n = sm.count;
@@ -761,47 +883,30 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
           atomicMax(&sm0.highest, hi);
         }
       };
-      if (bin + 1 < kTail && tokens * 1.05 < (double)kList) {  // (masses tell their tokens' number to within 2^(1/16))
+      if (bin + 1 < last && tokens * 1.05 < (double)kList) {  // (masses tell their tokens' number to within 2^(1/16))
         const float edge = (float)(bin + (masses ? 2 : 1));
-        gather([&](float v) { return step_of(v) < edge; });
+        gather(step.floor(edge), [&](float v) { return step_of(v) < edge; });
         done = true;
         if (C > 1) cluster.sync();
         else __syncthreads();
         if (rank == 0) {
           const Row rest{step, a.V, by_mass, k, p, least, u, a.out + row};
-          u64 *const room = reinterpret_cast<u64 *>(row_data - tid);
-          const int n = sm.count;
+          unsigned *const room = reinterpret_cast<unsigned *>(row_data - tid);
+          const int n = min(sm.count, kList);
           if (n <= kSampleThreads) finish<1>(sm, room, mass_of, rest, n, bin, masses, target * one, above);
           else finish<kList / kSampleThreads>(sm, room, mass_of, rest, n, bin, masses, target * one, above);
         }
         return;
       }
-      // with masses: what lies above the bin, exactly, and in the groups.  The exact sums have the last word on the bin.
+      // with masses: what lies above the bin, exactly.  The exact sums have the last word on the bin.
       u64 sure = 0;
       while (masses) {
         Pair mine{0, 0};
-        __syncthreads();
-        fill_groups([&](const Vec<TI> &vec, int i0, u64 *w) {
-          unsigned hits = 0, here = 0;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float v = vec.at(e);
-            const int b = bin_of(step_of(v));
-            if (stays(v, i0 + e)) {
-              hits |= (unsigned)(b < bin) << e;
-              here |= (unsigned)(b == bin) << e;
-            }
-            w[e] = 0;
-          }
-          if (__any_sync(~0u, (hits | here) != 0)) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const u64 m = mass_of(vec.at(e));
-              mine.x += hits >> e & 1 ? m : 0;
-              mine.y += here >> e & 1 ? m : 0;
-              w[e] = (hits >> e & 1) && m >= least ? m : 0;
-            }
-          }
+        each_value(bin < last ? step.floor((float)(bin + 1)) : -INFINITY, [&](float v, int i, int, bool valid) {
+          const int b = bin_of(step_of(v));
+          const u64 m = valid && stays(v, i) ? mass_of(v) : 0;
+          mine.x += b < bin ? m : 0;
+          mine.y += b == bin ? m : 0;
         });
         Pair s = sum_over_cta(sm, mine);
         if (C > 1) {
@@ -817,12 +922,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         }
         sure = s.x;
         if (bin > 0 && (double)s.x >= target * one) --bin;
-        else if (bin < kTail && (double)(s.x + s.y) < target * one) ++bin;
+        else if (bin < last && (double)(s.x + s.y) < target * one) ++bin;
         else break;
-      }
-      if (masses) {
-        summed = true;
-        above = (double)sure * (1.0 / one);
       }
       // gathers the bin's tokens; divides it while they are too many
       unsigned low = 0, high = ~0u;  // keys
@@ -833,23 +934,24 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       int n;
       bool divided = false;
       for (;;) {
-        gather(inside);
-        extremes(inside);
+        gather(bin < last ? step.floor((float)(bin + 1)) : -INFINITY, inside);
         if (C > 1) cluster.sync();
         else __syncthreads();
         sm.hist[tid] = 0;  // (everybody has read the histograms)
         n = sm0.count;
-        const unsigned all_lo = sm0.lowest, all_hi = sm0.highest;
+        if (n > kList) {
+          extremes(inside);
+          if (C > 1) cluster.sync();
+          else __syncthreads();
+          low = sm0.lowest;
+          high = sm0.highest;
+        }
         if (C > 1) cluster.sync();
         else __syncthreads();
         if (rank == 0 && tid == 0) {
           sm.count = 0;
           sm.lowest = ~0u;
           sm.highest = 0;
-        }
-        if (n > 0) {
-          low = all_lo;
-          high = all_hi;
         }
         if (n <= kList || low == high) break;
         divided = true;
@@ -869,13 +971,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       if (masses && divided && n > 0) {  // the bin's tokens above what is left of it join what lies above
         const float highest = value_of(high);
         u64 more = 0;
-        EACH({
-          if (stays(v, i) && bin_of(step_of(v)) == bin && v > highest) {
-            const u64 m = mass_of(v);
-            more += m;
-            if (m >= least) atomicAdd(&sm.group[j * kSampleWarps + warp], m);
-          }
-        })
+        each_value(highest, [&](float v, int i, int, bool valid) {
+          if (valid && stays(v, i) && bin_of(step_of(v)) == bin && v > highest) more += mass_of(v);
+        });
         more = cta_sum(more);
         if (C > 1) {
           spread_u(more);
@@ -889,7 +987,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       if (n == 0) return;  // (a tail without tokens)
       if (n <= kList) {
         if (rank == 0) {
-          border_of<kList / kSampleThreads>(sm, mass_of, n, masses ? target * one - (double)sure : target - above, masses);
+          const double need = masses ? target * one - (double)sure : target - above;
+          if (n <= kSampleThreads) border_of<1>(sm, mass_of, n, need, masses);
+          else border_of<kList / kSampleThreads>(sm, mass_of, n, need, masses);
+          __syncthreads();
           if (tid == 0) {
             sm.border_x = value_of((unsigned)(sm.border >> 32));
             sm.border_i = (int)~(unsigned)sm.border;
@@ -899,14 +1000,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         else __syncthreads();
         border_x = sm0.border_x;
         border_i = sm0.border_i;
-        if (masses) {  // the list's tokens that stay join the groups
-          EACH({
-            if (stays(v, i) && inside(v)) {
-              const u64 m = mass_of(v);
-              if (m >= least) atomicAdd(&sm.group[j * kSampleWarps + warp], m);
-            }
-          })
-        }
       } else {  // many tokens of one value: their number decides, and the index of the last
         const float value = value_of(high);
         const u64 m = mass_of(value);
@@ -923,16 +1016,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         else __syncthreads();
         border_i = sm0.border_i;
         border_x = value;
-        summed = false;
       }
       if (C > 1) cluster.sync();
       else __syncthreads();
     };
-    if (by_rank) narrow(false);
+    if (by_rank) narrow(std::false_type());
     if (done) return;  // (nobody reads or writes another CTA's memory after the last barrier)
-    if (by_mass) narrow(true);
+    if (by_mass) narrow(std::true_type());
     if (done) return;
-    if (!summed) fill_groups(kept);
+    __syncthreads();
+    if (tid < NV * kSampleWarps) sm.group[tid] = 0;
+    __syncthreads();
+    each_value(fmaxf(border_x, -3.402823466e38f), [&](float v, int i, int j, bool valid) {
+      u64 m = valid && stays(v, i) ? mass_of(v) : 0;
+      if (m < least) m = 0;
+      unsigned left = __ballot_sync(~0u, m != 0);
+      while (left) {  // (a warp's values come in the order of its vectors: two or three of them)
+        const int lead = __ffs(left) - 1, one_of = __shfl_sync(~0u, j, lead);
+        const bool same = m != 0 && j == one_of;
+        const unsigned mask = __ballot_sync(~0u, same);
+        const unsigned lo = __reduce_add_sync(~0u, same ? (unsigned)m & 0x3fffffu : 0);
+        const unsigned hi = __reduce_add_sync(~0u, same ? (unsigned)(m >> 22) : 0);
+        if (lane == lead) sm.group[one_of * kSampleWarps + warp] += ((u64)hi << 22) + lo;
+        __syncwarp();
+        left &= ~mask;
+      }
+    });
   } else {
     fill_groups(kept);
   }

@@ -1,5 +1,5 @@
 """Gated delta rule and sampling without a GPU: what the C entry points and the Python functions refuse, and the float64
-checkers against differences and by hand."""
+oracles against differences and by hand."""
 
 from __future__ import annotations
 
