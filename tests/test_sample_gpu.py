@@ -83,6 +83,28 @@ def test_wide_nuclei_draw_exactly(dtype, b, V, spread):
     check(logits, u, 0.9, V // 2, top_p, 0.001)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("gap,below", [(12.0, 1e-3), (16.0, 1e-4), (25.0, 2.0 ** -23)])
+def test_borders_far_below_the_largest(dtype, gap, below):
+    """One token far above tens of thousands, of which a filter keeps some: steps, bins and small masses at their ends."""
+    V = 50021
+    logits, _ = rows(8, V, dtype, seed=7, spread=1.0)
+    logits[:, 17] = gap + 4.5
+    u = 1.0 - below * torch.rand(8, generator=torch.Generator().manual_seed(8), dtype=torch.float64).cuda()
+    for k, p in ((0, 1.0 - below), (1000, 1.0), (1000, 1.0 - below), (30000, 1.0 - below), (50, 1.0)):
+        check(logits, u, 1.0, k, p, 0.0)
+        check(logits, u, 0.4, k, p, 0.0)
+
+
+@pytest.mark.parametrize("k,p", [(700, 1.0), (2500, 0.9), (0, 0.3), (3900, 0.95)])
+def test_few_values_shared_by_many_tokens(k, p):
+    gen = torch.Generator().manual_seed(11)
+    values = torch.tensor([2.0, 1.0, 0.5, -40.0])
+    logits = values[torch.randint(0, 4, (16, 6000), generator=gen)].to(torch.bfloat16).cuda()
+    logits[8:] += (0.01 * torch.randn(8, 6000, generator=gen)).bfloat16().cuda()
+    check(logits, torch.rand(16, generator=gen).cuda(), 0.7, k, p, 0.0)
+
+
 def test_signed_zeros_are_one_value():
     logits = torch.tensor([[-0.0, 0.0, -0.0, -1.0]], device="cuda").repeat(3, 1)
     got = check(logits, torch.tensor([0.0, 0.4, 0.9]).cuda(), 1.0, 2, 1.0, 0.0)
