@@ -311,16 +311,17 @@ __device__ __forceinline__ void tile_rows(float (&c)[8][4], const Frag<SA> &a, c
   mma_group<SA, SB, 4>(c, 0, a, b);
 }
 // c (16 x W) += a (16 x 16 tokens) B for rows 16 kb .. of a row-major tile of W columns (planes `plane` apart)
-template <int SA, int SB, int W>
+// (group: blocks of B that are held at a time)
+template <int SA, int SB, int W, int group = 4>
 __device__ __forceinline__ void tile_cols(float (&c)[W / 8][4], const Frag<SA> &a, const __half *tile, int plane, int kb) {
 #pragma unroll
-  for (int n0 = 0; n0 < W / 16; n0 += 4) {
-    uint32_t b[4][SB][4];
+  for (int n0 = 0; n0 < W / 16; n0 += group) {
+    uint32_t b[group][SB][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < group; ++i)
 #pragma unroll
       for (int s = 0; s < SB; ++s) b_kn(b[i][s], tile + s * plane + 16 * kb * (W + 8) + 16 * (n0 + i), W + 8);
-    mma_group<SA, SB, 4>(c, n0, a, b);
+    mma_group<SA, SB, group>(c, n0, a, b);
   }
 }
 template <int n>
@@ -356,12 +357,14 @@ __device__ __forceinline__ const TI *head_base(const Rows &r, int b, int h, int 
 }
 
 // A tile of 64 tokens x W columns from global memory in 16-byte pieces, `per` of a thread, zeros outside rows and cols.
+// (By the first kThreads threads of a CTA.)
 template <typename TI, int W>
 struct Pieces {
   static constexpr int V = 16 / (int)sizeof(TI), per = L * W / V / kThreads;
   uint4 x[per];
   static __device__ __forceinline__ int row(int i) { return (i * kThreads + (int)threadIdx.x) / (W / V); }
   static __device__ __forceinline__ int col(int i) { return (i * kThreads + (int)threadIdx.x) % (W / V) * V; }
+  static __device__ __forceinline__ void meet() { asm volatile("barrier.sync 2, %0;" ::"n"(kThreads) : "memory"); }
   // (room: as many bytes of shared memory as the tile has, for rows that no 16-byte access fits)
   __device__ __forceinline__ void load(const TI *src, int64_t st, int rows, int cols, bool vec, void *room) {
     if (!vec) {
@@ -371,7 +374,7 @@ struct Pieces {
         const int r = i / W, c = i % W;
         raw[i] = r < rows && c < cols ? src[r * st + c] : from_f<TI>(0.f);
       }
-      __syncthreads();
+      meet();
     }
 #pragma unroll
     for (int i = 0; i < per; ++i) {
@@ -380,7 +383,7 @@ struct Pieces {
       if (!vec) x[i] = static_cast<const uint4 *>(room)[i * kThreads + threadIdx.x];
       else if (r < rows && c < cols) x[i] = *reinterpret_cast<const uint4 *>(src + r * st + c);
     }
-    if (!vec) __syncthreads();
+    if (!vec) meet();
   }
   __device__ __forceinline__ unsigned max_bits() const {  // of the largest magnitude, as fp32
     unsigned m = 0;

@@ -29,8 +29,10 @@ constexpr int chunk_smem() {
   return chunk_tiles<NT, SI>() + L * kAld * 4;
 }
 
+// The upper part is rounded to nearest: what is left is then at most 2^-11 of x and of either sign, and the product of two
+// such parts, which is left out, 2^-22.  (Cut off, it would be 2^-20, always of the result's sign.)  A NaN stays one in lo.
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
-  hi = __float_as_uint(x) & 0xffffe000u;
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 // c (16 x 16, two n8 tiles) += sign * A B^T for A in accumulator layout (two n8 tiles) and B rows (n) of row-major fp32.
