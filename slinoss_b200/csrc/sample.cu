@@ -22,6 +22,7 @@
 #include <cooperative_groups.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 
@@ -463,6 +464,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), C = (int)cluster.num_blocks();
   SampleShared &sm0 = *cluster.map_shared_rank(&sm, 0);
+  auto started = cluster.barrier_arrive();  // (waited for before the first access to another CTA's memory)
   const int row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const TI *x = static_cast<const TI *>(a.logits) + row * a.stride;
   const float temperature = a.temperature ? a.temperature[row] : a.temperature0;
@@ -543,6 +545,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
     top = value_of(__reduce_max_sync(~0u, sm.maxima[lane & (kSampleWarps - 1)]));
     least_of = __reduce_min_sync(~0u, sm.bounds[lane & (kSampleWarps - 1)]);
     if (least_of) bound = value_of(least_of);
+    cluster.barrier_wait(std::move(started));
     if (C > 1) {
       if (tid < C) {
         SampleShared &to = *cluster.map_shared_rank(&sm, tid);
