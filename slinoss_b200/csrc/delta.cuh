@@ -385,18 +385,24 @@ struct Pieces {
     }
     if (!vec) meet();
   }
-  __device__ __forceinline__ unsigned max_bits() const {  // of the largest magnitude, as fp32
-    unsigned m = 0;
+  __device__ __forceinline__ unsigned max_bits() const {  // of the largest magnitude, as fp32 (a NaN is the largest)
+    if constexpr (sizeof(TI) == 4) {
+      unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < per; ++i) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      for (int i = 0; i < per; ++i) m = max(max(max(m, x[i].x & 0x7fffffffu), max(x[i].y & 0x7fffffffu, x[i].z & 0x7fffffffu)), x[i].w & 0x7fffffffu);
+      return m;
+    } else {
+      __nv_bfloat162 m[2] = {__float2bfloat162_rn(0.f), __float2bfloat162_rn(0.f)};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(TI) == 4) m = max(m, w[j] & 0x7fffffffu);
-        else m = max(m, max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));  // bf16
+      for (int i = 0; i < per; ++i) {
+        const __nv_bfloat162 *w = reinterpret_cast<const __nv_bfloat162 *>(&x[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m[j & 1] = __hmax2_nan(m[j & 1], __habs2(w[j]));
       }
+      const __nv_bfloat162 r = __hmax2_nan(m[0], m[1]);
+      const uint32_t bits = *reinterpret_cast<const uint32_t *>(&r);
+      return max((bits << 16) & 0x7fffffffu, bits & 0x7fff0000u);
     }
-    return m;
   }
   // as scaled fp16, to an operand tile in shared memory and (COPY) to a copy of it in global memory
   template <int SI, bool COPY>
@@ -420,9 +426,13 @@ struct Pieces {
         uint4 h = x[i];
         if constexpr (!std::is_same<TI, __half>::value) {
           uint32_t *w = reinterpret_cast<uint32_t *>(&h);
+          const __nv_bfloat162 s2 = __float2bfloat162_rn(s);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            w[j] = pack(__uint_as_float(w[j] << 16) * s, __uint_as_float(w[j] & 0xffff0000u) * s);
+          for (int j = 0; j < 4; ++j) {  // (times a power of two: exact, but for what fp16 rounds to zero)
+            const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&w[j]), s2);
+            const uint32_t b = *reinterpret_cast<const uint32_t *>(&y);
+            w[j] = pack(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
+          }
         }
         *reinterpret_cast<uint4 *>(tile + at) = h;
         if constexpr (COPY) *reinterpret_cast<uint4 *>(copy + at) = h;
