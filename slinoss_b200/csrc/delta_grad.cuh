@@ -10,6 +10,10 @@
 // there).  One CTA of four warps per chunk and head; a warp owns 16 tokens, as t for dq and as s for Z, with its result rows
 // in accumulators; Q and H are formed in both orientations, in registers, which costs 1/8 more products than passing them
 // through shared memory would save barriers.
+//
+// 16384 chunks of one head each (N 128, P 64, bf16): 898 us at two CTAs an SM (103 KB and 255 registers a thread); 160 KB a chunk
+// through HBM would take 400.  Eight warps a CTA, four for dO, Q and dq and four for dX, H and dk, take 1123 us: at 128 registers
+// they spill, with one CTA an SM nothing hides the loads.
 #pragma once
 
 #include "delta.cuh"
