@@ -108,6 +108,31 @@ __device__ __forceinline__ void store_grad(TO *out, const float (&c)[NT / 8][4],
   }
 }
 
+// Where products join sums that are there already.  The matrix instructions cut off what they add below the accumulator's last
+// bit, always towards zero: sixty steps onto one accumulator were 1.2e-6 of dk, and by product they are 8e-7.  Where results are not rounded to bf16
+// anyway, each product has accumulators of its own, which are added by themselves.
+template <int NT, int SC>
+struct Onto {
+  float (&sum)[NT / 8][4];
+  float own[SC == 2 ? NT / 8 : 1][4];
+  __device__ __forceinline__ Onto(float (&c)[NT / 8][4]) : sum(c) {
+    if constexpr (SC == 2) zero(own);
+  }
+  template <int SB>
+  __device__ __forceinline__ void add(const Frag<SC> &f, const __half *tile, int plane, int kb) {
+    if constexpr (SC == 2) tile_cols<SC, SB, NT, 2>(own, f, tile, plane, kb);
+    else tile_cols<SC, SB, NT>(sum, f, tile, plane, kb);
+  }
+  __device__ __forceinline__ void join() {
+    if constexpr (SC == 2) {
+#pragma unroll
+      for (int j = 0; j < NT / 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[j][i] += own[j][i];
+    }
+  }
+};
+
 template <int NT, int SI, int SC, typename TI>
 __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
   using Op = Operand<SI, NT>;
@@ -276,21 +301,29 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       times_rows(acc, closing[r0] * u, closing[r1] * u);
     }
     const float s1 = fq * pow2(-e1), s2 = fh * pow2(-e2);
+    {
+      Onto<NT, SC> to(acc);
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-      if (kb >= warp) {
-        Frag<SC> f;
-        frag_of<SC>(f, Q[2 * kb], Q[2 * kb + 1], s1);
-        tile_cols<SC, SI, NT>(acc, f, qs, Op::plane, kb);
-      }
+      for (int kb = 0; kb < 4; ++kb)
+        if (kb >= warp) {
+          Frag<SC> f;
+          frag_of<SC>(f, Q[2 * kb], Q[2 * kb + 1], s1);
+          to.template add<SI>(f, qs, Op::plane, kb);
+        }
+      to.join();
+    }
     times(acc, pow2(e1 + eq - (e2 + ek)));
+    {
+      Onto<NT, SC> to(acc);
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-      if (kb >= warp) {
-        Frag<SC> f;
-        frag_of<SC>(f, H[2 * kb], H[2 * kb + 1], s2);
-        tile_cols<SC, SI, NT>(acc, f, ks, Op::plane, kb);
-      }
+      for (int kb = 0; kb < 4; ++kb)
+        if (kb >= warp) {
+          Frag<SC> f;
+          frag_of<SC>(f, H[2 * kb], H[2 * kb + 1], s2);
+          to.template add<SI>(f, ks, Op::plane, kb);
+        }
+      to.join();
+    }
     unit = e2 + ek;  // (acc is Z without its unit)
     db = row_dots<NT, SI>(acc, krow, ek);
     db.x *= pow2(unit);
@@ -328,6 +361,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       if (is_q) zero(acc);
       else times_rows(acc, b0 * u, b1 * u);
     }
+    Onto<NT, SC> onto(acc);
 #pragma unroll 1
     for (int pt = 0; pt < tiles; ++pt) {
       if (tiles > 1) {
@@ -358,9 +392,10 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
             load_b(bb, ys, sb, kb);
             mma_split<SC, SC>(H[2 * sb], H[2 * sb + 1], fa, bb);
           }
-        tile_cols<SC, SC, NT>(acc, fg, ss, splane, kb);
+        onto.template add<SC>(fg, ss, splane, kb);
       }
     }
+    onto.join();
 #pragma unroll
     for (int sb = 0; sb < 4; ++sb)
       if (sb <= warp) {
@@ -388,13 +423,17 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     const int e = floor_exp(warp_exp(H) + ya_top + above(f), warp_exp(acc) + unit, ek);
     times(acc, pow2(unit - (e + ek)));
     const float s = f * pow2(ya_top - e);
+    {
+      Onto<NT, SC> to(acc);
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-      if (kb <= warp) {
-        Frag<SC> fh2;
-        frag_of<SC>(fh2, H[2 * kb], H[2 * kb + 1], s);
-        tile_cols<SC, SI, NT>(acc, fh2, ks, Op::plane, kb);
-      }
+      for (int kb = 0; kb < 4; ++kb)
+        if (kb <= warp) {
+          Frag<SC> fh2;
+          frag_of<SC>(fh2, H[2 * kb], H[2 * kb + 1], s);
+          to.template add<SI>(fh2, ks, Op::plane, kb);
+        }
+      to.join();
+    }
     times(acc, pow2(e + ek));
     dots_k = dots_q;
     dots_q = row_dots<NT, SI>(acc, (is_q ? qs : ks) + 16 * warp * ld, is_q ? eq : ek);
