@@ -109,22 +109,23 @@ __device__ __forceinline__ void store_grad(TO *out, const float (&c)[NT / 8][4],
 }
 
 // Where products join sums that are there already.  The matrix instructions cut off what they add below the accumulator's last
-// bit, always towards zero: sixty steps onto one accumulator were 1.2e-6 of dk, and by product they are 8e-7.  Where results are not rounded to bf16
-// anyway, each product has accumulators of its own, which are added by themselves.
-template <int NT, int SC>
+// bit, always towards zero: sixty steps onto one accumulator were 1.2e-6 of dk in fp32, and by product they are 6e-7.  So each
+// product of fp32 tensors has accumulators of its own, which are added by themselves (fp16's rounding hides it: 2 % of its time).
+template <int NT, int SI, int SC>
 struct Onto {
+  static constexpr bool apart = SI == 2;
   float (&sum)[NT / 8][4];
-  float own[SC == 2 ? NT / 8 : 1][4];
+  float own[apart ? NT / 8 : 1][4];
   __device__ __forceinline__ Onto(float (&c)[NT / 8][4]) : sum(c) {
-    if constexpr (SC == 2) zero(own);
+    if constexpr (apart) zero(own);
   }
   template <int SB>
   __device__ __forceinline__ void add(const Frag<SC> &f, const __half *tile, int plane, int kb) {
-    if constexpr (SC == 2) tile_cols<SC, SB, NT, 2>(own, f, tile, plane, kb);
+    if constexpr (apart) tile_cols<SC, SB, NT, 2>(own, f, tile, plane, kb);
     else tile_cols<SC, SB, NT>(sum, f, tile, plane, kb);
   }
   __device__ __forceinline__ void join() {
-    if constexpr (SC == 2) {
+    if constexpr (apart) {
 #pragma unroll
       for (int j = 0; j < NT / 8; ++j)
 #pragma unroll
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     }
     const float s1 = fq * pow2(-e1), s2 = fh * pow2(-e2);
     {
-      Onto<NT, SC> to(acc);
+      Onto<NT, SI, SC> to(acc);
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
         if (kb >= warp) {
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     }
     times(acc, pow2(e1 + eq - (e2 + ek)));
     {
-      Onto<NT, SC> to(acc);
+      Onto<NT, SI, SC> to(acc);
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
         if (kb >= warp) {
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       if (is_q) zero(acc);
       else times_rows(acc, b0 * u, b1 * u);
     }
-    Onto<NT, SC> onto(acc);
+    Onto<NT, SI, SC> onto(acc);
 #pragma unroll 1
     for (int pt = 0; pt < tiles; ++pt) {
       if (tiles > 1) {
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     times(acc, pow2(unit - (e + ek)));
     const float s = f * pow2(ya_top - e);
     {
-      Onto<NT, SC> to(acc);
+      Onto<NT, SI, SC> to(acc);
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
         if (kb <= warp) {

@@ -92,6 +92,17 @@ __device__ __forceinline__ void minus_cols(float (&c)[8][4], const float (&v)[8]
     c[j][3] = fmaf(b, c[j][3], v[j][3]);
   }
 }
+// c = f c + s d.  Where fp32 and fp16 results are wanted, sums over a chunk's tokens have accumulators of their own: the matrix
+// instructions cut off what they add below an accumulator's last bit, and the state, which goes on for the whole sequence, would
+// shrink by that at every step (d_initial of 700 tokens in fp32 2.2e-6, so 6e-7).  With bf16 it would not show, and the passes of
+// the teams take 2 and 7 % longer; fp16's pass back by warps would take 25 % longer for its registers and goes without.
+template <int n>
+__device__ __forceinline__ void join(float (&c)[n][4], float f, const float (&d)[n][4], float s) {
+#pragma unroll
+  for (int j = 0; j < n; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[j][i] = fmaf(c[j][i], f, d[j][i] * s);
+}
 template <int S>
 __device__ __forceinline__ void frags_of(Frag<S> (&f)[4], const float (&c)[8][4], int e) {
   const float s = pow2(-e);
@@ -99,6 +110,22 @@ __device__ __forceinline__ void frags_of(Frag<S> (&f)[4], const float (&c)[8][4]
   for (int kb = 0; kb < 4; ++kb) frag_of<S>(f[kb], c[2 * kb], c[2 * kb + 1], s);
 }
 __device__ __forceinline__ int4 exps_of(const Record *r) { return __ldg(reinterpret_cast<const int4 *>(&r->eT)); }
+
+// c = f c + a B, over the 64 tokens of an operand tile B
+template <bool own, int SI, int NT>
+__device__ __forceinline__ void onto(float (&c)[NT / 8][4], float f, const Frag<2> (&a)[4], const __half *tile) {
+  if constexpr (own) {
+    float d[NT / 8][4];
+    zero(d);
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(d, a[kb], tile, Operand<SI, NT>::plane, kb);
+    join(c, f, d, 1.f);
+  } else {
+    times(c, f);
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(c, a[kb], tile, Operand<SI, NT>::plane, kb);
+  }
+}
 
 template <int NT, int SI, int SC, typename TI>
 __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
@@ -223,10 +250,8 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
     if (more) issue_rest(c + 1);
     cp_commit();
     if (active) {
-      times(S, top * pow2(unit - (eC + ek)));
+      onto<SC == 2, SI, NT>(S, top * pow2(unit - (eC + ek)), fc, kt);
       unit = eC + ek;
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(S, fc[kb], kt, Op::plane, kb);
     }
     ex = nx;
   }
@@ -366,13 +391,9 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
     if (c > 0) issue_rest(c - 1);
     cp_commit();
     if (active) {
-      times(R, top * pow2(unit - (e1 + eq)));
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(R, f1[kb], qs, Op::plane, kb);
-      times(R, pow2(e1 + eq - (e2 + ek)));
+      onto<SI == 2, SI, NT>(R, top * pow2(unit - (e1 + eq)), f1, qs);
+      onto<SI == 2, SI, NT>(R, pow2(e1 + eq - (e2 + ek)), f2, kt);
       unit = e2 + ek;
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb) tile_cols<2, SI, NT>(R, f2[kb], kt, Op::plane, kb);
     }
     ex = nx;
   }

@@ -255,17 +255,6 @@ __device__ __forceinline__ void write_state16(void *dst, int dtype, size_t base,
     }
 }
 
-// c = f c + s d.  Where fp32 and fp16 results are wanted, sums over a chunk's tokens have accumulators of their own: the matrix
-// instructions cut off what they add below an accumulator's last bit, and the state, which goes on for the whole sequence, would
-// shrink by that at every step (d_initial of 300 tokens in fp32 1.2e-6, so 5e-7).  With bf16 it would not show, and the passes
-// take 2 and 7 % longer.
-template <int n>
-__device__ __forceinline__ void join(float (&c)[n][4], float f, const float (&d)[n][4], float s) {
-#pragma unroll
-  for (int j = 0; j < n; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[j][i] = fmaf(c[j][i], f, d[j][i] * s);
-}
 // hi + lo of a fragment as accumulators, times s
 template <int S>
 __device__ __forceinline__ void frag_values(float (&c)[2][4], const Frag<S> &f, float s) {
