@@ -80,6 +80,8 @@ __global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_c
   const int chunk = blockIdx.x, b = blockIdx.y / a.key_heads, kh = blockIdx.y % a.key_heads;
   const int share = a.heads / a.key_heads, t0 = chunk * L, rows = min(L, a.T - t0);
 
+  const bool train = a.st;  // (the backward reads the tables and the lower plane of P; with bf16 the forward reads neither)
+
   // near pairs of block w lie in a block of A above the diagonal
   auto near_at = [&](int w, int r, int c) -> float & { return A[((w < 3 ? 0 : 16) + r) * kAld + (w < 3 ? 16 * w + 16 : 32) + c]; };
   In kx, qx;  // (on their way while the gates are read)
@@ -130,7 +132,8 @@ __global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_c
     __syncthreads();
     if (tid < L) {
       const float x = expf((float)(G[tid] - (tid < 16 ? 0.0 : G[(tid & ~15) - 1])));
-      rise[tid] = rec->rise[tid] = x;
+      rise[tid] = x;
+      if (train) rec->rise[tid] = x;
       rec->gamma[tid] = expf((float)G[tid]);
     } else {
       rec->closing[tid - L] = expf((float)(G[L - 1] - G[tid - L]));
@@ -138,13 +141,15 @@ __global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_c
     if (tid < 96) {
       const int i = tid < 16 ? 1 : tid < 48 ? 2 : 3;
       const float x = expf((float)(G[16 * i - 1] - G[tid - fall_at(i)]));
-      fall[tid] = rec->fall[tid] = x;
+      fall[tid] = x;
+      if (train) rec->fall[tid] = x;
     }
 #pragma unroll 4
     for (int i = lane; i < 256; i += 32) {  // this warp's block of near pairs
       const int r = i / 16, c = i % 16;
       const float x = c <= r ? expf((float)(G[16 * warp + r] - G[16 * warp + c])) : 0.f;
-      near_at(warp, r, c) = rec->near[warp][r * kNearLd + c] = x;
+      near_at(warp, r, c) = x;
+      if (train) rec->near[warp][r * kNearLd + c] = x;
     }
   };
   auto record_of = [&](int h) { return a.rec + (size_t)(b * a.heads + h) * a.NC + chunk; };
@@ -314,7 +319,8 @@ __global__ void __launch_bounds__(kThreads, NT == 64 || SI == 1 ? 4 : 1) delta_c
     uint4 *dst = reinterpret_cast<uint4 *>(rec);
     const uint4 *src = reinterpret_cast<const uint4 *>(tri);
 #pragma unroll
-    for (int i = 0; i < 4 * kTri / 8 / kThreads; ++i) dst[tid + i * kThreads] = src[tid + i * kThreads];
+    for (int i = 0; i < 4 * kTri / 8 / kThreads; ++i)
+      if (i < 3 * kTri / 8 / kThreads || train || !std::is_same<TI, __nv_bfloat16>::value) dst[tid + i * kThreads] = src[tid + i * kThreads];
     if (tid == 0) *reinterpret_cast<int4 *>(&rec->eT) = make_int4(eT, eQ, eq, ek);
     if (hs + 1 < share) {  // G, beta, A and tri are written again
       __syncthreads();
