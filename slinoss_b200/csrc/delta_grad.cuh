@@ -481,15 +481,34 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
   }
 }
 
-// dq and dk of key heads that several value heads share: the sums of theirs, in the order of the heads
-template <typename TI>
-__global__ void __launch_bounds__(256) delta_share_kernel(const float *pq, const float *pk, TI *dq, TI *dk, int share, int64_t per,
-                                                          int64_t total) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const float *src = (blockIdx.y ? pk : pq) + (i / per) * share * per + i % per;
-    float s = 0.f;
-    for (int h = 0; h < share; ++h) s += src[h * per];
-    (blockIdx.y ? dk : dq)[i] = from_f<TI>(s);
+// dq and dk of key heads that several value heads share: the sums of theirs, in the order of the heads.  per: values of a head,
+// V of them a thread at a time (4, where they divide into fours: 3 heads of 1537 x 64 values, 12 key heads, 5 us; one at a time 12).
+template <int V, typename TI>
+__global__ void __launch_bounds__(256) delta_share_kernel(const float *pq, const float *pk, TI *dq, TI *dk, int share, int64_t per) {
+  const float *src = (blockIdx.z ? pk : pq) + blockIdx.y * (share * per);
+  TI *dst = (blockIdx.z ? dk : dq) + blockIdx.y * per;
+  for (int64_t i = (blockIdx.x * 256 + threadIdx.x) * V; i < per; i += (int64_t)gridDim.x * 256 * V) {
+    float s[V] = {0.f};
+    for (int h = 0; h < share; ++h) {
+      if constexpr (V == 4) {
+        const float4 x = __ldcs(reinterpret_cast<const float4 *>(src + h * per + i));
+        s[0] += x.x;
+        s[1] += x.y;
+        s[2] += x.z;
+        s[3] += x.w;
+      } else {
+        s[0] += src[h * per + i];
+      }
+    }
+    if constexpr (V == 4) {
+      alignas(16) TI out[V];
+#pragma unroll
+      for (int n = 0; n < V; ++n) out[n] = from_f<TI>(s[n]);
+      using Wide = std::conditional_t<sizeof(TI) == 4, uint4, uint2>;
+      *reinterpret_cast<Wide *>(dst + i) = *reinterpret_cast<const Wide *>(out);
+    } else {
+      dst[i] = from_f<TI>(s[0]);
+    }
   }
 }
 

@@ -70,11 +70,13 @@ static int launch_bwd(const Args &a, void *dq, void *dk, int warps, cudaStream_t
     if (const int rc = check_launch("delta_grad_kernel")) return rc;
   }
   if (a.heads != a.key_heads) {
-    const int64_t per = (int64_t)a.T * a.N, total = per * a.batch * a.key_heads;
-    const int64_t want = (total + 255) / 256;
-    delta_share_kernel<TI><<<dim3((unsigned)(want < 8 * kB200Sms ? want : 8 * kB200Sms), 2), 256, 0, st>>>(
+    const int64_t per = (int64_t)a.T * a.N;
+    const bool wide = per % 4 == 0 && ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk)) & 15) == 0;
+    const int64_t want = (per + (wide ? 1023 : 255)) / (wide ? 1024 : 256), fill = 16 * kB200Sms / (a.batch * a.key_heads) + 1;
+    auto kernel = wide ? delta_share_kernel<4, TI> : delta_share_kernel<1, TI>;
+    kernel<<<dim3((unsigned)(want < fill ? want : fill), a.batch * a.key_heads, 2), 256, 0, st>>>(
         static_cast<const float *>(a.dq), static_cast<const float *>(a.dk), static_cast<TI *>(dq), static_cast<TI *>(dk),
-        a.heads / a.key_heads, per, total);
+        a.heads / a.key_heads, per);
     return check_launch("delta_share_kernel");
   }
   return SLX_OK;

@@ -110,6 +110,7 @@ def compare(inp, got, want):
     (1, 2, 2, 150, 128, 128),  # two tiles of value channels
     (1, 1, 1, 100, 96, 200),  # four, the last one ragged
     (2, 6, 2, 257, 64, 64),
+    (1, 4, 2, 67, 33, 16),    # shared keys, whose gradients do not divide into fours
 ])
 def test_forward_and_gradients(dtype, b, h, hk, T, N, P):
     inp = make(b, h, hk, T, N, P, dtype, seed=T + N + P)
