@@ -13,7 +13,8 @@
 //
 // 16384 chunks of one head each (N 128, P 64, bf16): 898 us at two CTAs an SM (103 KB and 255 registers a thread); 160 KB a chunk
 // through HBM would take 400.  Eight warps a CTA, four for dO, Q and dq and four for dX, H and dk, take 1123 us: at 128 registers
-// they spill, with one CTA an SM nothing hides the loads.
+// they spill, with one CTA an SM nothing hides the loads.  fp16 with 64 columns (900 chunks, 108 KB): 74 us at two CTAs an SM,
+// 107 at one, which a second plane of dO made it.
 #pragma once
 
 #include "delta.cuh"
@@ -23,7 +24,7 @@ namespace delta {
 
 template <int NT, int SI, int SC>
 constexpr int grad_smem() {
-  return 2 * Operand<SI, NT>::halves * 2 + 3 * SC * kTile * 2 + 2 * SC * 64 * (NT + 8) * 2 + kVectorBytes;
+  return 2 * Operand<SI, NT>::halves * 2 + (SI + 2 * SC) * kTile * 2 + 2 * SC * 64 * (NT + 8) * 2 + kVectorBytes;
 }
 
 // sum over n of the rows' accumulators times the operand tile's rows (16 of them from `tile`); both rows of the thread
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
   constexpr int ld = NT + 8, splane = 64 * ld;
   extern __shared__ __align__(128) char smem[];
   __half *ks = reinterpret_cast<__half *>(smem), *qs = ks + Op::halves;
-  __half *os = qs + Op::halves, *xs = os + SC * kTile, *ys = xs + SC * kTile;  // tokens x channels: dO, dX, Y
+  __half *os = qs + Op::halves, *xs = os + SI * kTile, *ys = xs + SC * kTile;  // tokens x channels: dO, dX, Y
   __half *ss = ys + SC * kTile, *rs = ss + SC * splane;                          // channels x N: S0, R
   float *gamma = reinterpret_cast<float *>(rs + SC * splane), *closing = gamma + L, *beta = closing + L;
   float *rise = beta + L + 32, *fall = rise + L, *near = fall + 96;
@@ -186,22 +187,23 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     Pieces<TI, 64> o;
     o.load(head_base<TI>(a.dO, b, h, t0) + 64 * pt, a.dO.st, rows, a.P - 64 * pt, a.dO.vec, os);
     o.template store<SI, false>(os, nullptr, eo_top);
-    if constexpr (SI < SC) {  // (a second plane of zeros: one code for dO and dX)
-      for (int i = tid * 8; i < kTile; i += kThreads * 8) *reinterpret_cast<uint4 *>(os + kTile + i) = make_uint4(0, 0, 0, 0);
-    }
     cp_wait<0>();
     __syncthreads();
   };
   auto below = [&](int e, int top, int pt, int kb) { return __shfl_sync(~0u, e, 4 * pt + kb) - top; };
   const int r0 = 16 * warp + g, r1 = r0 + 8;
   const __half *krow = ks + 16 * warp * ld;
-  auto load_a = [&](Frag<SC> &f, const __half *tile, int kb) {
+  auto load_a = [&](Frag<SC> &f, const __half *tile, int planes, int kb) {  // (dO may have one where dX has two)
 #pragma unroll
-    for (int s = 0; s < SC; ++s) a_mk(f.r[s], tile + s * kTile + 16 * warp * kTileLd + 16 * kb, kTileLd);
+    for (int s = 0; s < SC; ++s) {
+      if (s < planes) a_mk(f.r[s], tile + s * kTile + 16 * warp * kTileLd + 16 * kb, kTileLd);
+      else f.r[s][0] = f.r[s][1] = f.r[s][2] = f.r[s][3] = 0;
+    }
   };
-  auto load_b = [&](uint32_t (&f)[SC][4], const __half *tile, int rb, int kb) {
+  auto load_b = [&](auto &f, const __half *tile, int rb, int kb) {
+    constexpr int planes = sizeof(f) / 16;
 #pragma unroll
-    for (int s = 0; s < SC; ++s) b_nk(f[s], tile + s * kTile + 16 * rb * kTileLd + 16 * kb, kTileLd);
+    for (int s = 0; s < planes; ++s) b_nk(f[s], tile + s * kTile + 16 * rb * kTileLd + 16 * kb, kTileLd);
   };
   float acc[NT / 8][4];
   // ---- Z, this warp's tokens as s
@@ -224,15 +226,15 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
 #pragma unroll 1
       for (int kb = 0; kb < blocks; ++kb) {
         Frag<SC> fy;
-        load_a(fy, ys, kb);
+        load_a(fy, ys, SC, kb);
         const Frag<SC> f1 = scaled(fy, below(ey, y_top, pt, kb)), f2 = scaled(fy, below(yx, yx_top, pt, kb));
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb)
           if (tb >= warp) {
-            uint32_t bo[SC][4], bx[SC][4];
+            uint32_t bo[SI][4], bx[SC][4];
             load_b(bo, os, tb, kb);
             load_b(bx, xs, tb, kb);
-            mma_split<SC, SC>(Q[2 * tb], Q[2 * tb + 1], f1, bo);
+            mma_split<SC, SI>(Q[2 * tb], Q[2 * tb + 1], f1, bo);
             mma_split<SC, SC>(H[2 * tb], H[2 * tb + 1], f2, bx);
           }
         tile_cols<SC, SC, NT>(acc, scaled(fy, below(yr, yr_top, pt, kb)), rs, splane, kb);
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
 #pragma unroll 1
       for (int kb = 0; kb < blocks; ++kb) {
         Frag<SC> fa, fg;
-        load_a(fa, tile, kb);
+        load_a(fa, tile, is_q ? SI : SC, kb);
         const float m = pow2(below(sa, unit, pt, kb)), f0 = g0 * m, f1 = g1 * m;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
