@@ -70,7 +70,7 @@ struct alignas(16) SampleShared {  // (the row's vectors follow it)
   u64 gather_u[2][kMaxCluster], gather_v[2][kMaxCluster];
   double pick_before, pick_tokens;
   u64 start, border;
-  int pick_bin, found;
+  int pick_bin, pick_upto, found;
   // of CTA 0
   int count;
   unsigned lowest, highest;
@@ -303,11 +303,11 @@ struct Row {  // of one row, what its last steps need
   double u;
   int64_t *out;
 };
-// n tokens are in CTA 0's list.  With masses all down to the bin after `bin`, near which top_p's border lies, at the mass
-// `want`; else all down to `bin`, which holds top_k's, `above` tokens lying in the bins before.
+// n tokens are in CTA 0's list, all down to the bin `last`.  With masses top_p's border, at the mass `want`, is among them, in
+// `bin` or near it; else `bin` is the last and holds top_k's, `above` tokens lying in the bins before.
 template <int per>
-__device__ __noinline__ void finish(SampleShared &sm, unsigned *runs, Mass mass_of, Row row, int n, int bin, bool masses,
-                                    double want, double above) {
+__device__ __noinline__ void finish(SampleShared &sm, unsigned *runs, Mass mass_of, Row row, int n, int bin, int last,
+                                    bool masses, double want, double above) {
   const int tid = threadIdx.x;
   u64 entry[per], m[per], z;
   int bins[per];
@@ -323,7 +323,6 @@ __device__ __noinline__ void finish(SampleShared &sm, unsigned *runs, Mass mass_
       bins[c] = (int)row.step.of(v);
     }
   }
-  const int last = masses ? bin + 1 : bin;  // (no entry lies in a later bin)
   // Of the entries of one bin, by themselves, what lies below the one that reaches `need` is dropped.
   auto cut = [&](int at_bin, double need, bool by) {
     u64 *const weight = sm.list + kList - kSampleThreads;
@@ -745,7 +744,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       const Steps scale = masses || bound == -INFINITY ? step : Steps{top, (float)(kTail - 1) / (top - bound)};
       auto step_of = [&](float v) { return scale.of(v); };
       auto bin_of = [&](float t) { return t < (float)last ? (int)t : last; };
-      u64 mass = 0;
+      u64 mass = 0, beyond = 0;  // of all tokens, of those in the last bin
       unsigned tail = 0;
       if (masses) {
         // The many tokens below 2^-20 need no more than an exponential in 32 bits: off by 2^-21 of themselves, in no common
@@ -758,8 +757,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         auto weigh = [&](float v) {
           const float t = step_of(v);
           const int b = bin_of(t);
+          const u64 m = mass_of(v);
           if (b < last) atomicAdd(&sm.hist[b], weight15(t - (float)b));
-          mass += mass_of(v);
+          else beyond += m;
+          mass += m;
         };
         auto add_up = [&](auto all) {  // (all: no border lies before this one)
           int waiting = 0;
@@ -790,6 +791,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         };
         if (border_x == -INFINITY) add_up(std::true_type());
         else add_up(std::false_type());
+        beyond += 2 * (u64)light;
         mass += 2 * (u64)light;
       } else {
         each_above(bound, [&](const Vec<TI> &vec, int, bool valid) {
@@ -804,11 +806,18 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
           }
         });
       }
-      if (masses) spread_u(cta_sum(mass));
+      if (masses) {
+        const Pair s = sum_over_cta(sm, Pair{mass, beyond});
+        spread_u(s.x);
+        if (tid < C) cluster.map_shared_rank(&sm, tid)->gather_v[turn][rank] = s.y;
+      }
       else if ((tail = __reduce_add_sync(~0u, tail)) && lane == 0) atomicAdd(&sm.hist[kTail], tail);
       // Picks the bin: every CTA the same from everybody's histograms.  unit: of a bin's weights; above: what lies before the
-      // first, then before the bin; tokens: about how many lie above the lower edge of the bin after it.
+      // first, then before the bin; upto: the bin by which the target is met whatever the histogram's rounding (2^-15 of a
+      // weight); tokens: about how many lie above its lower edge; listed: the tokens of all bins but the last meet the target.
       double target = (double)k, above = 0.0, tokens = 0.0;
+      int upto = 0;
+      bool listed = false;
       auto pick = [&](double unit, bool first) {
         if (C > 1) cluster.sync();
         else __syncthreads();
@@ -833,28 +842,36 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
           sm.scan[warp] = run;
           sm.scan2[warp] = few;
         }
-        if (tid == 0) sm.pick_bin = kBins;
+        if (tid == 0) sm.pick_bin = sm.pick_upto = kBins;
         __syncthreads();
-        double upto = (lane < kSampleWarps ? sm.scan : sm.scan2)[lane % kSampleWarps];  // each in half of the warp
+        double passed = (lane < kSampleWarps ? sm.scan : sm.scan2)[lane % kSampleWarps];  // each in half of the warp
         for (int d = 1; d < kSampleWarps; d <<= 1) {
-          const double o = __shfl_up_sync(~0u, upto, d, kSampleWarps);
-          if (lane % kSampleWarps >= d) upto += o;
+          const double o = __shfl_up_sync(~0u, passed, d, kSampleWarps);
+          if (lane % kSampleWarps >= d) passed += o;
         }
-        const double run_before = __shfl_sync(~0u, upto, max(warp - 1, 0)), few_before = __shfl_sync(~0u, upto, 16 + max(warp - 1, 0));
-        const double start = above + (warp ? run_before : 0.0), all = above + __shfl_sync(~0u, upto, kSampleWarps - 1);
+        const double run_before = __shfl_sync(~0u, passed, max(warp - 1, 0)), few_before = __shfl_sync(~0u, passed, 16 + max(warp - 1, 0));
+        const double start = above + (warp ? run_before : 0.0), all = above + __shfl_sync(~0u, passed, kSampleWarps - 1);
         few += warp ? few_before : 0.0;
         if (masses && first) {
-          u64 whole = 0;
-          for (int c = 0; c < C; ++c) whole += sm.gather_u[turn][c];
+          u64 whole = 0, left = 0;
+          for (int c = 0; c < C; ++c) {
+            whole += sm.gather_u[turn][c];
+            left += sm.gather_v[turn][c];
+          }
           target = (double)p * (double)whole * (1.0 / one);
+          listed = (double)(whole - left) >= target * one;
         }
         const bool reached = start + run >= target;
         const unsigned votes = __ballot_sync(~0u, reached);
         if (reached && lane == __ffs(votes) - 1) atomicMin(&sm.pick_bin, tid);
+        const bool surely = start + run >= (masses ? target * (1.0 + 1.0 / 8192) : target);
+        const unsigned sure_votes = __ballot_sync(~0u, surely);
+        if (surely && lane == __ffs(sure_votes) - 1) atomicMin(&sm.pick_upto, tid);
         __syncthreads();
         const int b = sm.pick_bin;
         if (b == tid || (b == kBins && tid == kBins - 1)) sm.pick_before = b == tid ? start + run - w : all;
-        if (tid == min(b + 1, kBins - 1)) sm.pick_tokens = few;
+        upto = sm.pick_upto;
+        if (tid == min(upto, kBins - 1)) sm.pick_tokens = few;
         __syncthreads();
         above = sm.pick_before;
         tokens = sm.pick_tokens;
@@ -917,8 +934,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
           atomicMax(&sm0.highest, hi);
         }
       };
-      if (bin + 1 < last && tokens * 1.05 < (double)kList) {  // (masses tell their tokens' number to within 2^(1/16))
-        const float edge = (float)(bin + (masses ? 2 : 1));
+      if ((upto < last || listed) && tokens * 1.05 < (double)kList) {  // (masses tell their tokens' number to within 2^(1/16))
+        upto = min(upto, last - 1);
+        const float edge = (float)(upto + 1);
         gather(scale.floor(edge), [&](float v) { return step_of(v) < edge; });
         done = true;
         if (C > 1) cluster.sync();
@@ -927,9 +945,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
           const Row rest{scale, a.V, by_mass, k, p, least, u, a.out + row};
           unsigned *const room = reinterpret_cast<unsigned *>(row_data - tid);
           const int n = min(sm.count, kList);
-          if (n <= kSampleThreads) finish<1>(sm, room, mass_of, rest, n, bin, masses, target * one, above);
-          else if (n <= 3 * kSampleThreads) finish<3>(sm, room, mass_of, rest, n, bin, masses, target * one, above);
-          else finish<kList / kSampleThreads>(sm, room, mass_of, rest, n, bin, masses, target * one, above);
+          if (n <= kSampleThreads) finish<1>(sm, room, mass_of, rest, n, min(bin, upto), upto, masses, target * one, above);
+          else if (n <= 3 * kSampleThreads) finish<3>(sm, room, mass_of, rest, n, min(bin, upto), upto, masses, target * one, above);
+          else finish<kList / kSampleThreads>(sm, room, mass_of, rest, n, min(bin, upto), upto, masses, target * one, above);
         }
         return;
       }

@@ -105,6 +105,21 @@ def test_few_values_shared_by_many_tokens(k, p):
     check(logits, torch.rand(16, generator=gen).cuda(), 0.7, k, p, 0.0)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_borders_between_tokens_far_apart(dtype):
+    """top_p a millionth above what some of the tokens hold: the next one counts, however far below it lies."""
+    b = 400
+    gen = torch.Generator().manual_seed(12)
+    logits = (4.0 * torch.randn(b, 10, generator=gen)).to(DT[dtype])
+    mass = torch.exp(logits.double() - logits.double().amax(-1, keepdim=True)).sort(-1, descending=True)[0]
+    share = mass.cumsum(-1) / mass.sum(-1, keepdim=True)
+    some = torch.randint(0, 5, (b,), generator=gen)
+    top_p = share.gather(1, some[:, None])[:, 0] * torch.where(torch.arange(b) % 2 == 0, 1 + 1e-6, 1 - 1e-6)
+    top_p = top_p.float().clamp(max=1 - 2.0 ** -23)
+    check(logits.cuda(), (1.0 - 1e-9 * torch.rand(b, generator=gen, dtype=torch.float64)).cuda(), 1.0, 0, top_p.cuda(), 0.0)
+    check(logits.cuda(), torch.rand(b, generator=gen).cuda(), 1.0, 0, top_p.cuda(), 0.0)
+
+
 def test_signed_zeros_are_one_value():
     logits = torch.tensor([[-0.0, 0.0, -0.0, -1.0]], device="cuda").repeat(3, 1)
     got = check(logits, torch.tensor([0.0, 0.4, 0.9]).cuda(), 1.0, 2, 1.0, 0.0)
