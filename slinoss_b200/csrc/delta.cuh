@@ -99,8 +99,9 @@ constexpr int kZeroExp = -100;  // of a tile of zeros
 // Of a tile that holds an infinity or NaN: its powers are NaN, so that everything computed from the tile is NaN and not a
 // finite value that scaling by the infinity has wiped out.
 constexpr int kNanExp = 2000;
+// (zero below the normal range)
 __device__ __forceinline__ float pow2(int e) {
-  return abs(e) > 1000 ? __int_as_float(0x7fc00000) : __int_as_float((min(max(e, -126), 127) + 127) << 23);
+  return e > 1000 ? __int_as_float(0x7fc00000) : __int_as_float((min(max(e, -127), 127) + 127) << 23);
 }
 // e with max * 2^-e in [2^14, 2^15), from the bits of the largest magnitude
 __device__ __forceinline__ int exp_of(unsigned bits) {
@@ -112,8 +113,9 @@ __device__ __forceinline__ int above(float x) {
   return b >= 0x7f800000u ? kNanExp : (int)(b >> 23) - 126;
 }
 // an exponent for a product's operand such that an accumulator of exponent ec, brought to the product's unit e + eb, stays
-// far inside the range (what the raising rounds away is 2^-40 of the accumulator)
-__device__ __forceinline__ int floor_exp(int e, int ec, int eb) { return max(e, ec - eb - 40); }
+// far inside the range (what the raising rounds away is 2^-40 of the accumulator), and the unit does too
+constexpr int kLowestUnit = -100;
+__device__ __forceinline__ int floor_exp(int e, int ec, int eb) { return max(e, max(ec - 40, kLowestUnit) - eb); }
 __device__ __forceinline__ unsigned mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 template <int n>
 __device__ __forceinline__ unsigned max_mag(const float (&c)[n][4]) {

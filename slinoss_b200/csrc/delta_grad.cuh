@@ -477,7 +477,10 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (2 * lane + i < rows) {
-        store_as(a.dg, a.g_dtype, row + i, i == 0 ? after + x : after + y);
+        // (a gate that drops the state has no gradient, which the sum meets but for its roundings)
+        const int t = 2 * lane + i;
+        const float open = t == 0 ? gamma[0] : t % 16 == 0 ? rise[t] : near[t * kNearLd + t % 16 - 1];
+        store_as(a.dg, a.g_dtype, row + i, open == 0.f ? 0.f : i == 0 ? after + x : after + y);
         store_as(a.dbeta, a.beta_dtype, row + i, dbs[2 * lane + i]);
       }
   }

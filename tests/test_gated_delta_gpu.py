@@ -143,6 +143,32 @@ def test_many_heads_are_as_few(dtype):
         assert rel_err(_np(grads[n][:2]), _np(grads2[n])) <= 2 * tolerance(dt, n, grads2[n].dtype), n
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("b", [2, 60])
+def test_states_that_fade(dtype, b):
+    """The state decays by 2^-100 and more while nothing is written: small values keep their scale, down to zero."""
+    inp = make(b, 3, 3, 129, 128, 32, dtype, seed=33)
+    inp["g"] = torch.full_like(inp["g"], -1.0)
+    inp["beta"][:, :, 64:] = 0
+    _, final, _ = run(inp)
+    _, want, _ = odelta.forward(*(_np(inp[n]) for n in NAMES[:5]), 128 ** -0.5, _np(inp["init"]))
+    assert rel_err(_np(final), want) <= tolerance(inp["q"].dtype, "final", final.dtype)
+    inp["g"] = torch.full_like(inp["g"], -2.0)  # e^-130 of a state near one
+    _, final, _ = run(inp)
+    assert torch.isfinite(final).all() and float(final.detach().abs().max()) < 1e-37
+
+
+def test_a_dropped_state_has_no_gate_gradient():
+    inp = make(2, 2, 2, 150, 64, 32, "bf16", seed=34)
+    for t in (0, 1, 16, 63, 64, 97, 149):
+        inp["g"][:, :, t] = -torch.inf
+    grads = run(inp)[2]
+    assert (grads["g"][:, :, [0, 1, 16, 63, 64, 97, 149]] == 0).all() and (grads["g"][:, :, 2] != 0).all()
+    one = make(1, 2, 2, 1, 64, 16, "fp32", seed=35)
+    one["g"].fill_(-torch.inf)
+    assert (run(one)[2]["g"] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
 def test_special_rows_among_many(dtype):
     inp = make(84, 2, 2, 140, 64, 32, dtype, seed=32)
