@@ -978,6 +978,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         else if (bin < last && (double)(s.x + s.y) < target * one) ++bin;
         else break;
       }
+      if (masses) above = (double)sure * (1.0 / one);  // (what the bin's division goes on from, of the bin that it has become)
       // gathers the bin's tokens; divides it while they are too many
       unsigned low = 0, high = ~0u;  // keys
       auto inside = [&](float v) {
