@@ -818,7 +818,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       double target = (double)k, above = 0.0, tokens = 0.0;
       int upto = 0;
       bool listed = false;
-      auto pick = [&](double unit, bool first) {
+      auto pick = [&](double unit) {
         if (C > 1) cluster.sync();
         else __syncthreads();
         unsigned n[kMaxCluster];
@@ -852,7 +852,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         const double run_before = __shfl_sync(~0u, passed, max(warp - 1, 0)), few_before = __shfl_sync(~0u, passed, 16 + max(warp - 1, 0));
         const double start = above + (warp ? run_before : 0.0), all = above + __shfl_sync(~0u, passed, kSampleWarps - 1);
         few += warp ? few_before : 0.0;
-        if (masses && first) {
+        if (masses) {
           u64 whole = 0, left = 0;
           for (int c = 0; c < C; ++c) {
             whole += sm.gather_u[turn][c];
@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       // (bins' edges are powers of 2^(1/16), from the table of 2^(i/64): 2^(-b/16) = 2^(-b>>4) 2^((-b&15)/16))
       const int e16 = -tid;
       const double edge0 = masses ? sm.table[(e16 & 15) * 4] * __hiloint2double((1023 + (e16 >> 4)) << 20, 0) * (1.0 / 32768) : 1.0;
-      int bin = pick(edge0, true);
+      int bin = pick(edge0);
       if (masses) turn ^= 1;
       if (bin > last) bin = last;
       // the tokens of CTA 0's list: those that stay and are `in`
@@ -978,15 +978,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         else if (bin < last && (double)(s.x + s.y) < target * one) ++bin;
         else break;
       }
-      if (masses) above = (double)sure * (1.0 / one);  // (what the bin's division goes on from, of the bin that it has become)
-      // gathers the bin's tokens; divides it while they are too many
+      // Gathers the bin's tokens; divides it while they are too many: by the keys of its logits, with sums that are exact in
+      // every part.  (Rounded weights would be off alike for all tokens of one value, by as much as the whole of another.)
+      const double goal = masses ? target * one : target;
+      if (!masses) sure = (u64)above;
       unsigned low = 0, high = ~0u;  // keys
       auto inside = [&](float v) {
         const unsigned key = key_of(v);
         return key >= low && key <= high && bin_of(step_of(v)) == bin;
       };
+      u64 *const parts = sm.list;  // of every CTA, between two gatherings
       int n;
-      bool divided = false;
       for (;;) {
         gather(bin < last ? scale.floor((float)(bin + 1)) : -INFINITY, inside);
         if (C > 1) cluster.sync();
@@ -1008,40 +1010,35 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
           sm.highest = 0;
         }
         if (n <= kList || low == high) break;
-        divided = true;
-        // by keys, the highest first
-        const int cut = max(0, 32 - __clz(high - low) - 9);
-        const float edge = step_of(value_of(high));
+        const int cut = max(0, 32 - __clz(high - low) - 9);  // (at most kBins parts, the highest keys first)
+        parts[tid] = 0;
+        __syncthreads();
         EACH({
-          if (stays(v, i) && inside(v))
-            atomicAdd(&sm.hist[(high - key_of(v)) >> cut], masses ? weight15(step_of(v) - edge) : 1u);
+          if (stays(v, i) && inside(v)) atomicAdd(&parts[(high - key_of(v)) >> cut], masses ? mass_of(v) : (u64)1);
         })
-        int b = pick(masses ? exp2((double)edge * (-1.0 / 16)) * (1.0 / 32768) : 1.0, false);
-        if (b == kBins) b = (int)((high - low) >> cut);  // (weights that rounded away: the lowest)
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        u64 w = 0, whole;
+        for (int c = 0; c < C; ++c) w += cluster.map_shared_rank(&sm, c)->list[tid];
+        const u64 before = sure + cta_scan(w, whole);
+        // the first part that reaches the goal (the last one, should the sums' roundings keep the goal above them all)
+        if (tid == 0) sm.pick_bin = (int)((high - low) >> cut);
+        __syncthreads();
+        if ((double)(before + w) >= goal) atomicMin(&sm.pick_bin, tid);
+        __syncthreads();
+        const int b = sm.pick_bin;
+        if (tid == b) sm.start = before;
+        if (C > 1) cluster.sync();  // (and nobody reads the parts any more)
+        else __syncthreads();
+        sure = sm.start;
         const unsigned from = high - ((unsigned)b << cut);
         low = max(low, cut ? from - ((1u << cut) - 1) : from);
         high = from;
       }
-      if (masses && divided && n > 0) {  // the bin's tokens above what is left of it join what lies above
-        const float highest = value_of(high);
-        u64 more = 0;
-        each_value(highest, [&](float v, int i, int, bool valid) {
-          if (valid && stays(v, i) && bin_of(step_of(v)) == bin && v > highest) more += mass_of(v);
-        });
-        more = cta_sum(more);
-        if (C > 1) {
-          spread_u(more);
-          cluster.sync();
-          more = 0;
-          for (int c = 0; c < C; ++c) more += sm.gather_u[turn][c];
-          turn ^= 1;
-        }
-        sure += more;
-      }
       if (n == 0) return;  // (a tail without tokens)
       if (n <= kList) {
         if (rank == 0) {
-          const double need = masses ? target * one - (double)sure : target - above;
+          const double need = goal - (double)sure;
           if (n <= kSampleThreads) border_of<1>(sm, mass_of, n, need, masses);
           else border_of<kList / kSampleThreads>(sm, mass_of, n, need, masses);
           __syncthreads();
@@ -1057,7 +1054,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       } else {  // many tokens of one value: their number decides, and the index of the last
         const float value = value_of(high);
         const u64 m = mass_of(value);
-        const double want = masses ? (m ? ceil((target * one - (double)sure) / (double)m) : (double)n) : target - above;
+        const double want = masses ? (m ? ceil((goal - (double)sure) / (double)m) : (double)n) : goal - (double)sure;
         const u64 ties = (u64)fmin(fmax(want, 1.0), (double)n);
         auto is_tie = [&](const Vec<TI> &vec, int i0, u64 *w) {
 #pragma unroll
