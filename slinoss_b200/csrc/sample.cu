@@ -882,6 +882,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
       const double edge0 = masses ? sm.table[(e16 & 15) * 4] * __hiloint2double((1023 + (e16 >> 4)) << 20, 0) * (1.0 / 32768) : 1.0;
       int bin = pick(edge0);
       if (masses) turn ^= 1;
+      if (!masses && bin == kBins) {  // fewer than k tokens above -inf: all of them stay
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        sm.hist[tid] = 0;  // (everybody has read the histograms)
+        __syncthreads();
+        return;
+      }
       if (bin > last) bin = last;
       // the tokens of CTA 0's list: those that stay and are `in`
       // (each CTA lists its own; the others' lists then join CTA 0's)

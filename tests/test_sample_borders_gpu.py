@@ -111,3 +111,22 @@ def test_borders_among_equal_masses_in_wide_bins(dtype):
     compare(row, 30.0, top_p, torch.rand(120, generator=gen, dtype=torch.float64).numpy())
     fine = torch.randn(100003, generator=gen).to(dtype).cuda()
     compare(fine, 30.0, top_p, torch.rand(120, generator=gen, dtype=torch.float64).numpy())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("finite,k", [(5000, 6000), (9000, 9999), (300, 700), (6000, 6001)])
+def test_top_k_beyond_the_tokens_that_a_mask_leaves(dtype, finite, k):
+    """All of them stay, the small masses behind the first one too."""
+    import slinoss_b200 as sb
+    gen = torch.Generator().manual_seed(4)
+    V = 10000
+    row = torch.full((V,), -torch.inf)
+    some = torch.randperm(V - 1, generator=gen)[:finite]
+    row[some] = -18.0 - 2.0 * torch.rand(finite, generator=gen)
+    row[V - 1] = 0.0
+    row = row.to(dtype).cuda()
+    tail = float(torch.exp(row.double()).sum()) - 1.0
+    u = (tail * torch.rand(60, generator=gen, dtype=torch.float64)).numpy()
+    for p in (1.0, float(np.float32(1 - 0.3 * tail))):
+        got = sb.sample_b200(row.expand(60, -1), torch.as_tensor(u, device="cuda"), top_k=k, top_p=p).cpu().numpy()
+        assert (far_off(row, 1.0, np.full(60, p), u, got) <= 3 * V * 2.0 ** -44).all()
