@@ -4,12 +4,16 @@
 //     dq = scale gamma (dO S0) + (Q beta) k
 //     Z  = closing (Y R) + Q^T q - H^T k                      (all that reaches k_s through the row written at s, over beta_s)
 //     dk = beta Z - gamma (dX S0) - (H beta) k                (the rest reaches k_t through the error at t)
-//     dbeta_s = k_s.Z_s
-//     dG_t = q_t.dq_t + k_t.dk_t - 2 beta_t dbeta_t,  dG_63 += <R, S1>,   dg_t = sum of dG over the chunk's tokens >= t
-// (no product of 64 x 64 matrices with the decays is formed for dg: the row sums that it needs are dots of rows that are
-// there).  One CTA of four warps per chunk and head; a warp owns 16 tokens, as t for dq and as s for Z, with its result rows
-// in accumulators; Q and H are formed in both orientations, in registers, which costs 1/8 more products than passing them
-// through shared memory would save barriers.
+// What the row written at s passes to a later t is beta_s C_ts, C_ts = Q_ts q_t.k_s - H_ts k_t.k_s, and with that
+//     dbeta_s = closing_s Y_s.(R k_s) + sum of C_ts over t >= s
+//     dg_t = gamma_63 <R, S0> + sum over r >= t of gamma_r (scale dO_r.(S0 q_r) - dX_r.(S0 k_r))
+//            + sum over s < t of beta_s closing_s Y_s.(R k_s) + sum over s < t <= r of beta_s C_rs
+// : all that crosses the gate at t, term by term with its decay, so that a gate which is nearly closed has a gradient as small
+// and as exact as what it lets through.  (The suffix sum of q.dq + k.dk - 2 beta dbeta is the same in exact arithmetic, but its
+// terms of order one cancel: with g = -5 throughout it was off by 0.3 of dg in fp32 and by 180 times dg in bf16.)
+// One CTA of four warps per chunk and head; a warp owns 16 tokens, as t for dq and as s for Z, with its result rows in
+// accumulators; Q and H are formed in both orientations, in registers, which costs 1/8 more products than passing them through
+// shared memory would save barriers.
 //
 // 16384 chunks of one head each (N 128, P 64, bf16): 898 us at two CTAs an SM (103 KB and 255 registers a thread); 160 KB a chunk
 // through HBM would take 400.  Eight warps a CTA, four for dO, Q and dq and four for dX, H and dk, take 1123 us: at 128 registers
@@ -49,6 +53,16 @@ __device__ __forceinline__ float2 row_dots(const float (&c)[NT / 8][4], const __
   }
   const float f = pow2(e);
   return make_float2(x * f, y * f);
+}
+
+__device__ __forceinline__ float over_quad(float x) {
+  x += __shfl_xor_sync(~0u, x, 1);
+  return x + __shfl_xor_sync(~0u, x, 2);
+}
+__device__ __forceinline__ float over_rows(float x) {  // of the eight quads
+  x += __shfl_xor_sync(~0u, x, 4);
+  x += __shfl_xor_sync(~0u, x, 8);
+  return x + __shfl_xor_sync(~0u, x, 16);
 }
 
 // A warp's 16 rows of dq or dk, from accumulators: half types through `buf` (16 x (NT + 8) halves of the warp's own) in
@@ -145,7 +159,10 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
   __half *ss = ys + SC * kTile, *rs = ss + SC * splane;                          // channels x N: S0, R
   float *gamma = reinterpret_cast<float *>(rs + SC * splane), *closing = gamma + L, *beta = closing + L;
   float *rise = beta + L + 32, *fall = rise + L, *near = fall + 96;
-  __shared__ float dGs[L], dbs[L], wsum[L], dots[4];
+  // per token: what it reads of S0, dbeta, what its row passes on behind the chunk; what crosses its gate from the tokens of its
+  // block of 16, and (by block) from each earlier block to it
+  __shared__ float reads[L], dbs[L], wsum[L], dots[4];
+  __shared__ __align__(8) float near_cross[L], far_cross[3][L];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int chunk = blockIdx.x, bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads, kh = h / (a.heads / a.key_heads);
@@ -296,6 +313,85 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       }
     // Q and H still lack a factor each, which joins their scaling; the sum takes closing and its unit in one
     const float fq = a.scale * pow2(y_top + eo_top), fh = -pow2(yx_top);
+    {  // C, a block of 16 x 16 at a time: rows s, columns t
+      const float fk = pow2(ek), fqk = pow2(eq), b0 = beta[r0], b1 = beta[r1];
+      float later0 = 0.f, later1 = 0.f, own0 = 0.f, own1 = 0.f;  // row sums, over later blocks and over this one
+      float c[2][4];
+#pragma unroll
+      for (int i = 3; i >= 0; --i) {
+        if (i < warp) continue;
+        const int tb = i;
+        float qk[2][4], kk[2][4];
+        zero(qk);
+        zero(kk);
+#pragma unroll 2
+        for (int nb = 0; nb < NT / 16; ++nb) {
+          Frag<SI> f;
+          uint32_t bq[SI][4], bk[SI][4];
+#pragma unroll
+          for (int s = 0; s < SI; ++s) {
+            a_mk(f.r[s], krow + s * Op::plane + 16 * nb, ld);
+            b_nk(bq[s], qs + s * Op::plane + 16 * tb * ld + 16 * nb, ld);
+            b_nk(bk[s], ks + s * Op::plane + 16 * tb * ld + 16 * nb, ld);
+          }
+          mma_split<SI, SI>(qk[0], qk[1], f, bq);
+          mma_split<SI, SI>(kk[0], kk[1], f, bk);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            c[j][e] = Q[2 * tb + j][e] * fq * (qk[j][e] * fk * fqk) + H[2 * tb + j][e] * fh * (kk[j][e] * fk * fk);
+        const float x0 = (c[0][0] + c[0][1]) + (c[1][0] + c[1][1]), x1 = (c[0][2] + c[0][3]) + (c[1][2] + c[1][3]);
+        if (tb > warp) {
+          later0 += x0;
+          later1 += x1;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float u = over_rows(fmaf(b0, c[j][0], b1 * c[j][2])), v = over_rows(fmaf(b0, c[j][1], b1 * c[j][3]));
+            if (g == 0) *reinterpret_cast<float2 *>(&far_cross[warp][16 * tb + 8 * j + 2 * q]) = make_float2(u, v);
+          }
+        } else {
+          own0 = x0;
+          own1 = x1;
+        }
+      }
+      later0 = over_quad(later0);
+      later1 = over_quad(later1);
+      db.x = w.x + later0 + over_quad(own0);
+      db.y = w.y + later1 + over_quad(own1);
+      // c is the diagonal block: per row, sums over the columns from t on and over the later blocks; of these the rows before t
+      float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int s = g + 8 * n;
+        const float later = n ? later1 : later0, be = n ? b1 : b0;
+        float from[2];  // over this thread's columns of the tile and those to their right
+#pragma unroll
+        for (int j = 1; j >= 0; --j) {
+          float run = c[j][2 * n] + c[j][2 * n + 1];
+#pragma unroll
+          for (int d = 1; d < 4; d <<= 1) {
+            const float o = __shfl_down_sync(~0u, run, d, 4);
+            if (q + d < 4) run += o;
+          }
+          float right = __shfl_down_sync(~0u, run, 1, 4);  // (taken from the neighbour: a difference would keep roundings)
+          if (q == 3) right = 0.f;
+          const float behind = j ? later : later + __shfl_sync(~0u, from[1], lane & ~3);
+          if (j) from[1] = run;
+          const int t = 8 * j + 2 * q;
+          right += behind;
+          const float at1 = c[j][2 * n + 1] + right, at0 = c[j][2 * n] + at1;
+          if (s < t) sum[j][0] = fmaf(be, at0, sum[j][0]);
+          if (s < t + 1) sum[j][1] = fmaf(be, at1, sum[j][1]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float u = over_rows(sum[j][0]), v = over_rows(sum[j][1]);
+        if (g == 0) *reinterpret_cast<float2 *>(&near_cross[16 * warp + 8 * j + 2 * q]) = make_float2(u, v);
+      }
+    }
     const float top = __uint_as_float(__reduce_max_sync(~0u, max(mag(closing[r0]), mag(closing[r1]))));
     const int ec = warp_exp(acc) + yr_top + above(top), e1 = floor_exp(warp_exp(Q) + above(fq), ec, eq);
     const int e2 = floor_exp(warp_exp(H) + yx_top, max(ec, e1 + eq + 21) + 1, ek);
@@ -328,15 +424,12 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       to.join();
     }
     unit = e2 + ek;  // (acc is Z without its unit)
-    db = row_dots<NT, SI>(acc, krow, ek);
-    db.x *= pow2(unit);
-    db.y *= pow2(unit);
   }
   __syncthreads();  // (R is not read any more: its room takes results on their way out)
   __half *buf = rs + warp * 16 * ld;
   // ---- this warp's tokens as t: dk = beta Z + f gamma (dX S0) + f (H beta) k with f = -1, then the same with dO, Q and
   // f = scale: dq (whose sum starts at zero and has t itself)
-  float2 dots_k = make_float2(0.f, 0.f), dots_q = dots_k;
+  float2 read = make_float2(0.f, 0.f);  // of S0, by this warp's tokens
 #pragma unroll 1
   for (int part = 0; part < 2; ++part) {
     const bool is_q = part == 1;
@@ -347,9 +440,11 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     zero(H);
     const int ya = ey + ea, sa = es + ea;
     const int ya_top = __reduce_max_sync(~0u, ya), sa_top = __reduce_max_sync(~0u, sa);
-    // f gamma times the tile as an operand: the factor, which exceeds one where gates do, enters the product's unit
+    // dk: f gamma times the tile as an operand; the factor, which exceeds one where gates do, enters the product's unit.  dq,
+    // whose sum starts here: the tile as it is, and the factor on the sum.
     const float g0 = f * gamma[r0], g1 = f * gamma[r1];
-    const int top = __reduce_max_sync(~0u, max(mag(g0), mag(g1)));
+    const int top = is_q ? 0 : __reduce_max_sync(~0u, max(mag(g0), mag(g1)));
+    float d0 = 0.f, d1 = 0.f;  // dX.(S0 k)
     float b0 = 0.f, b1 = 0.f;  // dk takes beta Z over
     int held = kZeroExp;
     if (!is_q) {
@@ -376,16 +471,33 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       for (int kb = 0; kb < blocks; ++kb) {
         Frag<SC> fa, fg;
         load_a(fa, tile, is_q ? SI : SC, kb);
-        const float m = pow2(below(sa, unit, pt, kb)), f0 = g0 * m, f1 = g1 * m;
+        if (is_q) fg = scaled(fa, below(sa, unit, pt, kb));
+        else {
+          float sk[2][4];  // S0 k: tokens x channels, as the fragment of dX lies
+          zero(sk);
+#pragma unroll 2
+          for (int nb = 0; nb < NT / 16; ++nb) {
+            Frag<SI> fk;
+            uint32_t bs[SC][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float2 x = unpack(fa.r[0][i]);
-          if constexpr (SC == 2) {
-            const float2 y = unpack(fa.r[1][i]);
-            x.x += y.x;
-            x.y += y.y;
+            for (int s = 0; s < SI; ++s) a_mk(fk.r[s], krow + s * Op::plane + 16 * nb, ld);
+#pragma unroll
+            for (int s = 0; s < SC; ++s) b_nk(bs[s], ss + s * splane + 16 * kb * ld + 16 * nb, ld);
+            mma_split<SI, SC>(sk[0], sk[1], fk, bs);
           }
-          split<SC>(x.x * (i & 1 ? f1 : f0), x.y * (i & 1 ? f1 : f0), &fg.r[0][i], &fg.r[SC - 1][i]);
+          const float m = pow2(below(sa, unit, pt, kb)), f0 = g0 * m, f1 = g1 * m, n = pow2(below(sa, sa_top, pt, kb));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float2 x = unpack(fa.r[0][i]);
+            if constexpr (SC == 2) {
+              const float2 y = unpack(fa.r[1][i]);
+              x.x += y.x;
+              x.y += y.y;
+            }
+            float &d = i & 1 ? d1 : d0;
+            d = fmaf(n, fmaf(x.x, sk[i >> 1][(i & 1) * 2], x.y * sk[i >> 1][(i & 1) * 2 + 1]), d);
+            split<SC>(x.x * (i & 1 ? f1 : f0), x.y * (i & 1 ? f1 : f0), &fg.r[0][i], &fg.r[SC - 1][i]);
+          }
         }
         fa = scaled(fa, below(ya, ya_top, pt, kb));
 #pragma unroll
@@ -399,6 +511,17 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       }
     }
     onto.join();
+    if (is_q) {
+      const float2 d = row_dots<NT, SI>(acc, qs + 16 * warp * ld, eq);
+      const float u = pow2(unit);
+      read.x = fmaf(d.x * u, g0, read.x);
+      read.y = fmaf(d.y * u, g1, read.y);
+      times_rows(acc, g0, g1);
+    } else {
+      const float u = pow2(sa_top);
+      read.x = over_quad(d0) * u * pow2(ek) * g0;
+      read.y = over_quad(d1) * u * pow2(ek) * g1;
+    }
 #pragma unroll
     for (int sb = 0; sb < 4; ++sb)
       if (sb <= warp) {
@@ -438,8 +561,6 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       to.join();
     }
     times(acc, pow2(e + ek));
-    dots_k = dots_q;
-    dots_q = row_dots<NT, SI>(acc, (is_q ? qs : ks) + 16 * warp * ld, is_q ? eq : ek);
     if (tiles > 1) __syncthreads();  // (the last tile's R has been loaded by all threads)
     const bool shared = a.heads != a.key_heads;
     const size_t row0 = ((size_t)(shared ? bh : b * a.key_heads + kh) * a.T + t0 + 16 * warp) * a.N;
@@ -452,35 +573,56 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
   for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(~0u, dot, d);
   if (lane == 0) dots[warp] = dot;
   if (q == 0) {
-    dGs[r0] = dots_q.x + dots_k.x - 2.f * beta[r0] * db.x;
-    dGs[r1] = dots_q.y + dots_k.y - 2.f * beta[r1] * db.y;
+    reads[r0] = read.x;
+    reads[r1] = read.y;
     dbs[r0] = db.x;
     dbs[r1] = db.y;
     wsum[r0] = beta[r0] * w.x;
     wsum[r1] = beta[r1] * w.y;
   }
   __syncthreads();
-  if (warp == 0) {
-    float last = wsum[lane] + wsum[lane + 32];
+  if (warp == 0) {  // tokens 2 lane and 2 lane + 1
+    // sums over a pair's lane and all later ones, or all earlier ones; neighbours hand over what excludes the own
+    auto from_here = [&](float x, float y, float &at_x, float &at_y) {
+      float run = x + y;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) last += __shfl_xor_sync(~0u, last, d);
-    last = fmaf(gamma[L - 1], dots[0] + dots[1] + dots[2] + dots[3], last);  // <R, S1>
-    const float y = dGs[2 * lane + 1], x = dGs[2 * lane] + y;
-    float run = x;  // of this lane's tokens and all later ones
+      for (int d = 1; d < 32; d <<= 1) {
+        const float o = __shfl_down_sync(~0u, run, d);
+        if (lane + d < 32) run += o;
+      }
+      float rest = __shfl_down_sync(~0u, run, 1);
+      if (lane == 31) rest = 0.f;
+      at_y += y + rest;
+      at_x += x + (y + rest);
+    };
+    const float state = gamma[L - 1] * (dots[0] + dots[1] + dots[2] + dots[3]);
+    float x = state + near_cross[2 * lane], y = state + near_cross[2 * lane + 1];
+    from_here(reads[2 * lane], reads[2 * lane + 1], x, y);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {  // from block n to the later ones
+      const bool in = lane >= 8 * (n + 1);
+      float u = 0.f, v = 0.f;
+      from_here(in ? far_cross[n][2 * lane] : 0.f, in ? far_cross[n][2 * lane + 1] : 0.f, u, v);
+      if (in) {
+        x += u;
+        y += v;
+      }
+    }
+    float run = wsum[2 * lane] + wsum[2 * lane + 1];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const float o = __shfl_down_sync(~0u, run, d);
-      if (lane + d < 32) run += o;
+      const float o = __shfl_up_sync(~0u, run, d);
+      if (lane >= d) run += o;
     }
+    float before = __shfl_up_sync(~0u, run, 1);
+    if (lane == 0) before = 0.f;
+    x += before;
+    y += before + wsum[2 * lane];
     const size_t row = (size_t)bh * a.T + t0 + 2 * lane;
-    const float after = last + run - x;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (2 * lane + i < rows) {
-        // (a gate that drops the state has no gradient, which the sum meets but for its roundings)
-        const int t = 2 * lane + i;
-        const float open = t == 0 ? gamma[0] : t % 16 == 0 ? rise[t] : near[t * kNearLd + t % 16 - 1];
-        store_as(a.dg, a.g_dtype, row + i, open == 0.f ? 0.f : i == 0 ? after + x : after + y);
+        store_as(a.dg, a.g_dtype, row + i, i ? y : x);
         store_as(a.dbeta, a.beta_dtype, row + i, dbs[2 * lane + i]);
       }
   }
