@@ -112,8 +112,12 @@ __device__ __forceinline__ int above(float x) {
   const unsigned b = __float_as_uint(x) & 0x7fffffffu;
   return b >= 0x7f800000u ? kNanExp : (int)(b >> 23) - 126;
 }
+// x 2^e in two steps: e may pass the range where the product does not
+__device__ __forceinline__ float times_pow2(float x, int e) { return x * pow2(e >> 1) * pow2(e - (e >> 1)); }
 // an exponent for a product's operand such that an accumulator of exponent ec, brought to the product's unit e + eb, stays
-// far inside the range (what the raising rounds away is 2^-40 of the accumulator), and the unit does too
+// far inside the range (what the raising rounds away is 2^-40 of the accumulator), and the unit does too.  (ec: of what the
+// accumulator will be when the product joins it, behind its decay: a state that a gate has closed on keeps what was written
+// before the gate.)
 constexpr int kLowestUnit = -100;
 __device__ __forceinline__ int floor_exp(int e, int ec, int eb) { return max(e, max(ec - 40, kLowestUnit) - eb); }
 __device__ __forceinline__ unsigned mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }

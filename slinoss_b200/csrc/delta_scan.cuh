@@ -242,15 +242,15 @@ __global__ void __launch_bounds__(kThreads) delta_fwd_kernel(Args a, int pw) {
         store_rows<TI>(static_cast<TI *>(a.o) + ((size_t)bh * a.T + c * L) * a.P + p0, a.P, min(L, a.T - c * L), a.P - p0, O, buf);
       }
       times_cols(X, closing, 1.f);
-      eC = floor_exp(eY + y + max4(tops[2]), eS, ek);
-      frags_of<2>(fc, X, eC - y);
       top = gamma[L - 1];
+      eC = floor_exp(eY + y + max4(tops[2]), eS + above(top), ek);
+      frags_of<2>(fc, X, eC - y);
     }
     __syncthreads();
     if (more) issue_rest(c + 1);
     cp_commit();
     if (active) {
-      onto<SC == 2, SI, NT>(S, top * pow2(unit - (eC + ek)), fc, kt);
+      onto<SC == 2, SI, NT>(S, times_pow2(top, unit - (eC + ek)), fc, kt);
       unit = eC + ek;
     }
     ex = nx;
@@ -378,20 +378,21 @@ __global__ void __launch_bounds__(kThreads) delta_bwd_kernel(Args a, int pw) {
       }
       // (exponents from bounds: by the largest gamma)
       times_cols(dO, gamma, a.scale);
-      e1 = floor_exp(eG + max4(tops[0]) + above(a.scale), eR, eq);
+      top = gamma[L - 1];
+      const int eD = eR + above(top);  // of the decayed R
+      e1 = floor_exp(eG + max4(tops[0]) + above(a.scale), eD, eq);
       frags_of<2>(f1, dO, e1);
       times_cols(W, gamma, -1.f);
       // (64 products of values below 2^15 join R between the two)
-      e2 = floor_exp(eW + max4(tops[0]), max(eR, e1 + eq + 21) + 1, ek);
+      e2 = floor_exp(eW + max4(tops[0]), max(eD, e1 + eq + 21) + 1, ek);
       frags_of<2>(f2, W, e2);
-      top = gamma[L - 1];
     }
     cp_wait<1>();
     __syncthreads();
     if (c > 0) issue_rest(c - 1);
     cp_commit();
     if (active) {
-      onto<SI == 2, SI, NT>(R, top * pow2(unit - (e1 + eq)), f1, qs);
+      onto<SI == 2, SI, NT>(R, times_pow2(top, unit - (e1 + eq)), f1, qs);
       onto<SI == 2, SI, NT>(R, pow2(e1 + eq - (e2 + ek)), f2, kt);
       unit = e2 + ek;
     }

@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kTeamThreads) delta_fwd_team_kernel(Args a) {
         }
       }
       team_barrier();
-      const int eC = floor_exp(max4(exps[kC]), eS, ek);
+      const int eC = floor_exp(max4(exps[kC]), eS + above(st.gamma[L - 1]), ek);
       if constexpr (SC == 2) {
         float D[NT / 32][4];
         zero(D);
@@ -577,8 +577,9 @@ __global__ void __launch_bounds__(kTeamThreads) delta_bwd_team_kernel(Args a) {
         }
       }
       team_barrier();
-      const int u1 = floor_exp(max4(exps[kG]), eR, eq);
-      const int u2 = floor_exp(max4(exps[kN]), max(eR, u1 + eq + 21) + 1, ek);
+      const int eD = eR + above(st.gamma[L - 1]);  // of the decayed R
+      const int u1 = floor_exp(max4(exps[kG]), eD, eq);
+      const int u2 = floor_exp(max4(exps[kN]), max(eD, u1 + eq + 21) + 1, ek);
       if constexpr (SC == 2) {
         float D[NT / 32][4], E[NT / 32][4];
         zero(D);

@@ -68,3 +68,30 @@ def test_many_heads_that_close(dtype):
     inp["g"][:, ::2] = -10.0
     err, _ = gate_errors(inp, 2)
     assert err.max() <= TOL[dtype], err.max()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("b", [2, 40])
+@pytest.mark.parametrize("g", [-12.0, -30.0, -60.0])
+def test_states_behind_closed_gates_keep_their_scale(dtype, b, g):
+    """A gate that closes and nothing written behind it: the state is e^g of what it was, rows written before it in the same
+    chunk included.  The other way round, the initial state's gradient where only what lies behind the gate is read: a gate
+    inside a chunk enters by the chunk's triangular matrices, whose entries are pairs of fp16 beside a largest of one (off by
+    2^-39 each); over 64 tokens and the three operands made with them that is 3 * 64 * 2^-39 < 2^-31 of what an open gate
+    would give."""
+    from oracle import delta as odelta
+    from test_gated_delta_gpu import NAMES, tolerance
+    from util import rel_err
+    for t, T in [(20, 64), (63, 70), (64, 130), (100, 130)]:
+        inp = make(b, 4, 4, T, 64, 32, dtype, seed=45 + t, gates="fp32")
+        inp["g"][:, :, t] = g
+        late = {n: x.clone() for n, x in inp.items()}
+        late["beta"][:, :, t:] = 0
+        _, final, _ = run(late)
+        _, want, _ = odelta.forward(*(_np(late[n]) for n in NAMES[:5]), 0.125, _np(late["init"]))
+        assert rel_err(_np(final), want) <= tolerance(inp["q"].dtype, "final", final.dtype), t
+        inp["do"][:, :, :t] = 0
+        got, ref = _np(run(inp)[2]["init"]), reference(inp)[2]["init"]
+        inp["g"][:, :, t] = 0
+        size = np.linalg.norm(reference(inp)[2]["init"])
+        assert np.linalg.norm(got - ref) <= 1e-5 * np.linalg.norm(ref) + 2.0 ** -31 * size, t
