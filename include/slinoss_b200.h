@@ -472,7 +472,9 @@ int slx_gate_skip_bwd_as(const slx_glue_shape *s, const void *y, const void *u,
  * batch, head and token (a dense last axis; in elements, >= 0); the strides of an axis of one
  * element are not read.  States are (batch, heads, P, N).
  * g is a log decay; -inf (and anything below -110) drops the state.  A non-finite value in any
- * other place makes outputs of its head from its chunk of 64 tokens on NaN. */
+ * other place makes NaN of: all outputs from its chunk of 64 tokens on, of the heads that read
+ * it (k, g, beta); those of its block of 16 value channels (v, initial_state); the outputs of its
+ * chunk (q).  batch * heads <= 65535 (not for the step). */
 typedef struct {
   int32_t batch, heads, key_heads, T, P, N; /* N <= 128, P <= 256, heads a multiple of key_heads */
   int32_t dtype;                            /* slx_dtype of q, k, v, o and their gradients       */

@@ -72,8 +72,19 @@ def gated_delta_rule_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: 
 
     ``g`` is a log decay (usually negative); ``-inf`` drops the state, which separates documents packed into one
     sequence.  Tokens with ``beta = 0`` and ``g = 0`` leave the state as it is, which pads sequences.  The recurrence is
-    stable for ``beta |k|^2 < 2``; keys usually come normalised.  A non-finite value among the inputs (``-inf`` in ``g``
-    apart) makes its head's outputs NaN from its chunk of 64 tokens on.
+    stable for ``beta |k|^2 < 2``; keys usually come normalised.  At most 65535 heads (``batch * heads``).
+
+    A non-finite value among the inputs (``-inf`` in ``g`` apart) makes NaN of what is scaled together with it: from its
+    chunk of 64 tokens on all outputs of the heads that read it for ``k``, ``g`` and ``beta``, those of its block of 16
+    value channels for ``v`` and ``initial_state``, and the outputs of its chunk alone for ``q``.  Gradients are NaN where
+    they meet one of these.
+
+    Accuracy.  fp32 and fp16 results and all states are formed from operands of 22 bits, bfloat16 ones from operands of 11:
+    gradients of fp32 gates beside bfloat16 activations are right to about ``1e-3``.  Values are held relative to the
+    largest of their chunk of 64 tokens: what a closing gate inside a chunk makes smaller than ``2^-31`` of it (``2^-24``
+    for bfloat16 results) may come back as zero.  The carried state and the gradient of the gate itself keep their own
+    scale; below ``2^-100`` anything may be taken for zero.  With ``N < 16`` keys are alike, and the initial state's and
+    the gates' gradients are differences of sums over a chunk: off by up to ``2^-15``.
 
     ``residual`` chooses what autograd keeps: ``"keep"`` (default) what the forward has made of its inputs, and none of
     them: per 64 tokens and value head the triangular matrices of the chunk, the state before it and the prediction
