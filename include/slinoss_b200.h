@@ -530,7 +530,8 @@ typedef struct {
  * (ties: lower index first); the first top_k stay (<= 0: all), of these the shortest run that
  * holds at least top_p of their mass (>= 1: all), of these the ones with at least min_p of the
  * largest mass; the draw takes, in the order of the indices, the first token at which the running
- * mass exceeds u times the whole.  Masses are exp((logit - largest) / temperature) in 64 bits.
+ * mass exceeds u times the whole.  Masses are exp((logit - largest) / temperature) in 64 bits,
+ * rounded to multiples of 2^-44 (none 31 temperatures below the largest).
  * temperature <= 0 takes the first largest logit.  NaN logits count as -inf; a row without a
  * logit above -inf gives -1.  (No counterpart in the reference.) */
 int slx_sample(const slx_sample_shape *s, const void *logits, const void *u,

@@ -6,15 +6,18 @@
 //
 // A row is read once: a cluster of up to eight CTAs holds it in shared memory, and everything after that runs there.
 //   * The border of a filter (k tokens, or a share of the mass) is narrowed down by a histogram over steps of the logit
-//     (for masses of 1/16 in their logarithm), counted in 32-bit integers (masses relative to their bin's edge, 15 bits: a
-//     CTA's 2^17 tokens may all fall into one): one bin holds the border.
+//     (for masses of 1/16 in their logarithm), counted in 32-bit integers (masses relative to their bin's edge, 15 bits: all of
+//     a CTA's tokens may fall into one): one bin holds the border.
 //   * Where no more than a few thousand tokens lie above the bin's lower edge, CTA 0 gathers them and finishes the row, and
 //     the other CTAs are done.  Otherwise only the bin's own tokens are gathered for the border (a bin with too many is
-//     divided again by the integer keys of its logits), and the draw sums the tokens that stay where they are.
+//     divided again by the integer keys of its logits, with exact sums of every part), and the draw sums the tokens that stay
+//     where they are.
 //   * Masses that decide anything are exponentials in 64 bits, held as integers of 2^-44 of the largest: their sums do not
-//     depend on an order.  The whole mass that top_p refers to is such a sum over every token: an error of 10^-6 in it moves
-//     the border past a token in ten, every draw by that token's mass, and one draw in a hundred into the neighbour, where ten
-//     thousand tokens stay.  Only the histogram is coarser; it names a bin, and its neighbours are looked at too.
+//     depend on an order.  (A token 31 temperatures below the largest has none and is never drawn.)  The whole mass that top_p
+//     refers to is a sum over every token, of which those below 2^-20 take exponentials in 32 bits, off by 2^-41 of the
+//     largest each: an error of 10^-6 in it would move the border past a token in ten, every draw by that token's mass, and
+//     one draw in a hundred into the neighbour, where ten thousand tokens stay.  Only the histogram is coarser; it names a bin,
+//     and its neighbours are looked at too.
 //   * What costs is instructions: two CTAs of an SM go through 32 to 64 logits a thread.  A filter touches few of them, so
 //     warps first collect the values above a bound (a compare and a vote each) and then work on 32 at a time: the histogram
 //     of 192 rows of 150001 bf16 logits takes 5 thousand clocks instead of 13, their gathering 5 instead of 11.
@@ -55,6 +58,7 @@ constexpr int kQueue = 32 + 32 * 8;  // values of a warp that wait for their mas
 constexpr int kMaxVecs = 17;     // of a thread: eight CTAs hold 262144 fp32 logits that begin inside a vector
 constexpr int kMaxGroups = kMaxVecs * kSampleWarps;
 constexpr int kMaxCluster = 8;
+static_assert((u64)kMaxVecs * kSampleThreads * 8 << 15 < (u64)1 << 32, "a bin holds the 15-bit masses of all tokens of a CTA");
 static_assert(kBins == kSampleThreads, "threads scan the bins one each");
 
 struct alignas(16) SampleShared {  // (the row's vectors follow it)
@@ -1020,12 +1024,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
         const int cut = max(0, 32 - __clz(high - low) - 9);  // (at most kBins parts, the highest keys first)
         parts[tid] = 0;
         __syncthreads();
-        EACH({
-          if (stays(v, i) && inside(v)) atomicAdd(&parts[(high - key_of(v)) >> cut], masses ? mass_of(v) : (u64)1);
-        })
+        each_value(value_of(low), [&](float v, int i, int, bool valid) {
+          if (valid && stays(v, i) && inside(v)) atomicAdd(&parts[(high - key_of(v)) >> cut], masses ? mass_of(v) : (u64)1);
+        });
         if (C > 1) cluster.sync();
         else __syncthreads();
         u64 w = 0, whole;
+#pragma unroll 1
         for (int c = 0; c < C; ++c) w += cluster.map_shared_rank(&sm, c)->list[tid];
         const u64 before = sure + cta_scan(w, whole);
         // the first part that reaches the goal (the last one, should the sums' roundings keep the goal above them all)
@@ -1110,7 +1115,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a,
 #undef EACH_VECTOR
 }
 
-// A row's cluster: few vectors a thread where the rows leave SMs for more CTAs (two to an SM).
+// A row's cluster: few vectors a thread while two CTAs an SM have not been filled, then more, up to eight, so that rows take
+// fewer CTAs; more than eight only where a row needs them.  Measured with top_p 0.95, us: 192 rows of 150001 bf16 logits 330 with
+// up to two or four vectors, 270 with eight, 468 with 17 (too few CTAs an SM); 64 rows of 131072 fp32 111 with up to eight, 124 with
+// 17.  (256 rows of 65536 bf16 are the other way round, 219 and 187: at eight the third CTA of a row holds its last vector alone.)
+// Filling one CTA an SM or four in the place of two: 148 rows of 20000 fp32 logits 46 and 56 against 37, the others alike.
 template <typename TI>
 static int launch_sample(const SampleArgs &a, int rows, cudaStream_t st) {
   constexpr int VEC = 16 / sizeof(TI);

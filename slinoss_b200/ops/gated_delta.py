@@ -81,10 +81,11 @@ def gated_delta_rule_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: 
 
     Accuracy.  fp32 and fp16 results and all states are formed from operands of 22 bits, bfloat16 ones from operands of 11:
     gradients of fp32 gates beside bfloat16 activations are right to about ``1e-3``.  Values are held relative to the
-    largest of their chunk of 64 tokens: what a closing gate inside a chunk makes smaller than ``2^-31`` of it (``2^-24``
-    for bfloat16 results) may come back as zero.  The carried state and the gradient of the gate itself keep their own
-    scale; below ``2^-100`` anything may be taken for zero.  With ``N < 16`` keys are alike, and the initial state's and
-    the gates' gradients are differences of sums over a chunk: off by up to ``2^-15``.
+    largest of their chunk of 64 tokens: what a closing gate inside a chunk makes smaller than ``2^-31`` of it may come back
+    as zero.  The carried state and the gradient of the gate itself keep their own scale; below ``2^-100`` anything may be
+    taken for zero.  With ``N < 16`` keys are alike, and the initial state's and the gates' gradients are differences of sums
+    over a chunk, each right to ``2^-16`` of its terms: ``2^-15`` of the result for unit keys and tokens of like size, less
+    (``1e-3`` at ``N = 1``) where ``beta`` is near 2 or tokens differ in size a thousandfold.
 
     ``residual`` chooses what autograd keeps: ``"keep"`` (default) what the forward has made of its inputs, and none of
     them: per 64 tokens and value head the triangular matrices of the chunk, the state before it and the prediction

@@ -27,8 +27,10 @@ def sample_b200(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k
     Tokens are ranked by logit (ties: the lower index first).  The first ``top_k`` stay (``<= 0``: all); of these the
     shortest run that holds at least ``top_p`` of their mass; of these the ones with at least ``min_p`` of the largest
     mass (the first always stays).  The draw takes, in the order of the indices, the first token at which the running
-    mass exceeds ``u`` times the whole.  Masses are ``exp((logit - largest) / temperature)`` in 64 bits, so that a draw
-    depends on nothing but its row: not on the batch, the device's load or the run.
+    mass exceeds ``u`` times the whole.  Masses are ``exp((logit - largest) / temperature)`` in 64 bits, rounded to
+    multiples of ``2^-44``, so that a draw depends on nothing but its row: not on the batch, the device's load or the run.
+    (A token more than 31 temperatures below the largest has no mass; borders and draws that lie within ``V 2^-44`` of a
+    token's running mass may go either way.)
 
     Each setting is a number, or a tensor ``(b,)`` with one value per row (values of tensors are not checked:
     ``temperature <= 0``, ``top_p <= 0`` and ``min_p > 1`` take the first largest logit, ``top_p >= 1`` keeps all).
