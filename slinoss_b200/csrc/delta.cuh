@@ -317,11 +317,11 @@ __device__ __forceinline__ void tile_rows(float (&c)[8][4], const Frag<SA> &a, c
   mma_group<SA, SB, 4>(c, 0, a, b);
 }
 // c (16 x W) += a (16 x 16 tokens) B for rows 16 kb .. of a row-major tile of W columns (planes `plane` apart)
-// (group: blocks of B that are held at a time)
-template <int SA, int SB, int W, int group = 4>
-__device__ __forceinline__ void tile_cols(float (&c)[W / 8][4], const Frag<SA> &a, const __half *tile, int plane, int kb) {
+// (group: blocks of B that are held at a time; cols: columns from `tile` on, all W of them or fewer)
+template <int SA, int SB, int W, int group = 4, int cols = W>
+__device__ __forceinline__ void tile_cols(float (&c)[cols / 8][4], const Frag<SA> &a, const __half *tile, int plane, int kb) {
 #pragma unroll
-  for (int n0 = 0; n0 < W / 16; n0 += group) {
+  for (int n0 = 0; n0 < cols / 16; n0 += group) {
     uint32_t b[group][SB][4];
 #pragma unroll
     for (int i = 0; i < group; ++i)

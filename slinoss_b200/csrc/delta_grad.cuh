@@ -31,30 +31,6 @@ constexpr int grad_smem() {
   return 2 * Operand<SI, NT>::halves * 2 + (SI + 2 * SC) * kTile * 2 + 2 * SC * 64 * (NT + 8) * 2 + kVectorBytes;
 }
 
-// sum over n of the rows' accumulators times the operand tile's rows (16 of them from `tile`); both rows of the thread
-template <int NT, int SI>
-__device__ __forceinline__ float2 row_dots(const float (&c)[NT / 8][4], const __half *tile, int e) {
-  constexpr int ld = NT + 8, plane = L * ld;
-  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  float x = 0.f, y = 0.f;
-#pragma unroll
-  for (int j = 0; j < NT / 8; ++j)
-#pragma unroll
-    for (int s = 0; s < SI; ++s) {
-      const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(tile + s * plane + g * ld + 8 * j + 2 * q));
-      const float2 w = __half22float2(*reinterpret_cast<const __half2 *>(tile + s * plane + (g + 8) * ld + 8 * j + 2 * q));
-      x = fmaf(c[j][0], u.x, fmaf(c[j][1], u.y, x));
-      y = fmaf(c[j][2], w.x, fmaf(c[j][3], w.y, y));
-    }
-#pragma unroll
-  for (int d = 1; d < 4; d <<= 1) {
-    x += __shfl_xor_sync(~0u, x, d);
-    y += __shfl_xor_sync(~0u, y, d);
-  }
-  const float f = pow2(e);
-  return make_float2(x * f, y * f);
-}
-
 __device__ __forceinline__ float over_quad(float x) {
   x += __shfl_xor_sync(~0u, x, 1);
   return x + __shfl_xor_sync(~0u, x, 2);
@@ -63,6 +39,25 @@ __device__ __forceinline__ float over_rows(float x) {  // of the eight quads
   x += __shfl_xor_sync(~0u, x, 4);
   x += __shfl_xor_sync(~0u, x, 8);
   return x + __shfl_xor_sync(~0u, x, 16);
+}
+
+// This thread's part of the sums over n of the rows' accumulators (n of 8 columns) times the operand tile's rows (16 of them from
+// `tile`); both rows of the thread
+template <int NT, int SI, int n>
+__device__ __forceinline__ float2 row_dots(const float (&c)[n][4], const __half *tile) {
+  constexpr int ld = NT + 8, plane = L * ld;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  float x = 0.f, y = 0.f;
+#pragma unroll
+  for (int j = 0; j < n; ++j)
+#pragma unroll
+    for (int s = 0; s < SI; ++s) {
+      const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(tile + s * plane + g * ld + 8 * j + 2 * q));
+      const float2 w = __half22float2(*reinterpret_cast<const __half2 *>(tile + s * plane + (g + 8) * ld + 8 * j + 2 * q));
+      x = fmaf(c[j][0], u.x, fmaf(c[j][1], u.y, x));
+      y = fmaf(c[j][2], w.x, fmaf(c[j][3], w.y, y));
+    }
+  return make_float2(x, y);
 }
 
 // A warp's 16 rows of dq or dk, from accumulators: half types through `buf` (16 x (NT + 8) halves of the warp's own) in
@@ -282,9 +277,9 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     }
     dot *= pow2(sr_top);
     const float fr = pow2(yr_top);
-    w = row_dots<NT, SI>(acc, krow, ek);
-    w.x *= closing[r0] * fr;
-    w.y *= closing[r1] * fr;
+    w = row_dots<NT, SI>(acc, krow);
+    w.x = over_quad(w.x) * pow2(ek) * (closing[r0] * fr);
+    w.y = over_quad(w.y) * pow2(ek) * (closing[r1] * fr);
 #pragma unroll
     for (int tb = 0; tb < 4; ++tb)
       if (tb >= warp) {
@@ -440,11 +435,11 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
     zero(H);
     const int ya = ey + ea, sa = es + ea;
     const int ya_top = __reduce_max_sync(~0u, ya), sa_top = __reduce_max_sync(~0u, sa);
-    // dk: f gamma times the tile as an operand; the factor, which exceeds one where gates do, enters the product's unit.  dq,
-    // whose sum starts here: the tile as it is, and the factor on the sum.
+    // The product with S0 has sums of its own, half of the columns at a time: times q or k they are what the gates let through
+    // to this token, and times f gamma (in fp32: beside open gates a closed one would leave nothing in fp16) they join dq or dk.
     const float g0 = f * gamma[r0], g1 = f * gamma[r1];
-    const int top = is_q ? 0 : __reduce_max_sync(~0u, max(mag(g0), mag(g1)));
-    float d0 = 0.f, d1 = 0.f;  // dX.(S0 k)
+    const int top = __reduce_max_sync(~0u, max(mag(g0), mag(g1)));
+    float2 d = make_float2(0.f, 0.f);
     float b0 = 0.f, b1 = 0.f;  // dk takes beta Z over
     int held = kZeroExp;
     if (!is_q) {
@@ -459,7 +454,6 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
       if (is_q) zero(acc);
       else times_rows(acc, b0 * u, b1 * u);
     }
-    Onto<NT, SI, SC> onto(acc);
 #pragma unroll 1
     for (int pt = 0; pt < tiles; ++pt) {
       if (tiles > 1) {
@@ -467,60 +461,45 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
         load(pt);
       }
       const int blocks = min(4, PB - 4 * pt);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float sum[NT / 16][4];
+        zero(sum);
 #pragma unroll 1
-      for (int kb = 0; kb < blocks; ++kb) {
-        Frag<SC> fa, fg;
-        load_a(fa, tile, is_q ? SI : SC, kb);
-        if (is_q) fg = scaled(fa, below(sa, unit, pt, kb));
-        else {
-          float sk[2][4];  // S0 k: tokens x channels, as the fragment of dX lies
-          zero(sk);
-#pragma unroll 2
-          for (int nb = 0; nb < NT / 16; ++nb) {
-            Frag<SI> fk;
-            uint32_t bs[SC][4];
+        for (int kb = 0; kb < blocks; ++kb) {
+          Frag<SC> fa;
+          load_a(fa, tile, is_q ? SI : SC, kb);
+          if (half == 0) {
+            const Frag<SC> fh = scaled(fa, below(ya, ya_top, pt, kb));
 #pragma unroll
-            for (int s = 0; s < SI; ++s) a_mk(fk.r[s], krow + s * Op::plane + 16 * nb, ld);
-#pragma unroll
-            for (int s = 0; s < SC; ++s) b_nk(bs[s], ss + s * splane + 16 * kb * ld + 16 * nb, ld);
-            mma_split<SI, SC>(sk[0], sk[1], fk, bs);
+            for (int sb = 0; sb < 4; ++sb)
+              if (sb <= warp) {
+                uint32_t bb[SC][4];
+                load_b(bb, ys, sb, kb);
+                mma_split<SC, SC>(H[2 * sb], H[2 * sb + 1], fh, bb);
+              }
           }
-          const float m = pow2(below(sa, unit, pt, kb)), f0 = g0 * m, f1 = g1 * m, n = pow2(below(sa, sa_top, pt, kb));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float2 x = unpack(fa.r[0][i]);
-            if constexpr (SC == 2) {
-              const float2 y = unpack(fa.r[1][i]);
-              x.x += y.x;
-              x.y += y.y;
-            }
-            float &d = i & 1 ? d1 : d0;
-            d = fmaf(n, fmaf(x.x, sk[i >> 1][(i & 1) * 2], x.y * sk[i >> 1][(i & 1) * 2 + 1]), d);
-            split<SC>(x.x * (i & 1 ? f1 : f0), x.y * (i & 1 ? f1 : f0), &fg.r[0][i], &fg.r[SC - 1][i]);
-          }
+          tile_cols<SC, SC, NT, NT == 128 && SC == 1 ? 4 : 2, NT / 2>(sum, scaled(fa, below(sa, sa_top, pt, kb)),
+                                                                      ss + half * (NT / 2), splane, kb);
         }
-        fa = scaled(fa, below(ya, ya_top, pt, kb));
+        const float2 x = row_dots<NT, SI>(sum, (is_q ? qs : ks) + 16 * warp * ld + half * (NT / 2));
+        d.x += x.x;
+        d.y += x.y;
+        const float u = pow2(sa_top - unit), f0 = g0 * u, f1 = g1 * u;
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb)
-          if (sb <= warp) {
-            uint32_t bb[SC][4];
-            load_b(bb, ys, sb, kb);
-            mma_split<SC, SC>(H[2 * sb], H[2 * sb + 1], fa, bb);
-          }
-        onto.template add<SC>(fg, ss, splane, kb);
+        for (int j = 0; j < NT / 16; ++j) {
+          float(&to)[4] = acc[half * (NT / 16) + j];
+          to[0] = fmaf(f0, sum[j][0], to[0]);
+          to[1] = fmaf(f0, sum[j][1], to[1]);
+          to[2] = fmaf(f1, sum[j][2], to[2]);
+          to[3] = fmaf(f1, sum[j][3], to[3]);
+        }
       }
     }
-    onto.join();
-    if (is_q) {
-      const float2 d = row_dots<NT, SI>(acc, qs + 16 * warp * ld, eq);
-      const float u = pow2(unit);
-      read.x = fmaf(d.x * u, g0, read.x);
-      read.y = fmaf(d.y * u, g1, read.y);
-      times_rows(acc, g0, g1);
-    } else {
-      const float u = pow2(sa_top);
-      read.x = over_quad(d0) * u * pow2(ek) * g0;
-      read.y = over_quad(d1) * u * pow2(ek) * g1;
+    {
+      const float u = pow2(sa_top), v = pow2(is_q ? eq : ek);
+      read.x = fmaf(over_quad(d.x) * u * v, g0, read.x);
+      read.y = fmaf(over_quad(d.y) * u * v, g1, read.y);
     }
 #pragma unroll
     for (int sb = 0; sb < 4; ++sb)

@@ -73,3 +73,19 @@ def test_how_far_a_non_finite_value_reaches(dtype, many, name):
             hit_final[1, heads, channels] = True
         assert torch.equal(o.isnan(), hit) and torch.equal(final.isnan(), hit_final), value
         assert torch.equal(o[~hit], clean[~hit]) and torch.equal(final[~hit_final], clean_final[~hit_final]), value
+
+
+# Independent roundings add up like the root of their number.  bf16: a result's own (steps of at most 2^-7 of it: 2^-7 / sqrt 12 =
+# 2.3e-3) and eight operands' of 11 bits (2^-10 / sqrt 12 each, together 8e-4): 2.4e-3, held to 3e-3.  fp16: 2^-10 / sqrt 12 =
+# 2.8e-4 and operands that do not show: 3e-4.  fp32: eight operands of 22 bits (4e-7 together), left-out products of two low parts
+# (2^-22 each), and sums whose instructions cut off up to 2^-24 at each of a chunk's 8 steps of 8 products, all downwards
+# (64 * 2^-24 / 2 = 2e-6 at worst): 3e-6.
+@pytest.mark.parametrize("dtype,bound,wide", [("bf16", 3e-3, 3e-6), ("fp16", 3e-4, 3e-6), ("fp32", 3e-6, 3e-6)])
+@pytest.mark.parametrize("b,h,hk,T,N,P", [(2, 4, 2, 300, 128, 64), (20, 8, 8, 130, 64, 64), (1, 4, 4, 200, 128, 128)])
+def test_errors_are_those_of_the_roundings(dtype, bound, wide, b, h, hk, T, N, P):
+    inp = make(b, h, hk, T, N, P, dtype, seed=80)
+    o, final, grads = run(inp)
+    ro, rfinal, rgrads = reference(inp)
+    errs = {"o": rel_err(_np(o), ro), **{n: rel_err(_np(t), rgrads[n]) for n, t in grads.items()}}
+    assert rel_err(_np(final), rfinal) <= wide and errs.pop("init") <= wide
+    assert max(errs.values()) <= bound, errs
