@@ -96,8 +96,9 @@ struct Operand {
 
 // ---- exponents -----------------------------------------------------------------------------------------------------
 constexpr int kZeroExp = -100;  // of a tile of zeros
-// Of a tile that holds an infinity or NaN: its powers are NaN, so that everything computed from the tile is NaN and not a
-// finite value that scaling by the infinity has wiped out.
+// Of a tile that holds an infinity or NaN.  pow2 of it, by which results are brought back to their unit, is NaN, so that all of
+// them are NaN and not finite values that scaling by the infinity has wiped out.  (pow2 of its negative, by which the tile is
+// brought to fp16, is zero.)
 constexpr int kNanExp = 2000;
 // (zero below the normal range)
 __device__ __forceinline__ float pow2(int e) {

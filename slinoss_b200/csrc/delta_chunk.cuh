@@ -9,7 +9,7 @@
 // they lie, so that warps meet only at the diagonal blocks.  Decays are exponentials of differences of G held in 64 bits:
 // a large |g| anywhere in the chunk costs the later, slowly decaying tokens no precision.
 //
-// 16384 chunks of one head each (N 128, bf16): 532 us, 1.1 GB of which written; 1.5 instructions a clock and SM at 16 warps, a
+// 16384 chunks of one head each (N 128, bf16): 526 us, 1.1 GB written; 1.4 instructions a clock and SM at 16 warps, a
 // quarter of the waiting at barriers (the first warp takes the gates' sums, the inverse of block column 0 is the longest).
 // Letting the other warps convert k and q meanwhile gains 2 % there and loses 8 % with 64 columns, for registers.
 #pragma once

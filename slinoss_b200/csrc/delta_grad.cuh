@@ -15,10 +15,12 @@
 // accumulators; Q and H are formed in both orientations, in registers, which costs 1/8 more products than passing them through
 // shared memory would save barriers.
 //
-// 16384 chunks of one head each (N 128, P 64, bf16): 898 us at two CTAs an SM (103 KB and 255 registers a thread); 160 KB a chunk
-// through HBM would take 400.  Eight warps a CTA, four for dO, Q and dq and four for dX, H and dk, take 1123 us: at 128 registers
-// they spill, with one CTA an SM nothing hides the loads.  fp16 with 64 columns (900 chunks, 108 KB): 74 us at two CTAs an SM,
-// 107 at one, which a second plane of dO made it.
+// 16384 chunks of one head each (N 128, P 64, bf16): 1058 us at two CTAs an SM (106 KB and 241 registers a thread), of which the
+// gates' terms are 160; 160 KB a chunk through HBM would take 400.  1.5 instructions a clock and SM, the tensor pipe busy 23 %: a
+// warp waits for its own products and for what it reads.  fp16 with 64 columns (900 chunks, 110 KB): 85 us at two CTAs an SM.
+// Without the gates' terms: 898 and 74; then eight warps a CTA, four for dO, Q and dq and four for dX, H and dk, took 1123 (at 128
+// registers they spill, with one CTA an SM nothing hides the loads), and fp16 at one CTA an SM 107, which a second plane of dO
+// made it.
 #pragma once
 
 #include "delta.cuh"
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(kThreads) delta_grad_kernel(Args a) {
         float qk[2][4], kk[2][4];
         zero(qk);
         zero(kk);
-#pragma unroll 2
+#pragma unroll 4
         for (int nb = 0; nb < NT / 16; ++nb) {
           Frag<SI> f;
           uint32_t bq[SI][4], bk[SI][4];

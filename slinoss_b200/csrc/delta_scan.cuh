@@ -11,7 +11,7 @@
 // The tiles of the next chunk are on their way while this one is computed: k is double-buffered, the rest is loaded again
 // as soon as its last reader is through.
 //
-// 256 heads of 4096 tokens (N 128, P 64, bf16): 467 us forwards, 519 back, at two CTAs an SM; the state, two results and their
+// 256 heads of 4096 tokens (N 128, P 64, bf16): 466 us forwards, 513 back, at two CTAs an SM; the state, two results and their
 // fp16 parts fill the registers.  With one warp a scheduler the tensor pipe is busy 35 to 40 %: the rest is the chain of products
 // of one warp (11 thousand clocks a chunk alone, 14 with a second CTA beside it).
 #pragma once

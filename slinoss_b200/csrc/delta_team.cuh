@@ -8,7 +8,7 @@
 // warps copy the next chunk's tiles in, form the outputs (from the state's fragments, 16 tokens each) and write everything that
 // goes to memory.  Four barriers a chunk.  All tiles are double-buffered: a CTA has its SM to itself.
 //
-// 32 heads of 32768 tokens (N 128, P 64, bf16): 1104 us forwards, 1177 back, 4100 clocks a chunk (11 thousand for a warp by
+// 32 heads of 32768 tokens (N 128, P 64, bf16): 1083 us forwards, 1178 back, 4100 clocks a chunk (11 thousand for a warp by
 // itself).  What is left is the chain: partial sums, X, Tm X and the state's update, each behind a barrier; fragments fetched
 // ahead of their barrier made it slower.
 #pragma once

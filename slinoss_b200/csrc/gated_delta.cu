@@ -81,10 +81,10 @@ static Args args_of(const slx_gated_delta_shape *s, const Dims &d) {
 
 // Zero: teams of eight warps on 16 value channels, where each can have an SM to itself, or two rounds of teams fill the SMs well.
 // Else the warps of a CTA that hold 16 channels each: as many as there are, up to four, which share a CTA's tiles.  Measured
-// (T 2048, N 128, P 64, bf16, forward and training, us) with 128 blocks of 16 channels: teams 107 / 265, warps 178 / 433; with
-// 256: 201 / 493 and 215 / 529; with 320: 281 / 679 and 232 / 578.  Between 148 and 222 blocks teams take what they take with
+// (T 2048, N 128, P 64, bf16, forward and training, us) with 128 blocks of 16 channels: teams 102 / 275, warps 176 / 444; with
+// 256: 194 / 511 and 209 / 550; with 320: 270 / 700 and 231 / 617.  Between 148 and 222 blocks teams take what they take with
 // 256, and the warps, whose time grows with the blocks, less.  Fewer than four warps a CTA are never faster (512 blocks: four
-// 286 / 725, two 332 / 836, one 424 / 1027).
+// 275 / 767, two 323 / 873, one 413 / 1065).
 static int scan_warps(const Dims &d) {
   const int64_t blocks = d.BH * d.PB, two_rounds = 2 * kB200Sms;
   if (blocks <= kB200Sms || (4 * blocks >= 3 * two_rounds && blocks <= two_rounds)) return 0;

@@ -3,8 +3,9 @@
 // The state is read and written once, 8 P N bytes per head, and that is what the step costs: both dots of a state row are
 // taken in one pass over it (k.q is known beforehand), so a row goes from memory through registers and back.  Sixteen lanes
 // share a row of more than 32 values (E vectors of four each), fewer a shorter one: the rows side by side in a warp meet for
-// their dots in one set of exchanges.  Batch 256, 32 heads, 64 x 128 states (536 MB): 86.0 us, as a plain copy of the states
-// takes; 32 lanes a row 102 us, eight 87.6; four groups of rows in flight 95 and 108.
+// their dots in one set of exchanges.  Batch 256, 32 heads, 64 x 128 states (536 MB): 90 us a call among others with other states
+// (6030 GB/s), as a plain copy of the states takes; the kernel on one set of states 86, with 32 lanes a row 102, with eight 87.6;
+// four groups of rows in flight 95 and 108.
 #include "common.cuh"
 
 namespace slx {
